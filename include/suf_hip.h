@@ -889,6 +889,155 @@ int sufhip_beaver_matmul2_mfma_batched(const int8_t* d_Dp, const int8_t* d_Ep,
                                        int M, int K, int N, uint64_t* d_out0, uint64_t* d_out1,
                                        void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* Attention over a paged cache of keys and values, both parties on one    */
+/* GPU: rotary positions, the append, and the two products of packed       */
+/* sequences of different lengths with grouped heads.  The reference keeps */
+/* a cache of shares (include/nn/kv_cache.hpp) and opens every key again   */
+/* for each new token; here a key or value is opened once, when it is      */
+/* appended, under a mask that stays with it: the cache holds the public   */
+/* E = value - b and both parties' shares of b.  A later product needs     */
+/* only a fresh mask A of its own left operand, and the dealer's C = A b.  */
+/* ---------------------------------------------------------------------- */
+/* One party pair of packed rows: value i of head h of token t of party p at
+ * p[p][t * token_stride + h * head_stride + i] (u64 units, strides >= 0). */
+typedef struct sufhip_rows2 {
+  const uint64_t* p[2];
+  int64_t token_stride, head_stride;
+} sufhip_rows2;
+
+/* A public rotary table: d_table [positions][rot / 2][cos, sin] int32
+ * fixed-point factors (8-byte aligned), rot even, 0 <= rot <= the head's
+ * dim.  Pair i of a head's first rot values, (u, v) = (x[i], x[rot / 2 + i])
+ * or, with interleaved, (x[2 i], x[2 i + 1]), becomes (u c - v s, u s + v c)
+ * at the token's position; the other values are multiplied by pass_mul (the
+ * table's 1, so that the whole head has one scale).  d_table may be NULL when
+ * rot is 0. */
+typedef struct sufhip_rotary {
+  const int32_t* d_table;
+  int positions, rot, interleaved;
+  int64_t pass_mul;
+} sufhip_rotary;
+
+/* Rotary positions on both parties' shares of tokens x heads x dim values:
+ * the map is linear with public factors, so each party's is local and exact
+ * mod 2^64.  d_positions [tokens]; a token whose position is outside
+ * [0, positions) is padding and its output rows are left as they were.
+ * out[p] with its own strides may be x.p[p] with the same strides (in
+ * place); any other overlap is undefined, and so are output rows that
+ * overlap each other.  trunc (optional): the open out_0 + out_1 + mask feeds
+ * this prepared GapARS table gate (no addend), whose outputs trunc->y are
+ * written at the output positions instead of out. */
+typedef struct sufhip_rotary2_args {
+  sufhip_rows2 x;
+  int tokens, heads, dim;
+  sufhip_rotary rot;
+  const int32_t* d_positions;
+  uint64_t* out[2];
+  int64_t out_token_stride, out_head_stride;
+  const sufhip_trunc_epilogue* trunc;
+  uint64_t mask;
+} sufhip_rotary2_args;
+int sufhip_rotary2(const sufhip_rotary2_args* args, void* stream);
+
+/* The packed new tokens of a batch of sequences and the pages of their
+ * caches.  Sequence s's new tokens are rows d_cu_tokens[s] ..
+ * d_cu_tokens[s + 1] - 1 of every token array ([seqs + 1], not decreasing);
+ * rows in no sequence are padding: nothing of them is read or written.
+ * d_kv_lens [seqs]: keys of each sequence, its new tokens (the last ones)
+ * included.  d_pages [seqs][max_pages]: the pool page of each page_tokens
+ * keys; entries past a sequence's length are not used.  A page number outside
+ * the pool stands for no page: an append skips its tokens, the products take
+ * its keys and values as zeros.  max_new, max_keys: the most new tokens and
+ * keys of a sequence, by which a launch is laid out; the results do not
+ * depend on them, so a captured launch may keep bounds. */
+typedef struct sufhip_kv_batch {
+  int seqs, tokens;
+  const int32_t* d_cu_tokens;
+  const int32_t* d_kv_lens;
+  const int32_t* d_pages;
+  int max_pages;
+  int max_new, max_keys;
+} sufhip_kv_batch;
+
+/* Pages of keys or of values: e (the open value - b) and b[p] (party p's
+ * share of the mask), each [pages][kv_heads][page_tokens][dim] u64;
+ * page_tokens a power of two, 1 <= dim <= SUFHIP_KV_MAX_DIM. */
+#define SUFHIP_KV_MAX_DIM 256
+typedef struct sufhip_kv_pool {
+  uint64_t* e;
+  uint64_t* b[2];
+  int pages, page_tokens, kv_heads, dim;
+} sufhip_kv_pool;
+
+/* Appends the new tokens' rows to the pages of their sequences: for every
+ * new token and cached head, value - (mask_0 + mask_1) opened into e and the
+ * masks into b.  mask[p] [tokens][kv_heads][dim] (the dealer's shares of a
+ * mask used for nothing else).  Two parts at most, the keys and the values
+ * (e.g. part[0] rotated, part[1] not); a part with pool.e = NULL is absent.
+ * rot, unless its table is NULL and it has no positions: the rows are rotated
+ * on the way, by d_positions [tokens] if given, else by their places in their
+ * sequences; outside the table's positions nothing is written.  trunc (optional): the (rotated) rows are
+ * truncated before the open, by the gate fed with x_0 + x_1 + mask_trunc; its
+ * y[p] receive the truncated shares [tokens][kv_heads][dim], or are both NULL.
+ * Places not appended to keep their contents.  A place written twice by one
+ * call (a page listed twice) holds one of the writes or a mix. */
+typedef struct sufhip_kv_append_part {
+  sufhip_rows2 x;
+  const uint64_t* mask[2];
+  sufhip_kv_pool pool;
+  sufhip_rotary rot;
+  const int32_t* d_positions;
+  const sufhip_trunc_epilogue* trunc;
+  uint64_t trunc_mask;
+} sufhip_kv_append_part;
+typedef struct sufhip_kv_append2_args {
+  sufhip_kv_batch batch;
+  sufhip_kv_append_part part[2];
+} sufhip_kv_append2_args;
+int sufhip_kv_append2(const sufhip_kv_append2_args* args, void* stream);
+
+/* The two products of attention, exact mod 2^64.  Query head h of heads (a
+ * multiple of kv_heads) uses cached head h / (heads / kv_heads).  Packed
+ * rows: row (h, t) starts at element d_row_offsets[h * tokens + t] and holds
+ * d_row_offsets[h * tokens + t + 1] - d_row_offsets[h * tokens + t] elements
+ * ([heads * tokens + 1], not decreasing), one for each of its sequence's
+ * first keys (causal: keys up to the token's own; a row may be empty).  Of a
+ * row longer than its sequence the elements past the last key are not used;
+ * a row that does not lie within the n packed elements counts as empty.
+ *   scores (row (h, t), key j), over i < dim:
+ *     Z_p = C_p + sum_i D_i b_p[j][i] + (A_p,i + [p = 0] D_i) e[j][i]
+ *     x, a, D per value of the token's head; c, out per packed element
+ *   values (row (h, t), column i), over the row's keys j:
+ *     Z_p = C_p + sum_j D_j b_p[j][i] + (A_p,j + [p = 0] D_j) e[j][i]
+ *     x, a, D per packed element; c, out [tokens][heads][dim]
+ * with D = (x_0 - a_0) + (x_1 - a_1) opened on the way.  scores: x.p with
+ * strides, a[p] [tokens][heads][dim].  values: x.p packed, its strides not
+ * used.  An empty row's values are C_p.  n: packed elements (at most
+ * 2^31 - 1).  trunc (optional): the open Z_0 + Z_1 + mask feeds this prepared
+ * GapARS table gate (no addend), whose outputs y are written in place of out.
+ * d_work (values): sufhip_kv_values2_work_bytes() bytes, 16-byte aligned,
+ * used by this call only until it ends; 0 bytes: none needed. */
+typedef struct sufhip_kv_product2_args {
+  sufhip_kv_batch batch;
+  sufhip_kv_pool pool;
+  int heads;
+  sufhip_rows2 x;
+  const uint64_t* a[2];
+  const uint64_t* c[2];
+  const int32_t* d_row_offsets;
+  size_t n;
+  uint64_t* out[2];
+  const sufhip_trunc_epilogue* trunc;
+  uint64_t mask;
+  void* d_work;
+  size_t work_bytes;
+} sufhip_kv_product2_args;
+int sufhip_kv_scores2(const sufhip_kv_product2_args* args, void* stream);
+size_t sufhip_kv_values2_work_bytes(const sufhip_kv_batch* batch, const sufhip_kv_pool* pool,
+                                    int heads);
+int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream);
+
 /* Share x public weight for both parties (nn::matmul_publicW_gpu,
  * src/nn/matmul_gpu.cu:388-720; CPU form src/nn/matmul_publicW.cpp:17-36):
  * Y_p = X_p * W mod 2^64, X_p [M x K] u64 shares, W [K x N] public int64, on

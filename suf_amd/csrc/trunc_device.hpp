@@ -195,7 +195,9 @@ __device__ __forceinline__ void put_open(const TruncEpi& e, const EpiHdrs& eh, u
 }
 
 // Validates an epilogue for n elements and converts it (NULL -> off).
-inline int make_epi(const sufhip_trunc_epilogue* t, size_t n, const char* what, TruncEpi* out) {
+// need_y false: the outputs may be absent, both of them.
+inline int make_epi(const sufhip_trunc_epilogue* t, size_t n, const char* what, TruncEpi* out,
+                    bool need_y = true) {
   *out = TruncEpi{{nullptr, nullptr}, {nullptr, nullptr}, {nullptr, nullptr}, {nullptr, nullptr},
                   0, 0};
   if (!t) return SUFHIP_OK;
@@ -204,7 +206,8 @@ inline int make_epi(const sufhip_trunc_epilogue* t, size_t n, const char* what, 
     return SUFHIP_ERR_INVALID;
   }
   const bool ok = t->frac_bits >= 1 && t->frac_bits <= kTruncTableBits && t->key[0] &&
-                  t->key[1] && t->table[0] && t->table[1] && t->y[0] && t->y[1] &&
+                  t->key[1] && t->table[0] && t->table[1] &&
+                  (need_y ? t->y[0] && t->y[1] : (t->y[0] == nullptr) == (t->y[1] == nullptr)) &&
                   (reinterpret_cast<uintptr_t>(t->key[0]) & 7) == 0 &&
                   (reinterpret_cast<uintptr_t>(t->key[1]) & 7) == 0 &&
                   (reinterpret_cast<uintptr_t>(t->table[0]) & 15) == 0 &&

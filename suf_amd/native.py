@@ -102,6 +102,11 @@ _SIGS = {
     "sufhip_beaver_matmul2_mfma_batched": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                                    c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp,
                                                    c_vp]),
+    "sufhip_rotary2": (c_int, [c_vp, c_vp]),
+    "sufhip_kv_append2": (c_int, [c_vp, c_vp]),
+    "sufhip_kv_scores2": (c_int, [c_vp, c_vp]),
+    "sufhip_kv_values2_work_bytes": (c_sz, [c_vp, c_vp, c_int]),
+    "sufhip_kv_values2": (c_int, [c_vp, c_vp]),
     "sufhip_public_w_digits": (c_int, [c_vp, c_sz]),
     "sufhip_public_w_planes_bytes": (c_sz, [c_int, c_int, c_int]),
     "sufhip_public_w_prepare": (c_int, [c_vp, c_int, c_int, c_int, c_vp, c_vp]),
@@ -260,6 +265,60 @@ class KbOpenJob(ctypes.Structure):
                 ("rows", c_int), ("cols", c_int), ("k_is_col", c_int), ("planes_a0", c_vp),
                 ("a0", c_vp), ("a_stride", ctypes.c_int64 * 3), ("valid_rows", c_int),
                 ("valid_cols", c_int)]
+
+
+class Rows2(ctypes.Structure):
+    """sufhip_rows2 (include/suf_hip.h)."""
+    _fields_ = [("p", c_vp * 2), ("token_stride", c_i64), ("head_stride", c_i64)]
+
+
+class RotaryTable(ctypes.Structure):
+    """sufhip_rotary (include/suf_hip.h)."""
+    _fields_ = [("d_table", c_vp), ("positions", c_int), ("rot", c_int), ("interleaved", c_int),
+                ("pass_mul", c_i64)]
+
+
+class Rotary2Args(ctypes.Structure):
+    """sufhip_rotary2_args (include/suf_hip.h)."""
+    _fields_ = [("x", Rows2), ("tokens", c_int), ("heads", c_int), ("dim", c_int),
+                ("rot", RotaryTable), ("d_positions", c_vp), ("out", c_vp * 2),
+                ("out_token_stride", c_i64), ("out_head_stride", c_i64),
+                ("trunc", ctypes.POINTER(TruncEpilogue)), ("mask", c_u64)]
+
+
+KV_MAX_DIM = 256
+
+
+class KvBatch(ctypes.Structure):
+    """sufhip_kv_batch (include/suf_hip.h)."""
+    _fields_ = [("seqs", c_int), ("tokens", c_int), ("d_cu_tokens", c_vp), ("d_kv_lens", c_vp),
+                ("d_pages", c_vp), ("max_pages", c_int), ("max_new", c_int), ("max_keys", c_int)]
+
+
+class KvPool(ctypes.Structure):
+    """sufhip_kv_pool (include/suf_hip.h)."""
+    _fields_ = [("e", c_vp), ("b", c_vp * 2), ("pages", c_int), ("page_tokens", c_int),
+                ("kv_heads", c_int), ("dim", c_int)]
+
+
+class KvAppendPart(ctypes.Structure):
+    """sufhip_kv_append_part (include/suf_hip.h)."""
+    _fields_ = [("x", Rows2), ("mask", c_vp * 2), ("pool", KvPool), ("rot", RotaryTable),
+                ("d_positions", c_vp), ("trunc", ctypes.POINTER(TruncEpilogue)),
+                ("trunc_mask", c_u64)]
+
+
+class KvAppend2Args(ctypes.Structure):
+    """sufhip_kv_append2_args (include/suf_hip.h)."""
+    _fields_ = [("batch", KvBatch), ("part", KvAppendPart * 2)]
+
+
+class KvProduct2Args(ctypes.Structure):
+    """sufhip_kv_product2_args (include/suf_hip.h)."""
+    _fields_ = [("batch", KvBatch), ("pool", KvPool), ("heads", c_int), ("x", Rows2),
+                ("a", c_vp * 2), ("c", c_vp * 2), ("d_row_offsets", c_vp), ("n", c_sz),
+                ("out", c_vp * 2), ("trunc", ctypes.POINTER(TruncEpilogue)), ("mask", c_u64),
+                ("d_work", c_vp), ("work_bytes", c_sz)]
 
 
 class Triple2(ctypes.Structure):
