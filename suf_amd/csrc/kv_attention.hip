@@ -19,6 +19,7 @@ struct ProductArgs {
   KvBatch b;
   KvPool pool;
   int heads, group;
+  FastDiv by_group;
   const uint64_t* x[2];
   int64_t xts, xhs;
   const uint64_t* a[2];
@@ -42,16 +43,30 @@ __device__ __forceinline__ Span span_of(const ProductArgs& a, int h, int t, int 
   return {int(f), int(l < kv ? l : kv)};
 }
 
-// Both parties' finished values of output element i.
-__device__ __forceinline__ void put2(const ProductArgs& a, const EpiHdrs& eh, int64_t i,
-                                     uint64_t z0, uint64_t z1) {
-  if (a.epi.on) {
-    put_open(a.epi, eh, nullptr, size_t(i), z0 + z1 + a.mask);
-  } else {
+// Both parties' finished values of output element i: to the outputs, or the
+// open through the truncation gate.
+template <bool kTrunc>
+struct Put {
+  __device__ __forceinline__ explicit Put(const ProductArgs&) {}
+  __device__ __forceinline__ void operator()(const ProductArgs& a, int64_t i, uint64_t z0,
+                                             uint64_t z1) const {
     a.out[0][i] = z0;
     a.out[1][i] = z1;
   }
-}
+};
+template <>
+struct Put<true> {
+  EpiHdrs eh;
+  __device__ __forceinline__ explicit Put(const ProductArgs& a) : eh(epi_hdrs(a.epi)) {}
+  __device__ __forceinline__ void operator()(const ProductArgs& a, int64_t i, uint64_t z0,
+                                             uint64_t z1) const {
+    const uint64_t open = z0 + z1 + a.mask;
+    const uint64_t w0 = trunc_table_word(eh.h[0], a.epi.table[0], a.epi.f, open);
+    const uint64_t w1 = trunc_table_word(eh.h[1], a.epi.table[1], a.epi.f, open);
+    a.epi.y[0][i] = trunc_table_out(eh.h[0], a.epi.f, open, w0);
+    a.epi.y[1][i] = trunc_table_out(eh.h[1], a.epi.f, open, w1);
+  }
+};
 
 // ---- digits ----
 //
@@ -105,17 +120,6 @@ __device__ __forceinline__ uint64_t from_sums(const v4i (&acc)[kDigitPlanes], in
   return lo + (uint64_t(hi) << 32);
 }
 
-// acc += l r over the digit pairs of weight below 256^8.
-__device__ __forceinline__ void mul_digits(const v4i (&l)[kDigitPlanes],
-                                           const v4i (&r)[kDigitPlanes],
-                                           v4i (&acc)[kDigitPlanes]) {
-#pragma unroll
-  for (int i = 0; i < kDigitPlanes; ++i)
-#pragma unroll
-    for (int j = 0; i + j < kDigitPlanes; ++j)
-      acc[i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(l[i], r[j], acc[i + j], 0, 0, 0);
-}
-
 // ---- left operands in LDS ----
 //
 // One 16 x 64 tile (16 rows, 64 of k) of the three left operands D, L_0, L_1
@@ -124,49 +128,91 @@ __device__ __forceinline__ void mul_digits(const v4i (&l)[kDigitPlanes],
 // 16-byte read and a wave reads a plane's 1 KB in order.
 constexpr int kTileBytes = 3 * kDigitPlanes * 1024;
 
-__device__ __forceinline__ void put_left(int8_t* tile, int r, int g, int q, const uint64_t (&x0)[4],
-                                         const uint64_t (&x1)[4], const uint64_t (&a0)[4],
-                                         const uint64_t (&a1)[4]) {
-  uint64_t d[4], l0[4];
+// kN of a row's k from byte j0 of group g on (kN = 2 or 4, j0 a multiple).
+template <int kN>
+__device__ __forceinline__ void put_digits(int8_t* plane0, const uint64_t (&v)[kN]) {
+  if constexpr (kN == 4) {
+    uint32_t pl[8];
+    digits_of4(v, pl);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    d[k] = (x0[k] - a0[k]) + (x1[k] - a1[k]);
-    l0[k] = a0[k] + d[k];
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(plane0 + i * 1024) = pl[i];
+  } else {
+    const uint64_t u0 = (v[0] + kBias) ^ kBias, u1 = (v[1] + kBias) ^ kBias;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t w0 = uint32_t(u0 >> (32 * h)), w1 = uint32_t(u1 >> (32 * h));
+      const uint32_t a = __builtin_amdgcn_perm(w1, w0, 0x05010400u);
+      const uint32_t b = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+      int8_t* p = plane0 + 4096 * h;
+      *reinterpret_cast<uint16_t*>(p) = uint16_t(a);
+      *reinterpret_cast<uint16_t*>(p + 1024) = uint16_t(a >> 16);
+      *reinterpret_cast<uint16_t*>(p + 2048) = uint16_t(b);
+      *reinterpret_cast<uint16_t*>(p + 3072) = uint16_t(b >> 16);
+    }
   }
-  uint32_t pl[8];
-  uint32_t* w = reinterpret_cast<uint32_t*>(tile) + (r * 4 + g) * 4 + q;
-  digits_of4(d, pl);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i * 256] = pl[i];
-  digits_of4(l0, pl);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[2048 + i * 256] = pl[i];
-  digits_of4(a1, pl);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[4096 + i * 256] = pl[i];
 }
 
-// Operand o's planes for lane l (row l % 16, k group l / 16).
-__device__ __forceinline__ void get_left(const int8_t* tile, int o, int l,
-                                         v4i (&pl)[kDigitPlanes]) {
-  const int8_t* p = tile + o * 8192 + ((l & 15) * 4 + (l >> 4)) * 16;
+// kN words of each array a left operand is formed from.
+template <int kN>
+struct Raw {
+  uint64_t x0[kN], x1[kN], a0[kN], a1[kN];
+};
+template <int kN>
+__device__ __forceinline__ void put_left(int8_t* tile, int r, int g, int j0, const Raw<kN>& v) {
+  uint64_t d[kN], l0[kN];
 #pragma unroll
-  for (int i = 0; i < kDigitPlanes; ++i) pl[i] = *reinterpret_cast<const v4i*>(p + i * 1024);
+  for (int k = 0; k < kN; ++k) {
+    d[k] = (v.x0[k] - v.a0[k]) + (v.x1[k] - v.a1[k]);
+    l0[k] = v.a0[k] + d[k];
+  }
+  int8_t* p = tile + (r * 4 + g) * 16 + j0;
+  put_digits<kN>(p, d);
+  put_digits<kN>(p + 8192, l0);
+  put_digits<kN>(p + 16384, v.a1);
 }
 
-// Both parties' digit products of a left tile with the right operands.
+// Plane i of operand o for lane l (row l % 16, k group l / 16).
+__device__ __forceinline__ v4i get_left(const int8_t* tile, int o, int l, int i) {
+  return *reinterpret_cast<const v4i*>(tile + o * 8192 + i * 1024 + ((l & 15) * 4 + (l >> 4)) * 16);
+}
+
+// acc += (left operand o) r over the digit pairs of weight below 256^8.
+__device__ __forceinline__ void mul_left(const int8_t* tile, int o, int l,
+                                         const v4i (&r)[kDigitPlanes],
+                                         v4i (&acc)[kDigitPlanes]) {
+#pragma unroll
+  for (int i = 0; i < kDigitPlanes; ++i) {
+    const v4i x = get_left(tile, o, l, i);
+#pragma unroll
+    for (int j = 0; i + j < kDigitPlanes; ++j)
+      acc[i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, r[j], acc[i + j], 0, 0, 0);
+  }
+}
+
+// Both parties' digit products of a left tile with the right operands: D with
+// the parties' masks, then all of them.
+__device__ __forceinline__ void mul_opened(const int8_t* tile, int l,
+                                           const v4i (&b0)[kDigitPlanes],
+                                           const v4i (&b1)[kDigitPlanes],
+                                           v4i (&acc)[2][kDigitPlanes]) {
+#pragma unroll
+  for (int i = 0; i < kDigitPlanes; ++i) {
+    const v4i x = get_left(tile, 0, l, i);
+#pragma unroll
+    for (int j = 0; i + j < kDigitPlanes; ++j) {
+      acc[0][i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, b0[j], acc[0][i + j], 0, 0, 0);
+      acc[1][i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, b1[j], acc[1][i + j], 0, 0, 0);
+    }
+  }
+}
+
 __device__ __forceinline__ void mul_tile(const int8_t* tile, int l, const v4i (&e)[kDigitPlanes],
                                          const v4i (&b0)[kDigitPlanes],
                                          const v4i (&b1)[kDigitPlanes],
                                          v4i (&acc)[2][kDigitPlanes]) {
-  v4i x[kDigitPlanes];
-  get_left(tile, 0, l, x);
-  mul_digits(x, b0, acc[0]);
-  mul_digits(x, b1, acc[1]);
-  get_left(tile, 1, l, x);
-  mul_digits(x, e, acc[0]);
-  get_left(tile, 2, l, x);
-  mul_digits(x, e, acc[1]);
+  mul_opened(tile, l, b0, b1, acc);
+  mul_left(tile, 1, l, e, acc[0]);
+  mul_left(tile, 2, l, e, acc[1]);
 }
 
 __device__ __forceinline__ void clear(v4i (&acc)[2][kDigitPlanes]) {
@@ -181,10 +227,10 @@ __device__ __forceinline__ void clear(v4i (&acc)[2][kDigitPlanes]) {
 struct Seq {
   int s, hk, t0, rows, kv;
 };
-__device__ __forceinline__ Seq seq_at(const ProductArgs& a, int64_t z) {
+__device__ __forceinline__ Seq seq_at(const ProductArgs& a, int z) {
   Seq q;
-  q.s = int(z / a.pool.heads);
-  q.hk = int(z - int64_t(q.s) * a.pool.heads);
+  q.s = z / a.pool.heads;
+  q.hk = z - q.s * a.pool.heads;
   const int lo = a.b.cu[q.s], hi = a.b.cu[q.s + 1];
   q.t0 = lo > 0 ? lo : 0;
   const int t1 = hi < a.b.tokens ? hi : a.b.tokens;
@@ -193,43 +239,60 @@ __device__ __forceinline__ Seq seq_at(const ProductArgs& a, int64_t z) {
   return q;
 }
 
+// Row m of a sequence: its token, head and packed elements (m past the last
+// row: token -1, no elements).
+struct Row {
+  int t, h, first, len;
+};
+__device__ __forceinline__ Row row_at(const ProductArgs& a, const Seq& q, int m) {
+  if (m >= q.rows) return {-1, 0, 0, 0};
+  const int tl = int(div_by(a.by_group, uint32_t(m)));
+  const int t = q.t0 + tl, h = q.hk * a.group + (m - tl * a.group);
+  const Span sp = span_of(a, h, t, q.kv);
+  return {t, h, sp.first, sp.len};
+}
+
 // ---- scores ----
 //
-// A workgroup of 4 waves takes 64 keys of one cached head, 16 to a wave (the
-// columns of a 16 x 16 tile), and runs over row tiles.  The keys' digits are
-// formed once, in registers, straight from the pages; the row tiles' pass
-// through LDS.  k order: byte j = 2 i + e of group g stands for dim 8 i + 2 g
-// + e of a 64-wide chunk, so each of a lane's 16-byte loads has its
-// neighbours' beside it (64 contiguous bytes a key).
-constexpr int kKeyTile = 64;
-constexpr int kRowGroup = 16;  // row tiles whose spans are read at once
+// A wave takes 16 keys of one cached head (the columns of a 16 x 16 tile), a
+// workgroup 16 for each of its waves.  The keys' digits are formed in
+// registers straight from the pages, the rows' pass through LDS.  k order:
+// byte j = 2 i + e of group g stands for dim 8 i + 2 g + e of a 64-wide
+// chunk, so each of a lane's 16-byte loads has its neighbours' beside it (64
+// contiguous bytes a key).
+//
+// Every lane loads from its page or, where there is none (past the last key,
+// a page number outside the pool), from the pool's first word: a key reaches
+// its own column alone, and that column's product is dropped.  Values past a
+// head's last meet zero digits of the left operand.  So no load is
+// conditional, and the loads of a tile leave together.
 
-template <bool kVec>
-__device__ __forceinline__ void load_keys(const uint64_t* p, bool ok, int g, int left,
-                                          uint64_t (&v)[16]) {
+// kFull: dim is a multiple of 64.
+template <bool kVec, bool kFull>
+__device__ __forceinline__ void load_keys(const uint64_t* p, int g, int left, uint64_t (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int d = 8 * i + 2 * g;
     if constexpr (kVec) {
-      ulonglong2 w = make_ulonglong2(0, 0);
-      if (ok && d < left) w = *reinterpret_cast<const ulonglong2*>(p + d);
+      const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(p + (kFull || d < left ? d : 0));
       v[2 * i] = w.x;
       v[2 * i + 1] = w.y;
     } else {
-      v[2 * i] = ok && d < left ? p[d] : 0;
-      v[2 * i + 1] = ok && d + 1 < left ? p[d + 1] : 0;
+      v[2 * i] = p[d < left ? d : 0];
+      v[2 * i + 1] = p[d + 1 < left ? d + 1 : 0];
     }
   }
 }
 
-template <bool kVec>
-__device__ __forceinline__ void load_left4(const uint64_t* p, int d, int left, uint64_t (&v)[4]) {
+// Words at dims d (+ 8 for the second pair).
+template <int kN, bool kVec, bool kFull>
+__device__ __forceinline__ void load_left(const uint64_t* p, int d, int left, uint64_t (&v)[kN]) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < kN / 2; ++h) {
     const int o = d + 8 * h;
     if constexpr (kVec) {
       ulonglong2 w = make_ulonglong2(0, 0);
-      if (o < left) w = *reinterpret_cast<const ulonglong2*>(p + o);
+      if (kFull || o < left) w = *reinterpret_cast<const ulonglong2*>(p + o);
       v[2 * h] = w.x;
       v[2 * h + 1] = w.y;
     } else {
@@ -239,124 +302,226 @@ __device__ __forceinline__ void load_left4(const uint64_t* p, int d, int left, u
   }
 }
 
-// kHeld: 64-wide chunks of the keys held as digits over all row tiles (0:
-// any number of chunks, loaded for each row tile again).
-template <int kHeld, bool kVec>
-__global__ void __launch_bounds__(256, kHeld == 2 ? 1 : 2) kv_scores2_kernel(ProductArgs a,
-                                                                             int chunks) {
+// kN of a 64-wide chunk of a row's left operands, of 64 / kN threads a row:
+// thread part takes group part % 4, bytes kN (part / 4) on.  A thread whose
+// words lie past the head's last leaves v as it is (zeros from the start).
+template <int kN, bool kVec, bool kFull>
+__device__ __forceinline__ void load_raw(const ProductArgs& a, const Row& r, int c, int part,
+                                         Raw<kN>& v) {
+  const int d = 4 * kN * (part >> 2) + 2 * (part & 3), left = a.pool.dim - 64 * c;
+  if (r.t < 0 || d >= left) return;
+  const int64_t xo = int64_t(r.t) * a.xts + int64_t(r.h) * a.xhs + 64 * c;
+  const int64_t ao = (int64_t(r.t) * a.heads + r.h) * a.pool.dim + 64 * c;
+  load_left<kN, kVec, kFull || (kVec && kN == 2)>(a.x[0] + xo, d, left, v.x0);
+  load_left<kN, kVec, kFull || (kVec && kN == 2)>(a.x[1] + xo, d, left, v.x1);
+  load_left<kN, kVec, kFull || (kVec && kN == 2)>(a.a[0] + ao, d, left, v.a0);
+  load_left<kN, kVec, kFull || (kVec && kN == 2)>(a.a[1] + ao, d, left, v.a1);
+}
+// Rows past the last write what their registers hold: a row of the left
+// operand reaches that row of the product alone, and it is not stored.
+template <int kN>
+__device__ __forceinline__ void put_raw(int8_t* tile, int row, int part, const Raw<kN>& v) {
+  put_left<kN>(tile, row, part & 3, kN * (part >> 2), v);
+}
+
+// Few rows: a workgroup keeps one row tile in LDS and streams its share of
+// the keys, 64 at a time.  Bound by HBM: an array's 16 words a lane are
+// turned into digits, the next tile's loads leave into the same registers,
+// and the matrix cores run under them, so a wave has up to 24 KB in flight.
+constexpr int kKeyTile = 64;
+
+template <bool kVec, bool kFull, bool kTrunc>
+__global__ void __launch_bounds__(256, kVec && !kTrunc ? 2 : 1)
+    kv_scores2_few_kernel(ProductArgs a, int chunks) {
   extern __shared__ __align__(16) int8_t tiles[];
-  __shared__ int first[kRowGroup * 16];
-  __shared__ int len[kRowGroup * 16];
-  __shared__ unsigned active;
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  __shared__ Row rows[16];
+  const int tid = threadIdx.x, l = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = l >> 4, n = l & 15;
   const int dim = a.pool.dim;
-  const EpiHdrs eh = epi_hdrs(a.epi);
-  for (int64_t z = blockIdx.z; z < int64_t(a.b.seqs) * a.pool.heads; z += gridDim.z) {
-    const Seq q = seq_at(a, z);
-    const int row_tiles = (q.rows + 15) / 16;
-    for (int64_t k0 = int64_t(blockIdx.x) * kKeyTile; k0 < q.kv;
-         k0 += int64_t(gridDim.x) * kKeyTile) {
-      const int64_t key = k0 + 16 * w + n;
-      const int64_t place = key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
-      const bool ok = place >= 0;
-      constexpr int kC = kHeld ? kHeld : 1;
-      v4i K[kC][3][kDigitPlanes];
-      auto load_chunk = [&](int c, v4i (&to)[3][kDigitPlanes]) {
-        uint64_t v[3][16];
-        const int64_t o = place + 64 * c;
-        load_keys<kVec>(a.pool.e + o, ok, g, dim - 64 * c, v[0]);
-        load_keys<kVec>(a.pool.b[0] + o, ok, g, dim - 64 * c, v[1]);
-        load_keys<kVec>(a.pool.b[1] + o, ok, g, dim - 64 * c, v[2]);
+  const Put<kTrunc> put(a);
+  const Seq q = seq_at(a, int(blockIdx.x));
+  for (int m0 = blockIdx.z * 16; m0 < q.rows; m0 += gridDim.z * 16) {
+    __syncthreads();
+    if (tid < 16) rows[tid] = row_at(a, q, m0 + tid);
+    __syncthreads();
+    for (int c = 0; c < chunks; ++c) {
+      Raw<4> v{};
+      load_raw<4, kVec, kFull>(a, rows[tid >> 4], c, tid & 15, v);
+      put_raw<4>(tiles + c * kTileBytes, tid >> 4, tid & 15, v);
+    }
+    __syncthreads();
+    int most = 0;
 #pragma unroll
-        for (int o3 = 0; o3 < 3; ++o3) digits_of16(v[o3], to[o3]);
-      };
-      if constexpr (kHeld > 0) {
+    for (int r = 0; r < 16; ++r) most = rows[r].len > most ? rows[r].len : most;
+    most = __builtin_amdgcn_readfirstlane(most);
+    const int all = (most + kKeyTile - 1) / kKeyTile;
+    const int per = (all + int(gridDim.y) - 1) / int(gridDim.y);
+    const int tb = int(blockIdx.y) * per, te = tb + per < all ? tb + per : all;
+    if (tb >= te) continue;
+    const auto place_of = [&](int t) -> int64_t {
+      const int key = t * kKeyTile + 16 * w + n;
+      return key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
+    };
+    int64_t here = place_of(tb), next = place_of(tb + 1);
+    uint64_t raw[3][16];
+    const auto issue = [&](int k, int64_t place, int c) {
+      const uint64_t* src = k == 0 ? a.pool.b[0] : k == 1 ? a.pool.b[1] : a.pool.e;
+      load_keys<kVec, kFull>(src + (place < 0 ? 0 : place) + 64 * c, g, dim - 64 * c, raw[k]);
+    };
 #pragma unroll
-        for (int c = 0; c < kC; ++c) load_chunk(c, K[c]);
-      }
-      for (int rb = blockIdx.y; rb < row_tiles; rb += gridDim.y * kRowGroup) {
-        // Spans of up to 16 row tiles, and which of them see these keys.
-        __syncthreads();
-        {
-          const int m = (rb + (tid >> 4) * int(gridDim.y)) * 16 + (tid & 15);
-          Span sp{0, 0};
-          if (m < q.rows && m >= 0) {
-            const int tl = m / a.group;
-            sp = span_of(a, q.hk * a.group + (m - tl * a.group), q.t0 + tl, q.kv);
-          }
-          first[tid] = sp.first;
-          len[tid] = sp.len;
-          if (tid == 0) active = 0;
-          const uint64_t seen = __ballot(sp.len > k0);
-          __syncthreads();
-          if (l == 0) {
-            unsigned bits = 0;
-            for (int i = 0; i < 4; ++i)
-              if ((seen >> (16 * i)) & 0xffff) bits |= 1u << (4 * w + i);
-            if (bits) atomicOr(&active, bits);
-          }
+    for (int k = 0; k < 3; ++k) issue(k, here, 0);
+    v4i acc[2][kDigitPlanes];
+    clear(acc);
+    int t = tb, c = 0;
+    for (int u = (te - tb) * chunks; u > 0; --u) {
+      const bool last = c + 1 == chunks;
+      const int64_t np = last ? next : here;
+      const int nc = last ? 0 : c + 1;
+      const int8_t* tile = tiles + c * kTileBytes;
+      v4i y[kDigitPlanes];
+      digits_of16(raw[0], y);
+      issue(0, np, nc);
+      mul_left(tile, 0, l, y, acc[0]);
+      digits_of16(raw[1], y);
+      issue(1, np, nc);
+      mul_left(tile, 0, l, y, acc[1]);
+      digits_of16(raw[2], y);
+      issue(2, np, nc);
+      mul_left(tile, 1, l, y, acc[0]);
+      mul_left(tile, 2, l, y, acc[1]);
+      c = nc;
+      if (last) {
+        const int key = t * kKeyTile + 16 * w + n;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const Row& row = rows[4 * g + r];
+          if (key >= row.len) continue;
+          const int64_t o = int64_t(row.first) + key;
+          const uint64_t z0 = here < 0 ? 0 : from_sums(acc[0], r);
+          const uint64_t z1 = here < 0 ? 0 : from_sums(acc[1], r);
+          put(a, o, z0 + a.c[0][o], z1 + a.c[1][o]);
         }
+        clear(acc);
+        ++t;
+        here = next;
+        next = place_of(t + 1);
+      }
+    }
+  }
+}
+
+// Many rows: a workgroup of 4 kGroups waves keeps the digits of its keys in
+// registers, kHeld 64-wide chunks of them, and runs over row tiles.  Each
+// thread loads its words of the next row tile, and writes their digits into
+// the other half of LDS while the matrix cores work on the present one (one
+// barrier a tile).
+template <int kHeld, int kGroups, bool kVec, bool kFull, bool kTrunc>
+__global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(ProductArgs a) {
+  constexpr int kRows = 256 * kGroups;  // rows looked up at once
+  constexpr int kKeys = 64 * kGroups;
+  constexpr int kHalf = kHeld * kTileBytes;
+  extern __shared__ __align__(16) int8_t tiles[];
+  __shared__ Row rows[kRows];
+  __shared__ unsigned active;
+  const int tid = threadIdx.x, l = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = l >> 4, n = l & 15;
+  const int dim = a.pool.dim;
+  const Put<kTrunc> put(a);
+  const Seq q = seq_at(a, int(blockIdx.x));
+  const int row_tiles = (q.rows + 15) / 16;
+  for (int k0 = int(blockIdx.y) * kKeys; k0 < q.kv; k0 += int(gridDim.y) * kKeys) {
+    const int key = k0 + 16 * w + n;
+    const int64_t place = key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
+    v4i K[kHeld][3][kDigitPlanes];
+    // The lane's offsets are formed again for each key tile: kept over the
+    // loop they would take registers that it does not have.
+    int lane_g = g;
+    asm volatile("" : "+v"(lane_g));
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c) {
+      const int64_t o = (place < 0 ? 0 : place) + 64 * c;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        uint64_t v[16];
+        load_keys<kVec, kFull>((k == 0 ? a.pool.e : a.pool.b[k - 1]) + o, lane_g, dim - 64 * c,
+                               v);
+        digits_of16(v, K[c][k]);
+      }
+    }
+    for (int rb = blockIdx.z; rb < row_tiles; rb += gridDim.z * (kRows / 16)) {
+      // Up to kRows / 16 row tiles, and which of them see these keys.
+      __syncthreads();
+      const Row mine = row_at(a, q, (rb + (tid >> 4) * int(gridDim.z)) * 16 + (tid & 15));
+      rows[tid] = mine;
+      if (tid == 0) active = 0;
+      const uint64_t seen = __ballot(mine.len > k0);
+      __syncthreads();
+      if (l == 0) {
+        unsigned bits = 0;
+        for (int i = 0; i < 4; ++i)
+          if ((seen >> (16 * i)) & 0xffff) bits |= 1u << (4 * w + i);
+        if (bits) atomicOr(&active, bits);
+      }
+      __syncthreads();
+      unsigned todo = __builtin_amdgcn_readfirstlane(active);
+      if (!todo) continue;
+      constexpr int kN = 4 / kGroups;
+      const int row = tid / (64 / kN), part = tid % (64 / kN);
+      Raw<kN> raw[kHeld] = {};
+      const auto fetch = [&](unsigned bits) {
+        if (!bits) return;
+        const Row r = rows[__builtin_ctz(bits) * 16 + row];
+#pragma unroll
+        for (int c = 0; c < kHeld; ++c) load_raw<kN, kVec, kFull>(a, r, c, part, raw[c]);
+      };
+      const auto write = [&](int it) {
+        int8_t* to = tiles + (it & 1) * kHalf;
+#pragma unroll
+        for (int c = 0; c < kHeld; ++c) put_raw<kN>(to + c * kTileBytes, row, part, raw[c]);
+      };
+      fetch(todo);
+      write(0);
+      fetch(todo & (todo - 1));
+      for (int it = 0; todo; ++it) {
+        const int ti = __builtin_ctz(todo);
+        todo &= todo - 1;
         __syncthreads();
-        for (unsigned todo = active; todo; todo &= todo - 1) {
-          const int ti = __builtin_ctz(todo);
-          const int m0 = (rb + ti * int(gridDim.y)) * 16;
-          // The tile's left operands: thread (row, part) takes 4 of k in each
-          // chunk.  Rows past the last stay as they are: a row of the left
-          // operand reaches that row of the product alone.
-          {
-            const int r = tid >> 4, m = m0 + r, lg = tid & 3, lq = (tid >> 2) & 3;
-            if (m < q.rows) {
-              const int tl = m / a.group, t = q.t0 + tl;
-              const int h = q.hk * a.group + (m - tl * a.group);
-              const int64_t xo = int64_t(t) * a.xts + int64_t(h) * a.xhs;
-              const int64_t ao = (int64_t(t) * a.heads + h) * dim;
-              for (int c = 0; c < chunks; ++c) {
-                const int d = 16 * lq + 2 * lg, left = dim - 64 * c;
-                uint64_t x0[4], x1[4], a0[4], a1[4];
-                load_left4<kVec>(a.x[0] + xo + 64 * c, d, left, x0);
-                load_left4<kVec>(a.x[1] + xo + 64 * c, d, left, x1);
-                load_left4<kVec>(a.a[0] + ao + 64 * c, d, left, a0);
-                load_left4<kVec>(a.a[1] + ao + 64 * c, d, left, a1);
-                put_left(tiles + c * kTileBytes, r, lg, lq, x0, x1, a0, a1);
-              }
-            }
-          }
-          // The product's shares of C for this lane's elements.
-          uint64_t cw[2][4];
-          int at[4];
+        if (todo) {
+          write(it + 1);
+          fetch(todo & (todo - 1));
+        }
+        const int8_t* tile = tiles + (it & 1) * kHalf;
+        v4i acc[2][kDigitPlanes];
+        clear(acc);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = 4 * g + r;
-            at[r] = key < len[ti * 16 + row] ? first[ti * 16 + row] + int(key) : -1;
-          }
-          const auto load_c = [&] {
+        for (int c = 0; c < kHeld; ++c)
+          mul_opened(tile + c * kTileBytes, l, K[c][1], K[c][2], acc);
+        // C's words load under the other half of the products.
+        __builtin_amdgcn_sched_barrier(0);
+        uint64_t cw[2][4];
+        int at[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              cw[0][r] = at[r] >= 0 ? a.c[0][at[r]] : 0;
-              cw[1][r] = at[r] >= 0 ? a.c[1][at[r]] : 0;
-            }
-          };
-          if constexpr (kHeld > 0) load_c();
-          __syncthreads();
-          v4i acc[2][kDigitPlanes];
-          clear(acc);
-          if constexpr (kHeld > 0) {
+        for (int r = 0; r < 4; ++r) {
+          const Row& row = rows[ti * 16 + 4 * g + r];
+          at[r] = key < row.len ? row.first + key : -1;
+          const int o = at[r] < 0 ? 0 : at[r];
+          cw[0][r] = a.c[0][o];
+          cw[1][r] = a.c[1][o];
+        }
 #pragma unroll
-            for (int c = 0; c < kC; ++c)
-              mul_tile(tiles + c * kTileBytes, l, K[c][0], K[c][1], K[c][2], acc);
-          } else {
-            for (int c = 0; c < chunks; ++c) {
-              load_chunk(c, K[0]);
-              mul_tile(tiles + c * kTileBytes, l, K[0][0], K[0][1], K[0][2], acc);
-            }
-            load_c();
-          }
+        for (int c = 0; c < kHeld; ++c) {
+          mul_left(tile + c * kTileBytes, 1, l, K[c][0], acc[0]);
+          mul_left(tile + c * kTileBytes, 2, l, K[c][0], acc[1]);
+        }
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (at[r] >= 0)
-              put2(a, eh, at[r], from_sums(acc[0], r) + cw[0][r], from_sums(acc[1], r) + cw[1][r]);
-          __syncthreads();
+        for (int r = 0; r < 4; ++r) {
+          if (at[r] < 0) continue;
+          const uint64_t z0 = place < 0 ? 0 : from_sums(acc[0], r);
+          const uint64_t z1 = place < 0 ? 0 : from_sums(acc[1], r);
+          put(a, at[r], z0 + cw[0][r], z1 + cw[1][r]);
+          if constexpr (kTrunc) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -380,39 +545,29 @@ struct ValuesArgs {
 // at most 2^14 at 64 of k are 2^24 a chunk.
 constexpr int kSumChunks = 64;
 
-template <int kWaves>
+template <int kWaves, bool kTrunc>
 __global__ void __launch_bounds__(64 * kWaves, 2) kv_values2_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;
   __shared__ __align__(16) int8_t tile[kTileBytes];
   __shared__ int64_t base[kKeyTile];
-  __shared__ int first[16];
-  __shared__ int len[16];
+  __shared__ Row rows[16];
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
   const int g = l >> 4, n = l & 15;
   const int dim = a.pool.dim;
-  const EpiHdrs eh = epi_hdrs(a.epi);
+  const Put<kTrunc> put(a);
   const int blocks = (dim + va.cols - 1) / va.cols;
-  const int split = int(blockIdx.x) % va.splits;
-  const int col = (int(blockIdx.x) / va.splits) * va.cols + 16 * w + n;
-  if (int(blockIdx.x) / va.splits >= blocks) return;
-  for (int64_t z = blockIdx.z; z < int64_t(a.b.seqs) * a.pool.heads; z += gridDim.z) {
-    const Seq q = seq_at(a, z);
-    for (int64_t m0 = int64_t(blockIdx.y) * 16; m0 < q.rows; m0 += int64_t(gridDim.y) * 16) {
+  const int split = int(blockIdx.y) % va.splits;
+  const int col = (int(blockIdx.y) / va.splits) * va.cols + 16 * w + n;
+  if (int(blockIdx.y) / va.splits >= blocks) return;
+  {
+    const Seq q = seq_at(a, int(blockIdx.x));
+    for (int m0 = int(blockIdx.z) * 16; m0 < q.rows; m0 += int(gridDim.z) * 16) {
       __syncthreads();
-      if (tid < 16) {
-        const int m = int(m0) + tid;
-        Span sp{0, 0};
-        if (m < q.rows) {
-          const int tl = m / a.group;
-          sp = span_of(a, q.hk * a.group + (m - tl * a.group), q.t0 + tl, q.kv);
-        }
-        first[tid] = sp.first;
-        len[tid] = sp.len;
-      }
+      if (tid < 16) rows[tid] = row_at(a, q, m0 + tid);
       __syncthreads();
       int most = 0;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) most = len[r] > most ? len[r] : most;
+      for (int r = 0; r < 16; ++r) most = rows[r].len > most ? rows[r].len : most;
       const int chunks = (most + kKeyTile - 1) / kKeyTile;
       const int per = (chunks + va.splits - 1) / va.splits;
       const int c0 = split * per, c1 = c0 + per < chunks ? c0 + per : chunks;
@@ -427,20 +582,21 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv_values2_kernel(ValuesArgs v
           base[tid] = key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
         }
         for (int u = tid; u < 256; u += 64 * kWaves) {
-          const int r = u >> 4, part = u & 15, ln = len[r];
-          if (m0 + r < q.rows) {
-            uint64_t x0[4], x1[4], a0[4], a1[4];
+          const int r = u >> 4, part = u & 15;
+          const Row row = rows[r];
+          if (row.t >= 0) {
+            Raw<4> v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int64_t key = k0 + 16 * i + part;
-              const bool in = key < ln;
-              const int64_t o = int64_t(first[r]) + key;
-              x0[i] = in ? a.x[0][o] : 0;
-              x1[i] = in ? a.x[1][o] : 0;
-              a0[i] = in ? a.a[0][o] : 0;
-              a1[i] = in ? a.a[1][o] : 0;
+              const bool in = key < row.len;
+              const int64_t o = int64_t(row.first) + key;
+              v.x0[i] = in ? a.x[0][o] : 0;
+              v.x1[i] = in ? a.x[1][o] : 0;
+              v.a0[i] = in ? a.a[0][o] : 0;
+              v.a1[i] = in ? a.a[1][o] : 0;
             }
-            put_left(tile, r, part & 3, part >> 2, x0, x1, a0, a1);
+            put_left<4>(tile, r, part & 3, 4 * (part >> 2), v);
           }
         }
         __syncthreads();
@@ -470,17 +626,16 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv_values2_kernel(ValuesArgs v
       if (col >= dim) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int m = int(m0) + 4 * g + r;
-        if (m >= q.rows) continue;
-        const int tl = m / a.group;
-        const int64_t row = int64_t(q.t0 + tl) * a.heads + q.hk * a.group + (m - tl * a.group);
+        const Row at = rows[4 * g + r];
+        if (at.t < 0) continue;
+        const int64_t row = int64_t(at.t) * a.heads + at.h;
         const int64_t o = row * dim + col;
         if (va.splits > 1) {
           const int64_t all = int64_t(a.b.tokens) * a.heads * dim;
           va.part[2 * split * all + o] = sum[0][r];
           va.part[(2 * split + 1) * all + o] = sum[1][r];
         } else {
-          put2(a, eh, o, sum[0][r] + a.c[0][o], sum[1][r] + a.c[1][o]);
+          put(a, o, sum[0][r] + a.c[0][o], sum[1][r] + a.c[1][o]);
         }
       }
     }
@@ -488,12 +643,13 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv_values2_kernel(ValuesArgs v
 }
 
 // Adds the splits' sums: 32 outputs a workgroup, 8 lanes over the splits.
+template <bool kTrunc>
 __global__ void __launch_bounds__(256) kv_values2_join_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;
   __shared__ uint64_t s[2][8][32];
   const int64_t all = int64_t(a.b.tokens) * a.heads * a.pool.dim;
   const int u = threadIdx.x & 31, lane = threadIdx.x >> 5;
-  const EpiHdrs eh = epi_hdrs(a.epi);
+  const Put<kTrunc> put(a);
   for (int64_t o0 = int64_t(blockIdx.x) * 32; o0 < all; o0 += int64_t(gridDim.x) * 32) {
     const int64_t o = o0 + u;
     uint64_t z0 = 0, z1 = 0;
@@ -513,7 +669,7 @@ __global__ void __launch_bounds__(256) kv_values2_join_kernel(ValuesArgs va) {
         z0 += s[0][k][u];
         z1 += s[1][k][u];
       }
-      put2(a, eh, o, z0, z1);
+      put(a, o, z0, z1);
     }
   }
 }
@@ -525,11 +681,13 @@ int product_args(const sufhip_kv_product2_args* args, bool values, const char* w
   ProductArgs a{};
   if (int rc = kv_batch_of(g.batch, what, &a.b)) return rc;
   if (int rc = kv_pool_of(g.pool, what, &a.pool)) return rc;
+  if (g.pool.pages < 1) return kv_fail(what, "the pool has no pages");
   if (g.heads < 1 || g.heads % g.pool.kv_heads)
     return kv_fail(what, "heads must be a multiple of the pool's kv_heads");
   if (g.n > 0x7fffffffu) return kv_fail(what, "at most 2^31 - 1 packed elements");
   const size_t rows = size_t(a.b.tokens) * size_t(g.heads);
-  if (rows > (1u << 30)) return kv_fail(what, "at most 2^30 rows");
+  if (rows > (1u << 30) || size_t(a.b.seqs) * size_t(a.pool.heads) > (1u << 30))
+    return kv_fail(what, "at most 2^30 rows, and sequences times cached heads");
   *empty = a.b.seqs == 0 || rows == 0 || (!values && g.n == 0);
   if (*empty) return SUFHIP_OK;
   const size_t n_out = values ? rows * size_t(g.pool.dim) : g.n;
@@ -546,6 +704,7 @@ int product_args(const sufhip_kv_product2_args* args, bool values, const char* w
     return kv_fail(what, "strides must be >= 0");
   a.heads = g.heads;
   a.group = g.heads / g.pool.kv_heads;
+  a.by_group = fast_div(uint32_t(a.group));
   a.xts = g.x.token_stride;
   a.xhs = g.x.head_stride;
   a.offsets = g.d_row_offsets;
@@ -582,15 +741,66 @@ int cu_total() {
   return cus;
 }
 
-template <int kHeld, bool kVec>
-int launch_scores(const ProductArgs& a, const dim3& grid, int chunks, hipStream_t st) {
+// Dynamic LDS past the 64 KB that a kernel may take unasked.
+template <typename F>
+int allow_lds(F* f, size_t lds) {
+  if (lds > 64 * 1024)
+    SUFHIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(f),
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)),
+                 "dynamic LDS");
+  return SUFHIP_OK;
+}
+
+template <bool kVec, bool kFull, bool kTrunc>
+int launch_scores_few(const ProductArgs& a, const dim3& grid, int chunks, hipStream_t st) {
   const size_t lds = size_t(chunks) * kTileBytes;
-  const void* f = reinterpret_cast<const void*>(kv_scores2_kernel<kHeld, kVec>);
-  if (lds > 48 * 1024)
-    SUFHIP_CHECK(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)),
-                 "kv_scores2_kernel LDS");
-  hipLaunchKernelGGL((kv_scores2_kernel<kHeld, kVec>), grid, dim3(256), lds, st, a, chunks);
+  if (int rc = allow_lds(kv_scores2_few_kernel<kVec, kFull, kTrunc>, lds)) return rc;
+  hipLaunchKernelGGL((kv_scores2_few_kernel<kVec, kFull, kTrunc>), grid, dim3(256), lds, st, a,
+                     chunks);
+  return check_launch("kv_scores2_few_kernel");
+}
+
+template <int kHeld, int kGroups, bool kVec, bool kFull, bool kTrunc>
+int launch_scores_many(const ProductArgs& a, const dim3& grid, hipStream_t st) {
+  const size_t lds = 2 * size_t(kHeld) * kTileBytes;
+  if (int rc = allow_lds(kv_scores2_kernel<kHeld, kGroups, kVec, kFull, kTrunc>, lds)) return rc;
+  hipLaunchKernelGGL((kv_scores2_kernel<kHeld, kGroups, kVec, kFull, kTrunc>), grid,
+                     dim3(256 * kGroups), lds, st, a);
   return check_launch("kv_scores2_kernel");
+}
+
+template <bool kVec, bool kFull, bool kTrunc>
+int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st) {
+  const int chunks = (a.pool.dim + 63) / 64;
+  const int64_t row_tiles = (int64_t(b.max_new) * a.group + 15) / 16;
+  const int64_t zs = int64_t(a.b.seqs) * a.pool.heads;
+  const int cus = cu_total();
+  if (row_tiles <= 1 || chunks > 2) {
+    // Shares of the keys: four workgroups a CU, of four key tiles at least
+    // where that still gives every CU one.
+    const int64_t tiles = (int64_t(b.max_keys) + kKeyTile - 1) / kKeyTile;
+    const int64_t groups = zs * (row_tiles < 1 ? 1 : row_tiles);
+    int64_t y = (4 * int64_t(cus) + groups - 1) / groups;
+    if (y > (tiles + 3) / 4 && groups * ((tiles + 3) / 4) >= cus) y = (tiles + 3) / 4;
+    if (y > tiles) y = tiles;
+    const dim3 grid(unsigned(zs), clip(y, 65535), clip(row_tiles, 65535));
+    return launch_scores_few<kVec, kFull, kTrunc>(a, grid, chunks, st);
+  }
+  constexpr int kGroups = kVec ? 2 : 1;  // of one chunk's kernel
+  const int groups = chunks == 1 ? kGroups : 1;
+  const int64_t key_tiles = (int64_t(b.max_keys) + 64 * groups - 1) / (64 * groups);
+  // Row tiles are spread over workgroups until four of them share a CU.
+  const int64_t want = (4 * int64_t(cus) + key_tiles * zs) / (key_tiles * zs + 1);
+  const dim3 grid(unsigned(zs), clip(key_tiles, 65535),
+                  clip(want < row_tiles ? want : row_tiles, 65535));
+  if (chunks == 1) return launch_scores_many<1, kGroups, kVec, kFull, kTrunc>(a, grid, st);
+  return launch_scores_many<2, 1, kVec, kFull, kTrunc>(a, grid, st);
+}
+
+template <bool kVec, bool kFull>
+int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st) {
+  return a.epi.on ? launch_scores<kVec, kFull, true>(a, b, st)
+                  : launch_scores<kVec, kFull, false>(a, b, st);
 }
 
 // Shares of the keys: as many as fill the chip twice, each of two chunks of
@@ -631,24 +841,10 @@ int sufhip_kv_scores2(const sufhip_kv_product2_args* args, void* stream) {
   const bool vec = (a.pool.dim & 1) == 0 && at16(a.pool.e) && at16(a.pool.b[0]) &&
                    at16(a.pool.b[1]) && at16(a.x[0]) && at16(a.x[1]) && at16(a.a[0]) &&
                    at16(a.a[1]) && (a.xts & 1) == 0 && (a.xhs & 1) == 0;
-  const int chunks = (a.pool.dim + 63) / 64;
-  const int64_t key_tiles = (int64_t(args->batch.max_keys) + kKeyTile - 1) / kKeyTile;
-  const int64_t row_tiles = (int64_t(args->batch.max_new) * a.group + 15) / 16;
-  const int64_t zs = int64_t(a.b.seqs) * a.pool.heads;
-  // Row tiles are spread over workgroups until four of them share a CU.
-  const int64_t want = (4 * 4 * int64_t(cu_total()) + key_tiles * zs) / (key_tiles * zs + 1);
-  const dim3 grid(clip(key_tiles, 1 << 20), clip(want < row_tiles ? want : row_tiles, 65535),
-                  clip(zs, 65535));
   const hipStream_t st = as_stream(stream);
-  const bool reuse = row_tiles > int64_t(grid.y);  // a workgroup runs over several row tiles
-  if (chunks == 1)
-    return vec ? launch_scores<1, true>(a, grid, chunks, st)
-               : launch_scores<1, false>(a, grid, chunks, st);
-  if (chunks == 2 && reuse)
-    return vec ? launch_scores<2, true>(a, grid, chunks, st)
-               : launch_scores<2, false>(a, grid, chunks, st);
-  return vec ? launch_scores<0, true>(a, grid, chunks, st)
-             : launch_scores<0, false>(a, grid, chunks, st);
+  if (!vec) return launch_scores<false, false>(a, args->batch, st);
+  return a.pool.dim % 64 ? launch_scores<true, false>(a, args->batch, st)
+                         : launch_scores<true, true>(a, args->batch, st);
 }
 
 size_t sufhip_kv_values2_work_bytes(const sufhip_kv_batch* batch, const sufhip_kv_pool* pool,
@@ -675,17 +871,25 @@ int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
                    "sufhip_kv_values2: d_work smaller than its work bytes, or not 16-byte aligned");
     va.part = static_cast<uint64_t*>(args->d_work);
   }
-  const dim3 grid(unsigned(v.splits * v.blocks), clip(v.row_tiles, 65535), clip(v.zs, 65535));
+  const dim3 grid(unsigned(v.zs), unsigned(v.splits * v.blocks), clip(v.row_tiles, 65535));
   const hipStream_t st = as_stream(stream);
-  if (v.waves == 4)
-    hipLaunchKernelGGL((kv_values2_kernel<4>), grid, dim3(256), 0, st, va);
+  const bool trunc = va.p.epi.on && v.splits == 1;
+  if (v.waves == 4 && trunc)
+    hipLaunchKernelGGL((kv_values2_kernel<4, true>), grid, dim3(256), 0, st, va);
+  else if (v.waves == 4)
+    hipLaunchKernelGGL((kv_values2_kernel<4, false>), grid, dim3(256), 0, st, va);
+  else if (trunc)
+    hipLaunchKernelGGL((kv_values2_kernel<8, true>), grid, dim3(512), 0, st, va);
   else
-    hipLaunchKernelGGL((kv_values2_kernel<8>), grid, dim3(512), 0, st, va);
+    hipLaunchKernelGGL((kv_values2_kernel<8, false>), grid, dim3(512), 0, st, va);
   if (int rc = check_launch("kv_values2_kernel")) return rc;
   if (v.splits == 1) return SUFHIP_OK;
   const int64_t all = int64_t(va.p.b.tokens) * va.p.heads * va.p.pool.dim;
-  hipLaunchKernelGGL(kv_values2_join_kernel, dim3(clip((all + 31) / 32, 1 << 20)), dim3(256), 0, st,
-                     va);
+  const dim3 join(clip((all + 31) / 32, 1 << 20));
+  if (va.p.epi.on)
+    hipLaunchKernelGGL(kv_values2_join_kernel<true>, join, dim3(256), 0, st, va);
+  else
+    hipLaunchKernelGGL(kv_values2_join_kernel<false>, join, dim3(256), 0, st, va);
   return check_launch("kv_values2_join_kernel");
 }
 
