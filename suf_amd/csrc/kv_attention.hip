@@ -533,116 +533,199 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
 // A workgroup takes 16 rows, 16 columns a wave, and a share of the keys in
 // chunks of 64 (the k of the product).  k order: byte j of group g stands for
 // key 16 (j % 4) + 4 (j / 4) + g of a chunk, so that the left operand's loads
-// (4 keys a thread) and the pages' (one column of 16 keys a lane) both run
-// over neighbouring words.
+// and the pages' (one column of 16 keys a lane) both run over neighbouring
+// words, and the 16 keys of one j % 4 are in one page when pages hold 16.
+//
+// The left operand (one row of packed elements a k) passes through LDS, the
+// next chunk's written while the present one multiplies; the pages' words go
+// to registers, an array's turned into digits and the next chunk's loaded in
+// their place, as for the scores.
 struct ValuesArgs {
   ProductArgs p;
   int splits, cols;   // shares of the keys; columns of a workgroup
   uint64_t* part;     // splits > 1: [splits][2][tokens * heads][dim] sums
+  uint64_t* out[2];   // one split: the values, before a truncation if one follows
 };
 
 // Chunks whose digit sums stay within int32: 2 products of 8 digit pairs of
 // at most 2^14 at 64 of k are 2^24 a chunk.
 constexpr int kSumChunks = 64;
 
-template <int kWaves, bool kTrunc>
-__global__ void __launch_bounds__(64 * kWaves, 2) kv_values2_kernel(ValuesArgs va) {
+// kWide: pages of at least 16 keys.
+template <int kWaves, bool kWide>
+__global__ void __launch_bounds__(64 * kWaves, kWide ? 2 : 1) kv_values2_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;
-  __shared__ __align__(16) int8_t tile[kTileBytes];
-  __shared__ int64_t base[kKeyTile];
+  constexpr int kN = 16 / kWaves;  // words of a row's chunk a thread forms
+  __shared__ __align__(16) int8_t tiles[2][kTileBytes];
+  __shared__ uint64_t sums[64 * kWaves][8];
   __shared__ Row rows[16];
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x, l = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = l >> 4, n = l & 15;
-  const int dim = a.pool.dim;
-  const Put<kTrunc> put(a);
-  const int blocks = (dim + va.cols - 1) / va.cols;
+  const int dim = a.pool.dim, shift = a.pool.shift;
   const int split = int(blockIdx.y) % va.splits;
   const int col = (int(blockIdx.y) / va.splits) * va.cols + 16 * w + n;
-  if (int(blockIdx.y) / va.splits >= blocks) return;
-  {
-    const Seq q = seq_at(a, int(blockIdx.x));
-    for (int m0 = int(blockIdx.z) * 16; m0 < q.rows; m0 += int(gridDim.z) * 16) {
-      __syncthreads();
-      if (tid < 16) rows[tid] = row_at(a, q, m0 + tid);
-      __syncthreads();
-      int most = 0;
+  const uint32_t lane = 8 * uint32_t((kWide ? g * dim : 0) + (col < dim ? col : 0));
+  const Seq q = seq_at(a, int(blockIdx.x));
+  // First word of the present cached head's page that holds key j, j uniform
+  // over the wave (kWide) or a lane's own; -1: none.
+  const int32_t* table = a.b.table + int64_t(q.s) * a.b.max_pages;
+  const auto page_of = [&](int j) -> int {
+    const int at = j >> shift;
+    return j < q.kv && at < a.b.max_pages ? table[at] : -1;
+  };
+  const auto place_of = [&](int page, int j) -> int64_t {
+    if (page < 0 || page >= a.pool.pages) return -1;
+    return (((int64_t(page) * a.pool.heads + q.hk) << shift) + (j & ((1 << shift) - 1))) * dim;
+  };
+  const int row = tid / (64 / kN), part = tid % (64 / kN);
+  for (int m0 = int(blockIdx.z) * 16; m0 < q.rows; m0 += int(gridDim.z) * 16) {
+    __syncthreads();
+    if (tid < 16) rows[tid] = row_at(a, q, m0 + tid);
+    __syncthreads();
+    int most = 0;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) most = rows[r].len > most ? rows[r].len : most;
-      const int chunks = (most + kKeyTile - 1) / kKeyTile;
-      const int per = (chunks + va.splits - 1) / va.splits;
-      const int c0 = split * per, c1 = c0 + per < chunks ? c0 + per : chunks;
-      uint64_t sum[2][4] = {};
-      v4i acc[2][kDigitPlanes];
-      clear(acc);
-      for (int c = c0; c < c1; ++c) {
-        const int64_t k0 = int64_t(c) * kKeyTile;
-        __syncthreads();
-        if (tid < kKeyTile) {
-          const int64_t key = k0 + tid;
-          base[tid] = key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
-        }
-        for (int u = tid; u < 256; u += 64 * kWaves) {
-          const int r = u >> 4, part = u & 15;
-          const Row row = rows[r];
-          if (row.t >= 0) {
-            Raw<4> v;
+    for (int r = 0; r < 16; ++r) most = rows[r].len > most ? rows[r].len : most;
+    most = __builtin_amdgcn_readfirstlane(most);
+    const int chunks = (most + kKeyTile - 1) / kKeyTile;
+    const int per = (chunks + va.splits - 1) / va.splits;
+    const int c0 = split * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+    v4i acc[2][kDigitPlanes];
+    clear(acc);
+    bool flushed = false;
+    if (c0 < c1) {
+      constexpr int kP = kWide ? 4 : 16;  // pages of a lane's keys of a chunk
+      uint64_t raw[3][16];
+      Raw<kN> left = {};
+      const Row mine = rows[row];
+      // A chunk's pages (kWide: of its four runs of 16 keys).
+      const auto pages = [&](int c, int (&pg)[kP]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int64_t key = k0 + 16 * i + part;
-              const bool in = key < row.len;
-              const int64_t o = int64_t(row.first) + key;
-              v.x0[i] = in ? a.x[0][o] : 0;
-              v.x1[i] = in ? a.x[1][o] : 0;
-              v.a0[i] = in ? a.a[0][o] : 0;
-              v.a1[i] = in ? a.a[1][o] : 0;
+        for (int i = 0; i < kP; ++i)
+          pg[i] = c >= c1 ? -1
+                  : kWide ? page_of(c * kKeyTile + 16 * i)
+                          : page_of(c * kKeyTile + 16 * (i & 3) + 4 * (i >> 2) + g);
+      };
+      const auto issue = [&](int k, int c, const int (&pg)[kP]) {
+        const uint64_t* src = k == 0 ? a.pool.b[0] : k == 1 ? a.pool.b[1] : a.pool.e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (kWide) {
+            const int64_t base = place_of(__builtin_amdgcn_readfirstlane(pg[i]),
+                                          c * kKeyTile + 16 * i);
+            const char* run = reinterpret_cast<const char*>(src + (base < 0 ? 0 : base));
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+              raw[k][4 * m + i] =
+                  *reinterpret_cast<const uint64_t*>(run + (lane + uint32_t(32 * m * dim)));
+          } else {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const int64_t base = place_of(pg[4 * m + i], c * kKeyTile + 16 * i + 4 * m + g);
+              raw[k][4 * m + i] = src[(base < 0 ? 0 : base) + lane / 8];
             }
-            put_left<4>(tile, r, part & 3, 4 * (part >> 2), v);
           }
         }
+      };
+      // The left operand's words; past the row's end and for keys without a
+      // page the row's first element, dropped in `write`.
+      bool in[kN];
+      const auto fetch = [&](int c, const int (&pg)[kP]) {
+#pragma unroll
+        for (int k = 0; k < kN; ++k) {
+          const int j = kN * (part >> 2) + k;
+          const int key = c * kKeyTile + 16 * (j & 3) + 4 * (j >> 2) + (part & 3);
+          int page;
+          if constexpr (kWide)
+            page = kN == 4 ? pg[k] : (part & 4) ? pg[2 + k] : pg[k];
+          else
+            page = c < c1 ? page_of(key) : -1;
+          in[k] = key < mine.len && page >= 0 && page < a.pool.pages;
+          const int64_t o = int64_t(mine.first) + (in[k] ? key : 0);
+          left.x0[k] = a.x[0][o];
+          left.x1[k] = a.x[1][o];
+          left.a0[k] = a.a[0][o];
+          left.a1[k] = a.a[1][o];
+        }
+      };
+      const auto write = [&](int c) {
+#pragma unroll
+        for (int k = 0; k < kN; ++k) {
+          if (in[k]) continue;
+          left.x0[k] = left.x1[k] = left.a0[k] = left.a1[k] = 0;
+        }
+        put_left<kN>(tiles[c & 1], row, part & 3, kN * (part >> 2), left);
+      };
+      int pg[kP], pn[kP];
+      pages(c0, pg);
+      fetch(c0, pg);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) issue(k, c0, pg);
+      pages(c0 + 1, pg);
+      write(c0);
+      for (int c = c0; c < c1; ++c) {
+        const int8_t* tile = tiles[c & 1];
         __syncthreads();
-        v4i K[3][kDigitPlanes];
-        {
-          uint64_t v[3][16];
+        pages(c + 2, pn);
+        // An array's loads leave when its digits have been used: into their
+        // registers, with the other two arrays' still under way.
+        v4i y[kDigitPlanes];
+        digits_of16(raw[0], y);
+        mul_left(tile, 0, l, y, acc[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        issue(0, c + 1, pg);
+        fetch(c + 1, pg);
+        digits_of16(raw[1], y);
+        mul_left(tile, 0, l, y, acc[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        issue(1, c + 1, pg);
+        digits_of16(raw[2], y);
+        mul_left(tile, 1, l, y, acc[0]);
+        mul_left(tile, 2, l, y, acc[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        write(c + 1);
+        issue(2, c + 1, pg);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int64_t o = base[16 * (j & 3) + 4 * (j >> 2) + g];
-            const bool in = o >= 0 && col < dim;
-            v[0][j] = in ? a.pool.e[o + col] : 0;
-            v[1][j] = in ? a.pool.b[0][o + col] : 0;
-            v[2][j] = in ? a.pool.b[1][o + col] : 0;
-          }
-#pragma unroll
-          for (int o3 = 0; o3 < 3; ++o3) digits_of16(v[o3], K[o3]);
-        }
-        mul_tile(tile, l, K[0], K[1], K[2], acc);
-        if (c - c0 + 1 == c1 - c0 || (c - c0) % kSumChunks == kSumChunks - 1) {
+        for (int i = 0; i < kP; ++i) pg[i] = pn[i];
+        if ((c - c0) % kSumChunks == kSumChunks - 1) {
 #pragma unroll
           for (int p = 0; p < 2; ++p)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum[p][r] += from_sums(acc[p], r);
+            for (int r = 0; r < 4; ++r) {
+              uint64_t v = from_sums(acc[p], r);
+              if (flushed) v += sums[tid][4 * p + r];
+              sums[tid][4 * p + r] = v;
+            }
+          flushed = true;
           clear(acc);
         }
       }
-      if (col >= dim) continue;
+    }
+    if (col >= dim) continue;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const Row at = rows[4 * g + r];
-        if (at.t < 0) continue;
-        const int64_t row = int64_t(at.t) * a.heads + at.h;
-        const int64_t o = row * dim + col;
-        if (va.splits > 1) {
-          const int64_t all = int64_t(a.b.tokens) * a.heads * dim;
-          va.part[2 * split * all + o] = sum[0][r];
-          va.part[(2 * split + 1) * all + o] = sum[1][r];
-        } else {
-          put(a, o, sum[0][r] + a.c[0][o], sum[1][r] + a.c[1][o]);
-        }
+    for (int r = 0; r < 4; ++r) {
+      const Row at = rows[4 * g + r];
+      if (at.t < 0) continue;
+      const int64_t o = (int64_t(at.t) * a.heads + at.h) * dim + col;
+      uint64_t z0 = from_sums(acc[0], r), z1 = from_sums(acc[1], r);
+      if (flushed) {
+        z0 += sums[tid][r];
+        z1 += sums[tid][4 + r];
+      }
+      if (va.splits > 1) {
+        const int64_t all = int64_t(a.b.tokens) * a.heads * dim;
+        va.part[2 * split * all + o] = z0;
+        va.part[(2 * split + 1) * all + o] = z1;
+      } else {
+        va.out[0][o] = z0 + a.c[0][o];
+        va.out[1][o] = z1 + a.c[1][o];
       }
     }
   }
 }
 
-// Adds the splits' sums: 32 outputs a workgroup, 8 lanes over the splits.
+// Adds the splits' sums and C, 32 outputs a workgroup, 8 lanes over the
+// splits; with one split (a truncation follows) the values are in va.out.
 template <bool kTrunc>
 __global__ void __launch_bounds__(256) kv_values2_join_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;
@@ -653,7 +736,7 @@ __global__ void __launch_bounds__(256) kv_values2_join_kernel(ValuesArgs va) {
   for (int64_t o0 = int64_t(blockIdx.x) * 32; o0 < all; o0 += int64_t(gridDim.x) * 32) {
     const int64_t o = o0 + u;
     uint64_t z0 = 0, z1 = 0;
-    if (o < all)
+    if (o < all && va.splits > 1)
       for (int k = lane; k < va.splits; k += 8) {
         z0 += va.part[2 * k * all + o];
         z1 += va.part[(2 * k + 1) * all + o];
@@ -663,8 +746,8 @@ __global__ void __launch_bounds__(256) kv_values2_join_kernel(ValuesArgs va) {
     s[1][lane][u] = z1;
     __syncthreads();
     if (lane == 0 && o < all && seq_of(a.b, int(o / (int64_t(a.heads) * a.pool.dim))) >= 0) {
-      z0 = a.c[0][o];
-      z1 = a.c[1][o];
+      z0 = va.splits > 1 ? a.c[0][o] : va.out[0][o];
+      z1 = va.splits > 1 ? a.c[1][o] : va.out[1][o];
       for (int k = 0; k < 8; ++k) {
         z0 += s[0][k][u];
         z1 += s[1][k][u];
@@ -815,10 +898,12 @@ int values_splits(int64_t groups, int64_t max_keys, int cus) {
 struct ValuesPlan {
   int cols, waves, blocks, splits;
   int64_t row_tiles, zs;
+  bool wide;
 };
 ValuesPlan plan_values(const sufhip_kv_batch& b, const sufhip_kv_pool& p, int heads) {
   ValuesPlan v{};
-  v.waves = p.dim <= 64 ? 4 : 8;
+  v.wide = p.page_tokens >= 16;
+  v.waves = p.dim <= 64 || !v.wide ? 4 : 8;
   v.cols = 16 * v.waves;
   v.blocks = (p.dim + v.cols - 1) / v.cols;
   const int64_t rows = int64_t(b.max_new) * (heads / p.kv_heads);
@@ -873,17 +958,15 @@ int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
   }
   const dim3 grid(unsigned(v.zs), unsigned(v.splits * v.blocks), clip(v.row_tiles, 65535));
   const hipStream_t st = as_stream(stream);
-  const bool trunc = va.p.epi.on && v.splits == 1;
-  if (v.waves == 4 && trunc)
-    hipLaunchKernelGGL((kv_values2_kernel<4, true>), grid, dim3(256), 0, st, va);
-  else if (v.waves == 4)
+  for (int p = 0; p < 2; ++p) va.out[p] = va.p.epi.on ? va.p.epi.y[p] : va.p.out[p];
+  if (!v.wide)
     hipLaunchKernelGGL((kv_values2_kernel<4, false>), grid, dim3(256), 0, st, va);
-  else if (trunc)
-    hipLaunchKernelGGL((kv_values2_kernel<8, true>), grid, dim3(512), 0, st, va);
+  else if (v.waves == 4)
+    hipLaunchKernelGGL((kv_values2_kernel<4, true>), grid, dim3(256), 0, st, va);
   else
-    hipLaunchKernelGGL((kv_values2_kernel<8, false>), grid, dim3(512), 0, st, va);
+    hipLaunchKernelGGL((kv_values2_kernel<8, true>), grid, dim3(512), 0, st, va);
   if (int rc = check_launch("kv_values2_kernel")) return rc;
-  if (v.splits == 1) return SUFHIP_OK;
+  if (v.splits == 1 && !va.p.epi.on) return SUFHIP_OK;
   const int64_t all = int64_t(va.p.b.tokens) * va.p.heads * va.p.pool.dim;
   const dim3 join(clip((all + 31) / 32, 1 << 20));
   if (va.p.epi.on)
