@@ -123,10 +123,15 @@ __device__ __forceinline__ uint64_t from_sums(const v4i (&acc)[kDigitPlanes], in
 // ---- left operands in LDS ----
 //
 // One 16 x 64 tile (16 rows, 64 of k) of the three left operands D, L_0, L_1
-// as digit planes: byte j of k group g of row r of plane i of operand o at
-// o * 8192 + i * 1024 + (r * 4 + g) * 16 + j, so a lane's operand is one
-// 16-byte read and a wave reads a plane's 1 KB in order.
+// as digit planes of 1 KB (plane i of operand o at o * 8192 + i * 1024), where
+// byte j of k group g of row r is byte j of the 16-byte cell below: a lane's
+// operand is one cell.  The rows are exchanged within a group so that neither
+// the 16-byte reads nor the writes of a wave (all groups of 2 rows) meet on
+// LDS banks.
 constexpr int kTileBytes = 3 * kDigitPlanes * 1024;
+__device__ __forceinline__ int cell(int r, int g) {
+  return (16 * g + (r ^ (2 * (g & 1) + 12 * (g >> 1)))) * 16;
+}
 
 // kN of a row's k from byte j0 of group g on (kN = 2 or 4, j0 a multiple).
 template <int kN>
@@ -165,7 +170,7 @@ __device__ __forceinline__ void put_left(int8_t* tile, int r, int g, int j0, con
     d[k] = (v.x0[k] - v.a0[k]) + (v.x1[k] - v.a1[k]);
     l0[k] = v.a0[k] + d[k];
   }
-  int8_t* p = tile + (r * 4 + g) * 16 + j0;
+  int8_t* p = tile + cell(r, g) + j0;
   put_digits<kN>(p, d);
   put_digits<kN>(p + 8192, l0);
   put_digits<kN>(p + 16384, v.a1);
@@ -173,7 +178,7 @@ __device__ __forceinline__ void put_left(int8_t* tile, int r, int g, int j0, con
 
 // Plane i of operand o for lane l (row l % 16, k group l / 16).
 __device__ __forceinline__ v4i get_left(const int8_t* tile, int o, int l, int i) {
-  return *reinterpret_cast<const v4i*>(tile + o * 8192 + i * 1024 + ((l & 15) * 4 + (l >> 4)) * 16);
+  return *reinterpret_cast<const v4i*>(tile + o * 8192 + i * 1024 + cell(l & 15, l >> 4));
 }
 
 // acc += (left operand o) r over the digit pairs of weight below 256^8.
@@ -227,10 +232,10 @@ __device__ __forceinline__ void clear(v4i (&acc)[2][kDigitPlanes]) {
 struct Seq {
   int s, hk, t0, rows, kv;
 };
-__device__ __forceinline__ Seq seq_at(const ProductArgs& a, int z) {
+__device__ __forceinline__ Seq seq_of_head(const ProductArgs& a, int s, int hk) {
   Seq q;
-  q.s = z / a.pool.heads;
-  q.hk = z - q.s * a.pool.heads;
+  q.s = s;
+  q.hk = hk;
   const int lo = a.b.cu[q.s], hi = a.b.cu[q.s + 1];
   q.t0 = lo > 0 ? lo : 0;
   const int t1 = hi < a.b.tokens ? hi : a.b.tokens;
@@ -239,17 +244,133 @@ __device__ __forceinline__ Seq seq_at(const ProductArgs& a, int z) {
   return q;
 }
 
+__device__ __forceinline__ Seq seq_at(const ProductArgs& a, int z) {
+  const int s = z / a.pool.heads;
+  return seq_of_head(a, s, z - s * a.pool.heads);
+}
+
 // Row m of a sequence: its token, head and packed elements (m past the last
-// row: token -1, no elements).
+// row: token -1, no elements; row_of: without the elements).
 struct Row {
   int t, h, first, len;
 };
-__device__ __forceinline__ Row row_at(const ProductArgs& a, const Seq& q, int m) {
+__device__ __forceinline__ Row row_of(const ProductArgs& a, const Seq& q, int m) {
   if (m >= q.rows) return {-1, 0, 0, 0};
   const int tl = int(div_by(a.by_group, uint32_t(m)));
-  const int t = q.t0 + tl, h = q.hk * a.group + (m - tl * a.group);
-  const Span sp = span_of(a, h, t, q.kv);
-  return {t, h, sp.first, sp.len};
+  return {q.t0 + tl, q.hk * a.group + (m - tl * a.group), 0, 0};
+}
+__device__ __forceinline__ Row row_at(const ProductArgs& a, const Seq& q, int m) {
+  Row r = row_of(a, q, m);
+  if (r.t < 0) return r;
+  const Span sp = span_of(a, r.h, r.t, q.kv);
+  r.first = sp.first;
+  r.len = sp.len;
+  return r;
+}
+
+// ---- even shares ----
+//
+// Few rows a sequence, and sequences of any lengths: the work is cut into
+// units of 64 keys of one item (row tile, column block, cached head of a
+// sequence), in that order within each sequence, and every workgroup takes
+// the same number of neighbouring units, across items and sequences.  The
+// lengths are in device memory, so each workgroup sums them up for itself
+// (one load of each length; 256 threads scan).  An item counts one unit more
+// than its keys, in front: what a workgroup spends on starting one.
+constexpr int kKeyTile = 64;
+
+struct Share {
+  int64_t unit, end, per;  // this workgroup's units; units of each workgroup
+};
+
+__device__ __forceinline__ int tiles_of(int kv) {
+  return kv > kKeyTile ? (kv + kKeyTile - 1) / kKeyTile : 1;
+}
+__device__ __forceinline__ int64_t units_of(const ProductArgs& a, int s, int blocks) {
+  const int lo = a.b.cu[s], hi = a.b.cu[s + 1];
+  const int t0 = lo > 0 ? lo : 0, t1 = hi < a.b.tokens ? hi : a.b.tokens;
+  const int64_t row_tiles = t1 > t0 ? ((t1 - t0) * a.group + 15) / 16 : 0;
+  return row_tiles * blocks * a.pool.heads * (tiles_of(a.b.lens[s]) + 1);
+}
+
+// Sums before each of the 256 threads' sequences into pre[0 .. 256] (a
+// workgroup of 256), and the workgroup's share.
+__device__ __forceinline__ Share share_of(const ProductArgs& a, int blocks, int64_t (&pre)[260]) {
+  const int tid = threadIdx.x, l = tid & 63;
+  if (a.b.seqs == 1) {  // nothing to scan
+    const int64_t all = units_of(a, 0, blocks);
+    const int64_t n = (all + gridDim.x - 1) / gridDim.x, u = int64_t(blockIdx.x) * n;
+    return {u, u + n < all ? u + n : all, n};
+  }
+  const int per = (a.b.seqs + 255) / 256;
+  int64_t mine = 0;
+  for (int s = tid * per; s < a.b.seqs && s < (tid + 1) * per; ++s) mine += units_of(a, s, blocks);
+  int64_t sum = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t v = __shfl_up(sum, d);
+    if (l >= d) sum += v;
+  }
+  if (l == 63) pre[256 + (tid >> 6)] = sum;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+  for (int w = 0; w < 4; ++w) {
+    if (w < (tid >> 6)) before += pre[256 + w];
+    all += pre[256 + w];
+  }
+  __syncthreads();
+  pre[tid] = before + sum - mine;
+  if (tid == 0) pre[256] = all;
+  __syncthreads();
+  const int64_t n = (all + gridDim.x - 1) / gridDim.x;
+  const int64_t u = int64_t(blockIdx.x) * n;
+  return {u, u + n < all ? u + n : all, n};
+}
+
+// The item of the share's next unit: key tiles [tile, tile + count) of its
+// `tiles` are the workgroup's (count 0: none), `first` and `last` the
+// workgroups of its first and last ones.  Steps the share past them.
+struct Piece {
+  Seq q;
+  int rt, block, tile, count, tiles, first, last;
+};
+__device__ __forceinline__ Piece piece_at(const ProductArgs& a, int blocks,
+                                          const int64_t (&pre)[260], Share& sh) {
+  int s = 0;
+  int64_t rem = sh.unit;
+  if (a.b.seqs > 1) {
+    int b = 0;
+#pragma unroll
+    for (int step = 128; step; step >>= 1)
+      if (pre[b + step] <= sh.unit) b += step;
+    const int per = (a.b.seqs + 255) / 256;
+    s = b * per;
+    rem = sh.unit - pre[b];
+    if (per > 1)
+      for (int64_t n; s + 1 < a.b.seqs && (n = units_of(a, s, blocks)) <= rem; ++s) rem -= n;
+  }
+  Piece p;
+  p.q = seq_of_head(a, s, 0);
+  p.tiles = tiles_of(p.q.kv);
+  const int64_t item = rem / (p.tiles + 1);
+  const int at = int(rem - item * (p.tiles + 1));  // 0: the unit in front
+  // Divided afresh for each piece: the divisors' reciprocals would be kept in
+  // registers over the caller's loop.
+  int heads = a.pool.heads;
+  asm volatile("" : "+s"(heads));
+  asm volatile("" : "+s"(blocks));
+  const int64_t row = item / heads;
+  p.q.hk = int(item - row * heads);
+  p.rt = int(row / blocks);
+  p.block = int(row - int64_t(p.rt) * blocks);
+  const int64_t begin = sh.unit - at + 1;
+  p.first = int(begin / sh.per);
+  p.last = int((begin + p.tiles - 1) / sh.per);
+  const int left = int(min(sh.end - sh.unit, int64_t(p.tiles + 1 - at)));
+  sh.unit += left;
+  p.tile = at > 0 ? at - 1 : 0;
+  p.count = at > 0 ? left : left - 1;
+  return p;
 }
 
 // ---- scores ----
@@ -324,41 +445,41 @@ __device__ __forceinline__ void put_raw(int8_t* tile, int row, int part, const R
   put_left<kN>(tile, row, part & 3, kN * (part >> 2), v);
 }
 
-// Few rows: a workgroup keeps one row tile in LDS and streams its share of
-// the keys, 64 at a time.  Bound by HBM: an array's 16 words a lane are
-// turned into digits, the next tile's loads leave into the same registers,
-// and the matrix cores run under them, so a wave has up to 24 KB in flight.
-constexpr int kKeyTile = 64;
+// The longest row of a tile.
+__device__ __forceinline__ int longest(const Row (&rows)[16]) {
+  int most = 0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) most = rows[r].len > most ? rows[r].len : most;
+  return __builtin_amdgcn_readfirstlane(most);
+}
+
+// Few rows: a workgroup keeps one row tile in LDS and streams its units of
+// the keys.  Bound by HBM: an array's 16 words a lane are turned into digits,
+// the next unit's loads leave into the same registers, and the matrix cores
+// run under them, so a wave has up to 24 KB in flight.
 
 template <bool kVec, bool kFull, bool kTrunc>
 __global__ void __launch_bounds__(256, kVec && !kTrunc ? 2 : 1)
     kv_scores2_few_kernel(ProductArgs a, int chunks) {
   extern __shared__ __align__(16) int8_t tiles[];
   __shared__ Row rows[16];
-  const int tid = threadIdx.x, l = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = l >> 4, n = l & 15;
+  const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   const int dim = a.pool.dim;
   const Put<kTrunc> put(a);
-  const Seq q = seq_at(a, int(blockIdx.x));
-  for (int m0 = blockIdx.z * 16; m0 < q.rows; m0 += gridDim.z * 16) {
-    __syncthreads();
-    if (tid < 16) rows[tid] = row_at(a, q, m0 + tid);
-    __syncthreads();
-    for (int c = 0; c < chunks; ++c) {
-      Raw<4> v{};
-      load_raw<4, kVec, kFull>(a, rows[tid >> 4], c, tid & 15, v);
-      put_raw<4>(tiles + c * kTileBytes, tid >> 4, tid & 15, v);
-    }
-    __syncthreads();
-    int most = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) most = rows[r].len > most ? rows[r].len : most;
-    most = __builtin_amdgcn_readfirstlane(most);
-    const int all = (most + kKeyTile - 1) / kKeyTile;
-    const int per = (all + int(gridDim.y) - 1) / int(gridDim.y);
-    const int tb = int(blockIdx.y) * per, te = tb + per < all ? tb + per : all;
-    if (tb >= te) continue;
+  __shared__ int64_t pre[260];
+  Share sh = share_of(a, 1, pre);
+  while (sh.unit < sh.end) {
+    const Piece pc = piece_at(a, 1, pre, sh);
+    const Seq& q = pc.q;
+    if (pc.count == 0) continue;
+    // The lane's offsets are formed again for each piece: kept over the loop
+    // they would take registers that it does not have.
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int l = tid & 63, g = l >> 4, n = l & 15;
+    // The first keys' pages and words, the rows' words and the rows' places
+    // are on their way together.
+    const int tb = pc.tile;
     const auto place_of = [&](int t) -> int64_t {
       const int key = t * kKeyTile + 16 * w + n;
       return key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
@@ -369,8 +490,22 @@ __global__ void __launch_bounds__(256, kVec && !kTrunc ? 2 : 1)
       const uint64_t* src = k == 0 ? a.pool.b[0] : k == 1 ? a.pool.b[1] : a.pool.e;
       load_keys<kVec, kFull>(src + (place < 0 ? 0 : place) + 64 * c, g, dim - 64 * c, raw[k]);
     };
+    const Row stage = row_of(a, q, 16 * pc.rt + (tid >> 4));
+    __syncthreads();
+    if (tid < 16) rows[tid] = row_at(a, q, 16 * pc.rt + tid);
+    for (int c = 0; c < chunks; ++c) {
+      Raw<4> v{};
+      load_raw<4, kVec, kFull>(a, stage, c, tid & 15, v);
+      if (c == 0) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) issue(k, here, 0);
+        for (int k = 0; k < 3; ++k) issue(k, here, 0);
+      }
+      put_raw<4>(tiles + c * kTileBytes, tid >> 4, tid & 15, v);
+    }
+    __syncthreads();
+    const int all = (longest(rows) + kKeyTile - 1) / kKeyTile;
+    const int te = tb + pc.count < all ? tb + pc.count : all;
+    if (tb >= te) continue;
     v4i acc[2][kDigitPlanes];
     clear(acc);
     int t = tb, c = 0;
@@ -379,6 +514,19 @@ __global__ void __launch_bounds__(256, kVec && !kTrunc ? 2 : 1)
       const int64_t np = last ? next : here;
       const int nc = last ? 0 : c + 1;
       const int8_t* tile = tiles + c * kTileBytes;
+      const int key = t * kKeyTile + 16 * w + n;
+      uint64_t cw[2][4];
+      int at[4];
+      if (last) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const Row& row = rows[4 * g + r];
+          at[r] = key < row.len ? row.first + key : -1;
+          const int o = at[r] < 0 ? 0 : at[r];
+          cw[0][r] = a.c[0][o];
+          cw[1][r] = a.c[1][o];
+        }
+      }
       v4i y[kDigitPlanes];
       digits_of16(raw[0], y);
       issue(0, np, nc);
@@ -392,15 +540,12 @@ __global__ void __launch_bounds__(256, kVec && !kTrunc ? 2 : 1)
       mul_left(tile, 2, l, y, acc[1]);
       c = nc;
       if (last) {
-        const int key = t * kKeyTile + 16 * w + n;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const Row& row = rows[4 * g + r];
-          if (key >= row.len) continue;
-          const int64_t o = int64_t(row.first) + key;
+          if (at[r] < 0) continue;
           const uint64_t z0 = here < 0 ? 0 : from_sums(acc[0], r);
           const uint64_t z1 = here < 0 ? 0 : from_sums(acc[1], r);
-          put(a, o, z0 + a.c[0][o], z1 + a.c[1][o]);
+          put(a, at[r], z0 + cw[0][r], z1 + cw[1][r]);
         }
         clear(acc);
         ++t;
@@ -431,7 +576,7 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
   const Put<kTrunc> put(a);
   const Seq q = seq_at(a, int(blockIdx.x));
   const int row_tiles = (q.rows + 15) / 16;
-  for (int k0 = int(blockIdx.y) * kKeys; k0 < q.kv; k0 += int(gridDim.y) * kKeys) {
+  for (int k0 = int(blockIdx.z) * kKeys; k0 < q.kv; k0 += int(gridDim.z) * kKeys) {
     const int key = k0 + 16 * w + n;
     const int64_t place = key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
     v4i K[kHeld][3][kDigitPlanes];
@@ -450,10 +595,10 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
         digits_of16(v, K[c][k]);
       }
     }
-    for (int rb = blockIdx.z; rb < row_tiles; rb += gridDim.z * (kRows / 16)) {
+    for (int rb = blockIdx.y; rb < row_tiles; rb += gridDim.y * (kRows / 16)) {
       // Up to kRows / 16 row tiles, and which of them see these keys.
       __syncthreads();
-      const Row mine = row_at(a, q, (rb + (tid >> 4) * int(gridDim.z)) * 16 + (tid & 15));
+      const Row mine = row_at(a, q, (rb + (tid >> 4) * int(gridDim.y)) * 16 + (tid & 15));
       rows[tid] = mine;
       if (tid == 0) active = 0;
       const uint64_t seen = __ballot(mine.len > k0);
@@ -498,7 +643,9 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
 #pragma unroll
         for (int c = 0; c < kHeld; ++c)
           mul_opened(tile + c * kTileBytes, l, K[c][1], K[c][2], acc);
-        // C's words load under the other half of the products.
+        // C's words load under the other half of the products (before the
+        // first half, or a tile ahead, they hold the wave up at the stores
+        // of the tile before: 143 and 149 us against 129 for three prompts).
         __builtin_amdgcn_sched_barrier(0);
         uint64_t cw[2][4];
         int at[4];
@@ -542,218 +689,302 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
 // their place, as for the scores.
 struct ValuesArgs {
   ProductArgs p;
-  int splits, cols;   // shares of the keys; columns of a workgroup
-  uint64_t* part;     // splits > 1: [splits][2][tokens * heads][dim] sums
-  uint64_t* out[2];   // one split: the values, before a truncation if one follows
+  int blocks;        // column blocks
+  uint64_t* part;    // few rows: two slots of sums a workgroup
+  int4* info;        // few rows: [tokens * heads][blocks]
+  uint64_t* out[2];  // the values, before a truncation if one follows
 };
+constexpr int kSlotWords = 2 * 16 * 64;  // both parties' sums of a 16 x 64 tile
 
 // Chunks whose digit sums stay within int32: 2 products of 8 digit pairs of
 // at most 2^14 at 64 of k are 2^24 a chunk.
 constexpr int kSumChunks = 64;
 
-// kWide: pages of at least 16 keys.
+// One row tile's product with the columns of a workgroup over chunks
+// [c0, c1): digit sums of the lane's column and 4 rows into acc, those of
+// earlier chunks, if there were too many for int32, into the lane's words of
+// `sums` (true).  The pages' first words are on their way while the caller's
+// `rows` arrive (a barrier).  kWide: pages of at least 16 keys.
+template <int kWaves, bool kWide>
+__device__ __forceinline__ bool values_run(const ProductArgs& a, const Seq& q, const Row (&rows)[16],
+                                           int8_t (*tiles)[kTileBytes], uint64_t* sums, int c0,
+                                           int c1, int col, v4i (&acc)[2][kDigitPlanes]) {
+  constexpr int kN = 16 / kWaves;      // words of a row's chunk a thread forms, in pairs
+  constexpr int kP = kWide ? 4 : 16;   // page lookups of a chunk: its runs of 16 keys,
+                                       // or a lane's own keys
+  // The lane's offsets are formed again in each call: kept over the caller's
+  // loop they would take registers that the chunk loop does not have.
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int l = tid & 63, g = l >> 4;
+  const int dim = a.pool.dim, shift = a.pool.shift;
+  const int row = tid / (64 / kN), part = tid % (64 / kN);
+  bool flushed = false;
+  clear(acc);
+  const uint32_t lane = 8 * uint32_t((kWide ? g * dim : 0) + (col < dim ? col : 0));
+  const int32_t* table = a.b.table + int64_t(q.s) * a.b.max_pages;
+  const auto page_of = [&](int c, int j) -> int {
+    const int at = j >> shift;
+    const bool in = c < c1 && j < q.kv && at < a.b.max_pages;
+    const int page = table[in ? at : 0];
+    return in ? page : -1;
+  };
+  const auto key_of = [&](int c, int i) {  // of lookup i
+    return c * kKeyTile + (kWide ? 16 * i : 16 * (i & 3) + 4 * (i >> 2) + g);
+  };
+  const auto lookup = [&](int c, int (&pg)[kP]) {
+#pragma unroll
+    for (int i = 0; i < kP; ++i) pg[i] = page_of(c, key_of(c, i));
+  };
+  // First word of each lookup's keys (the pool's first where there is no
+  // page) and, kWide, which of the four runs have a page.
+  int64_t base[kP];
+  unsigned held = 0;
+  const auto place = [&](int c, const int (&pg)[kP]) {
+    held = 0;
+#pragma unroll
+    for (int i = 0; i < kP; ++i) {
+      const int at = kWide ? __builtin_amdgcn_readfirstlane(pg[i]) : pg[i];
+      const bool ok = unsigned(at) < unsigned(a.pool.pages);
+      const int64_t head = int64_t(ok ? at : 0) * a.pool.heads + (ok ? q.hk : 0);
+      const int in = ok ? key_of(c, i) & ((1 << shift) - 1) : 0;
+      base[i] = ((head << shift) + in) * dim;
+      held |= ok ? 1u << i : 0u;
+    }
+  };
+  uint64_t raw[3][16];
+  const auto issue = [&](int k) {
+    const uint64_t* src = k == 0 ? a.pool.b[0] : k == 1 ? a.pool.b[1] : a.pool.e;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const char* at = reinterpret_cast<const char*>(src + base[kWide ? i & 3 : i]);
+      raw[k][i] = *reinterpret_cast<const uint64_t*>(
+          at + (lane + (kWide ? uint32_t(32 * (i >> 2) * dim) : 0u)));
+    }
+  };
+  // The left operand's words of pair h: keys of bytes j and j + 1, j = kN m +
+  // 2 h.  Past the row's end and for keys without a page the row's first
+  // element, which `write` drops.
+  Row mine;
+  const auto key0 = [&](int c, int h) {
+    const int j = kN * (part >> 2) + 2 * h;
+    return c * kKeyTile + 16 * (j & 3) + 4 * (j >> 2) + (part & 3);
+  };
+  const auto inside = [&](int c, int h, int k) {
+    const int key = key0(c, h) + 16 * k;
+    if constexpr (kWide) {
+      const int run = (kN == 4 ? 2 * h : (part >> 1) & 2) + k;
+      return key < mine.len && ((held >> run) & 1);
+    } else {
+      return key < mine.len && unsigned(page_of(c, key)) < unsigned(a.pool.pages);
+    }
+  };
+  Raw<2> left[kN / 2];
+  const auto fetch = [&](int c, int h) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int key = key0(c, h) + 16 * k;
+      const int64_t o = int64_t(mine.first) + (key < mine.len ? key : 0);
+      left[h].x0[k] = a.x[0][o];
+      left[h].x1[k] = a.x[1][o];
+      left[h].a0[k] = a.a[0][o];
+      left[h].a1[k] = a.a[1][o];
+    }
+  };
+  const auto write = [&](int c, int h) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (inside(c, h, k)) continue;
+      left[h].x0[k] = left[h].x1[k] = left[h].a0[k] = left[h].a1[k] = 0;
+    }
+    put_left<2>(tiles[c & 1], row, part & 3, kN * (part >> 2) + 2 * h, left[h]);
+  };
+  int pg[kP];
+  lookup(c0, pg);
+  place(c0, pg);
+  lookup(c0 + 1, pg);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) issue(k);
+  __syncthreads();
+  const int chunks = (longest(rows) + kKeyTile - 1) / kKeyTile;
+  c1 = c1 < chunks ? c1 : chunks;
+  if (c0 >= c1) return flushed;
+  mine = rows[row];
+#pragma unroll
+  for (int h = 0; h < kN / 2; ++h) fetch(c0, h);
+#pragma unroll
+  for (int h = 0; h < kN / 2; ++h) write(c0, h);
+  for (int c = c0; c < c1; ++c) {
+    const int8_t* tile = tiles[c & 1];
+    __syncthreads();
+    place(c + 1, pg);
+    lookup(c + 2, pg);
+    if constexpr (kN == 4) fetch(c + 1, 1);
+    // An array's loads leave when its digits have been used: into their
+    // registers, with the other two arrays' still under way.
+    v4i y[kDigitPlanes];
+    digits_of16(raw[0], y);
+    mul_left(tile, 0, l, y, acc[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(0);
+    fetch(c + 1, 0);
+    digits_of16(raw[1], y);
+    mul_left(tile, 0, l, y, acc[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kN == 4) write(c + 1, 1);
+    issue(1);
+    digits_of16(raw[2], y);
+    mul_left(tile, 1, l, y, acc[0]);
+    mul_left(tile, 2, l, y, acc[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    write(c + 1, 0);
+    issue(2);
+    if ((c - c0) % kSumChunks == kSumChunks - 1) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          uint64_t v = from_sums(acc[p], r);
+          if (flushed) v += sums[4 * p + r];
+          sums[4 * p + r] = v;
+        }
+      flushed = true;
+      clear(acc);
+    }
+  }
+  return flushed;
+}
+
+// Many rows: a workgroup a row tile, cached head and column block.
 template <int kWaves, bool kWide>
 __global__ void __launch_bounds__(64 * kWaves, kWide ? 2 : 1) kv_values2_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;
-  constexpr int kN = 16 / kWaves;  // words of a row's chunk a thread forms
   __shared__ __align__(16) int8_t tiles[2][kTileBytes];
   __shared__ uint64_t sums[64 * kWaves][8];
   __shared__ Row rows[16];
   const int tid = threadIdx.x, l = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = l >> 4, n = l & 15;
-  const int dim = a.pool.dim, shift = a.pool.shift;
-  const int split = int(blockIdx.y) % va.splits;
-  const int col = (int(blockIdx.y) / va.splits) * va.cols + 16 * w + n;
-  const uint32_t lane = 8 * uint32_t((kWide ? g * dim : 0) + (col < dim ? col : 0));
+  const int dim = a.pool.dim;
+  const int col = int(blockIdx.y) * 16 * kWaves + 16 * w + n;
   const Seq q = seq_at(a, int(blockIdx.x));
-  // First word of the present cached head's page that holds key j, j uniform
-  // over the wave (kWide) or a lane's own; -1: none.
-  const int32_t* table = a.b.table + int64_t(q.s) * a.b.max_pages;
-  const auto page_of = [&](int j) -> int {
-    const int at = j >> shift;
-    return j < q.kv && at < a.b.max_pages ? table[at] : -1;
-  };
-  const auto place_of = [&](int page, int j) -> int64_t {
-    if (page < 0 || page >= a.pool.pages) return -1;
-    return (((int64_t(page) * a.pool.heads + q.hk) << shift) + (j & ((1 << shift) - 1))) * dim;
-  };
-  const int row = tid / (64 / kN), part = tid % (64 / kN);
-  for (int m0 = int(blockIdx.z) * 16; m0 < q.rows; m0 += int(gridDim.z) * 16) {
+  // The last row tiles first: with causal rows they are the longest.
+  for (int m = (q.rows + 15) / 16 - 1 - int(blockIdx.z); m >= 0; m -= int(gridDim.z)) {
     __syncthreads();
-    if (tid < 16) rows[tid] = row_at(a, q, m0 + tid);
-    __syncthreads();
-    int most = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) most = rows[r].len > most ? rows[r].len : most;
-    most = __builtin_amdgcn_readfirstlane(most);
-    const int chunks = (most + kKeyTile - 1) / kKeyTile;
-    const int per = (chunks + va.splits - 1) / va.splits;
-    const int c0 = split * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+    if (tid < 16) rows[tid] = row_at(a, q, 16 * m + tid);
     v4i acc[2][kDigitPlanes];
-    clear(acc);
-    bool flushed = false;
-    if (c0 < c1) {
-      constexpr int kP = kWide ? 4 : 16;  // pages of a lane's keys of a chunk
-      uint64_t raw[3][16];
-      Raw<kN> left = {};
-      const Row mine = rows[row];
-      // A chunk's pages (kWide: of its four runs of 16 keys).
-      const auto pages = [&](int c, int (&pg)[kP]) {
-#pragma unroll
-        for (int i = 0; i < kP; ++i)
-          pg[i] = c >= c1 ? -1
-                  : kWide ? page_of(c * kKeyTile + 16 * i)
-                          : page_of(c * kKeyTile + 16 * (i & 3) + 4 * (i >> 2) + g);
-      };
-      const auto issue = [&](int k, int c, const int (&pg)[kP]) {
-        const uint64_t* src = k == 0 ? a.pool.b[0] : k == 1 ? a.pool.b[1] : a.pool.e;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (kWide) {
-            const int64_t base = place_of(__builtin_amdgcn_readfirstlane(pg[i]),
-                                          c * kKeyTile + 16 * i);
-            const char* run = reinterpret_cast<const char*>(src + (base < 0 ? 0 : base));
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-              raw[k][4 * m + i] =
-                  *reinterpret_cast<const uint64_t*>(run + (lane + uint32_t(32 * m * dim)));
-          } else {
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const int64_t base = place_of(pg[4 * m + i], c * kKeyTile + 16 * i + 4 * m + g);
-              raw[k][4 * m + i] = src[(base < 0 ? 0 : base) + lane / 8];
-            }
-          }
-        }
-      };
-      // The left operand's words; past the row's end and for keys without a
-      // page the row's first element, dropped in `write`.
-      bool in[kN];
-      const auto fetch = [&](int c, const int (&pg)[kP]) {
-#pragma unroll
-        for (int k = 0; k < kN; ++k) {
-          const int j = kN * (part >> 2) + k;
-          const int key = c * kKeyTile + 16 * (j & 3) + 4 * (j >> 2) + (part & 3);
-          int page;
-          if constexpr (kWide)
-            page = kN == 4 ? pg[k] : (part & 4) ? pg[2 + k] : pg[k];
-          else
-            page = c < c1 ? page_of(key) : -1;
-          in[k] = key < mine.len && page >= 0 && page < a.pool.pages;
-          const int64_t o = int64_t(mine.first) + (in[k] ? key : 0);
-          left.x0[k] = a.x[0][o];
-          left.x1[k] = a.x[1][o];
-          left.a0[k] = a.a[0][o];
-          left.a1[k] = a.a[1][o];
-        }
-      };
-      const auto write = [&](int c) {
-#pragma unroll
-        for (int k = 0; k < kN; ++k) {
-          if (in[k]) continue;
-          left.x0[k] = left.x1[k] = left.a0[k] = left.a1[k] = 0;
-        }
-        put_left<kN>(tiles[c & 1], row, part & 3, kN * (part >> 2), left);
-      };
-      int pg[kP], pn[kP];
-      pages(c0, pg);
-      fetch(c0, pg);
-#pragma unroll
-      for (int k = 0; k < 3; ++k) issue(k, c0, pg);
-      pages(c0 + 1, pg);
-      write(c0);
-      for (int c = c0; c < c1; ++c) {
-        const int8_t* tile = tiles[c & 1];
-        __syncthreads();
-        pages(c + 2, pn);
-        // An array's loads leave when its digits have been used: into their
-        // registers, with the other two arrays' still under way.
-        v4i y[kDigitPlanes];
-        digits_of16(raw[0], y);
-        mul_left(tile, 0, l, y, acc[0]);
-        __builtin_amdgcn_sched_barrier(0);
-        issue(0, c + 1, pg);
-        fetch(c + 1, pg);
-        digits_of16(raw[1], y);
-        mul_left(tile, 0, l, y, acc[1]);
-        __builtin_amdgcn_sched_barrier(0);
-        issue(1, c + 1, pg);
-        digits_of16(raw[2], y);
-        mul_left(tile, 1, l, y, acc[0]);
-        mul_left(tile, 2, l, y, acc[1]);
-        __builtin_amdgcn_sched_barrier(0);
-        write(c + 1);
-        issue(2, c + 1, pg);
-#pragma unroll
-        for (int i = 0; i < kP; ++i) pg[i] = pn[i];
-        if ((c - c0) % kSumChunks == kSumChunks - 1) {
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              uint64_t v = from_sums(acc[p], r);
-              if (flushed) v += sums[tid][4 * p + r];
-              sums[tid][4 * p + r] = v;
-            }
-          flushed = true;
-          clear(acc);
-        }
-      }
-    }
+    const bool flushed = values_run<kWaves, kWide>(a, q, rows, tiles, sums[tid], 0,
+                                                   tiles_of(q.kv), col, acc);
     if (col >= dim) continue;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const Row at = rows[4 * g + r];
       if (at.t < 0) continue;
       const int64_t o = (int64_t(at.t) * a.heads + at.h) * dim + col;
-      uint64_t z0 = from_sums(acc[0], r), z1 = from_sums(acc[1], r);
-      if (flushed) {
-        z0 += sums[tid][r];
-        z1 += sums[tid][4 + r];
-      }
-      if (va.splits > 1) {
-        const int64_t all = int64_t(a.b.tokens) * a.heads * dim;
-        va.part[2 * split * all + o] = z0;
-        va.part[(2 * split + 1) * all + o] = z1;
-      } else {
-        va.out[0][o] = z0 + a.c[0][o];
-        va.out[1][o] = z1 + a.c[1][o];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint64_t v = from_sums(acc[p], r) + a.c[p][o];
+        if (flushed) v += sums[tid][4 * p + r];
+        va.out[p][o] = v;
       }
     }
   }
 }
 
-// Adds the splits' sums and C, 32 outputs a workgroup, 8 lanes over the
-// splits; with one split (a truncation follows) the values are in va.out.
-template <bool kTrunc>
+// Few rows: even shares of the keys' units.  An item that lies within one
+// workgroup's share is finished there; the sums of one that does not go to
+// the workspace, where slot 2 w holds what workgroup w has of an item that
+// began before its share, slot 2 w + 1 of one that goes on after it.  For
+// each row and column block `info` keeps the first and last workgroup of its
+// item and its row in the tile, from which the join finds the slots.
+constexpr int kFewCols = 64;
+
+template <bool kWide>
+__global__ void __launch_bounds__(256, kWide ? 2 : 1) kv_values2_few_kernel(ValuesArgs va) {
+  const ProductArgs& a = va.p;
+  __shared__ __align__(16) int8_t tiles[2][kTileBytes];
+  __shared__ uint64_t sums[256][8];
+  __shared__ Row rows[16];
+  __shared__ int64_t pre[260];
+  const int dim = a.pool.dim, blocks = va.blocks;
+  Share sh = share_of(a, blocks, pre);
+  while (sh.unit < sh.end) {
+    const Piece pc = piece_at(a, blocks, pre, sh);
+    if (pc.count == 0) continue;
+    // As in values_run: offsets formed for each piece.
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int g = (tid >> 4) & 3, in = 16 * (tid >> 6) + (tid & 15);
+    const int col = pc.block * kFewCols + in;
+    __syncthreads();
+    if (tid < 16) {
+      const Row r = row_at(a, pc.q, 16 * pc.rt + tid);
+      rows[tid] = r;
+      if (pc.tile == 0 && r.t >= 0)
+        va.info[(int64_t(r.t) * a.heads + r.h) * blocks + pc.block] =
+            make_int4(pc.first, pc.last, tid, 0);
+    }
+    v4i acc[2][kDigitPlanes];
+    const bool flushed = values_run<4, kWide>(a, pc.q, rows, tiles, sums[tid], pc.tile,
+                                              pc.tile + pc.count, col, acc);
+    const bool whole = pc.count == pc.tiles;
+    uint64_t* slot = va.part + (2 * int64_t(blockIdx.x) + (pc.tile == 0 ? 1 : 0)) * kSlotWords;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const Row at = rows[4 * g + r];
+      if (at.t < 0 || col >= dim) continue;
+      const int64_t o = (int64_t(at.t) * a.heads + at.h) * dim + col;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint64_t v = from_sums(acc[p], r);
+        if (flushed) v += sums[tid][4 * p + r];
+        if (whole)
+          va.out[p][o] = v + a.c[p][o];
+        else
+          slot[(p * 16 + 4 * g + r) * kFewCols + in] = v;
+      }
+    }
+  }
+}
+
+// Joins the items that several workgroups have sums of, and truncates: kOut
+// columns of one row a workgroup, the other lanes over the slots.
+template <bool kTrunc, int kOut>
 __global__ void __launch_bounds__(256) kv_values2_join_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;
-  __shared__ uint64_t s[2][8][32];
-  const int64_t all = int64_t(a.b.tokens) * a.heads * a.pool.dim;
-  const int u = threadIdx.x & 31, lane = threadIdx.x >> 5;
+  constexpr int kLanes = 256 / kOut;
+  __shared__ uint64_t s[2][kLanes][kOut];
+  const int dim = a.pool.dim;
+  const int u = threadIdx.x % kOut, lane = threadIdx.x / kOut;
+  const int64_t row = blockIdx.x;
   const Put<kTrunc> put(a);
-  for (int64_t o0 = int64_t(blockIdx.x) * 32; o0 < all; o0 += int64_t(gridDim.x) * 32) {
-    const int64_t o = o0 + u;
+  if (seq_of(a.b, int(row / a.heads)) < 0) return;
+  const int col = int(blockIdx.y) * kOut + u;
+  const int64_t o = row * dim + col;
+  const int4 at = va.info ? va.info[row * va.blocks + int(blockIdx.y) * kOut / kFewCols]
+                          : make_int4(0, 0, 0, 0);
+  if (at.y > at.x) {
+    const int64_t in = at.z * kFewCols + col % kFewCols;
     uint64_t z0 = 0, z1 = 0;
-    if (o < all && va.splits > 1)
-      for (int k = lane; k < va.splits; k += 8) {
-        z0 += va.part[2 * k * all + o];
-        z1 += va.part[(2 * k + 1) * all + o];
-      }
-    __syncthreads();
+#pragma unroll 4
+    for (int w = at.x + lane; w <= at.y; w += kLanes) {
+      const uint64_t* slot = va.part + (2 * int64_t(w) + (w == at.x ? 1 : 0)) * kSlotWords + in;
+      z0 += slot[0];
+      z1 += slot[16 * kFewCols];
+    }
     s[0][lane][u] = z0;
     s[1][lane][u] = z1;
     __syncthreads();
-    if (lane == 0 && o < all && seq_of(a.b, int(o / (int64_t(a.heads) * a.pool.dim))) >= 0) {
-      z0 = va.splits > 1 ? a.c[0][o] : va.out[0][o];
-      z1 = va.splits > 1 ? a.c[1][o] : va.out[1][o];
-      for (int k = 0; k < 8; ++k) {
-        z0 += s[0][k][u];
-        z1 += s[1][k][u];
-      }
-      put(a, o, z0, z1);
+    if (lane || col >= dim) return;
+    z0 = a.c[0][o];
+    z1 = a.c[1][o];
+    for (int k = 0; k < kLanes; ++k) {
+      z0 += s[0][k][u];
+      z1 += s[1][k][u];
     }
+    put(a, o, z0, z1);
+  } else if (kTrunc && lane == 0 && col < dim) {
+    put(a, o, va.out[0][o], va.out[1][o]);
   }
 }
 
@@ -799,6 +1030,9 @@ int product_args(const sufhip_kv_product2_args* args, bool values, const char* w
     a.c[p] = g.c[p];
     a.out[p] = g.out[p];
   }
+  // A lookup that is not wanted reads a sequence's first page number; without
+  // pages a word that is there, and drops it.
+  if (a.b.max_pages == 0) a.b.table = a.b.cu;
   *out = a;
   return SUFHIP_OK;
 }
@@ -859,14 +1093,8 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
   const int64_t zs = int64_t(a.b.seqs) * a.pool.heads;
   const int cus = cu_total();
   if (row_tiles <= 1 || chunks > 2) {
-    // Shares of the keys: four workgroups a CU, of four key tiles at least
-    // where that still gives every CU one.
-    const int64_t tiles = (int64_t(b.max_keys) + kKeyTile - 1) / kKeyTile;
-    const int64_t groups = zs * (row_tiles < 1 ? 1 : row_tiles);
-    int64_t y = (4 * int64_t(cus) + groups - 1) / groups;
-    if (y > (tiles + 3) / 4 && groups * ((tiles + 3) / 4) >= cus) y = (tiles + 3) / 4;
-    if (y > tiles) y = tiles;
-    const dim3 grid(unsigned(zs), clip(y, 65535), clip(row_tiles, 65535));
+    const int64_t tiles = b.max_keys > kKeyTile ? (b.max_keys + kKeyTile - 1) / kKeyTile : 1;
+    const dim3 grid(clip(zs * (row_tiles < 1 ? 1 : row_tiles) * (tiles + 1), 2 * int64_t(cus)));
     return launch_scores_few<kVec, kFull, kTrunc>(a, grid, chunks, st);
   }
   constexpr int kGroups = kVec ? 2 : 1;  // of one chunk's kernel
@@ -874,8 +1102,8 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
   const int64_t key_tiles = (int64_t(b.max_keys) + 64 * groups - 1) / (64 * groups);
   // Row tiles are spread over workgroups until four of them share a CU.
   const int64_t want = (4 * int64_t(cus) + key_tiles * zs) / (key_tiles * zs + 1);
-  const dim3 grid(unsigned(zs), clip(key_tiles, 65535),
-                  clip(want < row_tiles ? want : row_tiles, 65535));
+  const dim3 grid(unsigned(zs), clip(want < row_tiles ? want : row_tiles, 65535),
+                  clip(key_tiles, 65535));
   if (chunks == 1) return launch_scores_many<1, kGroups, kVec, kFull, kTrunc>(a, grid, st);
   return launch_scores_many<2, 1, kVec, kFull, kTrunc>(a, grid, st);
 }
@@ -886,31 +1114,41 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
                   : launch_scores<kVec, kFull, false>(a, b, st);
 }
 
-// Shares of the keys: as many as fill the chip twice, each of two chunks of
-// keys at least.
-int values_splits(int64_t groups, int64_t max_keys, int cus) {
-  const int64_t want = (4 * int64_t(cus) + groups - 1) / groups;
-  const int64_t most = max_keys / (2 * kKeyTile);
-  const int64_t n = want < most ? want : most;
-  return n < 1 ? 1 : int(n < 1024 ? n : 1024);
-}
-
+// How a values call is laid out.  Few rows (up to kFewTiles row tiles a
+// sequence): even shares, `groups` workgroups.  Else a workgroup an item.
+constexpr int kFewTiles = 4;
 struct ValuesPlan {
-  int cols, waves, blocks, splits;
-  int64_t row_tiles, zs;
-  bool wide;
+  bool wide, few;
+  int waves, blocks;
+  int64_t row_tiles, zs, groups;
+  size_t part_bytes, info_bytes;
 };
 ValuesPlan plan_values(const sufhip_kv_batch& b, const sufhip_kv_pool& p, int heads) {
   ValuesPlan v{};
   v.wide = p.page_tokens >= 16;
-  v.waves = p.dim <= 64 || !v.wide ? 4 : 8;
-  v.cols = 16 * v.waves;
-  v.blocks = (p.dim + v.cols - 1) / v.cols;
   const int64_t rows = int64_t(b.max_new) * (heads / p.kv_heads);
   v.row_tiles = rows < 1 ? 1 : (rows + 15) / 16;
   v.zs = int64_t(b.seqs) * p.kv_heads;
-  v.splits = values_splits(v.row_tiles * v.zs * v.blocks, b.max_keys, cu_total());
+  v.few = v.row_tiles <= kFewTiles;
+  v.waves = v.few || !v.wide || p.dim <= 64 ? 4 : 8;
+  v.blocks = (p.dim + 16 * v.waves - 1) / (16 * v.waves);
+  if (v.few) {
+    const int64_t tiles = b.max_keys > kKeyTile ? (b.max_keys + kKeyTile - 1) / kKeyTile : 1;
+    v.groups = clip(v.zs * v.row_tiles * v.blocks * (tiles + 1), 2 * cu_total());
+    v.part_bytes = size_t(v.groups) * 2 * kSlotWords * 8;
+    v.info_bytes = size_t(b.tokens) * size_t(heads) * size_t(v.blocks) * 16;
+  }
   return v;
+}
+
+template <int kOut>
+void launch_join(const ValuesArgs& va, hipStream_t st) {
+  const dim3 grid(unsigned(va.p.b.tokens) * unsigned(va.p.heads),
+                  unsigned((va.p.pool.dim + kOut - 1) / kOut));
+  if (va.p.epi.on)
+    hipLaunchKernelGGL((kv_values2_join_kernel<true, kOut>), grid, dim3(256), 0, st, va);
+  else
+    hipLaunchKernelGGL((kv_values2_join_kernel<false, kOut>), grid, dim3(256), 0, st, va);
 }
 
 }  // namespace
@@ -938,8 +1176,7 @@ size_t sufhip_kv_values2_work_bytes(const sufhip_kv_batch* batch, const sufhip_k
       batch->seqs < 1 || heads % pool->kv_heads)
     return 0;
   const ValuesPlan v = plan_values(*batch, *pool, heads);
-  if (v.splits <= 1) return 0;
-  return size_t(v.splits) * 16 * size_t(batch->tokens) * size_t(heads) * size_t(pool->dim);
+  return v.part_bytes + v.info_bytes;
 }
 
 int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
@@ -948,17 +1185,29 @@ int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
   if (int rc = product_args(args, true, "sufhip_kv_values2", &va.p, &empty)) return rc;
   if (empty) return SUFHIP_OK;
   const ValuesPlan v = plan_values(args->batch, args->pool, args->heads);
-  va.splits = v.splits;
-  va.cols = v.cols;
-  if (v.splits > 1) {
-    const size_t need = sufhip_kv_values2_work_bytes(&args->batch, &args->pool, args->heads);
-    SUFHIP_REQUIRE(args->d_work && at16(args->d_work) && args->work_bytes >= need,
+  const hipStream_t st = as_stream(stream);
+  va.blocks = v.blocks;
+  for (int p = 0; p < 2; ++p) va.out[p] = va.p.epi.on ? va.p.epi.y[p] : va.p.out[p];
+  if (v.few) {
+    SUFHIP_REQUIRE(args->d_work && at16(args->d_work) &&
+                       args->work_bytes >= v.part_bytes + v.info_bytes,
                    "sufhip_kv_values2: d_work smaller than its work bytes, or not 16-byte aligned");
     va.part = static_cast<uint64_t*>(args->d_work);
+    va.info = reinterpret_cast<int4*>(static_cast<char*>(args->d_work) + v.part_bytes);
+    const dim3 grid{unsigned(v.groups)};
+    if (v.wide)
+      hipLaunchKernelGGL(kv_values2_few_kernel<true>, grid, dim3(256), 0, st, va);
+    else
+      hipLaunchKernelGGL(kv_values2_few_kernel<false>, grid, dim3(256), 0, st, va);
+    if (int rc = check_launch("kv_values2_few_kernel")) return rc;
+    // Slots of an item: over four, more lanes take them.
+    if (v.groups > 4 * v.zs * v.row_tiles * v.blocks)
+      launch_join<16>(va, st);
+    else
+      launch_join<64>(va, st);
+    return check_launch("kv_values2_join_kernel");
   }
-  const dim3 grid(unsigned(v.zs), unsigned(v.splits * v.blocks), clip(v.row_tiles, 65535));
-  const hipStream_t st = as_stream(stream);
-  for (int p = 0; p < 2; ++p) va.out[p] = va.p.epi.on ? va.p.epi.y[p] : va.p.out[p];
+  const dim3 grid(unsigned(v.zs), unsigned(v.blocks), clip(v.row_tiles, 65535));
   if (!v.wide)
     hipLaunchKernelGGL((kv_values2_kernel<4, false>), grid, dim3(256), 0, st, va);
   else if (v.waves == 4)
@@ -966,13 +1215,8 @@ int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
   else
     hipLaunchKernelGGL((kv_values2_kernel<8, true>), grid, dim3(512), 0, st, va);
   if (int rc = check_launch("kv_values2_kernel")) return rc;
-  if (v.splits == 1 && !va.p.epi.on) return SUFHIP_OK;
-  const int64_t all = int64_t(va.p.b.tokens) * va.p.heads * va.p.pool.dim;
-  const dim3 join(clip((all + 31) / 32, 1 << 20));
-  if (va.p.epi.on)
-    hipLaunchKernelGGL(kv_values2_join_kernel<true>, join, dim3(256), 0, st, va);
-  else
-    hipLaunchKernelGGL(kv_values2_join_kernel<false>, join, dim3(256), 0, st, va);
+  if (!va.p.epi.on) return SUFHIP_OK;
+  launch_join<64>(va, st);
   return check_launch("kv_values2_join_kernel");
 }
 
