@@ -44,69 +44,87 @@ def _fail(what, msg):
     raise ValueError("%s: %s" % (what, msg))
 
 
-def _check(t, shape, dtype, device, what, name):
+def _refuse(t, shape, d, what, name, dtype, dense):
+    """Says what is wrong with a tensor that _ptr did not take."""
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape):
         _fail(what, "%s must be a %s tensor of shape %s" % (name, dtype, list(shape)))
-    if t.device != device or device.type != "cuda":
-        _fail(what, "%s must be on the GPU, with the other tensors (%s)" % (name, device))
-    return t
-
-
-def _dense(t, shape, device, what, name, dtype=torch.int64):
-    if not _check(t, shape, dtype, device, what, name).is_contiguous():
+    if not t.is_cuda or t.get_device() != d:
+        _fail(what, "%s must be on the GPU, on one device with the other tensors" % name)
+    if dense and not t.is_contiguous():
         _fail(what, "%s must be contiguous" % name)
-    return t.data_ptr()
+    _fail(what, "%s is not usable" % name)
 
 
-def _dense2(arr, pair, shape, device, what, name):
+# The calls below take a few microseconds each and a step makes many of them, so
+# a tensor is checked in one expression; _refuse finds the reason.
+
+def _ptr(t, shape, d, what, name, dtype=torch.int64):
+    """Address of a contiguous tensor on GPU d."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and \
+            t.get_device() == d >= 0 and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(t, shape, d, what, name, dtype, True)
+
+
+def _two(pair, what, name):
+    try:
+        t0, t1 = pair
+    except (TypeError, ValueError):
+        _fail(what, "%s must be a pair (party 0, party 1)" % name)
+    return t0, t1
+
+
+def _ptr2(arr, pair, shape, d, what, name):
     """Both parties' contiguous tensors into a void*[2]."""
-    if len(pair) != 2:
-        _fail(what, "%s must be a pair (party 0, party 1)" % name)
-    arr[0] = _dense(pair[0], shape, device, what, name)
-    arr[1] = _dense(pair[1], shape, device, what, name)
+    t0, t1 = _two(pair, what, name)
+    arr[0] = _ptr(t0, shape, d, what, name)
+    arr[1] = _ptr(t1, shape, d, what, name)
 
 
-def _strides(pair, shape, device, what, name, written=False):
-    """Token and head stride of both parties' [tokens, heads, dim] tensors."""
-    if len(pair) != 2:
-        _fail(what, "%s must be a pair (party 0, party 1)" % name)
-    for t in pair:
-        _check(t, shape, torch.int64, device, what, name)
-        if shape[2] > 1 and t.stride(2) != 1:
+def _rows(arr, pair, shape, d, what, name, written=False):
+    """Both parties' [tokens, heads, dim] tensors into a void*[2]; their token
+    and head stride."""
+    t0, t1 = _two(pair, what, name)
+    st = None
+    for p, t in ((0, t0), (1, t1)):
+        if not (isinstance(t, torch.Tensor) and t.dtype is torch.int64 and t.shape == shape and
+                t.get_device() == d >= 0):
+            _refuse(t, shape, d, what, name, torch.int64, False)
+        s = t.stride()
+        if s[2] != 1 and shape[2] > 1:
             _fail(what, "the values of a head of %s must be neighbours" % name)
-    st = pair[0].stride()[:2]
-    if pair[1].stride()[:2] != st and pair[0].numel():
-        _fail(what, "both parties' %s must have the same strides" % name)
-    if written and any(n > 1 and s == 0 for n, s in zip(shape[:2], st)):
+        if st is None:
+            st = s
+        elif st[:2] != s[:2] and t.numel():
+            _fail(what, "both parties' %s must have the same strides" % name)
+        arr[p] = t.data_ptr()
+    if written and any(n > 1 and v == 0 for n, v in zip(shape[:2], st)):
         _fail(what, "rows of %s must not overlap" % name)
-    return st
+    return st[0], st[1]
 
 
-def _rows(out, pair, shape, device, what, name):
-    out.token_stride, out.head_stride = _strides(pair, shape, device, what, name)
-    out.p[0], out.p[1] = pair[0].data_ptr(), pair[1].data_ptr()
+def _device(t, what, name):
+    """Index of the GPU a call's first tensor is on."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _fail(what, "%s must be a tensor on the GPU" % name)
+    return t.get_device()
 
 
-class _Launch:
-    """The stream of `device`, and that device current while a call is made."""
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else \
-            torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_entries = {}
 
 
-def _call(name, args, device):
-    with _Launch(device) as stream:
-        native.call(name, ctypes.byref(args), stream)
+def _call(name, args, d):
+    """One library call on GPU d's current stream."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(native.load(), name)
+    if torch._C._cuda_getDevice() == d:
+        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(d))
+    else:
+        with torch.cuda.device(d):
+            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(d))
+    if rc != native.OK:
+        native.check(rc, name)
 
 
 def _epilogue(args, trunc, out, n, what):
@@ -129,11 +147,13 @@ class Rotary:
     1, multiplies the values past the rotated part."""
 
     def __init__(self, table, dim, interleaved=False, pass_mul=1 << 12):
+        _device(table, "Rotary", "the table")
         if table.dim() != 3 or table.shape[2] != 2 or 2 * table.shape[1] > dim:
             _fail("Rotary", "the table must be [positions, rot / 2, 2] with rot <= dim")
-        _dense(table, table.shape, table.device, "Rotary", "the table", torch.int32)
+        _ptr(table, table.shape, _device(table, "Rotary", "the table"), "Rotary", "the table",
+             torch.int32)
         self.table, self.dim, self.interleaved = table, int(dim), bool(interleaved)
-        self.pass_mul = int(pass_mul)
+        self.pass_mul, self.device = int(pass_mul), table.get_device()
         r = self.arg = native.RotaryTable()
         r.d_table = table.data_ptr() or None
         r.positions, r.rot = table.shape[0], 2 * table.shape[1]
@@ -197,15 +217,16 @@ class Pool:
     b); page_tokens a power of two."""
 
     def __init__(self, e, b0, b1):
-        if e.dim() != 4:
+        d, shape = _device(e, "Pool", "e"), e.shape
+        if len(shape) != 4:
             _fail("Pool", "the arrays must be [pages, kv_heads, page_tokens, dim]")
-        p = self.arg = native.KvPool()
-        p.e = _dense(e, e.shape, e.device, "Pool", "e")
-        p.b[0] = _dense(b0, e.shape, e.device, "Pool", "b0")
-        p.b[1] = _dense(b1, e.shape, e.device, "Pool", "b1")
-        p.pages, p.kv_heads, p.page_tokens, p.dim = e.shape
-        self.e, self.b, self.device = e, (b0, b1), e.device
-        self.kv_heads, self.dim = e.shape[1], e.shape[3]
+        self.arg = native.KvPool(_ptr(e, shape, d, "Pool", "e"),
+                                 (_ptr(b0, shape, d, "Pool", "b0"),
+                                  _ptr(b1, shape, d, "Pool", "b1")),
+                                 shape[0], shape[2], shape[1], shape[3])
+        self.e, self.b, self.device = e, (b0, b1), d
+        self.shape = shape
+        self.kv_heads, self.dim = shape[1], shape[3]
 
 
 class Batch:
@@ -217,17 +238,19 @@ class Batch:
     max_new, max_keys: bounds by which launches are laid out."""
 
     def __init__(self, cu, kv_lens, pages, tokens, max_new, max_keys):
+        d = _device(kv_lens, "Batch", "kv_lens")
         if kv_lens.dim() != 1 or pages.dim() != 2:
             _fail("Batch", "kv_lens must be [seqs], pages [seqs, max_pages]")
-        seqs, d = kv_lens.shape[0], kv_lens.device
+        seqs, width = kv_lens.shape[0], pages.shape[1]
         b = self.arg = native.KvBatch()
-        b.d_cu_tokens = _dense(cu, (seqs + 1,), d, "Batch", "cu", torch.int32)
-        b.d_kv_lens = _dense(kv_lens, (seqs,), d, "Batch", "kv_lens", torch.int32)
-        b.d_pages = _dense(pages, (seqs, pages.shape[1]), d, "Batch", "pages", torch.int32)
-        b.seqs, b.tokens, b.max_pages = seqs, int(tokens), pages.shape[1]
+        b.d_cu_tokens = _ptr(cu, (seqs + 1,), d, "Batch", "cu", torch.int32)
+        b.d_kv_lens = _ptr(kv_lens, (seqs,), d, "Batch", "kv_lens", torch.int32)
+        b.d_pages = _ptr(pages, (seqs, width), d, "Batch", "pages", torch.int32)
+        b.seqs, b.tokens, b.max_pages = seqs, int(tokens), width
         b.max_new, b.max_keys = int(max_new), int(max_keys)
         self.cu, self.kv_lens, self.pages = cu, kv_lens, pages
         self.tokens, self.device = int(tokens), d
+        self._work_bytes = {}
 
 
 def causal_row_offsets(new, lens, heads):
@@ -248,22 +271,22 @@ def rotary2(x, rotary, positions, out=None, trunc=None):
     x, which may be x itself, or None for new ones (zeros in padding rows).  trunc: a prepared
     tasks.Trunc the rotated values go through.  Returns out."""
     what = "rotary2"
-    shape, d = tuple(x[0].shape), x[0].device
+    d, shape = _device(x[0], what, "x"), x[0].shape
     if len(shape) != 3 or shape[2] != rotary.dim:
         _fail(what, "x must be [tokens, heads, %d]" % rotary.dim)
-    if rotary.table.device != d:
+    if rotary.device != d:
         _fail(what, "the table is on another device than x")
     if out is None:
-        out = tuple(torch.zeros(shape, dtype=torch.int64, device=d) for _ in range(2))
+        out = tuple(torch.zeros(shape, dtype=torch.int64, device=x[0].device) for _ in range(2))
     a = native.Rotary2Args()
-    _rows(a.x, x, shape, d, what, "x")
+    r = a.x
+    r.token_stride, r.head_stride = _rows(r.p, x, shape, d, what, "x")
     a.tokens, a.heads, a.dim = shape
     a.rot = rotary.arg
-    a.d_positions = _dense(positions, shape[:1], d, what, "positions", torch.int32)
-    a.out_token_stride, a.out_head_stride = _strides(out, shape, d, what, "out", written=True)
-    a.out[0], a.out[1] = out[0].data_ptr(), out[1].data_ptr()
-    epi = _epilogue(a, trunc, out, x[0].numel(), what)
-    if epi is not None:
+    a.d_positions = _ptr(positions, shape[:1], d, what, "positions", torch.int32)
+    a.out_token_stride, a.out_head_stride = _rows(a.out, out, shape, d, what, "out", written=True)
+    if trunc is not None:
+        epi = _epilogue(a, trunc, out, x[0].numel(), what)
         a.mask = trunc.mask & M64
     _call("sufhip_rotary2", a, d)
     return out
@@ -274,22 +297,22 @@ def _append_part(part, batch, pool, x, mask, rotary, positions, trunc, what, nam
     shape = (T, pool.kv_heads, pool.dim)
     if pool.device != d:
         _fail(what, "the pool and the batch are on different devices")
-    _rows(part.x, x, shape, d, what, name)
-    _dense2(part.mask, mask, shape, d, what, name + "_mask")
+    r = part.x
+    r.token_stride, r.head_stride = _rows(r.p, x, shape, d, what, name)
+    _ptr2(part.mask, mask, shape, d, what, name + "_mask")
     part.pool = pool.arg
     if rotary is not None:
-        if rotary.dim != pool.dim or rotary.table.device != d:
-            _fail(what, "the rotary table is for heads of %d on %s" %
-                  (rotary.dim, rotary.table.device))
+        if rotary.dim != pool.dim or rotary.device != d:
+            _fail(what, "the rotary table must be for heads of %d, on the pool's device" % pool.dim)
         part.rot = rotary.arg
         if positions is not None:
-            part.d_positions = _dense(positions, (T,), d, what, "positions", torch.int32)
+            part.d_positions = _ptr(positions, (T,), d, what, "positions", torch.int32)
     if trunc is None:
         return None
     gate, y = trunc if isinstance(trunc, tuple) else (trunc, None)
     if y is not None:
         for t in y:
-            _dense(t, shape, d, what, "the truncated shares")
+            _ptr(t, shape, d, what, "the truncated shares")
     epi = _epilogue(part, gate, y if y is not None else x, x[0].numel(), what)
     if y is None:
         epi.y[0] = epi.y[1] = None
@@ -323,8 +346,8 @@ def _product(batch, pool, offsets, heads, what):
     a.batch, a.pool, a.heads = batch.arg, pool.arg, heads
     if pool.device != batch.device:
         _fail(what, "the pool and the batch are on different devices")
-    a.d_row_offsets = _dense(offsets, (heads * batch.tokens + 1,), batch.device, what, "offsets",
-                             torch.int32)
+    a.d_row_offsets = _ptr(offsets, (heads * batch.tokens + 1,), batch.device, what, "offsets",
+                           torch.int32)
     return a
 
 
@@ -336,27 +359,40 @@ def scores2(batch, pool, q, a, c, offsets, out, trunc=None):
     [heads * tokens + 1], row (h, t) first element h * tokens + t.  trunc: a
     prepared tasks.Trunc the scores go through.  Returns out."""
     what, d = "scores2", batch.device
-    if q[0].dim() != 3 or q[0].shape[0] != batch.tokens or q[0].shape[2] != pool.dim:
+    _device(q[0], what, "q")
+    shape = q[0].shape
+    if len(shape) != 3 or shape[0] != batch.tokens or shape[2] != pool.dim:
         _fail(what, "q must be [%d, heads, %d]" % (batch.tokens, pool.dim))
-    shape = tuple(q[0].shape)
     g = _product(batch, pool, offsets, shape[1], what)
-    _rows(g.x, q, shape, d, what, "q")
-    _dense2(g.a, a, shape, d, what, "a")
-    g.n = out[0].numel()
-    _dense2(g.c, c, (g.n,), d, what, "c")
-    _dense2(g.out, out, (g.n,), d, what, "out")
-    epi = _epilogue(g, trunc, out, g.n, what)
-    if epi is not None:
+    r = g.x
+    r.token_stride, r.head_stride = _rows(r.p, q, shape, d, what, "q")
+    _ptr2(g.a, a, shape, d, what, "a")
+    _device(out[0], what, "out")
+    n = g.n = out[0].numel()
+    _ptr2(g.c, c, (n,), d, what, "c")
+    _ptr2(g.out, out, (n,), d, what, "out")
+    if trunc is not None:
+        epi = _epilogue(g, trunc, out, n, what)
         g.mask = trunc.mask & M64
     _call("sufhip_kv_scores2", g, d)
     return out
 
 
+def _work_words(batch, pool, heads):
+    key = (pool.shape, heads)
+    n = batch._work_bytes.get(key)
+    if n is None:
+        with torch.cuda.device(batch.device):
+            nb = native.load().sufhip_kv_values2_work_bytes(ctypes.byref(batch.arg),
+                                                            ctypes.byref(pool.arg), heads)
+        n = batch._work_bytes[key] = (nb + 7) // 8
+    return n
+
+
 def values_work(batch, pool, heads):
     """The workspace of a values2 call on this batch (None: none needed)."""
-    nb = native.load().sufhip_kv_values2_work_bytes(ctypes.byref(batch.arg),
-                                                    ctypes.byref(pool.arg), heads)
-    return torch.empty((nb + 7) // 8, dtype=torch.int64, device=batch.device) if nb else None
+    n = _work_words(batch, pool, heads)
+    return torch.empty(n, dtype=torch.int64, device=batch.kv_lens.device) if n else None
 
 
 def values2(batch, pool, p, a, c, offsets, out, trunc=None, work=None):
@@ -367,22 +403,24 @@ def values2(batch, pool, p, a, c, offsets, out, trunc=None, work=None):
     work: values_work(...) of a batch with the same extents, allocated here if
     it is not given.  Returns out."""
     what, d = "values2", batch.device
-    if out[0].dim() != 3 or out[0].shape[0] != batch.tokens or out[0].shape[2] != pool.dim:
+    _device(out[0], what, "out")
+    shape = out[0].shape
+    if len(shape) != 3 or shape[0] != batch.tokens or shape[2] != pool.dim:
         _fail(what, "out must be [%d, heads, %d]" % (batch.tokens, pool.dim))
-    shape = tuple(out[0].shape)
     g = _product(batch, pool, offsets, shape[1], what)
-    g.n = p[0].numel()
-    _dense2(g.x.p, p, (g.n,), d, what, "p")
-    _dense2(g.a, a, (g.n,), d, what, "a")
-    _dense2(g.c, c, shape, d, what, "c")
-    _dense2(g.out, out, shape, d, what, "out")
-    epi = _epilogue(g, trunc, out, out[0].numel(), what)
-    if epi is not None:
+    _device(p[0], what, "p")
+    n = g.n = p[0].numel()
+    _ptr2(g.x.p, p, (n,), d, what, "p")
+    _ptr2(g.a, a, (n,), d, what, "a")
+    _ptr2(g.c, c, shape, d, what, "c")
+    _ptr2(g.out, out, shape, d, what, "out")
+    if trunc is not None:
+        epi = _epilogue(g, trunc, out, out[0].numel(), what)
         g.mask = trunc.mask & M64
-    with _Launch(d) as stream:
-        if work is None:
-            work = values_work(batch, pool, shape[1])
-        if work is not None:
-            g.d_work, g.work_bytes = work.data_ptr(), work.numel() * 8
-        native.call("sufhip_kv_values2", ctypes.byref(g), stream)
+    if work is None:
+        work = values_work(batch, pool, shape[1])
+    if work is not None:
+        g.d_work = _ptr(work, work.shape, d, what, "work")
+        g.work_bytes = work.numel() * 8
+    _call("sufhip_kv_values2", g, d)
     return out
