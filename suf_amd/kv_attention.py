@@ -31,7 +31,7 @@ import math
 import numpy as np
 import torch
 
-from . import native, pfss
+from . import native
 from .softmax import SoftmaxBlock
 from .tasks import Dealer, Trunc, dev, dev_i32, prepare_batch
 
@@ -424,3 +424,156 @@ def values2(batch, pool, p, a, c, offsets, out, trunc=None, work=None):
         g.work_bytes = work.numel() * 8
     _call("sufhip_kv_values2", g, d)
     return out
+
+
+# ---- a cache of many sequences, and a step of attention over it ----
+
+class PagedCache:
+    """Pages of keys and values for many sequences of any lengths.  open()
+    starts a sequence, extend() gives its new tokens pages, close() takes its
+    pages back; k and v are the Pools.  A page that is used again gets new
+    masks with its new tokens."""
+
+    def __init__(self, pages, page_tokens, kv_heads, dim, v_dim=None, device="cuda"):
+        shape = (pages, kv_heads, page_tokens)
+        self.k, self.v = (
+            Pool(*(torch.zeros(shape + (n,), dtype=torch.int64, device=device)
+                   for _ in range(3))) for n in (dim, dim if v_dim is None else v_dim))
+        self.page_tokens, self.kv_heads, self.device = page_tokens, kv_heads, device
+        self.free = list(range(pages))[::-1]
+        self.seqs = {}
+        self._next = 0
+
+    def open(self):
+        """A new, empty sequence's number."""
+        s, self._next = self._next, self._next + 1
+        self.seqs[s] = {"pages": [], "length": 0}
+        return s
+
+    def close(self, seq):
+        self.free += self.seqs.pop(seq)["pages"][::-1]
+
+    def length(self, seq):
+        return self.seqs[seq]["length"]
+
+    def extend(self, seqs, new):
+        """Room for new[i] more tokens of sequence seqs[i]; the Batch of these
+        tokens.  Raises, with nothing changed, when the pages do not suffice."""
+        if len(seqs) != len(new) or len(set(seqs)) != len(seqs) or min(new, default=1) < 0:
+            _fail("extend", "sequences must be different, each with a count of new tokens >= 0")
+        state = [self.seqs[s] for s in seqs]
+        lens = [st["length"] + n for st, n in zip(state, new)]
+        need = [-(-n // self.page_tokens) - len(st["pages"]) for n, st in zip(lens, state)]
+        if sum(need) > len(self.free):
+            raise RuntimeError("PagedCache: %d pages wanted, %d free" % (sum(need), len(self.free)))
+        for st, n, k in zip(state, lens, need):
+            st["pages"] += [self.free.pop() for _ in range(k)]
+            st["length"] = n
+        width = max([len(st["pages"]) for st in state] + [1])
+        table = np.full((len(seqs), width), -1, np.int32)
+        for row, st in zip(table, state):
+            row[:len(st["pages"])] = st["pages"]
+        cu = np.concatenate([[0], np.cumsum(np.asarray(new, dtype=np.int64))])
+        return Batch(dev_i32(cu, self.device), dev_i32(np.asarray(lens), self.device),
+                     dev_i32(table, self.device), tokens=int(cu[-1]), max_new=max(new, default=0),
+                     max_keys=max(lens, default=0))
+
+
+def _shares(dealer, shape, device):
+    """Uniform shares of a uniform value (a mask), both parties."""
+    n = int(np.prod(shape))
+    return tuple(dev(dealer.words(n), device).view(shape) for _ in range(2))
+
+
+class CachedAttention:
+    """Causal attention of new tokens over a PagedCache, grouped heads, with
+    rotary positions; Q(frac_bits) shares in and out:
+      q', k' = trunc(rot(q) / sqrt(dim)), trunc(rot(k))
+      scores = trunc(q' k'^T), p = Softmax(scores), out = trunc(p v)
+    deal(seqs, new) makes a step's dealer material and room in the cache,
+    step.run(q, k, v, out) computes it."""
+
+    def __init__(self, cache, heads, prg_state, max_positions, frac_bits=12, table_bits=12,
+                 rot=None, base=10000.0, interleaved=False, scaling=None, seed=21):
+        dim = cache.k.dim
+        if heads % cache.kv_heads:
+            _fail("CachedAttention", "heads must be a multiple of the cache's %d" % cache.kv_heads)
+        self.cache, self.heads, self.f, self.fc = cache, heads, frac_bits, table_bits
+        self.prg_state = bytes(prg_state)
+        self.max_positions = max_positions
+        kw = dict(rot=rot, base=base, frac_bits=table_bits, interleaved=interleaved,
+                  scaling=scaling, device=cache.device)
+        self.q_rotary = Rotary.build(dim, max_positions, scale=1.0 / math.sqrt(dim), **kw)
+        self.k_rotary = Rotary.build(dim, max_positions, **kw)
+        self.dealer = Dealer(seed)
+
+    def deal(self, seqs, new):
+        if min(new, default=0) < 1:
+            _fail("CachedAttention.deal", "every sequence needs a new token")
+        if max(self.cache.length(s) + n for s, n in zip(seqs, new)) > self.max_positions:
+            _fail("CachedAttention.deal", "a sequence grows past max_positions")
+        return AttentionStep(self, seqs, new)
+
+
+class AttentionStep:
+    """One step's tokens: its Batch, the dealer's masks, products and gates."""
+
+    def __init__(self, att, seqs, new):
+        cache, deal, H, f = att.cache, att.dealer, att.heads, att.f
+        device, Hk = cache.device, cache.kv_heads
+        self.att = att
+        self.batch = b = cache.extend(seqs, new)
+        lens = [cache.length(s) for s in seqs]
+        T, D, Dv = b.tokens, cache.k.dim, cache.v.dim
+        self.offsets = causal_row_offsets(new, lens, H)
+        self.off = dev_i32(self.offsets, device)
+        n = int(self.offsets[-1])
+        self.positions = dev_i32(np.concatenate([np.arange(L - k, L)
+                                                 for k, L in zip(new, lens)]), device)
+        self.work = values_work(b, cache.v, H)
+        # The new words' masks go to their pages at once (the append of zeros
+        # leaves -mask for E), so that the products below see all masks.
+        self.k_mask = _shares(deal, (T, Hk, D), device)
+        self.v_mask = _shares(deal, (T, Hk, Dv), device)
+        none = tuple(torch.zeros((T, Hk, max(D, Dv)), dtype=torch.int64, device=device)
+                     for _ in range(2))
+        append2(b, cache.k, tuple(t[..., :D] for t in none), self.k_mask, cache.v,
+                tuple(t[..., :Dv] for t in none), self.v_mask)
+        self.q_a, self.p_a = _shares(deal, (T, H, D), device), _shares(deal, (n,), device)
+        self.s_c = self._triple(scores2, cache.k, self.q_a, (n,), deal, {})
+        self.o_c = self._triple(values2, cache.v, self.p_a, (T, H, Dv), deal, {"work": self.work})
+        self.tr = {name: Trunc(deal, bits, size, att.prg_state, device=device)
+                   for name, bits, size in (("q", att.fc, T * H * D), ("k", att.fc, T * Hk * D),
+                                            ("s", f, n), ("o", f, T * H * Dv))}
+        self.softmax = SoftmaxBlock(self.offsets, att.prg_state, f, seed=deal.word() >> 1,
+                                    device=device)
+        self.q = tuple(torch.empty((T, H, D), dtype=torch.int64, device=device) for _ in range(2))
+        self.s, self.p = (tuple(torch.empty(n, dtype=torch.int64, device=device)
+                                for _ in range(2)) for _ in range(2))
+
+    def _triple(self, op, pool, a, shape, deal, kw):
+        """Shares of A b for the product's left mask A: the product itself with
+        b_1 in E's place, A opened and nothing else: Z_0 = A b_0 + A b_1."""
+        zero = tuple(torch.zeros_like(a[0]) for _ in range(2))
+        out = tuple(torch.zeros(shape, dtype=torch.int64, device=a[0].device) for _ in range(2))
+        op(self.batch, Pool(pool.b[1], pool.b[0], pool.b[0]), (a[0] + a[1], zero[1]), zero,
+           tuple(torch.zeros_like(v) for v in out), self.off, out, **kw)
+        c0 = dev(deal.words(out[0].numel()), out[0].device).view(shape)
+        return c0, out[0] - c0
+
+    def truncs(self):
+        return list(self.tr.values())
+
+    def run(self, q, k, v, out):
+        """q [tokens, heads, dim], k, v [tokens, kv_heads, dim]: pairs of shares
+        with any token and head strides (the parts of a fused product's rows);
+        out: contiguous [tokens, heads, dim of v].  Returns out."""
+        att, cache, b, tr = self.att, self.att.cache, self.batch, self.tr
+        prepare_batch(self.truncs())
+        rotary2(q, att.q_rotary, self.positions, self.q, trunc=tr["q"])
+        append2(b, cache.k, k, self.k_mask, cache.v, v, self.v_mask, rotary=att.k_rotary,
+                k_trunc=tr["k"])
+        scores2(b, cache.k, self.q, self.q_a, self.s_c, self.off, self.s, trunc=tr["s"])
+        self.softmax.eval2(self.s, self.p)
+        return values2(b, cache.v, self.p, self.p_a, self.o_c, self.off, out, trunc=tr["o"],
+                       work=self.work)
