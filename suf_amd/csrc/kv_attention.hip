@@ -229,9 +229,14 @@ __device__ __forceinline__ void clear(v4i (&acc)[2][kDigitPlanes]) {
 
 // A sequence's part of the batch for one cached head: its rows are (token,
 // head of the group) in that order, row m at token t0 + m / group.
+// kv: its keys, none of which a row of at most n elements can do without.
 struct Seq {
   int s, hk, t0, rows, kv;
 };
+__device__ __forceinline__ int keys_of(const ProductArgs& a, int s) {
+  const int kv = a.b.lens[s];
+  return int64_t(kv) < a.n ? kv : int(a.n);
+}
 __device__ __forceinline__ Seq seq_of_head(const ProductArgs& a, int s, int hk) {
   Seq q;
   q.s = s;
@@ -240,7 +245,7 @@ __device__ __forceinline__ Seq seq_of_head(const ProductArgs& a, int s, int hk) 
   q.t0 = lo > 0 ? lo : 0;
   const int t1 = hi < a.b.tokens ? hi : a.b.tokens;
   q.rows = t1 > q.t0 ? (t1 - q.t0) * a.group : 0;
-  q.kv = a.b.lens[q.s];
+  q.kv = keys_of(a, s);
   return q;
 }
 
@@ -290,7 +295,7 @@ __device__ __forceinline__ int64_t units_of(const ProductArgs& a, int s, int blo
   const int lo = a.b.cu[s], hi = a.b.cu[s + 1];
   const int t0 = lo > 0 ? lo : 0, t1 = hi < a.b.tokens ? hi : a.b.tokens;
   const int64_t row_tiles = t1 > t0 ? ((t1 - t0) * a.group + 15) / 16 : 0;
-  return row_tiles * blocks * a.pool.heads * (tiles_of(a.b.lens[s]) + 1);
+  return row_tiles * blocks * a.pool.heads * (tiles_of(keys_of(a, s)) + 1);
 }
 
 // Sums before each of the 256 threads' sequences into pre[0 .. 256] (a
@@ -576,8 +581,9 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
   const Put<kTrunc> put(a);
   const Seq q = seq_at(a, int(blockIdx.x));
   const int row_tiles = (q.rows + 15) / 16;
-  for (int k0 = int(blockIdx.z) * kKeys; k0 < q.kv; k0 += int(gridDim.z) * kKeys) {
-    const int key = k0 + 16 * w + n;
+  for (int64_t first_key = int64_t(blockIdx.z) * kKeys; first_key < q.kv;
+       first_key += int64_t(gridDim.z) * kKeys) {
+    const int k0 = int(first_key), key = k0 + 16 * w + n;
     const int64_t place = key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
     v4i K[kHeld][3][kDigitPlanes];
     // The lane's offsets are formed again for each key tile: kept over the
@@ -956,35 +962,38 @@ __global__ void __launch_bounds__(256) kv_values2_join_kernel(ValuesArgs va) {
   __shared__ uint64_t s[2][kLanes][kOut];
   const int dim = a.pool.dim;
   const int u = threadIdx.x % kOut, lane = threadIdx.x / kOut;
-  const int64_t row = blockIdx.x;
   const Put<kTrunc> put(a);
-  if (seq_of(a.b, int(row / a.heads)) < 0) return;
-  const int col = int(blockIdx.y) * kOut + u;
-  const int64_t o = row * dim + col;
-  const int4 at = va.info ? va.info[row * va.blocks + int(blockIdx.y) * kOut / kFewCols]
-                          : make_int4(0, 0, 0, 0);
-  if (at.y > at.x) {
-    const int64_t in = at.z * kFewCols + col % kFewCols;
-    uint64_t z0 = 0, z1 = 0;
+  const int64_t all = int64_t(a.b.tokens) * a.heads;
+  for (int64_t row = blockIdx.x; row < all; row += gridDim.x) {
+    if (seq_of(a.b, int(row / a.heads)) < 0) continue;
+    const int col = int(blockIdx.y) * kOut + u;
+    const int64_t o = row * dim + col;
+    const int4 at = va.info ? va.info[row * va.blocks + int(blockIdx.y) * kOut / kFewCols]
+                            : make_int4(0, 0, 0, 0);
+    if (at.y > at.x) {
+      const int64_t in = at.z * kFewCols + col % kFewCols;
+      uint64_t z0 = 0, z1 = 0;
 #pragma unroll 4
-    for (int w = at.x + lane; w <= at.y; w += kLanes) {
-      const uint64_t* slot = va.part + (2 * int64_t(w) + (w == at.x ? 1 : 0)) * kSlotWords + in;
-      z0 += slot[0];
-      z1 += slot[16 * kFewCols];
+      for (int w = at.x + lane; w <= at.y; w += kLanes) {
+        const uint64_t* slot = va.part + (2 * int64_t(w) + (w == at.x ? 1 : 0)) * kSlotWords + in;
+        z0 += slot[0];
+        z1 += slot[16 * kFewCols];
+      }
+      __syncthreads();  // the sums of the row before have been used
+      s[0][lane][u] = z0;
+      s[1][lane][u] = z1;
+      __syncthreads();
+      if (lane || col >= dim) continue;
+      z0 = a.c[0][o];
+      z1 = a.c[1][o];
+      for (int k = 0; k < kLanes; ++k) {
+        z0 += s[0][k][u];
+        z1 += s[1][k][u];
+      }
+      put(a, o, z0, z1);
+    } else if (kTrunc && lane == 0 && col < dim) {
+      put(a, o, va.out[0][o], va.out[1][o]);
     }
-    s[0][lane][u] = z0;
-    s[1][lane][u] = z1;
-    __syncthreads();
-    if (lane || col >= dim) return;
-    z0 = a.c[0][o];
-    z1 = a.c[1][o];
-    for (int k = 0; k < kLanes; ++k) {
-      z0 += s[0][k][u];
-      z1 += s[1][k][u];
-    }
-    put(a, o, z0, z1);
-  } else if (kTrunc && lane == 0 && col < dim) {
-    put(a, o, va.out[0][o], va.out[1][o]);
   }
 }
 
@@ -1000,8 +1009,8 @@ int product_args(const sufhip_kv_product2_args* args, bool values, const char* w
     return kv_fail(what, "heads must be a multiple of the pool's kv_heads");
   if (g.n > 0x7fffffffu) return kv_fail(what, "at most 2^31 - 1 packed elements");
   const size_t rows = size_t(a.b.tokens) * size_t(g.heads);
-  if (rows > (1u << 30) || size_t(a.b.seqs) * size_t(a.pool.heads) > (1u << 30))
-    return kv_fail(what, "at most 2^30 rows, and sequences times cached heads");
+  if (rows > (1u << 30) || size_t(a.b.seqs) * size_t(a.pool.heads) > (1u << 22))
+    return kv_fail(what, "at most 2^30 rows, and 2^22 sequences times cached heads");
   *empty = a.b.seqs == 0 || rows == 0 || (!values && g.n == 0);
   if (*empty) return SUFHIP_OK;
   const size_t n_out = values ? rows * size_t(g.pool.dim) : g.n;
@@ -1092,8 +1101,13 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
   const int64_t row_tiles = (int64_t(b.max_new) * a.group + 15) / 16;
   const int64_t zs = int64_t(a.b.seqs) * a.pool.heads;
   const int cus = cu_total();
+  // One row tile a sequence streams the keys; with more, keys held as digits
+  // are used for all of them (4 cached heads of 64, 8 x 4 rows over 4 x 2048
+  // keys, two row tiles: 42 us streamed, 29 held; 24 row tiles: 284 and 155).
+  // Heads past 128 do not fit in registers.
   if (row_tiles <= 1 || chunks > 2) {
-    const int64_t tiles = b.max_keys > kKeyTile ? (b.max_keys + kKeyTile - 1) / kKeyTile : 1;
+    const int64_t tiles =
+        b.max_keys > kKeyTile ? (int64_t(b.max_keys) + kKeyTile - 1) / kKeyTile : 1;
     const dim3 grid(clip(zs * (row_tiles < 1 ? 1 : row_tiles) * (tiles + 1), 2 * int64_t(cus)));
     return launch_scores_few<kVec, kFull, kTrunc>(a, grid, chunks, st);
   }
@@ -1114,9 +1128,17 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
                   : launch_scores<kVec, kFull, false>(a, b, st);
 }
 
-// How a values call is laid out.  Few rows (up to kFewTiles row tiles a
-// sequence): even shares, `groups` workgroups.  Else a workgroup an item.
-constexpr int kFewTiles = 4;
+// How a values call is laid out: even shares of the keys over two workgroups a
+// CU (few), or a workgroup an item (row tile, cached head, column block).  An
+// item is one chain over its keys, so even shares win while items are fewer
+// than half the CUs, and, whatever their number, with one row tile a sequence,
+// where lengths differ most; from there on the items fill the chip and need no
+// join, as do short chains.  Us, even shares / items (4 cached heads of 64, new
+// tokens x 8 heads; keys in all):
+//   4 x 2048 keys:  32 items 41 / 131    96: 84 / 140   192: 139 / 145   384: 257 / 222
+//   1 x 300:         8 items 15 / 25     48: 24 / 32     96: 32 / 32
+//   8 x 100:        64 items 19 / 17    192: 31 / 18    768: 66 / 50
+constexpr int kFewMinTiles = 4;
 struct ValuesPlan {
   bool wide, few;
   int waves, blocks;
@@ -1129,11 +1151,12 @@ ValuesPlan plan_values(const sufhip_kv_batch& b, const sufhip_kv_pool& p, int he
   const int64_t rows = int64_t(b.max_new) * (heads / p.kv_heads);
   v.row_tiles = rows < 1 ? 1 : (rows + 15) / 16;
   v.zs = int64_t(b.seqs) * p.kv_heads;
-  v.few = v.row_tiles <= kFewTiles;
+  const int64_t tiles = b.max_keys > kKeyTile ? (int64_t(b.max_keys) + kKeyTile - 1) / kKeyTile : 1;
+  const int64_t items = v.zs * v.row_tiles * ((p.dim + 63) / 64);
+  v.few = tiles >= kFewMinTiles && (v.row_tiles == 1 || 2 * items <= cu_total());
   v.waves = v.few || !v.wide || p.dim <= 64 ? 4 : 8;
   v.blocks = (p.dim + 16 * v.waves - 1) / (16 * v.waves);
   if (v.few) {
-    const int64_t tiles = b.max_keys > kKeyTile ? (b.max_keys + kKeyTile - 1) / kKeyTile : 1;
     v.groups = clip(v.zs * v.row_tiles * v.blocks * (tiles + 1), 2 * cu_total());
     v.part_bytes = size_t(v.groups) * 2 * kSlotWords * 8;
     v.info_bytes = size_t(b.tokens) * size_t(heads) * size_t(v.blocks) * 16;
@@ -1143,7 +1166,7 @@ ValuesPlan plan_values(const sufhip_kv_batch& b, const sufhip_kv_pool& p, int he
 
 template <int kOut>
 void launch_join(const ValuesArgs& va, hipStream_t st) {
-  const dim3 grid(unsigned(va.p.b.tokens) * unsigned(va.p.heads),
+  const dim3 grid(clip(int64_t(va.p.b.tokens) * va.p.heads, 1 << 20),
                   unsigned((va.p.pool.dim + kOut - 1) / kOut));
   if (va.p.epi.on)
     hipLaunchKernelGGL((kv_values2_join_kernel<true, kOut>), grid, dim3(256), 0, st, va);

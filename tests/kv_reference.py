@@ -58,9 +58,10 @@ class Case:
         pg = self.table[s, j // self.page]
         return (pg, j % self.page) if 0 <= pg < self.pages else None
 
-    def cached(self, s, g, which):
-        """[length, dim] words of a pool array; zeros without a page."""
-        out = np.zeros((max(0, self.lens[s]), self.dim), U)
+    def cached(self, s, g, which, most):
+        """[length, dim] words of a pool array (no more keys than the longest
+        row's); zeros without a page."""
+        out = np.zeros((min(max(0, self.lens[s]), most), self.dim), U)
         for j in range(len(out)):
             at = self.spot(s, j)
             if at is not None:
@@ -108,10 +109,11 @@ def scores(case, heads, off, x, a, c, before):
     out = [b.copy() for b in before]
     d = (x[0] - a[0]) + (x[1] - a[1])
     left = (a[0] + d, a[1])
+    most = int(max(0, np.diff(off.astype(np.int64)).max(initial=0)))
     for s, n in enumerate(case.new):
         for h in range(heads):
             g = h // (heads // case.kv_heads)
-            E, B = case.cached(s, g, 0), (case.cached(s, g, 1), case.cached(s, g, 2))
+            E, *B = (case.cached(s, g, i, most) for i in range(3))
             for t in range(case.cu[s], case.cu[s] + n):
                 f, l = _span(off, h * case.tokens + t, len(out[0]), case.lens[s])
                 for p in range(2):
@@ -124,10 +126,11 @@ def values(case, heads, off, x, a, c, before):
     out = [b.copy() for b in before]
     d = (x[0] - a[0]) + (x[1] - a[1])
     left = (a[0] + d, a[1])
+    most = int(max(0, np.diff(off.astype(np.int64)).max(initial=0)))
     for s, n in enumerate(case.new):
         for h in range(heads):
             g = h // (heads // case.kv_heads)
-            E, B = case.cached(s, g, 0), (case.cached(s, g, 1), case.cached(s, g, 2))
+            E, *B = (case.cached(s, g, i, most) for i in range(3))
             for t in range(case.cu[s], case.cu[s] + n):
                 f, l = _span(off, h * case.tokens + t, len(d), case.lens[s])
                 for p in range(2):

@@ -243,4 +243,5 @@ def test_calls_refuse_wrong_tensors():
         odd = kv.Pool(*(z(4, 2, 3, 16) for _ in range(3)))
         kv.append2(b, odd, kx, kx)
     with pytest.raises(native.SufHipError, match="d_work"):
-        kv.values2(b, cache.v, p, p, x, off, x, work=z(2))
+        long = kv.Batch(b.cu, b.kv_lens, b.pages, tokens=3, max_new=3, max_keys=1000)
+        kv.values2(long, cache.v, p, p, x, off, x, work=z(2))

@@ -284,6 +284,119 @@ def test_product_bad_pages_are_zeros(kind):
     eq(run_product(*case, kind), getattr(ref, kind)(*case), kind)
 
 
+@pytest.mark.parametrize("kind", ["scores", "values"])
+def test_product_wrong_lengths_stay_inside(kind):
+    """Lengths that no pages cover, the largest and negative ones: keys without
+    a page are zeros, rows of a sequence without keys are empty."""
+    case = product_case([3, 1, 2, 1], [70, 300, 20, 9], 8, 2, 3, 64, 1, kind)
+    c = case[0]
+    c.lens = [2 ** 31 - 1, 2 ** 31 - 1, -5, -2 ** 31]
+    eq(run_product(*case, kind, max_keys=300), getattr(ref, kind)(*case), kind)
+
+
+@pytest.mark.parametrize("kind", ["scores", "values"])
+def test_product_of_many_sequences(kind):
+    """More sequences than a workgroup has threads, some without new tokens."""
+    rng = np.random.default_rng(3)
+    lens = [int(v) for v in rng.integers(1, 30, 700)]
+    lens[::50] = [257] * 14
+    new = [int(v) for v in rng.integers(0, 3, 700)]
+    new = [min(n, m) for n, m in zip(new, lens)]
+    case = product_case(new, lens, 16, 1, 2, 16, 2, kind)
+    eq(run_product(*case, kind), getattr(ref, kind)(*case), kind)
+
+
+def sparse_rows(c, H, long):
+    """Offsets with rows only for the (head, token) pairs in `long`."""
+    rows = np.zeros(H * c.tokens, np.int64)
+    for (h, t), n in long.items():
+        rows[h * c.tokens + t] = n
+    return np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+
+
+@pytest.mark.parametrize("page", [16, 4])
+@pytest.mark.parametrize("new,hk,group,dim,hint", [(130, 1, 16, 16, 9000),    # an item a workgroup
+                                                   (130, 1, 16, 80, 9000),
+                                                   (1, 1, 2, 16, 256),        # even shares of five
+                                                   (1, 2, 2, 2, 256)])
+@pytest.mark.parametrize("extreme", [False, True])
+def test_values_long_sums(page, new, hk, group, dim, hint, extreme):
+    """More keys than int32 digit sums hold in one workgroup; extreme: every
+    digit of the opened operand and of party 0's mask share is -128."""
+    L = 8400 if new > 1 else 30000
+    rng = np.random.default_rng(dim + L)
+    c = ref.Case(rng, [new], [L], page, hk, dim)
+    H = hk * group
+    off = sparse_rows(c, H, {(0, 0): L, (H - 1, new - 1): L - 1, (H // 2, new // 2): 4097})
+    n = int(off[-1])
+    x, a = ([ref.words(rng, n) for _ in range(2)] for _ in range(2))
+    if extreme:
+        low = np.uint64(0x7f7f7f7f7f7f7f80)  # sum of -128 * 256^i
+        x[0][:], x[1][:], a[0][:] = low, 0, 0
+        a[1][:] = 0
+        c.pool[0][:], c.pool[1][:] = low, low
+    cc, out = ([ref.words(rng, c.tokens, H, dim) for _ in range(2)] for _ in range(2))
+    case = (c, H, off, x, a, cc, out)
+    eq(run_product(*case, "values", max_keys=hint), ref.values(*case), "values")
+
+
+def test_scores_extreme_digits():
+    """Every digit of the operands of one party is -128, in a wide head."""
+    rng = np.random.default_rng(2)
+    for new, dim in ((1, 256), (40, 128)):
+        c = ref.Case(rng, [new], [130], 16, 1, dim)
+        off = c.causal(2)
+        n = int(off[-1])
+        low = np.uint64(0x7f7f7f7f7f7f7f80)
+        x = [np.full((new, 2, dim), v, np.uint64) for v in (low, 0)]
+        a = [np.zeros((new, 2, dim), np.uint64) for _ in range(2)]
+        c.pool[0][:], c.pool[1][:] = low, low
+        cc, out = ([ref.words(rng, n) for _ in range(2)] for _ in range(2))
+        case = (c, 2, off, x, a, cc, out)
+        eq(run_product(*case, "scores"), ref.scores(*case), "scores")
+
+
+def test_long_cache_offsets_pass_32_bits():
+    """A pool whose words lie past 2^32 bytes, and past 2^31 words."""
+    pages, page, dim = 9000, 128, 2048 // 8
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("30 GiB of device memory wanted")
+    shape = (pages, 8, page, dim)  # 2.36e9 words, 18.9 GB: e, b0, b1 share them
+    e = torch.empty(shape, dtype=torch.int64, device="cuda")
+    rng = np.random.default_rng(1)
+    pool = kv.Pool(e, e, e)  # written once below, only read by the products
+    table = np.array([[pages - 1, 3, pages - 2]], np.int32)
+    c = ref.Case.__new__(ref.Case)
+    c.new, c.lens, c.page, c.kv_heads, c.dim, c.width = [1], [300], page, 8, dim, 3
+    c.table, c.pages, c.cu, c.tokens = table, pages, np.array([0, 1], np.int32), 1
+    words = {int(pg): ref.words(rng, 8, page, dim) for pg in table[0]}
+    for pg, w in words.items():
+        e[pg].copy_(dev(w))
+
+    class Pages(dict):
+        def __getitem__(self, key):
+            return words[int(key[0])][key[1:]]
+    c.pool = [Pages()] * 3
+    off = c.causal(8)
+    n = int(off[-1])
+    for kind, shapes in (("scores", ((1, 8, dim), (n,))), ("values", ((n,), (1, 8, dim)))):
+        x, a = ([ref.words(rng, *shapes[0]) for _ in range(2)] for _ in range(2))
+        cc, out = ([ref.words(rng, *shapes[1]) for _ in range(2)] for _ in range(2))
+        o = dev2(out)
+        op = kv.scores2 if kind == "scores" else kv.values2
+        op(batch_of(c), pool, dev2(x), dev2(a), dev2(cc), i32(off), o)
+        eq(o, getattr(ref, kind)(c, 8, off, x, a, cc, out), kind)
+    # The append's far words: the last place of the last page, which here all
+    # three arrays of the pool share, so any of its words may be left there.
+    m, k = ([ref.words(rng, 1, 8, dim) for _ in range(2)] for _ in range(2))
+    c.lens, c.table = [page], np.array([[pages - 1, 0, 0]], np.int32)
+    kv.append2(batch_of(c), pool, dev2(k), dev2(m))
+    got = u64(e[pages - 1, :, page - 1])
+    assert any(np.array_equal(got, w) for w in (m[0][0], m[1][0],
+                                                 k[0][0] + k[1][0] - m[0][0] - m[1][0]))
+    assert np.array_equal(u64(e[pages - 1, :, page - 2]), words[pages - 1][:, page - 2])
+
+
 def test_scores_of_a_view():
     """Queries inside the rows of a fused product, 8-byte aligned."""
     for lead, gap in ((0, 64), (1, 0), (0, 1)):

@@ -188,6 +188,9 @@ def test_products_refuse(name):
     a.heads, a.batch.tokens = 2 << 10, 1 << 20
     refused(name, a, "rows")
     a = product_args()
+    a.batch.seqs = (1 << 21) + 1
+    refused(name, a, "sequences times")
+    a = product_args()
     a.trunc = trunc(frac_bits=0)
     refused(name, a, "frac_bits")
     for kw in ({"seqs": 0}, {"tokens": 0}):
@@ -199,6 +202,7 @@ def test_products_refuse(name):
 def test_values2_needs_its_workspace():
     lib = native.load()
     a = product_args()
+    batch(a.batch, max_keys=1000)
     need = lib.sufhip_kv_values2_work_bytes(ctypes.byref(a.batch), ctypes.byref(a.pool), a.heads)
     assert need > 0
     for work, nb in ((None, need), (PTR, need - 1), (PTR + 8, need)):
