@@ -464,7 +464,7 @@ __device__ __forceinline__ int longest(const Row (&rows)[16]) {
 // run under them, so a wave has up to 24 KB in flight.
 
 template <bool kVec, bool kFull, bool kTrunc>
-__global__ void __launch_bounds__(256, kVec && !kTrunc ? 2 : 1)
+__global__ void __launch_bounds__(256, kVec ? 2 : 1)
     kv_scores2_few_kernel(ProductArgs a, int chunks) {
   extern __shared__ __align__(16) int8_t tiles[];
   __shared__ Row rows[16];
@@ -551,6 +551,7 @@ __global__ void __launch_bounds__(256, kVec && !kTrunc ? 2 : 1)
           const uint64_t z0 = here < 0 ? 0 : from_sums(acc[0], r);
           const uint64_t z1 = here < 0 ? 0 : from_sums(acc[1], r);
           put(a, at[r], z0 + cw[0][r], z1 + cw[1][r]);
+          if constexpr (kTrunc) __builtin_amdgcn_sched_barrier(0);
         }
         clear(acc);
         ++t;

@@ -1,6 +1,8 @@
 """Rotary positions, the append to a paged cache and the two products of
 attention over it, against plain numpy forms: bit-equal shares (everything is
 an integer mod 2^64), and every word that a call must not touch as it was."""
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -19,6 +21,11 @@ STATE = ol.mt64_bytes(3, ol.PRG_STATE_BYTES).tobytes()
 @pytest.fixture(scope="module", autouse=True)
 def _init():
     native.call("sufhip_init", 0)
+    yield
+    # Nothing of these tests' stays in the allocator: what a later test is
+    # handed, and so the size that is counted for it, depends on free blocks.
+    gc.collect()
+    torch.cuda.empty_cache()
 
 
 def dev2(pair):
