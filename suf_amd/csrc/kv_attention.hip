@@ -6,6 +6,8 @@
 // E and B_p read from the cache's pages.
 #include <hip/hip_runtime.h>
 
+#include <atomic>
+
 #include "digit_planes.hpp"
 #include "kv_device.hpp"
 #include "suf_hip.h"
@@ -1058,13 +1060,24 @@ namespace {
 bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 unsigned clip(int64_t v, int64_t most) { return unsigned(v < 1 ? 1 : (v < most ? v : most)); }
 
+// Compute units of the current device (256 without one: sizes asked for on a
+// host alone); asked of the runtime once a device.
 int cu_total() {
-  int cus = 256, dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0) {
     (void)hipGetLastError();
-    cus = 256;
+    return 256;
   }
+  if (dev < 64)
+    if (const int n = known[dev].load(std::memory_order_relaxed)) return n;
+  int cus = 0;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+      cus < 1) {
+    (void)hipGetLastError();
+    return 256;
+  }
+  if (dev < 64) known[dev].store(cus, std::memory_order_relaxed);
   return cus;
 }
 

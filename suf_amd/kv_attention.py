@@ -55,51 +55,68 @@ def _refuse(t, shape, d, what, name, dtype, dense):
     _fail(what, "%s is not usable" % name)
 
 
-# The calls below take a few microseconds each and a step makes many of them, so
-# a tensor is checked in one expression; _refuse finds the reason.
-
-def _ptr(t, shape, d, what, name, dtype=torch.int64):
-    """Address of a contiguous tensor on GPU d."""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and \
-            t.get_device() == d >= 0 and t.is_contiguous():
-        return t.data_ptr()
-    _refuse(t, shape, d, what, name, dtype, True)
-
-
-def _two(pair, what, name):
-    try:
-        t0, t1 = pair
-    except (TypeError, ValueError):
+def _refuse_pair(pair, shape, d, what, name, dense):
+    if not isinstance(pair, (tuple, list)) or len(pair) != 2:
         _fail(what, "%s must be a pair (party 0, party 1)" % name)
-    return t0, t1
+    for t in pair:
+        if not (isinstance(t, torch.Tensor) and t.dtype is torch.int64 and t.shape == shape and
+                t.get_device() == d and (not dense or t.is_contiguous())):
+            _refuse(t, shape, d, what, name, torch.int64, dense)
+    _fail(what, "%s is not usable" % name)
+
+
+# A step makes many calls of a few microseconds each, so a pair of tensors is
+# checked in one expression; the functions above find the reason.
+
+_I64 = torch.int64
+
+
+def _ptr(t, shape, d, what, name, dtype=_I64):
+    """Address of a contiguous tensor on GPU d (>= 0)."""
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == d and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(t, shape, d, what, name, dtype, True)
 
 
 def _ptr2(arr, pair, shape, d, what, name):
     """Both parties' contiguous tensors into a void*[2]."""
-    t0, t1 = _two(pair, what, name)
-    arr[0] = _ptr(t0, shape, d, what, name)
-    arr[1] = _ptr(t1, shape, d, what, name)
+    try:
+        t0, t1 = pair
+        if t0.dtype is _I64 and t1.dtype is _I64 and t0.shape == shape and t1.shape == shape and \
+                t0.get_device() == d and t1.get_device() == d and t0.is_contiguous() and \
+                t1.is_contiguous():
+            arr[0], arr[1] = t0.data_ptr(), t1.data_ptr()
+            return
+    except (AttributeError, TypeError, ValueError):
+        pass
+    _refuse_pair(pair, shape, d, what, name, True)
 
 
 def _rows(arr, pair, shape, d, what, name, written=False):
     """Both parties' [tokens, heads, dim] tensors into a void*[2]; their token
     and head stride."""
-    t0, t1 = _two(pair, what, name)
-    st = None
-    for p, t in ((0, t0), (1, t1)):
-        if not (isinstance(t, torch.Tensor) and t.dtype is torch.int64 and t.shape == shape and
-                t.get_device() == d >= 0):
-            _refuse(t, shape, d, what, name, torch.int64, False)
-        s = t.stride()
-        if s[2] != 1 and shape[2] > 1:
+    try:
+        t0, t1 = pair
+        ok = t0.dtype is _I64 and t1.dtype is _I64 and t0.shape == shape and t1.shape == shape and \
+            t0.get_device() == d and t1.get_device() == d
+    except (AttributeError, TypeError, ValueError):
+        ok = False
+    if not ok:
+        _refuse_pair(pair, shape, d, what, name, False)
+    st = t0.stride()
+    if st != t1.stride():
+        if shape[2] > 1 and t1.stride()[2] != 1:
             _fail(what, "the values of a head of %s must be neighbours" % name)
-        if st is None:
-            st = s
-        elif st[:2] != s[:2] and t.numel():
+        if st[:2] != t1.stride()[:2] and t0.numel():
             _fail(what, "both parties' %s must have the same strides" % name)
-        arr[p] = t.data_ptr()
-    if written and any(n > 1 and v == 0 for n, v in zip(shape[:2], st)):
+    if st[2] != 1 and shape[2] > 1:
+        _fail(what, "the values of a head of %s must be neighbours" % name)
+    if written and ((st[0] == 0 and shape[0] > 1) or (st[1] == 0 and shape[1] > 1)):
         _fail(what, "rows of %s must not overlap" % name)
+    arr[0], arr[1] = t0.data_ptr(), t1.data_ptr()
     return st[0], st[1]
 
 
@@ -216,17 +233,18 @@ class Pool:
     page_tokens, dim] on the GPU (the open value - b, both parties' shares of
     b); page_tokens a power of two."""
 
+    __slots__ = ("arg", "e", "b", "device", "shape", "kv_heads", "dim")
+
     def __init__(self, e, b0, b1):
         d, shape = _device(e, "Pool", "e"), e.shape
         if len(shape) != 4:
             _fail("Pool", "the arrays must be [pages, kv_heads, page_tokens, dim]")
-        self.arg = native.KvPool(_ptr(e, shape, d, "Pool", "e"),
-                                 (_ptr(b0, shape, d, "Pool", "b0"),
-                                  _ptr(b1, shape, d, "Pool", "b1")),
-                                 shape[0], shape[2], shape[1], shape[3])
-        self.e, self.b, self.device = e, (b0, b1), d
-        self.shape = shape
-        self.kv_heads, self.dim = shape[1], shape[3]
+        p = self.arg = native.KvPool()
+        p.e = _ptr(e, shape, d, "Pool", "e")
+        _ptr2(p.b, (b0, b1), shape, d, "Pool", "b")
+        p.pages, self.kv_heads, p.page_tokens, self.dim = shape
+        p.kv_heads, p.dim = self.kv_heads, self.dim
+        self.e, self.b, self.device, self.shape = e, (b0, b1), d, shape
 
 
 class Batch:
