@@ -33,18 +33,6 @@ struct ProductArgs {
   uint64_t mask;
 };
 
-// The packed elements of row (h, t): where they start and how many of them
-// have a key (kv keys in the sequence).
-struct Span {
-  int first, len;
-};
-__device__ __forceinline__ Span span_of(const ProductArgs& a, int h, int t, int kv) {
-  const int64_t r = int64_t(h) * a.b.tokens + t;
-  const int64_t f = a.offsets[r], l = int64_t(a.offsets[r + 1]) - f;
-  if (f < 0 || l <= 0 || f + l > a.n) return {0, 0};
-  return {int(f), int(l < kv ? l : kv)};
-}
-
 // Both parties' finished values of output element i: to the outputs, or the
 // open through the truncation gate.
 template <bool kTrunc>
@@ -235,29 +223,25 @@ __device__ __forceinline__ void clear(v4i (&acc)[2][kDigitPlanes]) {
 struct Seq {
   int s, hk, t0, rows, kv;
 };
-__device__ __forceinline__ int keys_of(const ProductArgs& a, int s) {
-  const int kv = a.b.lens[s];
-  return int64_t(kv) < a.n ? kv : int(a.n);
-}
 __device__ __forceinline__ Seq seq_of_head(const ProductArgs& a, int s, int hk) {
+  const int lo = a.b.cu[s], hi = a.b.cu[s + 1], kv = a.b.lens[s];
   Seq q;
   q.s = s;
   q.hk = hk;
-  const int lo = a.b.cu[q.s], hi = a.b.cu[q.s + 1];
-  q.t0 = lo > 0 ? lo : 0;
-  const int t1 = hi < a.b.tokens ? hi : a.b.tokens;
-  q.rows = t1 > q.t0 ? (t1 - q.t0) * a.group : 0;
-  q.kv = keys_of(a, s);
+  q.t0 = max(lo, 0);
+  q.rows = max(min(hi, a.b.tokens) - q.t0, 0) * a.group;
+  q.kv = int(min(int64_t(kv), a.n));
   return q;
 }
-
 __device__ __forceinline__ Seq seq_at(const ProductArgs& a, int z) {
   const int s = z / a.pool.heads;
   return seq_of_head(a, s, z - s * a.pool.heads);
 }
 
-// Row m of a sequence: its token, head and packed elements (m past the last
-// row: token -1, no elements; row_of: without the elements).
+// Row m of a sequence: its token, its head, where its packed elements start
+// and how many of them have a key (m past the last row: token -1, no
+// elements; row_of: without the elements).  A row that does not lie within
+// the packed elements has none.
 struct Row {
   int t, h, first, len;
 };
@@ -266,13 +250,48 @@ __device__ __forceinline__ Row row_of(const ProductArgs& a, const Seq& q, int m)
   const int tl = int(div_by(a.by_group, uint32_t(m)));
   return {q.t0 + tl, q.hk * a.group + (m - tl * a.group), 0, 0};
 }
-__device__ __forceinline__ Row row_at(const ProductArgs& a, const Seq& q, int m) {
-  Row r = row_of(a, q, m);
-  if (r.t < 0) return r;
-  const Span sp = span_of(a, r.h, r.t, q.kv);
-  r.first = sp.first;
-  r.len = sp.len;
+// row_at in two halves: the row's offsets on their way, then its elements.
+struct RowLoad {
+  Row r;
+  int from, to;
+};
+__device__ __forceinline__ RowLoad load_row(const ProductArgs& a, const Seq& q, int m) {
+  RowLoad w{row_of(a, q, m), 0, 0};
+  const int64_t i = w.r.t < 0 ? 0 : int64_t(w.r.h) * a.b.tokens + w.r.t;
+  w.from = a.offsets[i];
+  w.to = a.offsets[i + 1];
+  return w;
+}
+__device__ __forceinline__ Row row_from(const ProductArgs& a, const Seq& q, const RowLoad& w) {
+  Row r = w.r;
+  const int64_t f = w.from, l = int64_t(w.to) - f;
+  if (r.t < 0 || f < 0 || l <= 0 || f + l > a.n) return r;
+  r.first = w.from;
+  r.len = int(l < q.kv ? l : q.kv);
   return r;
+}
+__device__ __forceinline__ Row row_at(const ProductArgs& a, const Seq& q, int m) {
+  return row_from(a, q, load_row(a, q, m));
+}
+
+// A key's page number on its way, then the first word of its head in the pool
+// (-1: no page holds it).
+struct Spot {
+  int64_t key;
+  int page;
+};
+__device__ __forceinline__ bool has_entry(const ProductArgs& a, const Seq& q, int64_t key) {
+  return key < q.kv && (key >> a.pool.shift) < a.b.max_pages;
+}
+__device__ __forceinline__ Spot load_spot(const ProductArgs& a, const Seq& q, int64_t key) {
+  const int64_t at = has_entry(a, q, key) ? key >> a.pool.shift : 0;
+  return {key, a.b.table[int64_t(q.s) * a.b.max_pages + at]};
+}
+__device__ __forceinline__ int64_t place_at(const ProductArgs& a, const Seq& q, const Spot& w) {
+  const bool ok = has_entry(a, q, w.key) && unsigned(w.page) < unsigned(a.pool.pages);
+  const int64_t row = ((int64_t(w.page) * a.pool.heads + q.hk) << a.pool.shift) +
+                      (w.key & ((1 << a.pool.shift) - 1));
+  return ok ? row * a.pool.dim : -1;
 }
 
 // ---- even shares ----
@@ -294,10 +313,8 @@ __device__ __forceinline__ int tiles_of(int kv) {
   return kv > kKeyTile ? (kv + kKeyTile - 1) / kKeyTile : 1;
 }
 __device__ __forceinline__ int64_t units_of(const ProductArgs& a, int s, int blocks) {
-  const int lo = a.b.cu[s], hi = a.b.cu[s + 1];
-  const int t0 = lo > 0 ? lo : 0, t1 = hi < a.b.tokens ? hi : a.b.tokens;
-  const int64_t row_tiles = t1 > t0 ? ((t1 - t0) * a.group + 15) / 16 : 0;
-  return row_tiles * blocks * a.pool.heads * (tiles_of(keys_of(a, s)) + 1);
+  const Seq q = seq_of_head(a, s, 0);
+  return int64_t((q.rows + 15) / 16) * blocks * a.pool.heads * (tiles_of(q.kv) + 1);
 }
 
 // Sums before each of the 256 threads' sequences into pre[0 .. 256] (a
@@ -484,29 +501,32 @@ __global__ void __launch_bounds__(256, kVec ? 2 : 1)
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
     const int l = tid & 63, g = l >> 4, n = l & 15;
-    // The first keys' pages and words, the rows' words and the rows' places
-    // are on their way together.
+    __syncthreads();
+    // The first keys' pages, the rows' words and the rows' offsets are on
+    // their way together, the keys' words with the writes to LDS.
     const int tb = pc.tile;
-    const auto place_of = [&](int t) -> int64_t {
-      const int key = t * kKeyTile + 16 * w + n;
-      return key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
+    const auto spot_of = [&](int t) {
+      return load_spot(a, q, int64_t(t) * kKeyTile + 16 * w + n);
     };
-    int64_t here = place_of(tb), next = place_of(tb + 1);
+    const Spot here = spot_of(tb);
+    Spot next = spot_of(tb + 1);
+    const RowLoad spans = load_row(a, q, 16 * pc.rt + n);
+    Raw<4> first{};
+    const Row stage = row_of(a, q, 16 * pc.rt + (tid >> 4));
+    load_raw<4, kVec, kFull>(a, stage, 0, tid & 15, first);
+    int64_t place = place_at(a, q, here);
     uint64_t raw[3][16];
     const auto issue = [&](int k, int64_t place, int c) {
       const uint64_t* src = k == 0 ? a.pool.b[0] : k == 1 ? a.pool.b[1] : a.pool.e;
       load_keys<kVec, kFull>(src + (place < 0 ? 0 : place) + 64 * c, g, dim - 64 * c, raw[k]);
     };
-    const Row stage = row_of(a, q, 16 * pc.rt + (tid >> 4));
-    __syncthreads();
-    if (tid < 16) rows[tid] = row_at(a, q, 16 * pc.rt + tid);
-    for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) issue(k, place, 0);
+    if (tid < 16) rows[tid] = row_from(a, q, spans);
+    put_raw<4>(tiles, tid >> 4, tid & 15, first);
+    for (int c = 1; c < chunks; ++c) {
       Raw<4> v{};
       load_raw<4, kVec, kFull>(a, stage, c, tid & 15, v);
-      if (c == 0) {
-#pragma unroll
-        for (int k = 0; k < 3; ++k) issue(k, here, 0);
-      }
       put_raw<4>(tiles + c * kTileBytes, tid >> 4, tid & 15, v);
     }
     __syncthreads();
@@ -518,8 +538,10 @@ __global__ void __launch_bounds__(256, kVec ? 2 : 1)
     int t = tb, c = 0;
     for (int u = (te - tb) * chunks; u > 0; --u) {
       const bool last = c + 1 == chunks;
-      const int64_t np = last ? next : here;
+      const int64_t np = last ? place_at(a, q, next) : place;
       const int nc = last ? 0 : c + 1;
+      // Read again for each chunk: no branch, and older than the loads below.
+      next = spot_of(last ? t + 2 : t + 1);
       const int8_t* tile = tiles + c * kTileBytes;
       const int key = t * kKeyTile + 16 * w + n;
       uint64_t cw[2][4];
@@ -550,15 +572,14 @@ __global__ void __launch_bounds__(256, kVec ? 2 : 1)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           if (at[r] < 0) continue;
-          const uint64_t z0 = here < 0 ? 0 : from_sums(acc[0], r);
-          const uint64_t z1 = here < 0 ? 0 : from_sums(acc[1], r);
+          const uint64_t z0 = place < 0 ? 0 : from_sums(acc[0], r);
+          const uint64_t z1 = place < 0 ? 0 : from_sums(acc[1], r);
           put(a, at[r], z0 + cw[0][r], z1 + cw[1][r]);
           if constexpr (kTrunc) __builtin_amdgcn_sched_barrier(0);
         }
         clear(acc);
         ++t;
-        here = next;
-        next = place_of(t + 1);
+        place = np;
       }
     }
   }
@@ -587,7 +608,7 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
   for (int64_t first_key = int64_t(blockIdx.z) * kKeys; first_key < q.kv;
        first_key += int64_t(gridDim.z) * kKeys) {
     const int k0 = int(first_key), key = k0 + 16 * w + n;
-    const int64_t place = key < q.kv ? kv_place(a.b, a.pool, q.s, q.hk, key) : -1;
+    const int64_t place = place_at(a, q, load_spot(a, q, key));
     v4i K[kHeld][3][kDigitPlanes];
     // The lane's offsets are formed again for each key tile: kept over the
     // loop they would take registers that it does not have.
