@@ -549,14 +549,12 @@ class AttentionStep:
         self.positions = dev_i32(np.concatenate([np.arange(L - k, L)
                                                  for k, L in zip(new, lens)]), device)
         self.work = values_work(b, cache.v, H)
-        # The new words' masks go to their pages at once (the append of zeros
-        # leaves -mask for E), so that the products below see all masks.
+        # The new words' masks go to their pages at once, so that the products
+        # below see all masks: appended as the values too, they leave E = 0
+        # there, which says nothing of them.
         self.k_mask = _shares(deal, (T, Hk, D), device)
         self.v_mask = _shares(deal, (T, Hk, Dv), device)
-        none = tuple(torch.zeros((T, Hk, max(D, Dv)), dtype=torch.int64, device=device)
-                     for _ in range(2))
-        append2(b, cache.k, tuple(t[..., :D] for t in none), self.k_mask, cache.v,
-                tuple(t[..., :Dv] for t in none), self.v_mask)
+        append2(b, cache.k, self.k_mask, self.k_mask, cache.v, self.v_mask, self.v_mask)
         self.q_a, self.p_a = _shares(deal, (T, H, D), device), _shares(deal, (n,), device)
         self.s_c = self._triple(scores2, cache.k, self.q_a, (n,), deal, {})
         self.o_c = self._triple(values2, cache.v, self.p_a, (T, H, Dv), deal, {"work": self.work})

@@ -177,6 +177,20 @@ def test_a_key_is_opened_under_its_own_mask():
     assert not bool((opens[0] == opens[1]).any())
 
 
+def test_dealing_opens_nothing():
+    """The masks are in their pages before the step's values are, beside an E
+    that does not depend on them."""
+    cache = kv.PagedCache(4, 4, 2, 8, 6)
+    att = kv.CachedAttention(cache, 2, STATE, 16)
+    s = cache.open()
+    step = att.deal([s], [5])
+    for pool, mask in ((cache.k, step.k_mask), (cache.v, step.v_mask)):
+        assert not bool(pool.e.any())
+        for p in (0, 1):
+            rows = torch.cat([pool.b[p][i].transpose(0, 1) for i in cache.seqs[s]["pages"]])
+            assert torch.equal(rows[:5], mask[p]) and not bool(rows[5:].any())
+
+
 def test_cache_bookkeeping():
     cache = kv.PagedCache(6, 4, 1, 8)
     att = kv.CachedAttention(cache, 2, STATE, 20)
