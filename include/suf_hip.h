@@ -943,7 +943,7 @@ int sufhip_rotary2(const sufhip_rotary2_args* args, void* stream);
 /* The packed new tokens of a batch of sequences and the pages of their
  * caches.  Sequence s's new tokens are rows d_cu_tokens[s] ..
  * d_cu_tokens[s + 1] - 1 of every token array ([seqs + 1], not decreasing);
- * rows in no sequence are padding: nothing of them is read or written.
+ * rows in no sequence are padding: nothing of them is used or written.
  * d_kv_lens [seqs]: keys of each sequence, its new tokens (the last ones)
  * included.  d_pages [seqs][max_pages]: the pool page of each page_tokens
  * keys; entries past a sequence's length are not used.  A page number outside
@@ -977,11 +977,12 @@ typedef struct sufhip_kv_pool {
  * (e.g. part[0] rotated, part[1] not); a part with pool.e = NULL is absent.
  * rot, unless its table is NULL and it has no positions: the rows are rotated
  * on the way, by d_positions [tokens] if given, else by their places in their
- * sequences; outside the table's positions nothing is written.  trunc (optional): the (rotated) rows are
- * truncated before the open, by the gate fed with x_0 + x_1 + mask_trunc; its
- * y[p] receive the truncated shares [tokens][kv_heads][dim], or are both NULL.
- * Places not appended to keep their contents.  A place written twice by one
- * call (a page listed twice) holds one of the writes or a mix. */
+ * sequences; outside the table's positions nothing is written.  trunc
+ * (optional): the (rotated) rows are truncated before the open, by the gate
+ * fed with x_0 + x_1 + trunc_mask; its y[p] receive the truncated shares
+ * [tokens][kv_heads][dim], or are both NULL.  At most 2^30 pairs of values a
+ * part.  Places not appended to keep their contents.  A place written twice by
+ * one call (a page listed twice) holds one of the writes or a mix. */
 typedef struct sufhip_kv_append_part {
   sufhip_rows2 x;
   const uint64_t* mask[2];
@@ -1014,7 +1015,8 @@ int sufhip_kv_append2(const sufhip_kv_append2_args* args, void* stream);
  * with D = (x_0 - a_0) + (x_1 - a_1) opened on the way.  scores: x.p with
  * strides, a[p] [tokens][heads][dim].  values: x.p packed, its strides not
  * used.  An empty row's values are C_p.  n: packed elements (at most
- * 2^31 - 1).  trunc (optional): the open Z_0 + Z_1 + mask feeds this prepared
+ * 2^31 - 256); at most 2^30 rows (tokens times heads), and 2^22 sequences
+ * times cached heads.  The pool has at least one page.  trunc (optional): the open Z_0 + Z_1 + mask feeds this prepared
  * GapARS table gate (no addend), whose outputs y are written in place of out.
  * d_work (values): sufhip_kv_values2_work_bytes() bytes, 16-byte aligned,
  * used by this call only until it ends; 0 bytes: none needed. */

@@ -1031,7 +1031,9 @@ int product_args(const sufhip_kv_product2_args* args, bool values, const char* w
   if (g.pool.pages < 1) return kv_fail(what, "the pool has no pages");
   if (g.heads < 1 || g.heads % g.pool.kv_heads)
     return kv_fail(what, "heads must be a multiple of the pool's kv_heads");
-  if (g.n > 0x7fffffffu) return kv_fail(what, "at most 2^31 - 1 packed elements");
+  // Two chunks past the last key are still numbered in 32 bits.
+  if (g.n > (size_t(1) << 31) - 256)
+    return kv_fail(what, "at most 2^31 - 256 packed elements");
   const size_t rows = size_t(a.b.tokens) * size_t(g.heads);
   if (rows > (1u << 30) || size_t(a.b.seqs) * size_t(a.pool.heads) > (1u << 22))
     return kv_fail(what, "at most 2^30 rows, and 2^22 sequences times cached heads");

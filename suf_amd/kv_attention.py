@@ -33,9 +33,11 @@ import torch
 
 from . import native
 from .softmax import SoftmaxBlock
-from .tasks import Dealer, Trunc, dev, dev_i32, prepare_batch
+from .tasks import TABLE_BITS, Dealer, Trunc, dev, dev_i32, prepare_batch
 
 M64 = (1 << 64) - 1
+I32 = (1 << 31) - 1       # the library counts tokens, heads and pages in 32 bits
+MAX_PACKED = (1 << 31) - 256
 
 
 # ---- arguments ----
@@ -144,7 +146,7 @@ def _call(name, args, d):
         native.check(rc, name)
 
 
-def _epilogue(args, trunc, out, n, what):
+def _epilogue(args, trunc, out, n, d, what):
     """trunc: a prepared tasks.Trunc whose outputs go to `out`."""
     if trunc is None:
         return None
@@ -152,6 +154,8 @@ def _epilogue(args, trunc, out, n, what):
         _fail(what, "the truncation must be a GapARS gate of at most 14 bits")
     if trunc.n < n:
         _fail(what, "the truncation is for %d elements, not %d" % (trunc.n, n))
+    if trunc.work[0].get_device() != d:
+        _fail(what, "the truncation is on another device")
     epi = trunc.epilogue(out)
     args.trunc = ctypes.pointer(epi)
     return epi
@@ -242,6 +246,8 @@ class Pool:
         p = self.arg = native.KvPool()
         p.e = _ptr(e, shape, d, "Pool", "e")
         _ptr2(p.b, (b0, b1), shape, d, "Pool", "b")
+        if max(shape) > I32:
+            _fail("Pool", "at most 2^31 - 1 pages")
         p.pages, self.kv_heads, p.page_tokens, self.dim = shape
         p.kv_heads, p.dim = self.kv_heads, self.dim
         self.e, self.b, self.device, self.shape = e, (b0, b1), d, shape
@@ -259,6 +265,8 @@ class Batch:
         d = _device(kv_lens, "Batch", "kv_lens")
         if kv_lens.dim() != 1 or pages.dim() != 2:
             _fail("Batch", "kv_lens must be [seqs], pages [seqs, max_pages]")
+        if not (0 <= tokens <= I32 and 0 <= max_new <= I32 and 0 <= max_keys <= I32):
+            _fail("Batch", "tokens, max_new and max_keys must be in [0, 2^31)")
         seqs, width = kv_lens.shape[0], pages.shape[1]
         b = self.arg = native.KvBatch()
         b.d_cu_tokens = _ptr(cu, (seqs + 1,), d, "Batch", "cu", torch.int32)
@@ -286,12 +294,15 @@ def rotary2(x, rotary, positions, out=None, trunc=None):
     """Rotates both parties' shares x (pair of int64 [tokens, heads, dim], any
     token and head strides) by the tokens' positions (int32 [tokens]; a token
     outside the table is padding and its rows of out stay).  out: a pair like
-    x, which may be x itself, or None for new ones (zeros in padding rows).  trunc: a prepared
-    tasks.Trunc the rotated values go through.  Returns out."""
+    x, which may be x itself, or None for new ones (zeros in padding rows).
+    trunc: a prepared tasks.Trunc the rotated values go through.  Returns
+    out."""
     what = "rotary2"
     d, shape = _device(x[0], what, "x"), x[0].shape
     if len(shape) != 3 or shape[2] != rotary.dim:
         _fail(what, "x must be [tokens, heads, %d]" % rotary.dim)
+    if shape[0] > I32 or shape[1] > I32:
+        _fail(what, "at most 2^31 - 1 tokens and heads")
     if rotary.device != d:
         _fail(what, "the table is on another device than x")
     if out is None:
@@ -304,7 +315,7 @@ def rotary2(x, rotary, positions, out=None, trunc=None):
     a.d_positions = _ptr(positions, shape[:1], d, what, "positions", torch.int32)
     a.out_token_stride, a.out_head_stride = _rows(a.out, out, shape, d, what, "out", written=True)
     if trunc is not None:
-        epi = _epilogue(a, trunc, out, x[0].numel(), what)
+        epi = _epilogue(a, trunc, out, x[0].numel(), d, what)
         a.mask = trunc.mask & M64
     _call("sufhip_rotary2", a, d)
     return out
@@ -331,7 +342,7 @@ def _append_part(part, batch, pool, x, mask, rotary, positions, trunc, what, nam
     if y is not None:
         for t in y:
             _ptr(t, shape, d, what, "the truncated shares")
-    epi = _epilogue(part, gate, y if y is not None else x, x[0].numel(), what)
+    epi = _epilogue(part, gate, y if y is not None else x, x[0].numel(), d, what)
     if y is None:
         epi.y[0] = epi.y[1] = None
         part.trunc = ctypes.pointer(epi)
@@ -361,6 +372,8 @@ def append2(batch, k_pool, k, k_mask, v_pool=None, v=None, v_mask=None, rotary=N
 
 def _product(batch, pool, offsets, heads, what):
     a = native.KvProduct2Args()
+    if heads > I32:
+        _fail(what, "at most 2^31 - 1 heads")
     a.batch, a.pool, a.heads = batch.arg, pool.arg, heads
     if pool.device != batch.device:
         _fail(what, "the pool and the batch are on different devices")
@@ -390,7 +403,7 @@ def scores2(batch, pool, q, a, c, offsets, out, trunc=None):
     _ptr2(g.c, c, (n,), d, what, "c")
     _ptr2(g.out, out, (n,), d, what, "out")
     if trunc is not None:
-        epi = _epilogue(g, trunc, out, n, what)
+        epi = _epilogue(g, trunc, out, n, d, what)
         g.mask = trunc.mask & M64
     _call("sufhip_kv_scores2", g, d)
     return out
@@ -433,7 +446,7 @@ def values2(batch, pool, p, a, c, offsets, out, trunc=None, work=None):
     _ptr2(g.c, c, shape, d, what, "c")
     _ptr2(g.out, out, shape, d, what, "out")
     if trunc is not None:
-        epi = _epilogue(g, trunc, out, out[0].numel(), what)
+        epi = _epilogue(g, trunc, out, out[0].numel(), d, what)
         g.mask = trunc.mask & M64
     if work is None:
         work = values_work(batch, pool, shape[1])
@@ -516,6 +529,8 @@ class CachedAttention:
         dim = cache.k.dim
         if heads % cache.kv_heads:
             _fail("CachedAttention", "heads must be a multiple of the cache's %d" % cache.kv_heads)
+        if not (0 < frac_bits <= TABLE_BITS and 0 < table_bits <= TABLE_BITS):
+            _fail("CachedAttention", "frac_bits and table_bits must be in [1, %d]" % TABLE_BITS)
         self.cache, self.heads, self.f, self.fc = cache, heads, frac_bits, table_bits
         self.prg_state = bytes(prg_state)
         self.max_positions = max_positions
@@ -530,6 +545,9 @@ class CachedAttention:
             _fail("CachedAttention.deal", "every sequence needs a new token")
         if max(self.cache.length(s) + n for s, n in zip(seqs, new)) > self.max_positions:
             _fail("CachedAttention.deal", "a sequence grows past max_positions")
+        keys = sum(n * self.cache.length(s) + n * (n + 1) // 2 for s, n in zip(seqs, new))
+        if self.heads * keys > MAX_PACKED:
+            _fail("CachedAttention.deal", "more than 2^31 - 256 scores in one step")
         return AttentionStep(self, seqs, new)
 
 

@@ -40,6 +40,10 @@ def whole(pair):
     return (u64(pair[0]) + u64(pair[1])).view(np.int64)
 
 
+def i32(a):
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+
 class Plain:
     """The keys and values of every sequence in the clear, and the stages."""
 
@@ -213,6 +217,68 @@ def test_cache_bookkeeping():
     assert len(cache.free) == 5 and a not in cache.seqs
     with pytest.raises(ValueError, match="multiple"):
         kv.CachedAttention(kv.PagedCache(1, 1, 2, 8), 3, STATE, 4)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Counts that the library would take modulo 2^32."""
+    z = lambda *n: torch.zeros(n, dtype=torch.int64, device="cuda")  # noqa: E731
+    cache = kv.PagedCache(4, 4, 1, 8)
+    s = cache.open()
+    b = cache.extend([s], [1])
+    for kw in ({"tokens": 1 << 32}, {"max_new": 1 << 31}, {"max_keys": 1 << 31}, {"tokens": -1}):
+        with pytest.raises(ValueError, match="2\\^31"):
+            kv.Batch(b.cu, b.kv_lens, b.pages, **dict({"tokens": 1, "max_new": 1, "max_keys": 1},
+                                                      **kw))
+    with pytest.raises(ValueError, match="2\\^31"):
+        kv.Pool(*(z(1 << 32, 0, 4, 8) for _ in range(3)))
+    r = kv.Rotary.build(8, 4)
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for shape in ((1, 1 << 32, 8), (1 << 32, 1, 8)):
+        x = tuple(z(1, 1, 8).expand(shape) for _ in range(2))
+        with pytest.raises(ValueError, match="2\\^31"):
+            kv.rotary2(x, r, pos.expand(shape[0]), out=x)
+    x = tuple(z(1, 1, 8).expand(1, 1 << 32, 8) for _ in range(2))
+    with pytest.raises(ValueError, match="2\\^31"):
+        kv.scores2(b, cache.k, x, x, (z(1), z(1)), pos, (z(1), z(1)))
+
+
+def test_a_step_of_too_many_scores_changes_nothing():
+    n = 1 << 16  # n (n + 1) / 2 scores a head
+    cache = kv.PagedCache(n // 64, 64, 1, 2)
+    att = kv.CachedAttention(cache, 1, STATE, n)
+    s = cache.open()
+    with pytest.raises(ValueError, match="2\\^31"):
+        att.deal([s], [n])
+    assert cache.length(s) == 0 and len(cache.free) == n // 64
+    for bits in ({"frac_bits": 0}, {"frac_bits": 15}, {"table_bits": 0}, {"table_bits": 15}):
+        with pytest.raises(ValueError, match="bits"):
+            kv.CachedAttention(cache, 1, STATE, 4, **bits)
+
+
+class OtherDevice:
+    """A prepared gate whose table is not on the tensors' GPU."""
+    n, mask, work = 1 << 20, 0, [torch.zeros(2, dtype=torch.int64)] * 2
+
+    def has_table(self):
+        return True
+
+    def epilogue(self, y):
+        raise AssertionError("used")
+
+
+def test_gates_on_another_device_are_refused():
+    cache = kv.PagedCache(4, 4, 1, 8)
+    s = cache.open()
+    b = cache.extend([s], [1])
+    z = lambda *n: torch.zeros(n, dtype=torch.int64, device="cuda")  # noqa: E731
+    x, p, off = (z(1, 1, 8), z(1, 1, 8)), (z(1), z(1)), i32([0, 1])
+    gate = OtherDevice()
+    for call in (lambda: kv.rotary2(x, kv.Rotary.build(8, 4), i32([0]), trunc=gate),
+                 lambda: kv.append2(b, cache.k, x, x, k_trunc=gate),
+                 lambda: kv.scores2(b, cache.k, x, x, p, off, p, trunc=gate),
+                 lambda: kv.values2(b, cache.v, p, p, x, off, x, trunc=gate)):
+        with pytest.raises(ValueError, match="another device"):
+            call()
 
 
 def test_calls_refuse_wrong_tensors():

@@ -199,6 +199,17 @@ def test_products_refuse(name):
         assert getattr(native.load(), name)(ctypes.byref(a), None) == 0
 
 
+@pytest.mark.parametrize("name", ["sufhip_kv_scores2", "sufhip_kv_values2"])
+def test_products_number_keys_in_32_bits(name):
+    """Two chunks of 64 keys past the last one are numbered too."""
+    a = product_args()
+    batch(a.batch, tokens=0)
+    a.n = (1 << 31) - 256
+    assert getattr(native.load(), name)(ctypes.byref(a), None) == 0
+    a.n += 1
+    refused(name, a, "packed elements")
+
+
 def test_values2_needs_its_workspace():
     lib = native.load()
     a = product_args()
