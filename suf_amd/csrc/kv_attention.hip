@@ -477,6 +477,14 @@ __device__ __forceinline__ int longest(const Row (&rows)[16]) {
   return __builtin_amdgcn_readfirstlane(most);
 }
 
+// The shortest.
+__device__ __forceinline__ int shortest(const Row (&rows)[16]) {
+  int least = rows[0].len;
+#pragma unroll
+  for (int r = 1; r < 16; ++r) least = rows[r].len < least ? rows[r].len : least;
+  return __builtin_amdgcn_readfirstlane(least);
+}
+
 // Few rows: a workgroup keeps one row tile in LDS and streams its units of
 // the keys.  Bound by HBM: an array's 16 words a lane are turned into digits,
 // the next unit's loads leave into the same registers, and the matrix cores
@@ -720,6 +728,8 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
 struct ValuesArgs {
   ProductArgs p;
   int blocks;        // column blocks
+  int8_t* planes;    // many rows: the values' digits (kPlanesBytes), or null
+  int room;          // many rows: key tiles a sequence has digits for
   uint64_t* part;    // few rows: two slots of sums a workgroup
   int4* info;        // few rows: [tokens * heads][blocks]
   uint64_t* out[2];  // the values, before a truncation if one follows
@@ -885,8 +895,156 @@ __device__ __forceinline__ bool values_run(const ProductArgs& a, const Seq& q, c
   return flushed;
 }
 
+// The values' digits, formed once for all row tiles: 64 keys of 16 columns are
+// the planes of b_0, b_1 and E (plane i of array k at (8 k + i) KB), 16 bytes a
+// lane in the lanes' order.  Keys without a page are zeros.
+constexpr int kPlanesBytes = 3 * kDigitPlanes * 1024;
+__device__ __forceinline__ int8_t* planes_at(const ValuesArgs& va, int z, int tile, int c16) {
+  const int per = (va.p.pool.dim + 15) / 16;
+  return va.planes + ((int64_t(z) * va.room + tile) * per + c16) * kPlanesBytes;
+}
+
+__global__ void __launch_bounds__(256, 2) kv_values2_digits_kernel(ValuesArgs va) {
+  const ProductArgs& a = va.p;
+  const int l = threadIdx.x & 63, g = l >> 4, n = l & 15;
+  const int c16 = 4 * int(blockIdx.y) + __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int dim = a.pool.dim;
+  if (16 * c16 >= dim) return;
+  const Seq q = seq_at(a, int(blockIdx.x));
+  const int tiles = tiles_of(q.kv);
+  if (q.rows == 0 || q.kv <= 0 || tiles > va.room) return;
+  const int col = 16 * c16 + n < dim ? 16 * c16 + n : 0;
+  for (int t = blockIdx.z; t < tiles; t += gridDim.z) {
+    int64_t place[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      place[i] = place_at(a, q, load_spot(a, q, t * kKeyTile + 16 * (i & 3) + 4 * (i >> 2) + g));
+    int8_t* to = planes_at(va, int(blockIdx.x), t, c16) + 16 * l;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const uint64_t* src = k == 2 ? a.pool.e : a.pool.b[k];
+      uint64_t v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = src[(place[i] < 0 ? 0 : place[i]) + col];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = place[i] < 0 ? 0 : v[i];
+      v4i y[kDigitPlanes];
+      digits_of16(v, y);
+#pragma unroll
+      for (int i = 0; i < kDigitPlanes; ++i)
+        *reinterpret_cast<v4i*>(to + (8 * k + i) * 1024) = y[i];
+    }
+  }
+}
+
+// values_run over digits that are there: from `from` (the wave's planes of the
+// first chunk, `step` bytes a chunk).
+template <int kWaves>
+__device__ __forceinline__ bool planes_run(const ProductArgs& a, const Row (&rows)[16],
+                                           int8_t (*tiles)[kTileBytes], uint64_t* sums,
+                                           const int8_t* from, int step, int c1,
+                                           v4i (&acc)[2][kDigitPlanes]) {
+  constexpr int kN = 16 / kWaves;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int l = tid & 63;
+  const uint32_t lane = 16 * uint32_t(l);
+  const int row = tid / (64 / kN), part = tid % (64 / kN);
+  bool flushed = false;
+  clear(acc);
+  v4i y[3][kDigitPlanes];
+  const auto issue = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < kDigitPlanes; ++i)
+      y[k][i] = *reinterpret_cast<const v4i*>(from + (8 * k + i) * 1024 + lane);
+  };
+#pragma unroll
+  for (int k = 0; k < 3; ++k) issue(k);
+  __syncthreads();
+  const int chunks = (longest(rows) + kKeyTile - 1) / kKeyTile;
+  c1 = c1 < chunks ? c1 : chunks;
+  if (c1 <= 0) return flushed;
+  // The left operand's words: byte j of a row's group g, j = kN (part / 4) + e,
+  // is key 16 e past the thread's first.  Chunks that all rows reach past need
+  // no bounds: their words lie at fixed distances from the thread's pointers.
+  const Row mine = rows[row];
+  const int within = shortest(rows);
+  const int first = kN == 4 ? part : 32 * ((part >> 2) & 1) + 4 * (part >> 3) + (part & 3);
+  const uint64_t* at[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    at[k] = (k < 2 ? a.x[k] : a.a[k - 2]) + int64_t(mine.first) + first;
+  Raw<kN> left;
+  const auto fetch = [&](int c) {
+    if ((c + 1) * kKeyTile <= within) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        left.x0[e] = at[0][16 * e];
+        left.x1[e] = at[1][16 * e];
+        left.a0[e] = at[2][16 * e];
+        left.a1[e] = at[3][16 * e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const int key = c * kKeyTile + first + 16 * e;
+        const int64_t o = int64_t(mine.first) + (key < mine.len ? key : 0);
+        left.x0[e] = a.x[0][o];
+        left.x1[e] = a.x[1][o];
+        left.a0[e] = a.a[0][o];
+        left.a1[e] = a.a[1][o];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) at[k] += kKeyTile;
+  };
+  const auto write = [&](int c) {
+    if ((c + 1) * kKeyTile > within) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        if (c * kKeyTile + first + 16 * e < mine.len) continue;
+        left.x0[e] = left.x1[e] = left.a0[e] = left.a1[e] = 0;
+      }
+    }
+    put_left<kN>(tiles[c & 1], row, part & 3, kN * (part >> 2), left);
+  };
+  fetch(0);
+  write(0);
+  fetch(1);
+  for (int c = 0; c < c1; ++c) {
+    const int8_t* tile = tiles[c & 1];
+    __syncthreads();
+    if (c + 1 < c1) from += step;
+    mul_left(tile, 0, l, y[0], acc[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(0);
+    mul_left(tile, 0, l, y[1], acc[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(1);
+    mul_left(tile, 1, l, y[2], acc[0]);
+    write(c + 1);
+    fetch(c + 2);
+    mul_left(tile, 2, l, y[2], acc[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(2);
+    if (c % kSumChunks == kSumChunks - 1) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          uint64_t v = from_sums(acc[p], r);
+          if (flushed) v += sums[4 * p + r];
+          sums[4 * p + r] = v;
+        }
+      flushed = true;
+      clear(acc);
+    }
+  }
+  return flushed;
+}
+
 // Many rows: a workgroup a row tile, cached head and column block.
-template <int kWaves, bool kWide>
+template <int kWaves, bool kWide, bool kPlanes>
 __global__ void __launch_bounds__(64 * kWaves, kWide ? 2 : 1) kv_values2_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;
   __shared__ __align__(16) int8_t tiles[2][kTileBytes];
@@ -903,8 +1061,17 @@ __global__ void __launch_bounds__(64 * kWaves, kWide ? 2 : 1) kv_values2_kernel(
     __syncthreads();
     if (tid < 16) rows[tid] = row_at(a, q, 16 * m + tid);
     v4i acc[2][kDigitPlanes];
-    const bool flushed = values_run<kWaves, kWide>(a, q, rows, tiles, sums[tid], 0,
-                                                   tiles_of(q.kv), col, acc);
+    bool flushed;
+    if (kPlanes && tiles_of(q.kv) <= va.room) {
+      const int per = (dim + 15) / 16;
+      const int c16 = min(int(blockIdx.y) * kWaves + w, per - 1);
+      flushed = planes_run<kWaves>(a, rows, tiles, sums[tid],
+                                   planes_at(va, int(blockIdx.x), 0, c16),
+                                   per * kPlanesBytes, tiles_of(q.kv), acc);
+    } else {
+      flushed = values_run<kWaves, kWide>(a, q, rows, tiles, sums[tid], 0, tiles_of(q.kv), col,
+                                          acc);
+    }
     if (col >= dim) continue;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -1175,12 +1342,21 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
 //   4 x 2048 keys:  32 items 41 / 131    96: 84 / 140   192: 139 / 145   384: 257 / 222
 //   1 x 300:         8 items 15 / 25     48: 24 / 32     96: 32 / 32
 //   8 x 100:        64 items 19 / 17    192: 31 / 18    768: 66 / 50
+// Items form the values' digits once for all of a sequence's row tiles
+// (planes), if those are several and the chains pay for the launch; in each
+// item / once:
+//   4 x 2048 keys:  heads of 64, 12 row tiles 144 / 119, 24: 221 / 192
+//                   heads of 128, 6 row tiles 201 / 153, 24: 395 / 313
+//   8 x 100 keys:   heads of 64, 4 row tiles 18 / 23, 24: 51 / 52
+// The digits take 24 bytes a value of max_keys for every sequence: not more
+// than twice what the pool itself holds, or they are formed in each item.
 constexpr int kFewMinTiles = 4;
+constexpr int kPlanesMinRows = 4;
 struct ValuesPlan {
   bool wide, few;
   int waves, blocks;
-  int64_t row_tiles, zs, groups;
-  size_t part_bytes, info_bytes;
+  int64_t row_tiles, zs, groups, room;
+  size_t part_bytes, info_bytes, planes_bytes;
 };
 ValuesPlan plan_values(const sufhip_kv_batch& b, const sufhip_kv_pool& p, int heads) {
   ValuesPlan v{};
@@ -1197,8 +1373,30 @@ ValuesPlan plan_values(const sufhip_kv_batch& b, const sufhip_kv_pool& p, int he
     v.groups = clip(v.zs * v.row_tiles * v.blocks * (tiles + 1), 2 * cu_total());
     v.part_bytes = size_t(v.groups) * 2 * kSlotWords * 8;
     v.info_bytes = size_t(b.tokens) * size_t(heads) * size_t(v.blocks) * 16;
+  } else if (v.row_tiles >= kPlanesMinRows && tiles >= kFewMinTiles &&
+             int64_t(b.seqs) * tiles * kKeyTile <= 2 * int64_t(p.pages) * p.page_tokens) {
+    v.room = tiles;
+    v.planes_bytes = size_t(v.zs) * size_t(tiles) * size_t((p.dim + 15) / 16) * kPlanesBytes;
   }
   return v;
+}
+
+template <int kWaves, bool kWide>
+void launch_values(const ValuesArgs& va, const dim3& grid, hipStream_t st) {
+  if (va.planes)
+    hipLaunchKernelGGL((kv_values2_kernel<kWaves, kWide, true>), grid, dim3(64 * kWaves), 0, st,
+                       va);
+  else
+    hipLaunchKernelGGL((kv_values2_kernel<kWaves, kWide, false>), grid, dim3(64 * kWaves), 0, st,
+                       va);
+}
+void launch_values(const ValuesArgs& va, const ValuesPlan& v, const dim3& grid, hipStream_t st) {
+  if (!v.wide)
+    launch_values<4, false>(va, grid, st);
+  else if (v.waves == 4)
+    launch_values<4, true>(va, grid, st);
+  else
+    launch_values<8, true>(va, grid, st);
 }
 
 template <int kOut>
@@ -1236,7 +1434,7 @@ size_t sufhip_kv_values2_work_bytes(const sufhip_kv_batch* batch, const sufhip_k
       batch->seqs < 1 || heads % pool->kv_heads)
     return 0;
   const ValuesPlan v = plan_values(*batch, *pool, heads);
-  return v.part_bytes + v.info_bytes;
+  return v.part_bytes + v.info_bytes + v.planes_bytes;
 }
 
 int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
@@ -1248,10 +1446,10 @@ int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
   const hipStream_t st = as_stream(stream);
   va.blocks = v.blocks;
   for (int p = 0; p < 2; ++p) va.out[p] = va.p.epi.on ? va.p.epi.y[p] : va.p.out[p];
+  const size_t need = v.part_bytes + v.info_bytes + v.planes_bytes;
+  SUFHIP_REQUIRE(need == 0 || (args->d_work && at16(args->d_work) && args->work_bytes >= need),
+                 "sufhip_kv_values2: d_work smaller than its work bytes, or not 16-byte aligned");
   if (v.few) {
-    SUFHIP_REQUIRE(args->d_work && at16(args->d_work) &&
-                       args->work_bytes >= v.part_bytes + v.info_bytes,
-                   "sufhip_kv_values2: d_work smaller than its work bytes, or not 16-byte aligned");
     va.part = static_cast<uint64_t*>(args->d_work);
     va.info = reinterpret_cast<int4*>(static_cast<char*>(args->d_work) + v.part_bytes);
     const dim3 grid{unsigned(v.groups)};
@@ -1267,13 +1465,16 @@ int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
       launch_join<64>(va, st);
     return check_launch("kv_values2_join_kernel");
   }
+  if (v.planes_bytes) {
+    va.planes = static_cast<int8_t*>(args->d_work);
+    va.room = int(v.room);
+    hipLaunchKernelGGL(kv_values2_digits_kernel,
+                       dim3(unsigned(v.zs), unsigned((va.p.pool.dim + 63) / 64), clip(v.room, 65535)),
+                       dim3(256), 0, st, va);
+    if (int rc = check_launch("kv_values2_digits_kernel")) return rc;
+  }
   const dim3 grid(unsigned(v.zs), unsigned(v.blocks), clip(v.row_tiles, 65535));
-  if (!v.wide)
-    hipLaunchKernelGGL((kv_values2_kernel<4, false>), grid, dim3(256), 0, st, va);
-  else if (v.waves == 4)
-    hipLaunchKernelGGL((kv_values2_kernel<4, true>), grid, dim3(256), 0, st, va);
-  else
-    hipLaunchKernelGGL((kv_values2_kernel<8, true>), grid, dim3(512), 0, st, va);
+  launch_values(va, v, grid, st);
   if (int rc = check_launch("kv_values2_kernel")) return rc;
   if (!va.p.epi.on) return SUFHIP_OK;
   launch_join<64>(va, st);

@@ -313,6 +313,19 @@ def test_product_of_many_sequences(kind):
     eq(run_product(*case, kind), getattr(ref, kind)(*case), kind)
 
 
+@pytest.mark.parametrize("page,hk,group,D", [(16, 4, 5, 64), (2, 8, 4, 33), (32, 3, 4, 80),
+                                             (64, 2, 8, 200)])
+@pytest.mark.parametrize("max_keys", [320, 256])
+def test_values_of_many_rows(page, hk, group, D, max_keys):
+    """Digits formed once for all row tiles (page numbers outside the pool
+    among them); 256: bounds that one of the sequences does not keep to."""
+    case = product_case([130, 0, 90, 3], [300, 5, 256, 70], page, hk, group, D, 2, "values")
+    c = case[0]
+    c.table[0, 1], c.table[2, 0] = -1, c.pages
+    say("many rows page=%d heads=%d x %d dim=%d max_keys=%d" % (page, hk, group, D, max_keys))
+    eq(run_product(*case, "values", max_keys=max_keys), ref.values(*case), "values")
+
+
 def sparse_rows(c, H, long):
     """Offsets with rows only for the (head, token) pairs in `long`."""
     rows = np.zeros(H * c.tokens, np.int64)
@@ -497,6 +510,41 @@ def test_captured_step_follows_the_lengths(kind):
         eager = dev2(host[3])
         op(batch, pool, x, a, cc, off, eager)
         want = getattr(ref, kind)(c, H, o, host[0], host[1], host[2], host[3])
+        eq(got, want, "replay")
+        eq(eager, want, "eager")
+
+
+def test_captured_values_of_many_rows():
+    """The same for prompts, whose digits pass through the workspace: a length
+    may leave the captured bounds and come back."""
+    D, hk, group, page = 64, 4, 5, 16
+    H, rng = hk * group, np.random.default_rng(19)
+    big = ref.Case(rng, [130, 60], [400, 400], page, hk, D)
+    cap = H * (130 + 60) * 400
+    lens, off = i32([130, 60]), i32(np.zeros(H * 190 + 1))
+    mk = lambda *n: tuple(torch.zeros(n, dtype=torch.int64, device="cuda")  # noqa: E731
+                          for _ in range(2))
+    x, a, cc, out = mk(cap), mk(cap), mk(190, H, D), mk(190, H, D)
+    pool = kv.Pool(*(dev(w) for w in big.pool))
+    batch = kv.Batch(i32(big.cu), lens, i32(big.table), tokens=190, max_new=130, max_keys=300)
+    work = kv.values_work(batch, pool, H)
+    graph = tasks.capture(lambda: kv.values2(batch, pool, x, a, cc, off, out, work=work))
+    for lens_now in ([300, 130], [140, 400], [299, 61]):
+        c = ref.Case.__new__(ref.Case)
+        c.__dict__.update(big.__dict__)
+        c.lens = lens_now
+        o = c.causal(H)
+        host = [[ref.words(rng, *s) for _ in range(2)] for s in ((cap,), (cap,), (190, H, D))]
+        for d, h in zip((x, a, cc), host):
+            for p in range(2):
+                d[p].copy_(dev(h[p]))
+        lens.copy_(i32(lens_now))
+        off.copy_(i32(o))
+        graph.replay()
+        got = tuple(v.clone() for v in out)
+        eager = mk(190, H, D)
+        kv.values2(batch, pool, x, a, cc, off, eager)
+        want = ref.values(c, H, o, *host, [np.zeros((190, H, D), np.uint64)] * 2)
         eq(got, want, "replay")
         eq(eager, want, "eager")
 
