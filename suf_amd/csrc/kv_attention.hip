@@ -3,7 +3,17 @@
 //
 // With D = (x_0 - a_0) + (x_1 - a_1) a party's share of a product is
 //   Z_p = C_p + D B_p + L_p E,   L_0 = A_0 + D,  L_1 = A_1,
-// E and B_p read from the cache's pages.
+// E and B_p read from the cache's pages: four products of u64 matrices.  Each
+// is 36 products of int8 digit matrices (digits i, j of weight 256^(i + j) below
+// 2^64), 144 matrix instructions for both parties' 16 x 16 results over 64 of
+// k; the digits' sums are exact in int32, and joined in 64 bits.
+//
+// What bounds them: single tokens read the cache once, 24 bytes a cached value,
+// at the rate of a large copy; prompts use each cached word for many rows, and
+// there the matrix instructions (16 cycles a SIMD) and what forms their digits
+// (4 to 5 cycles a vector instruction, of which the other wave of a SIMD
+// issues about two under each matrix instruction) share the time with the
+// packed elements' traffic, 32 bytes each.
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -488,8 +498,12 @@ __device__ __forceinline__ int shortest(const Row (&rows)[16]) {
 // Few rows: a workgroup keeps one row tile in LDS and streams its units of
 // the keys.  Bound by HBM: an array's 16 words a lane are turned into digits,
 // the next unit's loads leave into the same registers, and the matrix cores
-// run under them, so a wave has up to 24 KB in flight.
-
+// run under them, so a wave has up to 24 KB in flight.  Two workgroups a CU
+// (256 registers a wave).  16 sequences of up to 4096 keys, 8 cached heads of
+// 128, 4 queries each: 190 us, 852 MB at 4.5 TB/s.  One sequence of 300 keys,
+// 12 heads of 64: 11 us, a chain of loads that wait for one another (lengths,
+// page numbers, keys: 6 us), one unit's product (3) and the store (1.5); the
+// loads of one step leave together and without branches (12.3 with them).
 template <bool kVec, bool kFull, bool kTrunc>
 __global__ void __launch_bounds__(256, kVec ? 2 : 1)
     kv_scores2_few_kernel(ProductArgs a, int chunks) {
@@ -597,7 +611,11 @@ __global__ void __launch_bounds__(256, kVec ? 2 : 1)
 // registers, kHeld 64-wide chunks of them, and runs over row tiles.  Each
 // thread loads its words of the next row tile, and writes their digits into
 // the other half of LDS while the matrix cores work on the present one (one
-// barrier a tile).
+// barrier a tile).  Two groups of waves over one row tile (128 keys) where a
+// 64-wide chunk is all of a head: each thread then forms half as many digits.
+// Three prompts (1024, 517 after 200, 33), 12 heads of 64 on 4 cached ones:
+// 128 us, 342 MB; without its loads, stores and LDS writes the same work takes
+// seven tenths of that, two thirds of it matrix instructions.
 template <int kHeld, int kGroups, bool kVec, bool kFull, bool kTrunc>
 __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(ProductArgs a) {
   constexpr int kRows = 256 * kGroups;  // rows looked up at once
@@ -724,7 +742,8 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
 // The left operand (one row of packed elements a k) passes through LDS, the
 // next chunk's written while the present one multiplies; the pages' words go
 // to registers, an array's turned into digits and the next chunk's loaded in
-// their place, as for the scores.
+// their place, as for the scores.  Two row tiles a wave (the pages' digits used
+// twice, one wave a SIMD) took 190 us where this took 159.
 struct ValuesArgs {
   ProductArgs p;
   int blocks;        // column blocks
@@ -938,7 +957,10 @@ __global__ void __launch_bounds__(256, 2) kv_values2_digits_kernel(ValuesArgs va
 }
 
 // values_run over digits that are there: from `from` (the wave's planes of the
-// first chunk, `step` bytes a chunk).
+// first chunk, `step` bytes a chunk).  Nothing but the left operand is formed
+// here, 2.7 vector instructions for each matrix instruction instead of 5.2.
+// The place of the left words' loads and LDS writes among the products does
+// not matter (137 to 138 us for three prompts in five orders).
 template <int kWaves>
 __device__ __forceinline__ bool planes_run(const ProductArgs& a, const Row (&rows)[16],
                                            int8_t (*tiles)[kTileBytes], uint64_t* sums,
@@ -1043,7 +1065,11 @@ __device__ __forceinline__ bool planes_run(const ProductArgs& a, const Row (&row
   return flushed;
 }
 
-// Many rows: a workgroup a row tile, cached head and column block.
+// Many rows: a workgroup a row tile, cached head and column block.  Three
+// prompts (1024, 517 after 200, 33 tokens; 12 heads of 64 on 4 cached ones):
+// 126 us and 12 for the digits, 342 MB; the matrix cores are busy for 31% of
+// it.  The longest item is 16 chunks one after another; without the left
+// words' and the digits' traffic a chunk takes six tenths of its time.
 template <int kWaves, bool kWide, bool kPlanes>
 __global__ void __launch_bounds__(64 * kWaves, kWide ? 2 : 1) kv_values2_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;
@@ -1093,7 +1119,11 @@ __global__ void __launch_bounds__(64 * kWaves, kWide ? 2 : 1) kv_values2_kernel(
 // the workspace, where slot 2 w holds what workgroup w has of an item that
 // began before its share, slot 2 w + 1 of one that goes on after it.  For
 // each row and column block `info` keeps the first and last workgroup of its
-// item and its row in the tile, from which the join finds the slots.
+// item and its row in the tile, from which the join finds the slots.  Sums mod
+// 2^64 are the same in any order.  One sequence of 65536 keys, 2 cached heads
+// of 128, 4 queries each: 92 us, 420 MB at 4.6 TB/s, the join 5 of them; 16
+// sequences of up to 4096 keys 184 us (4.6 TB/s); 300 keys 14 us, 4 of them the
+// join's launch.
 constexpr int kFewCols = 64;
 
 template <bool kWide>
@@ -1318,7 +1348,8 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
   constexpr int kGroups = kVec ? 2 : 1;  // of one chunk's kernel
   const int groups = chunks == 1 ? kGroups : 1;
   const int64_t key_tiles = (int64_t(b.max_keys) + 64 * groups - 1) / (64 * groups);
-  // Row tiles are spread over workgroups until four of them share a CU.
+  // Row tiles are spread over workgroups until four of them share a CU (three
+  // prompts: 134 us then, 145 with eight, 175 with sixteen).
   const int64_t want = (4 * int64_t(cus) + key_tiles * zs) / (key_tiles * zs + 1);
   const dim3 grid(unsigned(zs), clip(want < row_tiles ? want : row_tiles, 65535),
                   clip(key_tiles, 65535));
