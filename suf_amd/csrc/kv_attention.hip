@@ -923,36 +923,39 @@ __device__ __forceinline__ int8_t* planes_at(const ValuesArgs& va, int z, int ti
   return va.planes + ((int64_t(z) * va.room + tile) * per + c16) * kPlanesBytes;
 }
 
-__global__ void __launch_bounds__(256, 2) kv_values2_digits_kernel(ValuesArgs va) {
+// A workgroup an array and 64 x 64 of its values: short chains of loads (lengths,
+// page numbers, words), and many of them.
+__global__ void __launch_bounds__(256) kv_values2_digits_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;
   const int l = threadIdx.x & 63, g = l >> 4, n = l & 15;
-  const int c16 = 4 * int(blockIdx.y) + __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int k = int(blockIdx.y) % 3;
+  const int c16 = 4 * (int(blockIdx.y) / 3) +
+                  __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   const int dim = a.pool.dim;
   if (16 * c16 >= dim) return;
   const Seq q = seq_at(a, int(blockIdx.x));
   const int tiles = tiles_of(q.kv);
   if (q.rows == 0 || q.kv <= 0 || tiles > va.room) return;
   const int col = 16 * c16 + n < dim ? 16 * c16 + n : 0;
+  const uint64_t* src = (k == 2 ? a.pool.e : a.pool.b[k]) + col;
   for (int t = blockIdx.z; t < tiles; t += gridDim.z) {
-    int64_t place[16];
+    Spot spot[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      place[i] = place_at(a, q, load_spot(a, q, t * kKeyTile + 16 * (i & 3) + 4 * (i >> 2) + g));
-    int8_t* to = planes_at(va, int(blockIdx.x), t, c16) + 16 * l;
+      spot[i] = load_spot(a, q, t * kKeyTile + 16 * (i & 3) + 4 * (i >> 2) + g);
+    uint64_t v[16];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const uint64_t* src = k == 2 ? a.pool.e : a.pool.b[k];
-      uint64_t v[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = src[(place[i] < 0 ? 0 : place[i]) + col];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = place[i] < 0 ? 0 : v[i];
-      v4i y[kDigitPlanes];
-      digits_of16(v, y);
-#pragma unroll
-      for (int i = 0; i < kDigitPlanes; ++i)
-        *reinterpret_cast<v4i*>(to + (8 * k + i) * 1024) = y[i];
+    for (int i = 0; i < 16; ++i) {
+      const int64_t at = place_at(a, q, spot[i]);
+      v[i] = src[at < 0 ? 0 : at];
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = place_at(a, q, spot[i]) < 0 ? 0 : v[i];
+    v4i y[kDigitPlanes];
+    digits_of16(v, y);
+    int8_t* to = planes_at(va, int(blockIdx.x), t, c16) + 8192 * k + 16 * l;
+#pragma unroll
+    for (int i = 0; i < kDigitPlanes; ++i) *reinterpret_cast<v4i*>(to + i * 1024) = y[i];
   }
 }
 
@@ -1067,7 +1070,7 @@ __device__ __forceinline__ bool planes_run(const ProductArgs& a, const Row (&row
 
 // Many rows: a workgroup a row tile, cached head and column block.  Three
 // prompts (1024, 517 after 200, 33 tokens; 12 heads of 64 on 4 cached ones):
-// 126 us and 12 for the digits, 342 MB; the matrix cores are busy for 31% of
+// 126 us and 9 for the digits, 342 MB; the matrix cores are busy for 31% of
 // it.  The longest item is 16 chunks one after another; without the left
 // words' and the digits' traffic a chunk takes six tenths of its time.
 template <int kWaves, bool kWide, bool kPlanes>
@@ -1500,7 +1503,8 @@ int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
     va.planes = static_cast<int8_t*>(args->d_work);
     va.room = int(v.room);
     hipLaunchKernelGGL(kv_values2_digits_kernel,
-                       dim3(unsigned(v.zs), unsigned((va.p.pool.dim + 63) / 64), clip(v.room, 65535)),
+                       dim3(unsigned(v.zs), unsigned(3 * ((va.p.pool.dim + 63) / 64)),
+                            clip(v.room, 65535)),
                        dim3(256), 0, st, va);
     if (int rc = check_launch("kv_values2_digits_kernel")) return rc;
   }
