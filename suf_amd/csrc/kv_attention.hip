@@ -151,8 +151,8 @@ __device__ __forceinline__ void put_digits(int8_t* plane0, const uint64_t (&v)[k
       int8_t* p = plane0 + 4096 * h;
       *reinterpret_cast<uint16_t*>(p) = uint16_t(a);
       *reinterpret_cast<uint16_t*>(p + 1024) = uint16_t(a >> 16);
-      *reinterpret_cast<uint16_t*>(p + 2048) = uint16_t(b);
-      *reinterpret_cast<uint16_t*>(p + 3072) = uint16_t(b >> 16);
+      *reinterpret_cast<uint16_t*>(p + 2 * 1024) = uint16_t(b);
+      *reinterpret_cast<uint16_t*>(p + 3 * 1024) = uint16_t(b >> 16);
     }
   }
 }
