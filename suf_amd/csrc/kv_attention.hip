@@ -1383,9 +1383,11 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
 //                   heads of 128, 6 row tiles 201 / 153, 24: 395 / 313
 //   8 x 100 keys:   heads of 64, 4 row tiles 18 / 23, 24: 51 / 52
 // The digits take 24 bytes a value of max_keys for every sequence: not more
-// than twice what the pool itself holds, or they are formed in each item.
+// than twice what the pool itself holds nor 2 GiB (beside caches of tens of
+// them), or they are formed in each item.
 constexpr int kFewMinTiles = 4;
 constexpr int kPlanesMinRows = 4;
+constexpr int64_t kPlanesMost = int64_t(1) << 31;
 struct ValuesPlan {
   bool wide, few;
   int waves, blocks;
@@ -1408,7 +1410,8 @@ ValuesPlan plan_values(const sufhip_kv_batch& b, const sufhip_kv_pool& p, int he
     v.part_bytes = size_t(v.groups) * 2 * kSlotWords * 8;
     v.info_bytes = size_t(b.tokens) * size_t(heads) * size_t(v.blocks) * 16;
   } else if (v.row_tiles >= kPlanesMinRows && tiles >= kFewMinTiles &&
-             int64_t(b.seqs) * tiles * kKeyTile <= 2 * int64_t(p.pages) * p.page_tokens) {
+             int64_t(b.seqs) * tiles * kKeyTile <= 2 * int64_t(p.pages) * p.page_tokens &&
+             v.zs * tiles * ((p.dim + 15) / 16) <= kPlanesMost / kPlanesBytes) {
     v.room = tiles;
     v.planes_bytes = size_t(v.zs) * size_t(tiles) * size_t((p.dim + 15) / 16) * kPlanesBytes;
   }

@@ -431,8 +431,8 @@ def values2(batch, pool, p, a, c, offsets, out, trunc=None, work=None):
     int64 [n]; the dealer's mask shares of p), c and out (pairs of contiguous
     int64 [tokens, heads, dim]: the shares of a's product with the values'
     masks; the weighted values, heads side by side).  offsets as in scores2.
-    work: values_work(...) of a batch with the same extents, allocated here if
-    it is not given.  Returns out."""
+    work: values_work(...) of a batch and a pool with the same extents,
+    allocated here if it is not given.  Returns out."""
     what, d = "values2", batch.device
     _device(out[0], what, "out")
     shape = out[0].shape

@@ -224,6 +224,25 @@ def test_values2_needs_its_workspace():
     assert lib.sufhip_kv_values2_work_bytes(ctypes.byref(a.batch), ctypes.byref(a.pool), 3) == 0
 
 
+def test_values2_work_bytes_are_bounded():
+    """Partial sums are two slots a workgroup, digits at most 2 GiB, also for
+    bounds that no cache holds."""
+    lib = native.load()
+    a = product_args()
+    pool(a.pool, pages=1 << 24, page_tokens=64, kv_heads=8, dim=128)
+
+    def need(seqs, new, keys):
+        batch(a.batch, seqs=seqs, tokens=seqs * new, max_new=new, max_keys=keys)
+        return lib.sufhip_kv_values2_work_bytes(ctypes.byref(a.batch), ctypes.byref(a.pool), 32)
+
+    assert need(1, 4096, 65536) == 8 * 1024 * 8 * 24576  # 24 bytes a value
+    assert 0 < need(16, 1, 1 << 20) < 32 << 20
+    for seqs, new, keys in ((64, 1024, 1 << 16), (1, 4096, 1 << 30), (1 << 16, 64, 2 ** 31 - 1)):
+        assert need(seqs, new, keys) <= 2 << 30
+    pool(a.pool, pages=16, page_tokens=64, kv_heads=8, dim=128)
+    assert need(1, 4096, 65536) == 0  # more than the pool holds
+
+
 def test_scores2_refuses_negative_strides():
     a = product_args()
     a.x.token_stride = -1
