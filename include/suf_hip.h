@@ -1018,8 +1018,9 @@ int sufhip_kv_append2(const sufhip_kv_append2_args* args, void* stream);
  * 2^31 - 256); at most 2^30 rows (tokens times heads), and 2^22 sequences
  * times cached heads.  The pool has at least one page.  trunc (optional): the open Z_0 + Z_1 + mask feeds this prepared
  * GapARS table gate (no addend), whose outputs y are written in place of out.
- * d_work (values): sufhip_kv_values2_work_bytes() bytes, 16-byte aligned,
- * used by this call only until it ends; 0 bytes: none needed. */
+ * d_work (values): sufhip_kv_values2_work_bytes() bytes (asked for the same
+ * extents with the call's device current), 16-byte aligned, used by this call
+ * only until it ends; 0 bytes: none needed. */
 typedef struct sufhip_kv_product2_args {
   sufhip_kv_batch batch;
   sufhip_kv_pool pool;
