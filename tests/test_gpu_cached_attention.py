@@ -137,6 +137,18 @@ def test_prompts_then_tokens(kv_heads, group, dim, v_dim, page, rot, neigh, scal
     run(att, plain, rng, [c, d, b], [1, 1, 1])
 
 
+def test_rows_past_the_one_launch_softmax():
+    """More keys than the softmax block takes in its one launch."""
+    rng = np.random.default_rng(8)
+    cache = kv.PagedCache(10, 64, 1, 8)
+    att = kv.CachedAttention(cache, 2, STATE, 600)
+    plain = Plain(att)
+    s = cache.open()
+    run(att, plain, rng, [s], [40])
+    run(att, plain, rng, [s], [500])
+    run(att, plain, rng, [s], [1])
+
+
 def test_captured_step_replays():
     """A step's launches as a graph, replayed with other shares of other
     values, beside eager work."""
