@@ -68,6 +68,72 @@ struct Put<true> {
   }
 };
 
+// A row's elements by key: where key's words of C are and its outputs go.
+// kBuffer: packed arrays of fewer than 2^29 elements as buffers, whose range
+// check drops a store past their end and reads zeros there.  Keys without an
+// element then need no branch, so the memory operations under way stay counted
+// and a wave waits for the words that it uses alone, not for the stores of the
+// tile before (32 row tiles of 4 x 2112 keys, 4 cached heads: 426 -> 380 us with
+// heads of 128, 222 -> 219 with 64).
+constexpr int64_t kBufferMost = (int64_t(1) << 29) - 1;
+template <bool kTrunc, bool kBuffer>
+struct Elements;
+template <bool kTrunc>
+struct Elements<kTrunc, false> {
+  Put<kTrunc> put_;
+  __device__ __forceinline__ explicit Elements(const ProductArgs& a) : put_(a) {}
+  __device__ __forceinline__ uint32_t at(int first, int len, int key) const {
+    return key < len ? uint32_t(first + key) : ~0u;
+  }
+  __device__ __forceinline__ uint64_t c(const ProductArgs& a, int p, uint32_t at) const {
+    return a.c[p][at == ~0u ? 0 : at];
+  }
+  __device__ __forceinline__ void put(const ProductArgs& a, uint32_t at, uint64_t z0,
+                                      uint64_t z1) const {
+    if (at != ~0u) put_(a, at, z0, z1);
+  }
+};
+template <bool kTrunc>
+struct Elements<kTrunc, true> {
+  EpiHdrs eh;
+  __amdgpu_buffer_rsrc_t c_[2], out[2];
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint64_t* p, int64_t n) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint64_t*>(p), 0, int(uint32_t(8 * n)),
+                                             0x00020000);
+  }
+  __device__ __forceinline__ explicit Elements(const ProductArgs& a) {
+    if constexpr (kTrunc) eh = epi_hdrs(a.epi);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      c_[p] = buffer(a.c[p], a.n);
+      out[p] = buffer(kTrunc ? a.epi.y[p] : a.out[p], a.n);
+    }
+  }
+  __device__ __forceinline__ uint32_t at(int first, int len, int key) const {
+    return key < len ? 8 * uint32_t(first + key) : 0xfffffff8u;
+  }
+  __device__ __forceinline__ uint64_t c(const ProductArgs&, int p, uint32_t at) const {
+    const auto w = __builtin_amdgcn_raw_buffer_load_b64(c_[p], at, 0, 0);
+    return uint64_t(w[0]) | uint64_t(w[1]) << 32;
+  }
+  __device__ __forceinline__ void store(int p, uint32_t at, uint64_t v) const {
+    typedef unsigned v2u __attribute__((ext_vector_type(2)));
+    __builtin_amdgcn_raw_buffer_store_b64(v2u{unsigned(v), unsigned(v >> 32)}, out[p], at, 0, 0);
+  }
+  __device__ __forceinline__ void put(const ProductArgs& a, uint32_t at, uint64_t z0,
+                                      uint64_t z1) const {
+    if constexpr (kTrunc) {
+      const uint64_t open = z0 + z1 + a.mask;
+      const uint64_t w0 = trunc_table_word(eh.h[0], a.epi.table[0], a.epi.f, open);
+      const uint64_t w1 = trunc_table_word(eh.h[1], a.epi.table[1], a.epi.f, open);
+      z0 = trunc_table_out(eh.h[0], a.epi.f, open, w0);
+      z1 = trunc_table_out(eh.h[1], a.epi.f, open, w1);
+    }
+    store(0, at, z0);
+    store(1, at, z1);
+  }
+};
+
 // ---- digits ----
 //
 // v = sum_i d_i 256^i with d_i in [-128, 127]: adding 128 to every byte (with
@@ -465,15 +531,17 @@ __device__ __forceinline__ void load_raw(const ProductArgs& a, const Row& r, int
                                          Raw<kN>& v) {
   const int d = 4 * kN * (part >> 2) + 2 * (part & 3), left = a.pool.dim - 64 * c;
   if (r.t < 0 || d >= left) return;
-  const int64_t xo = int64_t(r.t) * a.xts + int64_t(r.h) * a.xhs + 64 * c;
-  const int64_t ao = (int64_t(r.t) * a.heads + r.h) * a.pool.dim + 64 * c;
+  const int64_t t = max(r.t, 0);
+  const int64_t xo = t * a.xts + int64_t(r.h) * a.xhs + 64 * c;
+  const int64_t ao = (t * a.heads + r.h) * a.pool.dim + 64 * c;
   load_left<kN, kVec, kFull || (kVec && kN == 2)>(a.x[0] + xo, d, left, v.x0);
   load_left<kN, kVec, kFull || (kVec && kN == 2)>(a.x[1] + xo, d, left, v.x1);
   load_left<kN, kVec, kFull || (kVec && kN == 2)>(a.a[0] + ao, d, left, v.a0);
   load_left<kN, kVec, kFull || (kVec && kN == 2)>(a.a[1] + ao, d, left, v.a1);
 }
-// Rows past the last write what their registers hold: a row of the left
-// operand reaches that row of the product alone, and it is not stored.
+// Rows past the last write what their registers hold, or the first token's
+// words: a row of the left operand reaches that row of the product alone, and
+// it is not stored.
 template <int kN>
 __device__ __forceinline__ void put_raw(int8_t* tile, int row, int part, const Raw<kN>& v) {
   put_left<kN>(tile, row, part & 3, kN * (part >> 2), v);
@@ -616,7 +684,7 @@ __global__ void __launch_bounds__(256, kVec ? 2 : 1)
 // Three prompts (1024, 517 after 200, 33), 12 heads of 64 on 4 cached ones:
 // 128 us, 342 MB; without its loads, stores and LDS writes the same work takes
 // seven tenths of that, two thirds of it matrix instructions.
-template <int kHeld, int kGroups, bool kVec, bool kFull, bool kTrunc>
+template <int kHeld, int kGroups, bool kVec, bool kFull, bool kTrunc, bool kBuffer>
 __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(ProductArgs a) {
   constexpr int kRows = 256 * kGroups;  // rows looked up at once
   constexpr int kKeys = 64 * kGroups;
@@ -628,7 +696,7 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = l >> 4, n = l & 15;
   const int dim = a.pool.dim;
-  const Put<kTrunc> put(a);
+  const Elements<kTrunc, kBuffer> io(a);
   const Seq q = seq_at(a, int(blockIdx.x));
   const int row_tiles = (q.rows + 15) / 16;
   for (int64_t first_key = int64_t(blockIdx.z) * kKeys; first_key < q.kv;
@@ -672,8 +740,7 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
       const int row = tid / (64 / kN), part = tid % (64 / kN);
       Raw<kN> raw[kHeld] = {};
       const auto fetch = [&](unsigned bits) {
-        if (!bits) return;
-        const Row r = rows[__builtin_ctz(bits) * 16 + row];
+        const Row r = rows[(bits ? __builtin_ctz(bits) * 16 : 0) + row];
 #pragma unroll
         for (int c = 0; c < kHeld; ++c) load_raw<kN, kVec, kFull>(a, r, c, part, raw[c]);
       };
@@ -694,25 +761,24 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
           fetch(todo & (todo - 1));
         }
         const int8_t* tile = tiles + (it & 1) * kHalf;
+        // C's words load under the products; asked for before this tile's
+        // writes to LDS they gain nothing (128 to 133 us for three prompts in
+        // four places).
+        uint64_t cw[2][4];
+        uint32_t at[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const Row& row = rows[ti * 16 + 4 * g + r];
+          at[r] = io.at(row.first, row.len, key);
+          cw[0][r] = io.c(a, 0, at[r]);
+          cw[1][r] = io.c(a, 1, at[r]);
+        }
         v4i acc[2][kDigitPlanes];
         clear(acc);
 #pragma unroll
         for (int c = 0; c < kHeld; ++c)
           mul_opened(tile + c * kTileBytes, l, K[c][1], K[c][2], acc);
-        // C's words load under the other half of the products (before the
-        // first half, or a tile ahead, they hold the wave up at the stores
-        // of the tile before: 143 and 149 us against 129 for three prompts).
         __builtin_amdgcn_sched_barrier(0);
-        uint64_t cw[2][4];
-        int at[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const Row& row = rows[ti * 16 + 4 * g + r];
-          at[r] = key < row.len ? row.first + key : -1;
-          const int o = at[r] < 0 ? 0 : at[r];
-          cw[0][r] = a.c[0][o];
-          cw[1][r] = a.c[1][o];
-        }
 #pragma unroll
         for (int c = 0; c < kHeld; ++c) {
           mul_left(tile + c * kTileBytes, 1, l, K[c][0], acc[0]);
@@ -720,13 +786,125 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(Prod
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if (at[r] < 0) continue;
           const uint64_t z0 = place < 0 ? 0 : from_sums(acc[0], r);
           const uint64_t z1 = place < 0 ? 0 : from_sums(acc[1], r);
-          put(a, at[r], z0 + cw[0][r], z1 + cw[1][r]);
+          io.put(a, at[r], z0 + cw[0][r], z1 + cw[1][r]);
           if constexpr (kTrunc) __builtin_amdgcn_sched_barrier(0);
         }
       }
+    }
+  }
+}
+
+// Heads of 65 to 128: the digits of both chunks of a key do not fit in a wave's
+// registers beside a second wave on the SIMD, so two groups of four waves take
+// a chunk each, of the same 64 keys.  Each forms its own chunk of the left
+// operand; of a tile's 4 rows a lane, the first group finishes two and the
+// second two, with the other's sums through LDS, after the next tile's
+// barrier.  32 row tiles of 4 x 2112 keys, 4 cached heads of 128: 380 us; 460
+// with both chunks in one wave a SIMD.
+template <bool kFull, bool kTrunc, bool kBuffer>
+__global__ void __launch_bounds__(512, 2) kv_scores2_pair_kernel(ProductArgs a) {
+  constexpr int kRows = 512, kKeys = 64, kHalf = 2 * kTileBytes;
+  extern __shared__ __align__(16) int8_t tiles[];
+  __shared__ uint64_t sums[2][2][4][256];
+  __shared__ Row rows[kRows];
+  __shared__ unsigned active;
+  const int tid = threadIdx.x, l = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), half = w >> 2;
+  const int g = l >> 4, n = l & 15;
+  const int dim = a.pool.dim, in = tid & 255;
+  const Elements<kTrunc, kBuffer> io(a);
+  const Seq q = seq_at(a, int(blockIdx.x));
+  const int row_tiles = (q.rows + 15) / 16;
+  for (int64_t first_key = int64_t(blockIdx.z) * kKeys; first_key < q.kv;
+       first_key += int64_t(gridDim.z) * kKeys) {
+    const int k0 = int(first_key), key = k0 + 16 * (w & 3) + n;
+    const int64_t place = place_at(a, q, load_spot(a, q, key));
+    v4i K[3][kDigitPlanes];
+    int lane_g = g;
+    asm volatile("" : "+v"(lane_g));
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      uint64_t v[16];
+      load_keys<true, kFull>((k == 0 ? a.pool.e : a.pool.b[k - 1]) + (place < 0 ? 0 : place) +
+                                 64 * half,
+                             lane_g, dim - 64 * half, v);
+      digits_of16(v, K[k]);
+    }
+    for (int rb = blockIdx.y; rb < row_tiles; rb += gridDim.y * (kRows / 16)) {
+      __syncthreads();
+      const Row mine = row_at(a, q, (rb + (tid >> 4) * int(gridDim.y)) * 16 + (tid & 15));
+      rows[tid] = mine;
+      if (tid == 0) active = 0;
+      const uint64_t seen = __ballot(mine.len > k0);
+      __syncthreads();
+      if (l == 0) {
+        unsigned bits = 0;
+        for (int i = 0; i < 4; ++i)
+          if ((seen >> (16 * i)) & 0xffff) bits |= 1u << (4 * w + i);
+        if (bits) atomicOr(&active, bits);
+      }
+      __syncthreads();
+      unsigned todo = __builtin_amdgcn_readfirstlane(active);
+      if (!todo) continue;
+      Raw<4> raw = {};
+      const auto fetch = [&](unsigned bits) {
+        load_raw<4, true, kFull>(a, rows[(bits ? __builtin_ctz(bits) * 16 : 0) + (in >> 4)], half,
+                                 tid & 15, raw);
+      };
+      const auto write = [&](int it) {
+        put_raw<4>(tiles + (it & 1) * kHalf + half * kTileBytes, in >> 4, tid & 15, raw);
+      };
+      // The tile before: its C words, where they go, this group's sums.
+      uint64_t cw[2][2] = {}, own[2][2] = {};
+      uint32_t at[2] = {io.at(0, 0, 0), io.at(0, 0, 0)};  // none yet
+      const auto finish = [&](int it) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint64_t z0 = own[0][r] + sums[it & 1][half][r][in];
+          const uint64_t z1 = own[1][r] + sums[it & 1][half][2 + r][in];
+          io.put(a, at[r], (place < 0 ? 0 : z0) + cw[0][r], (place < 0 ? 0 : z1) + cw[1][r]);
+          if constexpr (kTrunc) __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      fetch(todo);
+      write(0);
+      fetch(todo & (todo - 1));
+      int it = 0;
+      for (; todo; ++it) {
+        const int ti = __builtin_ctz(todo);
+        todo &= todo - 1;
+        __syncthreads();
+        write(it + 1);
+        fetch(todo & (todo - 1));
+        finish(it - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const int8_t* tile = tiles + (it & 1) * kHalf + half * kTileBytes;
+        v4i acc[2][kDigitPlanes];
+        clear(acc);
+        mul_opened(tile, l, K[1], K[2], acc);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const Row& row = rows[ti * 16 + 4 * g + 2 * half + r];
+          at[r] = io.at(row.first, row.len, key);
+          cw[0][r] = io.c(a, 0, at[r]);
+          cw[1][r] = io.c(a, 1, at[r]);
+        }
+        mul_left(tile, 1, l, K[0], acc[0]);
+        mul_left(tile, 2, l, K[0], acc[1]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint64_t lo = from_sums(acc[p], r), hi = from_sums(acc[p], 2 + r);
+            own[p][r] = half ? hi : lo;
+            sums[it & 1][half ^ 1][2 * p + r][in] = half ? lo : hi;
+          }
+      }
+      __syncthreads();
+      finish(it - 1);
     }
   }
 }
@@ -1323,13 +1501,33 @@ int launch_scores_few(const ProductArgs& a, const dim3& grid, int chunks, hipStr
   return check_launch("kv_scores2_few_kernel");
 }
 
-template <int kHeld, int kGroups, bool kVec, bool kFull, bool kTrunc>
+template <int kHeld, int kGroups, bool kVec, bool kFull, bool kTrunc, bool kBuffer>
 int launch_scores_many(const ProductArgs& a, const dim3& grid, hipStream_t st) {
   const size_t lds = 2 * size_t(kHeld) * kTileBytes;
-  if (int rc = allow_lds(kv_scores2_kernel<kHeld, kGroups, kVec, kFull, kTrunc>, lds)) return rc;
-  hipLaunchKernelGGL((kv_scores2_kernel<kHeld, kGroups, kVec, kFull, kTrunc>), grid,
+  if (int rc = allow_lds(kv_scores2_kernel<kHeld, kGroups, kVec, kFull, kTrunc, kBuffer>, lds))
+    return rc;
+  hipLaunchKernelGGL((kv_scores2_kernel<kHeld, kGroups, kVec, kFull, kTrunc, kBuffer>), grid,
                      dim3(256 * kGroups), lds, st, a);
   return check_launch("kv_scores2_kernel");
+}
+
+template <bool kFull, bool kTrunc, bool kBuffer>
+int launch_scores_pair(const ProductArgs& a, const dim3& grid, hipStream_t st) {
+  const size_t lds = 4 * size_t(kTileBytes);
+  if (int rc = allow_lds(kv_scores2_pair_kernel<kFull, kTrunc, kBuffer>, lds)) return rc;
+  hipLaunchKernelGGL((kv_scores2_pair_kernel<kFull, kTrunc, kBuffer>), grid, dim3(512), lds, st, a);
+  return check_launch("kv_scores2_pair_kernel");
+}
+
+// Many rows, heads of up to 128.
+template <bool kVec, bool kFull, bool kTrunc, bool kBuffer>
+int launch_scores_many(const ProductArgs& a, const dim3& grid, hipStream_t st) {
+  if (a.pool.dim <= 64)
+    return launch_scores_many<1, kVec ? 2 : 1, kVec, kFull, kTrunc, kBuffer>(a, grid, st);
+  if constexpr (kVec)
+    return launch_scores_pair<kFull, kTrunc, kBuffer>(a, grid, st);
+  else
+    return launch_scores_many<2, 1, kVec, kFull, kTrunc, kBuffer>(a, grid, st);
 }
 
 template <bool kVec, bool kFull, bool kTrunc>
@@ -1356,8 +1554,8 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
   const int64_t want = (4 * int64_t(cus) + key_tiles * zs) / (key_tiles * zs + 1);
   const dim3 grid(unsigned(zs), clip(want < row_tiles ? want : row_tiles, 65535),
                   clip(key_tiles, 65535));
-  if (chunks == 1) return launch_scores_many<1, kGroups, kVec, kFull, kTrunc>(a, grid, st);
-  return launch_scores_many<2, 1, kVec, kFull, kTrunc>(a, grid, st);
+  return a.n <= kBufferMost ? launch_scores_many<kVec, kFull, kTrunc, true>(a, grid, st)
+                             : launch_scores_many<kVec, kFull, kTrunc, false>(a, grid, st);
 }
 
 template <bool kVec, bool kFull>

@@ -417,6 +417,35 @@ def test_long_cache_offsets_pass_32_bits():
     assert np.array_equal(u64(e[pages - 1, :, page - 2]), words[pages - 1][:, page - 2])
 
 
+@pytest.mark.parametrize("D", [64, 100])
+@pytest.mark.parametrize("n", [(1 << 29) - 1, (1 << 29) + 77])
+def test_scores_of_long_packed_arrays(D, n):
+    """Rows at the end of packed arrays on both sides of 2^29 elements, where
+    byte offsets pass 32 bits; every other element is left alone."""
+    rng = np.random.default_rng(D)
+    c = ref.Case(rng, [40], [150], 16, 1, D)
+    off = c.causal(1)
+    m = int(off[-1] - off[1])          # elements of the rows but the first
+    far = off.astype(np.int64) + (n - m - int(off[1]))
+    far[0] = 0                         # the first row's start; its rest has no keys
+    x, a = ([ref.words(rng, c.tokens, 1, D) for _ in range(2)] for _ in range(2))
+    cc = [ref.words(rng, int(off[-1])) for _ in range(2)]
+    want = ref.scores(c, 1, off, x, a, cc, [np.zeros(int(off[-1]), np.uint64)] * 2)
+    say("scores of %d packed elements, dim %d" % (n, D))
+    k0 = 150                           # the first row sees all of its sequence now
+    big = [torch.zeros(n, dtype=torch.int64, device="cuda") for _ in range(4)]
+    for p in range(2):
+        big[p][n - m:] = dev(cc[p][int(off[1]):])
+    out = (big[2], big[3])
+    kv.scores2(batch_of(c), kv.Pool(*(dev(w) for w in c.pool)), dev2(x), dev2(a),
+               (big[0], big[1]), i32(far), out)
+    for p in range(2):
+        assert np.array_equal(u64(out[p][n - m:]), want[p][int(off[1]):]), "party %d" % p
+        assert int(out[p][k0:n - m].count_nonzero()) == 0
+    del big, out
+    torch.cuda.empty_cache()
+
+
 def test_scores_of_a_view():
     """Queries inside the rows of a fused product, 8-byte aligned."""
     for lead, gap in ((0, 64), (1, 0), (0, 1)):
@@ -446,7 +475,9 @@ def test_pool_not_16_byte_aligned():
 
 @pytest.mark.parametrize("kind", ["scores", "values"])
 @pytest.mark.parametrize("new,lens,group,D", [([1, 1], [70, 300], 4, 64), ([40], [90], 2, 33),
-                                              ([1], [3000], 2, 128)])
+                                              ([1], [3000], 2, 128),
+                                              ([40], [90], 2, 64), ([3, 50], [9, 150], 3, 100),
+                                              ([130], [300], 8, 128)])
 def test_product_truncates(kind, new, lens, group, D):
     """Through the gate: the shares of the unfused product, open and gate,
     and rows in no sequence untouched."""
