@@ -1094,7 +1094,9 @@ __device__ __forceinline__ bool values_run(const ProductArgs& a, const Seq& q, c
 
 // The values' digits, formed once for all row tiles: 64 keys of 16 columns are
 // the planes of b_0, b_1 and E (plane i of array k at (8 k + i) KB), 16 bytes a
-// lane in the lanes' order.  Keys without a page are zeros.
+// lane in the lanes' order.  Keys without a page are zeros.  k order here:
+// byte j of group g stands for key 16 (j / 4) + 4 g + j % 4, so that a thread's
+// left words, bytes of one group, are neighbours.
 constexpr int kPlanesBytes = 3 * kDigitPlanes * 1024;
 __device__ __forceinline__ int8_t* planes_at(const ValuesArgs& va, int z, int tile, int c16) {
   const int per = (va.p.pool.dim + 15) / 16;
@@ -1120,7 +1122,7 @@ __global__ void __launch_bounds__(256) kv_values2_digits_kernel(ValuesArgs va) {
     Spot spot[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      spot[i] = load_spot(a, q, t * kKeyTile + 16 * (i & 3) + 4 * (i >> 2) + g);
+      spot[i] = load_spot(a, q, t * kKeyTile + 16 * (i >> 2) + 4 * g + (i & 3));
     uint64_t v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -1167,12 +1169,12 @@ __device__ __forceinline__ bool planes_run(const ProductArgs& a, const Row (&row
   const int chunks = (longest(rows) + kKeyTile - 1) / kKeyTile;
   c1 = c1 < chunks ? c1 : chunks;
   if (c1 <= 0) return flushed;
-  // The left operand's words: byte j of a row's group g, j = kN (part / 4) + e,
-  // is key 16 e past the thread's first.  Chunks that all rows reach past need
-  // no bounds: their words lie at fixed distances from the thread's pointers.
+  // The left operand's words, kN neighbours a thread.  Chunks that all rows
+  // reach past need no bounds: two words a load, 8-byte aligned.
+  typedef unsigned long long Two __attribute__((ext_vector_type(2), aligned(8)));
   const Row mine = rows[row];
   const int within = shortest(rows);
-  const int first = kN == 4 ? part : 32 * ((part >> 2) & 1) + 4 * (part >> 3) + (part & 3);
+  const int first = kN == 4 ? 4 * part : 16 * (part >> 3) + 4 * (part & 3) + 2 * ((part >> 2) & 1);
   const uint64_t* at[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -1181,16 +1183,21 @@ __device__ __forceinline__ bool planes_run(const ProductArgs& a, const Row (&row
   const auto fetch = [&](int c) {
     if ((c + 1) * kKeyTile <= within) {
 #pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        left.x0[e] = at[0][16 * e];
-        left.x1[e] = at[1][16 * e];
-        left.a0[e] = at[2][16 * e];
-        left.a1[e] = at[3][16 * e];
+      for (int e = 0; e < kN; e += 2) {
+        const auto two = [&](const uint64_t* from, uint64_t (&v)[kN]) {
+          const Two w = *reinterpret_cast<const Two*>(from + e);
+          v[e] = w[0];
+          v[e + 1] = w[1];
+        };
+        two(at[0], left.x0);
+        two(at[1], left.x1);
+        two(at[2], left.a0);
+        two(at[3], left.a1);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < kN; ++e) {
-        const int key = c * kKeyTile + first + 16 * e;
+        const int key = c * kKeyTile + first + e;
         const int64_t o = int64_t(mine.first) + (key < mine.len ? key : 0);
         left.x0[e] = a.x[0][o];
         left.x1[e] = a.x[1][o];
@@ -1205,7 +1212,7 @@ __device__ __forceinline__ bool planes_run(const ProductArgs& a, const Row (&row
     if ((c + 1) * kKeyTile > within) {
 #pragma unroll
       for (int e = 0; e < kN; ++e) {
-        if (c * kKeyTile + first + 16 * e < mine.len) continue;
+        if (c * kKeyTile + first + e < mine.len) continue;
         left.x0[e] = left.x1[e] = left.a0[e] = left.a1[e] = 0;
       }
     }
