@@ -1255,7 +1255,7 @@ __device__ __forceinline__ bool planes_run(const ProductArgs& a, const Row (&row
 
 // Many rows: a workgroup a row tile, cached head and column block.  Three
 // prompts (1024, 517 after 200, 33 tokens; 12 heads of 64 on 4 cached ones):
-// 126 us and 9 for the digits, 342 MB; the matrix cores are busy for 31% of
+// 123 us and 9 for the digits, 342 MB; the matrix cores are busy for 33% of
 // it.  The longest item is 16 chunks one after another; without the left
 // words' and the digits' traffic a chunk takes six tenths of its time.
 template <int kWaves, bool kWide, bool kPlanes>
