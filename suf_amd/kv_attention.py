@@ -31,8 +31,8 @@ import math
 import numpy as np
 import torch
 
-from . import native
-from .softmax import SoftmaxBlock
+from . import native, tables
+from .softmax import LONG_KEYS, LongRows, SoftmaxBlock
 from .tasks import TABLE_BITS, Dealer, Trunc, dev, dev_i32, prepare_batch
 
 M64 = (1 << 64) - 1
@@ -521,16 +521,36 @@ class CachedAttention:
     rotary positions; Q(frac_bits) shares in and out:
       q', k' = trunc(rot(q) / sqrt(dim)), trunc(rot(k))
       scores = trunc(q' k'^T), p = Softmax(scores), out = trunc(p v)
+    The queries' 1 / sqrt(dim) is part of their rotary table, so q' holds
+    frac_bits bits of the scaled query: each of its values is off by up to
+    2^-frac_bits and 2^-table_bits of the query's pair.
+
+    Softmax: steps of 2^-frac_bits in probabilities and reciprocals
+    (SoftmaxBlock) while an equal share of max_positions keys is at least six
+    of them; a row of n keys so loses up to about 1.4 n 2^-frac_bits of its
+    weight (4 % at 100 keys, 18 % at 600, frac_bits 12).  Beyond, and wherever
+    long_rows asks for it, weights of 24 bits are divided after the product
+    with the values (LongRows): off by less than 0.1 % up to 8192 keys, 1.3 %
+    at LONG_KEYS; the values have to stay below 2^(38 - frac_bits) over the
+    keys in size.
     deal(seqs, new) makes a step's dealer material and room in the cache,
     step.run(q, k, v, out) computes it."""
 
     def __init__(self, cache, heads, prg_state, max_positions, frac_bits=12, table_bits=12,
-                 rot=None, base=10000.0, interleaved=False, scaling=None, seed=21):
+                 rot=None, base=10000.0, interleaved=False, scaling=None, seed=21,
+                 long_rows=None):
         dim = cache.k.dim
         if heads % cache.kv_heads:
             _fail("CachedAttention", "heads must be a multiple of the cache's %d" % cache.kv_heads)
         if not (0 < frac_bits <= TABLE_BITS and 0 < table_bits <= TABLE_BITS):
             _fail("CachedAttention", "frac_bits and table_bits must be in [1, %d]" % TABLE_BITS)
+        # The block's gates have tables of up to 13 bits.
+        short = 6 * max_positions <= 1 << frac_bits and frac_bits < TABLE_BITS
+        self.long_rows = not short if long_rows is None else bool(long_rows)
+        if not self.long_rows and not short:
+            _fail("CachedAttention", "max_positions needs long_rows")
+        if max_positions > LONG_KEYS:
+            _fail("CachedAttention", "at most %d positions" % LONG_KEYS)
         self.cache, self.heads, self.f, self.fc = cache, heads, frac_bits, table_bits
         self.prg_state = bytes(prg_state)
         self.max_positions = max_positions
@@ -538,6 +558,9 @@ class CachedAttention:
                   scaling=scaling, device=cache.device)
         self.q_rotary = Rotary.build(dim, max_positions, scale=1.0 / math.sqrt(dim), **kw)
         self.k_rotary = Rotary.build(dim, max_positions, **kw)
+        # Of rows that the block takes, a reciprocal that holds at every sum.
+        self.recip_table = None if self.long_rows else tables.recip_wide_table(
+            frac_bits, 2.0 ** max(10, int(max_positions).bit_length()))
         self.dealer = Dealer(seed)
 
     def deal(self, seqs, new):
@@ -578,9 +601,19 @@ class AttentionStep:
         self.o_c = self._triple(values2, cache.v, self.p_a, (T, H, Dv), deal, {"work": self.work})
         self.tr = {name: Trunc(deal, bits, size, att.prg_state, device=device)
                    for name, bits, size in (("q", att.fc, T * H * D), ("k", att.fc, T * Hk * D),
-                                            ("s", f, n), ("o", f, T * H * Dv))}
-        self.softmax = SoftmaxBlock(self.offsets, att.prg_state, f, seed=deal.word() >> 1,
-                                    device=device)
+                                            ("s", f, n),
+                                            ("o", LongRows.z_bits() if att.long_rows else f,
+                                             T * H * Dv))}
+        seed = deal.word() >> 1
+        if att.long_rows:
+            row = np.arange(H) * T + np.arange(T)[:, None]  # of out's [tokens, heads]
+            self.softmax = LongRows(self.offsets, att.prg_state, f, np.repeat(row.ravel(), Dv),
+                                    seed=seed, device=device)
+            self.z = tuple(torch.empty((T, H, Dv), dtype=torch.int64, device=device)
+                           for _ in range(2))
+        else:
+            self.softmax = SoftmaxBlock(self.offsets, att.prg_state, f, seed=seed,
+                                        recip=att.recip_table, device=device)
         self.q = tuple(torch.empty((T, H, D), dtype=torch.int64, device=device) for _ in range(2))
         self.s, self.p = (tuple(torch.empty(n, dtype=torch.int64, device=device)
                                 for _ in range(2)) for _ in range(2))
@@ -603,11 +636,16 @@ class AttentionStep:
         with any token and head strides (the parts of a fused product's rows);
         out: contiguous [tokens, heads, dim of v].  Returns out."""
         att, cache, b, tr = self.att, self.att.cache, self.batch, self.tr
+        _ptr2([0, 0], out, (b.tokens, att.heads, cache.v.dim), b.device, "run", "out")
         prepare_batch(self.truncs())
         rotary2(q, att.q_rotary, self.positions, self.q, trunc=tr["q"])
         append2(b, cache.k, k, self.k_mask, cache.v, v, self.v_mask, rotary=att.k_rotary,
                 k_trunc=tr["k"])
         scores2(b, cache.k, self.q, self.q_a, self.s_c, self.off, self.s, trunc=tr["s"])
         self.softmax.eval2(self.s, self.p)
-        return values2(b, cache.v, self.p, self.p_a, self.o_c, self.off, out, trunc=tr["o"],
-                       work=self.work)
+        if not att.long_rows:
+            return values2(b, cache.v, self.p, self.p_a, self.o_c, self.off, out, trunc=tr["o"],
+                           work=self.work)
+        z = values2(b, cache.v, self.p, self.p_a, self.o_c, self.off, self.z, trunc=tr["o"],
+                    work=self.work)
+        return self.softmax.divide2(z, out)

@@ -280,3 +280,98 @@ class SoftmaxBlock:
         mul2x(operand(term(self.e)), operand(term(inv, index=self.row_index)), self.tri, self.n,
               into=(self.tr, out))
         return out
+
+
+LONG_KEYS = 1 << 17  # elements of a row
+HALF_BITS, WEIGHT_BITS, INV_BITS = 20, 24, 28
+
+
+class LongRows:
+    """Softmax of packed ragged Q(f) score rows of up to LONG_KEYS elements,
+    divided after the product with the values:
+      g = exp(-delta / 2) in Q(20), delta as RowMaxDiff's (CubicPolyTask's
+          chain: 20 bits keep its products of three factors below 2^62)
+      w = trunc(g g) in Q(24): the square halves a small weight's bits lost,
+          2^-23 g + 2^-24 of each, so that 2^17 of them do not add up
+      y = 1 / (row's sum of w) in Q(28), three Newton steps
+      quotient = trunc_28(trunc_24(z) y), z a row's sum of w times values
+    SoftmaxBlock's probabilities are whole steps of 2^-f, and so is its
+    reciprocal: of a row of n equal scores it keeps f - log2(n) bits.  Every
+    truncation by more bits than a gate's table has is two gates, one shift
+    after the other, but for the rows' few.  A row's sum of w times values has
+    to stay below 2^(38 - f) in size (Q(f + 24) below 2^62).
+
+    row_of: host int array, the row of each quotient."""
+
+    def __init__(self, offsets, prg_state, frac_bits, row_of, seed=11, device="cuda"):
+        self.offsets = np.asarray(offsets, dtype=np.int64)
+        self.n, self.rows = int(self.offsets[-1]), len(self.offsets) - 1
+        lens = np.diff(self.offsets)
+        if self.rows and int(lens.max()) > LONG_KEYS:
+            raise ValueError("LongRows: rows of at most %d elements" % LONG_KEYS)
+        if not 0 < frac_bits < HALF_BITS:
+            raise ValueError("LongRows: frac_bits must be in [1, %d]" % (HALF_BITS - 1))
+        self.f, self.prg_state = frac_bits, bytes(prg_state)
+        dealer = Dealer(seed)
+        self.rowmax = RowMaxDiff(self.offsets, dealer, device)
+        self.exp = spline.SplineGate(self.n, *tables.nexp_fine_table(HALF_BITS), self.prg_state,
+                                     HALF_BITS, seed=dealer.word() >> 1, nonce=dealer.word(),
+                                     device=device)
+        # A power of two above every sum (a weight is at most 1).
+        nmax = 2.0 ** max(1, int(lens.max(initial=1)).bit_length())
+        self.recip = Recip(self.rows, dealer, self.prg_state, INV_BITS,
+                           tables.recip_wide_table(INV_BITS, nmax), 3, device)
+        self.m = len(row_of)
+        self.quot_row = dev_i32(row_of, device)
+        self.offs_dev = dev_i32(self.offsets, device)
+        self.sq = Triples(dealer, self.n, device=device)
+        self.quot = Triples(dealer, self.m, row_of=row_of, device=device)
+        gate = lambda bits, n: Trunc(dealer, bits, n, self.prg_state, device=device)  # noqa: E731
+        cut = 2 * HALF_BITS - WEIGHT_BITS
+        self.tr_w = [gate(cut // 2, self.n), gate(cut - cut // 2, self.n)]
+        self.tr_z = gate(WEIGHT_BITS - self.z_bits(), self.m)
+        self.tr_q = [gate(INV_BITS // 2, self.m), gate(INV_BITS - INV_BITS // 2, self.m)]
+        self.side = torch.cuda.Stream(device=device)
+        self.delta, self.g = pair(self.n, device), pair(self.n, device)
+        self.s = pair(self.rows, device)
+        self.z, self.q = pair(self.m, device), pair(self.m, device)
+        for t in self.truncs():  # nothing is allocated by a call
+            if not t.has_table():
+                t.zhat_buf()
+
+    @staticmethod
+    def z_bits():
+        """Bits that z has lost already when it comes to divide2 (the first of
+        its two shifts, in the launch of the product)."""
+        return WEIGHT_BITS // 2
+
+    def truncs(self):
+        return (self.exp.truncs() + self.recip.truncs() + self.tr_w + [self.tr_z] + self.tr_q)
+
+    def eval2(self, x, w, prep=None):
+        """x: shares of the scores, w: the pair for those of the weights
+        (int64 [n], packed rows).  prep: as SoftmaxBlock.eval2's.  Returns w."""
+        if prep is None:
+            prep = (Prepared(self.side, [self.truncs()]), 0)
+        n = self.n
+        self.rowmax.eval2(x, self.delta)
+        lin2(operand(term(self.delta, shift=HALF_BITS - 1 - self.f)), n, out=self.g)
+        self.exp.eval2(self.g, self.delta, prep=prep, fused=False)
+        e = operand(term(self.delta))
+        mul2x(e, e, self.sq, n, into=(self.tr_w[0], self.g))
+        lin2(operand(term(self.g)), n, into=(self.tr_w[1], w))
+        row_sum2(operand(term(w, shift=INV_BITS - WEIGHT_BITS)), self.rows,
+                 offsets=self.offs_dev, sums=self.s)
+        self.recip.eval2(self.s, fused=False)
+        return w
+
+    def divide2(self, z, out):
+        """z: shares of the rows' sums of weights times values, truncated by
+        z_bits() (int64 [m], element i of row row_of[i]); out: the pair for
+        the Q(f) quotients.  Returns out."""
+        m = self.m
+        lin2(operand(term(z)), m, into=(self.tr_z, self.z))
+        mul2x(operand(term(self.z)), operand(term(self.recip.y, index=self.quot_row)), self.quot,
+              m, into=(self.tr_q[0], self.q))
+        lin2(operand(term(self.q)), m, into=(self.tr_q[1], out))
+        return out

@@ -14,6 +14,9 @@ interval LUT of the gate carries.
                recip_piecewise_affine_init.hpp:11-66) through the same
                expansion (RecipTask reads words 0 and 1,
                include/runtime/phase_tasks.hpp:3314-3326): 2 words.
+  recip_wide_table, nexp_fine_table
+               the two for rows longer than the reference's domains (its
+               reciprocal is a constant past an exp-sum of 1024): 2, 4 words.
   gelu_table   make_gelu_spline_spec (include/gates/tables/gelu_spline_table.hpp:
                57-92) through build_silu_suf_from_piecewise: 4 words.
   rsqrt_table  make_rsqrt_affine_init_spec (include/gates/tables/
@@ -207,6 +210,43 @@ def recip_table(frac_bits=12, nmax=1024.0):
     pieces.append((_enc(nmax, frac_bits) & M64, 0,
                    expand_to_x_coeffs(0, [_enc(1.0 / nmax, frac_bits)], 3, frac_bits)))
     return _finish(pieces, 2)
+
+
+def recip_wide_table(frac_bits, nmax):
+    """recip_table for long rows: its chords as far as their slopes,
+    -2^(f - 1 - 2 k) on [2^k, 2^(k+1)), are whole words (a slope rounded to a
+    whole word leads a Newton step away from 1/x), then constants, each within
+    9 % of 1/x on a quarter of an octave, up to nmax (a power of two)."""
+    exact = 2.0 ** ((frac_bits + 1) // 2)  # where the slopes stop being whole
+    alpha, coeffs = recip_table(frac_bits, min(exact, nmax))
+    pieces = [(int(a), 0, [int(w) for w in c]) for a, c in zip(alpha, coeffs)][:-1]
+    L = min(exact, nmax)
+    while L < nmax:
+        for i in range(4):
+            lo, hi = L * 2.0 ** (i / 4), L * 2.0 ** ((i + 1) / 4)
+            pieces.append((_enc(lo, frac_bits), 0, [_enc(2.0 / (lo + hi), frac_bits), 0]))
+        L *= 2.0
+    pieces.append((_enc(nmax, frac_bits), 0, [_enc(1.0 / nmax, frac_bits), 0]))
+    return _finish(pieces, 2)
+
+
+def nexp_fine_table(frac_bits):
+    """exp(-t) on [0, 16) in cubic pieces of half a unit (within h^4 / 384 =
+    1.7e-4 of itself), 0 from 16 on.  Word k of a piece in (t - start) is
+    rounded to a multiple of 2^k, so that its x-form, at starts of whole
+    halves, is made of whole words and no rounding of it is multiplied by t."""
+    pieces = []
+    for i in range(32):
+        start, end = 0.5 * i, 0.5 * (i + 1)
+        h = end - start
+        y0, y1 = math.exp(-start), math.exp(-end)
+        cs = [y0, -y0, (3.0 * (y1 - y0) + (2.0 * y0 + y1) * h) / (h * h),
+              (2.0 * (y0 - y1) - (y0 + y1) * h) / (h * h * h)]
+        cs = [_enc(c, frac_bits - k) << k for k, c in enumerate(cs)]
+        off = _enc(start, frac_bits)
+        pieces.append((off, off, expand_to_x_coeffs(off, cs, 3, frac_bits)))
+    pieces.append((_enc(16.0, frac_bits), 0, [0, 0, 0, 0]))
+    return _finish(pieces, 4)
 
 
 def rsqrt_table(frac_bits=12, eps=1.0 / 1024.0, vmax=16.0):
