@@ -296,6 +296,8 @@ __device__ __forceinline__ void clear(v4i (&acc)[2][kDigitPlanes]) {
 // A sequence's part of the batch for one cached head: its rows are (token,
 // head of the group) in that order, row m at token t0 + m / group.
 // kv: its keys, none of which a row of at most n elements can do without.
+// Wrong starts (any words, in any order) still give rows of the batch: both
+// ends are brought into [0, tokens] before they are subtracted.
 struct Seq {
   int s, hk, t0, rows, kv;
 };
@@ -304,8 +306,8 @@ __device__ __forceinline__ Seq seq_of_head(const ProductArgs& a, int s, int hk) 
   Seq q;
   q.s = s;
   q.hk = hk;
-  q.t0 = max(lo, 0);
-  q.rows = max(min(hi, a.b.tokens) - q.t0, 0) * a.group;
+  q.t0 = min(max(lo, 0), a.b.tokens);
+  q.rows = max(min(max(hi, 0), a.b.tokens) - q.t0, 0) * a.group;
   q.kv = int(min(int64_t(kv), a.n));
   return q;
 }
