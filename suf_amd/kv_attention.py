@@ -489,7 +489,8 @@ class PagedCache:
 
     def extend(self, seqs, new):
         """Room for new[i] more tokens of sequence seqs[i]; the Batch of these
-        tokens.  Raises, with nothing changed, when the pages do not suffice."""
+        tokens.  What it raises (the pages do not suffice, the device's memory
+        does not), it raises with nothing changed."""
         if len(seqs) != len(new) or len(set(seqs)) != len(seqs) or min(new, default=1) < 0:
             _fail("extend", "sequences must be different, each with a count of new tokens >= 0")
         state = [self.seqs[s] for s in seqs]
@@ -497,17 +498,30 @@ class PagedCache:
         need = [-(-n // self.page_tokens) - len(st["pages"]) for n, st in zip(lens, state)]
         if sum(need) > len(self.free):
             raise RuntimeError("PagedCache: %d pages wanted, %d free" % (sum(need), len(self.free)))
-        for st, n, k in zip(state, lens, need):
-            st["pages"] += [self.free.pop() for _ in range(k)]
-            st["length"] = n
-        width = max([len(st["pages"]) for st in state] + [1])
+        # The last free pages first, as many as each sequence needs.
+        ends = len(self.free) - np.concatenate([[0], np.cumsum(need, dtype=np.int64)])
+        pages = [st["pages"] + self.free[e:b][::-1] for st, b, e in zip(state, ends, ends[1:])]
+        width = max([len(p) for p in pages] + [1])
         table = np.full((len(seqs), width), -1, np.int32)
-        for row, st in zip(table, state):
-            row[:len(st["pages"])] = st["pages"]
+        for row, p in zip(table, pages):
+            row[:len(p)] = p
         cu = np.concatenate([[0], np.cumsum(np.asarray(new, dtype=np.int64))])
-        return Batch(dev_i32(cu, self.device), dev_i32(np.asarray(lens), self.device),
-                     dev_i32(table, self.device), tokens=int(cu[-1]), max_new=max(new, default=0),
-                     max_keys=max(lens, default=0))
+        batch = Batch(dev_i32(cu, self.device), dev_i32(np.asarray(lens), self.device),
+                      dev_i32(table, self.device), tokens=int(cu[-1]), max_new=max(new, default=0),
+                      max_keys=max(lens, default=0))
+        for st, n, p in zip(state, lens, pages):
+            st["pages"], st["length"] = p, n
+        del self.free[ends[-1]:]
+        return batch
+
+    def shrink(self, seqs, lens):
+        """Takes back what the last extend() gave: seqs[i] has lens[i] tokens
+        again, the pages past them are free."""
+        for s, n in reversed(list(zip(seqs, lens))):
+            st = self.seqs[s]
+            keep = -(-n // self.page_tokens)
+            self.free += st["pages"][keep:][::-1]
+            st["pages"], st["length"] = st["pages"][:keep], n
 
 
 def _shares(dealer, shape, device):
@@ -564,6 +578,8 @@ class CachedAttention:
         self.dealer = Dealer(seed)
 
     def deal(self, seqs, new):
+        """A step of new[i] tokens of sequence seqs[i].  What it raises, it
+        raises with the cache as it was."""
         if min(new, default=0) < 1:
             _fail("CachedAttention.deal", "every sequence needs a new token")
         if max(self.cache.length(s) + n for s, n in zip(seqs, new)) > self.max_positions:
@@ -571,17 +587,23 @@ class CachedAttention:
         keys = sum(n * self.cache.length(s) + n * (n + 1) // 2 for s, n in zip(seqs, new))
         if self.heads * keys > MAX_PACKED:
             _fail("CachedAttention.deal", "more than 2^31 - 256 scores in one step")
-        return AttentionStep(self, seqs, new)
+        before = [self.cache.length(s) for s in seqs]
+        batch = self.cache.extend(seqs, new)
+        try:
+            return AttentionStep(self, batch, seqs, new)
+        except BaseException:  # out of memory, an interrupt: no tokens without a step
+            self.cache.shrink(seqs, before)
+            raise
 
 
 class AttentionStep:
     """One step's tokens: its Batch, the dealer's masks, products and gates."""
 
-    def __init__(self, att, seqs, new):
+    def __init__(self, att, batch, seqs, new):
         cache, deal, H, f = att.cache, att.dealer, att.heads, att.f
         device, Hk = cache.device, cache.kv_heads
         self.att = att
-        self.batch = b = cache.extend(seqs, new)
+        self.batch = b = batch
         lens = [cache.length(s) for s in seqs]
         T, D, Dv = b.tokens, cache.k.dim, cache.v.dim
         self.offsets = causal_row_offsets(new, lens, H)
