@@ -27,6 +27,7 @@ src/nn/attention_block.cpp:931-1900.
 """
 import ctypes
 import math
+import warnings
 
 import numpy as np
 import torch
@@ -478,10 +479,13 @@ class PagedCache:
     def open(self):
         """A new, empty sequence's number."""
         s, self._next = self._next, self._next + 1
-        self.seqs[s] = {"pages": [], "length": 0}
+        self.seqs[s] = {"pages": [], "length": 0, "dealt": 0, "run": 0}
         return s
 
     def close(self, seq):
+        """Takes the sequence's pages back.  A step of it that was dealt and
+        has not run does not run any more, nor does a later one of another
+        sequence in that step, whose keys would miss: close that one too."""
         self.free += self.seqs.pop(seq)["pages"][::-1]
 
     def length(self, seq):
@@ -590,20 +594,26 @@ class CachedAttention:
         before = [self.cache.length(s) for s in seqs]
         batch = self.cache.extend(seqs, new)
         try:
-            return AttentionStep(self, batch, seqs, new)
+            step = AttentionStep(self, batch, seqs, new)
         except BaseException:  # out of memory, an interrupt: no tokens without a step
             self.cache.shrink(seqs, before)
             raise
+        for _, st, _ in step.turns:
+            st["dealt"] += 1
+        return step
 
 
 class AttentionStep:
-    """One step's tokens: its Batch, the dealer's masks, products and gates."""
+    """One step's tokens: its Batch, the dealer's masks, products and gates.
+    For one use, in the order in which the steps of a sequence were dealt."""
 
     def __init__(self, att, batch, seqs, new):
         cache, deal, H, f = att.cache, att.dealer, att.heads, att.f
         device, Hk = cache.device, cache.kv_heads
         self.att = att
         self.batch = b = batch
+        # Which step of each of its sequences this is.
+        self.turns = [(s, cache.seqs[s], cache.seqs[s]["dealt"]) for s in seqs]
         lens = [cache.length(s) for s in seqs]
         T, D, Dv = b.tokens, cache.k.dim, cache.v.dim
         self.offsets = causal_row_offsets(new, lens, H)
@@ -653,12 +663,40 @@ class AttentionStep:
     def truncs(self):
         return list(self.tr.values())
 
+    def _take_turn(self):
+        """Refuses a step whose keys would land in pages that are not its
+        sequences' any more, beside keys that are not there yet, or under keys
+        that a later step has used."""
+        again = False
+        for s, st, k in self.turns:
+            if self.att.cache.seqs.get(s) is not st:
+                raise RuntimeError("AttentionStep.run: sequence %d has been closed" % s)
+            if st["run"] < k:
+                raise RuntimeError("AttentionStep.run: an earlier step of sequence %d has not run"
+                                   % s)
+            if st["run"] > k + 1:
+                raise RuntimeError("AttentionStep.run: a later step of sequence %d has run" % s)
+            again = again or st["run"] > k
+        if again:
+            warnings.warn("AttentionStep.run: a step is for one use; a second one opens other "
+                          "values under the same masks, whose difference is then public",
+                          RuntimeWarning, stacklevel=3)
+        for _, st, k in self.turns:
+            st["run"] = k + 1
+
     def run(self, q, k, v, out):
         """q [tokens, heads, dim], k, v [tokens, kv_heads, dim]: pairs of shares
         with any token and head strides (the parts of a fused product's rows);
-        out: contiguous [tokens, heads, dim of v].  Returns out."""
+        out: contiguous [tokens, heads, dim of v].  Returns out.  Raises for a
+        step out of its order or of a closed sequence, and warns of a second
+        run (a captured one's replays are not seen here)."""
         att, cache, b, tr = self.att, self.att.cache, self.batch, self.tr
-        _ptr2([0, 0], out, (b.tokens, att.heads, cache.v.dim), b.device, "run", "out")
+        T, at = b.tokens, [0, 0]
+        _rows(at, q, (T, att.heads, cache.k.dim), b.device, "run", "q")
+        _rows(at, k, (T, cache.kv_heads, cache.k.dim), b.device, "run", "k")
+        _rows(at, v, (T, cache.kv_heads, cache.v.dim), b.device, "run", "v")
+        _ptr2(at, out, (T, att.heads, cache.v.dim), b.device, "run", "out")
+        self._take_turn()
         prepare_batch(self.truncs())
         rotary2(q, att.q_rotary, self.positions, self.q, trunc=tr["q"])
         append2(b, cache.k, k, self.k_mask, cache.v, v, self.v_mask, rotary=att.k_rotary,

@@ -1,6 +1,7 @@
 """The cache's state and the order of its steps: what raises leaves it as it
 was, and no step runs on pages that are not its own."""
 import gc
+import warnings
 
 import pytest
 import torch
@@ -60,3 +61,66 @@ def test_a_deal_that_fails_changes_nothing(monkeypatch, where):
     step = att.deal([b, a], [9, 3])
     assert [cache.length(s) for s in (a, b)] == [9, 10] and len(cache.free) == 8 - 3 - 3
     step.run(*one(att, 12))
+
+
+def test_steps_run_in_the_order_of_their_deal():
+    cache = kv.PagedCache(8, 4, 1, 8)
+    att = kv.CachedAttention(cache, 2, STATE, 20)
+    a, b = cache.open(), cache.open()
+    first, other = att.deal([a], [3]), att.deal([b], [2])
+    second = att.deal([b, a], [1, 1])
+    with pytest.raises(RuntimeError, match="earlier step"):
+        second.run(*one(att, 2))
+    first.run(*one(att, 3))
+    with pytest.raises(RuntimeError, match="earlier step"):
+        second.run(*one(att, 2))
+    assert not bool(cache.k.e[cache.seqs[b]["pages"][0]].any())  # nothing was opened
+    other.run(*one(att, 2))
+    second.run(*one(att, 2))
+    e = cache.k.e.clone()
+    for late, n in ((first, 3), (other, 2)):
+        with pytest.raises(RuntimeError, match="later step"):
+            late.run(*one(att, n))
+    assert torch.equal(cache.k.e, e)
+
+
+def test_a_closed_sequences_step_does_not_run():
+    """Its pages are another sequence's by then."""
+    cache = kv.PagedCache(2, 4, 1, 8)
+    att = kv.CachedAttention(cache, 2, STATE, 8)
+    a = cache.open()
+    old = att.deal([a], [8])
+    cache.close(a)
+    b = cache.open()
+    att.deal([b], [8]).run(*one(att, 8))
+    words = [t.clone() for p in (cache.k, cache.v) for t in (p.e,) + p.b]
+    with pytest.raises(RuntimeError, match="closed"):
+        old.run(*one(att, 8))
+    assert all(torch.equal(t, w) for t, w in
+               zip([t for p in (cache.k, cache.v) for t in (p.e,) + p.b], words))
+
+
+def test_a_second_run_is_warned_of():
+    cache = kv.PagedCache(4, 4, 1, 8)
+    att = kv.CachedAttention(cache, 2, STATE, 8)
+    step = att.deal([cache.open()], [1])
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        step.run(*one(att))
+    with pytest.warns(RuntimeWarning, match="one use"):
+        step.run(*one(att))
+
+
+def test_a_refused_call_does_not_use_a_step():
+    cache = kv.PagedCache(4, 4, 1, 8)
+    att = kv.CachedAttention(cache, 2, STATE, 8)
+    step = att.deal([cache.open()], [1])
+    q, k, v, out = one(att)
+    for bad in ((q, k, v, q[0]), (k, k, v, out), (q, q, v, out), (q, k, q, out),
+                (q[0], k, v, out), (q, k, None, out), (q, k, [t.float() for t in v], out)):
+        with pytest.raises((ValueError, TypeError)):
+            step.run(*bad)
+    assert not bool(cache.k.e.any())
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        step.run(q, k, v, out)
