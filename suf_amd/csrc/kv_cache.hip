@@ -367,14 +367,17 @@ int sufhip_kv_append2(const sufhip_kv_append2_args* args, void* stream) {
   SUFHIP_REQUIRE(args != nullptr, "sufhip_kv_append2: null args");
   AppendArgs a{};
   if (int rc = kv_batch_of(args->batch, what, &a.b)) return rc;
+  // No rows: arrays of none may be null.
+  const bool empty = a.b.seqs == 0 || a.b.tokens == 0;
   bool vec = true, trunc = false;
   for (int k = 0; k < 2; ++k) {
     const sufhip_kv_append_part& g = args->part[k];
     AppendPart& q = a.part[k];
     if (!g.pool.e) continue;
     if (int rc = kv_pool_of(g.pool, what, &q.pool)) return rc;
-    if (int rc = rows_of(g.x, what, &q.x)) return rc;
     if (int rc = rot_of(g.rot, g.pool.dim, what, &q.rot)) return rc;
+    if (empty) continue;
+    if (int rc = rows_of(g.x, what, &q.x)) return rc;
     SUFHIP_REQUIRE(g.mask[0] && g.mask[1], "sufhip_kv_append2: null mask");
     const size_t n = size_t(a.b.tokens) * size_t(q.pool.heads) * size_t(q.pool.dim);
     if (int rc = make_epi(g.trunc, n, what, &q.epi, false)) return rc;
@@ -388,7 +391,7 @@ int sufhip_kv_append2(const sufhip_kv_append2_args* args, void* stream) {
           at16(g.mask[0]) && at16(g.mask[1]) && at16(g.pool.e) && at16(g.pool.b[0]) &&
           at16(g.pool.b[1]) && at16(q.epi.y[0]) && at16(q.epi.y[1]);
   }
-  if (a.b.seqs == 0 || a.b.tokens == 0) return SUFHIP_OK;
+  if (empty) return SUFHIP_OK;
   uint64_t blocks[2] = {0, 0};
   for (int k = 0; k < 2; ++k) {
     AppendPart& q = a.part[k];

@@ -62,3 +62,24 @@ def test_wrong_starts_stay_inside(kind, new, lens, ends):
     op = kv.scores2 if kind == "scores" else kv.values2
     op(batch, kv.Pool(*(dev(w) for w in c.pool)), dev2(x), dev2(a), dev2(cc), i32(off), o)
     eq(o, want, kind)
+
+
+def test_calls_on_no_tokens():
+    """No sequences, sequences without new tokens, rows of padding alone."""
+    cache = kv.PagedCache(4, 4, 1, 8)
+    s = cache.open()
+    cache.extend([s], [3])
+    r = kv.Rotary.build(8, 4)
+    z = lambda *n: torch.zeros(n, dtype=torch.int64, device="cuda")  # noqa: E731
+    b = cache.extend([s], [0])
+    none = kv.Batch(i32([0]), i32([]), i32([]).reshape(0, 1), tokens=2, max_new=1, max_keys=4)
+    for batch, T in ((cache.extend([], []), 0), (b, 0), (none, 2)):
+        x = tuple(torch.full((T, 1, 8), 5, dtype=torch.int64, device="cuda") for _ in range(2))
+        p = (z(0), z(0))
+        off = i32([0] * (T + 1))
+        kv.append2(batch, cache.k, x, x, cache.v, x, x, rotary=r)
+        kv.scores2(batch, cache.k, x, x, p, off, p)
+        out = tuple(torch.full((T, 1, 8), 7, dtype=torch.int64, device="cuda") for _ in range(2))
+        kv.values2(batch, cache.v, p, p, x, off, out)
+        assert all(bool((t == 7).all()) for t in out)
+    assert not any(bool(t.any()) for c in (cache.k, cache.v) for t in (c.e,) + c.b)

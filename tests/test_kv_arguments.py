@@ -1,0 +1,21 @@
+"""Arguments of the cached-attention calls at their edges, on the CPU: what is
+taken and what is refused before any device work."""
+import ctypes
+
+import pytest
+
+from suf_amd import native
+from test_kv_attention import append_args, batch, refused
+
+
+@pytest.mark.parametrize("none", [{"seqs": 0}, {"tokens": 0}, {"seqs": 0, "tokens": 0}])
+def test_an_append_of_no_tokens_does_nothing(none):
+    """A tensor without elements has no address."""
+    a = append_args()
+    batch(a.batch, **none)
+    for p in a.part:
+        for i in range(2):
+            p.x.p[i] = p.mask[i] = None
+    assert native.load().sufhip_kv_append2(ctypes.byref(a), None) == 0
+    batch(a.batch)
+    refused("sufhip_kv_append2", a, "rows")
