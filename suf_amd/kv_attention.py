@@ -359,8 +359,12 @@ def append2(batch, k_pool, k, k_mask, v_pool=None, v=None, v_mask=None, rotary=N
     v if given.  k_mask, v_mask: pairs of the dealer's mask shares, contiguous
     [tokens, kv_heads, dim].  k_trunc, v_trunc: a prepared tasks.Trunc the rows
     go through before they are opened, or (Trunc, pair for the truncated
-    shares)."""
+    shares).  The two pools share no memory."""
     what = "append2"
+    if v_pool is None and not (v is None and v_mask is None and v_trunc is None):
+        _fail(what, "v, v_mask and v_trunc need v_pool")
+    if rotary is None and positions is not None:
+        _fail(what, "positions need rotary")
     a = native.KvAppend2Args()
     a.batch = batch.arg
     keep = [_append_part(a.part[0], batch, k_pool, k, k_mask, rotary, positions, k_trunc, what,

@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 
+from suf_amd import kv_attention as kv
 from suf_amd import native
 from test_kv_attention import append_args, batch, refused
 
@@ -19,3 +20,13 @@ def test_an_append_of_no_tokens_does_nothing(none):
     assert native.load().sufhip_kv_append2(ctypes.byref(a), None) == 0
     batch(a.batch)
     refused("sufhip_kv_append2", a, "rows")
+
+
+class Anything:
+    """Not read before the refusal."""
+
+
+@pytest.mark.parametrize("kw", [{"v": 1}, {"v_mask": 1}, {"v_trunc": 1}, {"positions": 1}])
+def test_append_arguments_without_their_part_are_refused(kw):
+    with pytest.raises(ValueError, match="need"):
+        kv.append2(Anything(), None, None, None, **kw)
