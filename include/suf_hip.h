@@ -974,7 +974,8 @@ typedef struct sufhip_kv_pool {
  * new token and cached head, value - (mask_0 + mask_1) opened into e and the
  * masks into b.  mask[p] [tokens][kv_heads][dim] (the dealer's shares of a
  * mask used for nothing else).  Two parts at most, the keys and the values
- * (e.g. part[0] rotated, part[1] not); a part with pool.e = NULL is absent.
+ * (e.g. part[0] rotated, part[1] not), whose pools share no memory; a part
+ * with pool.e = NULL is absent.
  * rot, unless its table is NULL and it has no positions: the rows are rotated
  * on the way, by d_positions [tokens] if given, else by their places in their
  * sequences; outside the table's positions nothing is written.  trunc

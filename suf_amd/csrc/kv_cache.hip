@@ -294,6 +294,22 @@ int rot_of(const sufhip_rotary& g, int dim, const char* what, Rot* out) {
   return SUFHIP_OK;
 }
 
+// Whether an array of one pool shares a word with one of the other's.
+bool pools_meet(const sufhip_kv_pool& a, const sufhip_kv_pool& b) {
+  const auto bytes = [](const sufhip_kv_pool& p) {
+    return 8 * size_t(p.pages) * size_t(p.kv_heads) * size_t(p.page_tokens) * size_t(p.dim);
+  };
+  const size_t na = bytes(a), nb = bytes(b);
+  const uint64_t* const pa[3] = {a.e, a.b[0], a.b[1]};
+  const uint64_t* const pb[3] = {b.e, b.b[0], b.b[1]};
+  for (const uint64_t* x : pa)
+    for (const uint64_t* y : pb) {
+      const uintptr_t u = reinterpret_cast<uintptr_t>(x), v = reinterpret_cast<uintptr_t>(y);
+      if (u < v + nb && v < u + na) return true;
+    }
+  return false;
+}
+
 int rows_of(const sufhip_rows2& g, const char* what, Rows* out) {
   if (!g.p[0] || !g.p[1] || g.token_stride < 0 || g.head_stride < 0)
     return kv_fail(what, "rows need both parties' pointers and strides >= 0");
@@ -405,6 +421,9 @@ int sufhip_kv_append2(const sufhip_kv_append2_args* args, void* stream) {
     blocks[k] = grid_for(q.total, kBlock);
   }
   if (blocks[0] + blocks[1] == 0) return SUFHIP_OK;
+  SUFHIP_REQUIRE(blocks[0] == 0 || blocks[1] == 0 ||
+                     !pools_meet(args->part[0].pool, args->part[1].pool),
+                 "sufhip_kv_append2: the parts' pools share memory");
   a.blocks0 = uint32_t(blocks[0]);
   const dim3 grid(unsigned(blocks[0] + blocks[1])), block(kBlock);
   const hipStream_t st = as_stream(stream);

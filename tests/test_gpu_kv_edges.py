@@ -83,3 +83,13 @@ def test_calls_on_no_tokens():
         kv.values2(batch, cache.v, p, p, x, off, out)
         assert all(bool((t == 7).all()) for t in out)
     assert not any(bool(t.any()) for c in (cache.k, cache.v) for t in (c.e,) + c.b)
+
+
+def test_one_pool_for_keys_and_values_is_refused():
+    cache = kv.PagedCache(4, 4, 1, 8)
+    b = cache.extend([cache.open()], [1])
+    x = tuple(torch.ones((1, 1, 8), dtype=torch.int64, device="cuda") for _ in range(2))
+    for pool in (cache.k, kv.Pool(cache.v.e, cache.v.b[0], cache.k.e)):
+        with pytest.raises(native.SufHipError, match="share memory"):
+            kv.append2(b, cache.k, x, x, pool, x, x)
+    assert not any(bool(t.any()) for c in (cache.k, cache.v) for t in (c.e,) + c.b)
