@@ -924,8 +924,9 @@ typedef struct sufhip_rotary {
  * mod 2^64.  d_positions [tokens]; a token whose position is outside
  * [0, positions) is padding and its output rows are left as they were.
  * out[p] with its own strides may be x.p[p] with the same strides (in
- * place); any other overlap is undefined, and so are output rows that
- * overlap each other.  trunc (optional): the open out_0 + out_1 + mask feeds
+ * place), or rows of the same buffer between x's rows, with the same strides;
+ * any other overlap is refused (with other strides wherever the extents meet),
+ * and so are output rows that overlap each other.  trunc (optional): the open out_0 + out_1 + mask feeds
  * this prepared GapARS table gate (no addend), whose outputs trunc->y are
  * written at the output positions instead of out. */
 typedef struct sufhip_rotary2_args {

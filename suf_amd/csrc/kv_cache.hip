@@ -23,6 +23,8 @@
 // so the row's own words are asked for first.
 #include <hip/hip_runtime.h>
 
+#include <utility>
+
 #include "kv_device.hpp"
 #include "suf_hip.h"
 #include "sufhip_internal.hpp"
@@ -317,6 +319,77 @@ int rows_of(const sufhip_rows2& g, const char* what, Rows* out) {
   return SUFHIP_OK;
 }
 
+// Rows of dim words each at p + t ts + h hs (words), t < tokens, h < heads.
+struct Lattice {
+  const uint64_t* p;
+  int64_t ts, hs;
+};
+
+// Whether the extents of two sets of rows meet.
+bool extents_meet(const Lattice& a, const Lattice& b, int tokens, int heads, int dim) {
+  const auto last = [&](const Lattice& r) {
+    return __int128(reinterpret_cast<uintptr_t>(r.p)) +
+           8 * ((__int128(tokens) - 1) * r.ts + (__int128(heads) - 1) * r.hs + dim);
+  };
+  return __int128(reinterpret_cast<uintptr_t>(a.p)) < last(b) &&
+         __int128(reinterpret_cast<uintptr_t>(b.p)) < last(a);
+}
+
+// Whether a row of one set shares a word with a row of another set of the same
+// strides `by` bytes after it; by = 0: with another row of the same set.  Two
+// rows i tokens and j heads apart do if |by + 8 (i ts + j hs)| < 8 dim: for each
+// step along the shorter axis the two steps along the longer one that come
+// nearest decide.
+bool rows_meet(__int128 by, int64_t ts, int64_t hs, int tokens, int heads, int dim) {
+  __int128 n[2] = {tokens, heads}, step[2] = {8 * __int128(ts), 8 * __int128(hs)};
+  const __int128 row = 8 * __int128(dim);
+  if (n[0] > n[1]) {
+    std::swap(n[0], n[1]);
+    std::swap(step[0], step[1]);
+  }
+  if (by == 0) {
+    // Rows side by side, and those as a whole: the usual layouts.
+    const int in = n[1] == 1 || (n[0] > 1 && step[0] < step[1]) ? 0 : 1;
+    if ((n[in] == 1 || step[in] >= row) &&
+        (n[1 - in] == 1 || step[1 - in] >= (n[in] - 1) * step[in] + row))
+      return false;
+  }
+  for (__int128 i = 1 - n[0]; i < n[0]; ++i) {
+    const __int128 at = by + i * step[0];
+    __int128 j = step[1] == 0 ? 0 : -at / step[1];
+    for (__int128 k = j - 1; k <= j + 1; ++k) {
+      if (k <= -n[1] || k >= n[1] || (by == 0 && i == 0 && k == 0)) continue;
+      const __int128 d = at + k * step[1];
+      if (d < row && -d < row) return true;
+    }
+  }
+  return false;
+}
+
+// What a rotation's outputs may not be: rows that share words with each other,
+// with the other party's, or with input rows other than their own.
+int rotary_overlap(const Rows& x, uint64_t* const (&y)[2], int64_t ots, int64_t ohs, int tokens,
+                   int heads, int dim, const char* what) {
+  const auto apart = [](const void* a, const void* b) {
+    return __int128(reinterpret_cast<uintptr_t>(a)) - __int128(reinterpret_cast<uintptr_t>(b));
+  };
+  const Lattice o[2] = {{y[0], ots, ohs}, {y[1], ots, ohs}};
+  if (rows_meet(0, ots, ohs, tokens, heads, dim) || y[0] == y[1] ||
+      (extents_meet(o[0], o[1], tokens, heads, dim) &&
+       rows_meet(apart(y[0], y[1]), ots, ohs, tokens, heads, dim)))
+    return kv_fail(what, "output rows overlap");
+  const bool like = (tokens == 1 || x.ts == ots) && (heads == 1 || x.hs == ohs);
+  for (int p = 0; p < 2; ++p)
+    for (int q = 0; q < 2; ++q) {
+      if (!extents_meet({x.p[p], x.ts, x.hs}, o[q], tokens, heads, dim)) continue;
+      if (like && (x.p[p] == y[q] ||
+                   !rows_meet(apart(x.p[p], y[q]), ots, ohs, tokens, heads, dim)))
+        continue;
+      return kv_fail(what, "outputs overlap other input rows than their own");
+    }
+  return SUFHIP_OK;
+}
+
 }  // namespace
 }  // namespace sufhip
 
@@ -355,6 +428,7 @@ int sufhip_rotary2(const sufhip_rotary2_args* args, void* stream) {
   a.units = units_of(vec ? 2 : 1, a.rot.half, g.dim);
   const uint64_t per_token = uint64_t(g.heads) * uint64_t(a.units);
   SUFHIP_REQUIRE(per_token <= kMaxUnits, "sufhip_rotary2: heads * dim too large");
+  if (int rc = rotary_overlap(a.x, y, a.ots, a.ohs, g.tokens, g.heads, g.dim, what)) return rc;
   a.by_units = fast_div(uint32_t(a.units));
   a.by_heads = fast_div(uint32_t(g.heads));
   const int step = int(kMaxUnits / per_token);  // tokens of one launch

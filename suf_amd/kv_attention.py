@@ -295,7 +295,8 @@ def rotary2(x, rotary, positions, out=None, trunc=None):
     """Rotates both parties' shares x (pair of int64 [tokens, heads, dim], any
     token and head strides) by the tokens' positions (int32 [tokens]; a token
     outside the table is padding and its rows of out stay).  out: a pair like
-    x, which may be x itself, or None for new ones (zeros in padding rows).
+    x, which may be x itself, or None for new ones (zeros in padding rows);
+    its rows overlap no others of x and none of each other.
     trunc: a prepared tasks.Trunc the rotated values go through.  Returns
     out."""
     what = "rotary2"

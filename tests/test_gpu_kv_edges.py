@@ -93,3 +93,50 @@ def test_one_pool_for_keys_and_values_is_refused():
         with pytest.raises(native.SufHipError, match="share memory"):
             kv.append2(b, cache.k, x, x, pool, x, x)
     assert not any(bool(t.any()) for c in (cache.k, cache.v) for t in (c.e,) + c.b)
+
+
+def test_rotary_takes_rows_between_rows():
+    """Outputs in the gaps of their inputs' buffers, in place, in the other
+    party's place: taken exactly where no word is another row's."""
+    from test_kv_arguments import meets
+    rng = np.random.default_rng(11)
+    r = kv.Rotary(i32(rng.integers(-99, 99, (50, 2, 2))), 5, pass_mul=3)
+    table = r.table.cpu().numpy()
+    taken = refusals = 0
+    for _ in range(400):
+        T, H, D = int(rng.integers(1, 4)), int(rng.integers(1, 4)), 5
+        hs = int(rng.choice([5, 6, 10, 15, 20, 40]))
+        ts = int(rng.choice([5, 10, 15, 30, 31, 60, 80]))
+        like = rng.random() < 0.8
+        os = (ts, hs) if like else (int(rng.choice([5, 20, 60])), int(rng.choice([5, 20, 60])))
+        x = [(int(v), ts, hs) for v in rng.choice([0, 300], 2, replace=False)]
+        out = [(b + int(rng.choice([0, 0, 5, 10, 20, 30, 7, 600])), *os) for b, _, _ in x]
+        if rng.random() < 0.3:
+            out = out[::-1]
+        words = ref.words(rng, 1600)
+        buf = dev(words)
+        view = lambda rows: torch.as_strided(buf, (T, H, D), (*rows[1:], 1), rows[0])  # noqa: E731
+        pos = rng.integers(0, 50, T)
+        xs = [u64(view(w).contiguous()) for w in x]
+        if len({w for a in x for w in [a[0] + t * ts + h * hs + i for t in range(T)
+                                       for h in range(H) for i in range(D)]}) < 2 * T * H * D:
+            continue  # the inputs themselves overlap: in place has no meaning
+        want = [ref.rotary(v, table, pos, False, 3, v) for v in xs]
+        bad = meets(T, H, D, x, out)
+        try:
+            kv.rotary2([view(w) for w in x], r, i32(pos), [view(w) for w in out])
+        except native.SufHipError as e:
+            assert "overlap" in str(e)
+            assert bad or not like, (T, H, x, out)
+            refusals += 1
+            continue
+        assert not bad, (T, H, x, out)
+        after = words.copy()
+        for p in range(2):
+            for t in range(T):
+                for h in range(H):
+                    o = out[p][0] + t * os[0] + h * os[1]
+                    after[o:o + D] = want[p][t, h]
+        assert np.array_equal(u64(buf), after), (T, H, x, out)
+        taken += 1
+    assert taken > 50 and refusals > 50

@@ -6,7 +6,7 @@ import pytest
 
 from suf_amd import kv_attention as kv
 from suf_amd import native
-from test_kv_attention import append_args, batch, refused
+from test_kv_attention import append_args, batch, refused, rotary_args
 
 
 @pytest.mark.parametrize("none", [{"seqs": 0}, {"tokens": 0}, {"seqs": 0, "tokens": 0}])
@@ -45,3 +45,76 @@ class Anything:
 def test_append_arguments_without_their_part_are_refused(kw):
     with pytest.raises(ValueError, match="need"):
         kv.append2(Anything(), None, None, None, **kw)
+
+
+# ---- a rotation's outputs ----
+
+def meets(T, H, D, x, out):
+    """By every word: whether an output word is another output's, or an input
+    word of another row or place (x, out: (address, token, head stride) of each
+    party, in words)."""
+    def words(rows):
+        base, ts, hs = rows
+        return {(t, h, i): base + t * ts + h * hs + i
+                for t in range(T) for h in range(H) for i in range(D)}
+    o = [words(r) for r in out]
+    if len(set(o[0].values()) | set(o[1].values())) < 2 * T * H * D:
+        return True
+    for q in o:
+        at = {w: k for k, w in q.items()}
+        for r in x:
+            if any(w in at and at[w] != k for k, w in words(r).items()):
+                return True
+    return False
+
+
+def rotary_of(T, H, D, x, out):
+    a = rotary_args(tokens=T, heads=H, dim=D)
+    a.rot.rot = 0
+    for p in range(2):
+        a.x.p[p], a.out[p] = 8 * x[p][0], 8 * out[p][0]
+    _, a.x.token_stride, a.x.head_stride = x[0]
+    _, a.out_token_stride, a.out_head_stride = out[0]
+    return a
+
+
+BASE = 1 << 20
+OVERLAPS = [
+    # tokens, heads, dim, strides of x, offset and strides of out in party 0's buffer
+    (3, 2, 8, (16, 8), 1, (16, 8)),       # a word further
+    (3, 2, 8, (16, 8), 8, (16, 8)),       # a head further
+    (3, 2, 8, (16, 8), 16, (16, 8)),      # a token further
+    (3, 2, 8, (16, 8), 0, (8, 24)),       # in place with the axes exchanged
+    (3, 2, 8, (48, 8), 12, (48, 8)),      # half a head into the next part
+    (3, 2, 8, (48, 24), 4, (48, 24)),
+    (5, 1, 8, (8, 8), 32, (8, 8)),
+    (1, 4, 6, (0, 6), 3, (0, 6)),
+]
+
+
+@pytest.mark.parametrize("T,H,D,xs,at,os", OVERLAPS)
+def test_rotary_refuses_outputs_over_other_inputs(T, H, D, xs, at, os):
+    x = [(BASE, *xs), (BASE + 5000, *xs)]
+    out = [(BASE + at, *os), (BASE + 9000, *os)]
+    assert meets(T, H, D, x, out)
+    refused("sufhip_rotary2", rotary_of(T, H, D, x, out), "overlap")
+    refused("sufhip_rotary2", rotary_of(T, H, D, x, out[::-1]), "overlap")
+
+
+@pytest.mark.parametrize("T,H,D,ts,hs", [(2, 2, 8, 8, 8), (3, 2, 8, 16, 7), (2, 3, 8, 4, 100),
+                                         (3, 4, 4, 12, 8), (2, 2, 8, 0, 8), (5, 7, 3, 9, 6)])
+def test_rotary_refuses_output_rows_over_each_other(T, H, D, ts, hs):
+    x = [(BASE, 1000, 100), (BASE + 10000, 1000, 100)]
+    out = [(BASE + 20000, ts, hs), (BASE + 30000, ts, hs)]
+    assert meets(T, H, D, x, out)
+    refused("sufhip_rotary2", rotary_of(T, H, D, x, out), "output rows overlap")
+
+
+@pytest.mark.parametrize("by", [0, 1, 8, 60])
+def test_rotary_refuses_one_output_for_both_parties(by):
+    x = [(BASE, 64, 8), (BASE + 10000, 64, 8)]
+    out = [(BASE + 20000, 64, 8), (BASE + 20000 + by, 64, 8)]
+    if meets(2, 6, 8, x, out):
+        refused("sufhip_rotary2", rotary_of(2, 6, 8, x, out), "output rows overlap")
+    else:
+        assert by == 48
