@@ -111,9 +111,12 @@ def _rows(arr, pair, shape, d, what, name, written=False):
         _refuse_pair(pair, shape, d, what, name, False)
     st = t0.stride()
     if st != t1.stride():
-        if shape[2] > 1 and t1.stride()[2] != 1:
+        # A stride along an axis of one says nothing.
+        other = t1.stride()
+        if shape[2] > 1 and other[2] != 1:
             _fail(what, "the values of a head of %s must be neighbours" % name)
-        if st[:2] != t1.stride()[:2] and t0.numel():
+        if t0.numel() and ((st[0] != other[0] and shape[0] > 1) or
+                           (st[1] != other[1] and shape[1] > 1)):
             _fail(what, "both parties' %s must have the same strides" % name)
     if st[2] != 1 and shape[2] > 1:
         _fail(what, "the values of a head of %s must be neighbours" % name)

@@ -3,6 +3,7 @@ taken and what is refused before any device work."""
 import ctypes
 
 import pytest
+import torch
 
 from suf_amd import kv_attention as kv
 from suf_amd import native
@@ -118,3 +119,34 @@ def test_rotary_refuses_one_output_for_both_parties(by):
         refused("sufhip_rotary2", rotary_of(2, 6, 8, x, out), "output rows overlap")
     else:
         assert by == 48
+
+
+# ---- strides of axes of one ----
+
+@pytest.mark.parametrize("shape", [(1, 4, 8), (4, 1, 8), (1, 1, 8), (3, 4, 1), (1, 1, 1), (0, 4, 8)])
+def test_strides_along_an_axis_of_one_do_not_matter(shape):
+    """A single token out of wider rows beside one of its own."""
+    base = torch.zeros(4096, dtype=torch.int64)
+    st = [1]
+    for n in shape[:0:-1]:
+        st.insert(0, st[0] * max(n, 1))
+    odd = [999 if n <= 1 else s for n, s in zip(shape, st)]
+    pair = (torch.as_strided(base, shape, st), torch.as_strided(base, shape, odd, 2048))
+    for p in (pair, pair[::-1]):
+        arr = [0, 0]
+        ts, hs = kv._rows(arr, p, shape, -1, "here", "x", written=True)
+        assert arr == [t.data_ptr() for t in p]
+        assert (shape[0] <= 1 or ts == st[0]) and (shape[1] <= 1 or hs == st[1])
+
+
+@pytest.mark.parametrize("shape,a,b", [((2, 3, 4), (12, 4, 1), (24, 4, 1)),
+                                       ((2, 3, 4), (12, 4, 1), (12, 8, 1)),
+                                       ((1, 3, 4), (12, 4, 1), (12, 8, 1)),
+                                       ((2, 3, 4), (12, 4, 1), (12, 1, 3)),
+                                       ((2, 3, 4), (12, 1, 3), (12, 1, 3))])
+def test_strides_that_differ_are_refused(shape, a, b):
+    base = torch.zeros(256, dtype=torch.int64)
+    for u, v in ((a, b), (b, a)):
+        with pytest.raises(ValueError, match="strides|neighbours"):
+            kv._rows([0, 0], (torch.as_strided(base, shape, u), torch.as_strided(base, shape, v)),
+                     shape, -1, "here", "x")
