@@ -179,8 +179,11 @@ class Rotary:
              torch.int32)
         self.table, self.dim, self.interleaved = table, int(dim), bool(interleaved)
         self.pass_mul, self.device = int(pass_mul), table.get_device()
+        # A table of no elements has no address, and no address is no rotation.
+        self._held = table if table.numel() else torch.zeros(2, dtype=torch.int32,
+                                                             device=table.device)
         r = self.arg = native.RotaryTable()
-        r.d_table = table.data_ptr() or None
+        r.d_table = self._held.data_ptr()
         r.positions, r.rot = table.shape[0], 2 * table.shape[1]
         r.interleaved, r.pass_mul = int(self.interleaved), self.pass_mul
 

@@ -140,3 +140,33 @@ def test_rotary_takes_rows_between_rows():
         assert np.array_equal(u64(buf), after), (T, H, x, out)
         taken += 1
     assert taken > 50 and refusals > 50
+
+
+@pytest.mark.parametrize("rot", [0, 4])
+@pytest.mark.parametrize("given", [False, True])
+def test_append_through_a_table_without_positions(rot, given):
+    """Every place is outside the table: nothing is written."""
+    cache = kv.PagedCache(4, 4, 2, 8)
+    b = cache.extend([cache.open()], [3])
+    x, m = (tuple(dev(ref.words(np.random.default_rng(i), 3, 2, 8)) for _ in range(2))
+            for i in (1, 2))
+    r = kv.Rotary(torch.zeros(0, rot // 2, 2, dtype=torch.int32, device="cuda"), 8)
+    kv.append2(b, cache.k, x, m, cache.v, x, m, rotary=r,
+               positions=i32([0, 1, 2]) if given else None)
+    assert not any(bool(t.any()) for t in (cache.k.e,) + cache.k.b)
+    rows = cache.v.b[0][cache.seqs[0]["pages"][0]].transpose(0, 1)[:3]
+    assert torch.equal(rows, m[0])  # the values are not rotated
+    kv.rotary2(x, r, i32([0, 1, 2]), x)
+    assert np.array_equal(u64(x[0]), ref.words(np.random.default_rng(1), 3, 2, 8))
+
+
+def test_append_through_a_table_that_rotates_nothing():
+    """rot 0 with positions: the words times the table's 1, inside it alone."""
+    cache = kv.PagedCache(4, 4, 1, 8)
+    b = cache.extend([cache.open()], [3])
+    x, m = ([ref.words(np.random.default_rng(i), 3, 1, 8) for _ in range(2)] for i in (1, 2))
+    r = kv.Rotary(torch.zeros(2, 0, 2, dtype=torch.int32, device="cuda"), 8, pass_mul=5)
+    kv.append2(b, cache.k, dev2(x), dev2(m), rotary=r)
+    e = u64(cache.k.e[cache.seqs[0]["pages"][0]])[0]
+    want = np.uint64(5) * (x[0] + x[1])[:, 0] - m[0][:, 0] - m[1][:, 0]
+    assert np.array_equal(e[:2], want[:2]) and not e[2:].any()
