@@ -200,7 +200,8 @@ class Rotary:
           ("parts", s, n, slow, fast)   pairs that turn at most `slow` times in
                             the n trained positions are stretched by s, those
                             that turn at least `fast` times not, the others in
-                            between; the table is scaled by 0.1 ln(s) + 1"""
+                            between; the table is scaled by 0.1 ln(s) + 1, its
+                            1 for the values past the rotated part too"""
         rot = dim if rot is None else rot
         table, one = rotary_table(positions, rot, base, frac_bits, scale, scaling)
         return cls(torch.from_numpy(table).to(device), dim, interleaved, one)
@@ -210,11 +211,15 @@ def rotary_table(positions, rot, base=10000.0, frac_bits=12, scale=1.0, scaling=
     """(int32 [positions, rot / 2, 2], the table's 1): Rotary.build's factors."""
     if rot < 0 or rot % 2 or positions < 0 or not 0 < frac_bits <= 28:
         _fail("rotary_table", "rot must be even, positions >= 0 and frac_bits in [1, 28]")
+    if not 0 < base < math.inf:
+        _fail("rotary_table", "base must be a positive number")
     i = np.arange(rot // 2, dtype=np.float64)
     freq = float(base) ** (-2.0 * i / max(rot, 1))
     if scaling is not None:
+        if len(scaling) != (5 if scaling and scaling[0] == "parts" else 2):
+            _fail("rotary_table", "scaling must be (kind, s) or (\"parts\", s, n, slow, fast)")
         kind, s = scaling[0], float(scaling[1])
-        if s < 1:
+        if not 1 <= s < math.inf:
             _fail("rotary_table", "positions are stretched by a factor of at least 1")
         if kind == "linear":
             freq = freq / s
@@ -223,8 +228,8 @@ def rotary_table(positions, rot, base=10000.0, frac_bits=12, scale=1.0, scaling=
                 freq = (float(base) * s ** (rot / (rot - 2.0))) ** (-2.0 * i / rot)
         elif kind == "parts":
             trained, slow, fast = (float(v) for v in scaling[2:])
-            if not 0 <= slow < fast:
-                _fail("rotary_table", "parts need 0 <= slow < fast")
+            if not (0 <= slow < fast < math.inf and 0 < trained < math.inf):
+                _fail("rotary_table", "parts need positions trained and 0 <= slow < fast")
             turns = trained * freq / (2.0 * math.pi)
             keep = np.clip((turns - slow) / (fast - slow), 0.0, 1.0)
             freq = freq * keep + freq / s * (1.0 - keep)
@@ -232,7 +237,7 @@ def rotary_table(positions, rot, base=10000.0, frac_bits=12, scale=1.0, scaling=
         else:
             _fail("rotary_table", "unknown scaling %r" % (kind,))
     one = scale * (1 << frac_bits)
-    if abs(one) >= 1 << 31:
+    if not abs(one) < (1 << 31) - 0.5:  # or it rounds past a word
         _fail("rotary_table", "scale * 2^frac_bits must stay below 2^31")
     ang = np.arange(positions, dtype=np.float64)[:, None] * freq
     table = np.rint(np.stack([np.cos(ang), np.sin(ang)], -1) * one).astype(np.int32)

@@ -150,3 +150,28 @@ def test_strides_that_differ_are_refused(shape, a, b):
         with pytest.raises(ValueError, match="strides|neighbours"):
             kv._rows([0, 0], (torch.as_strided(base, shape, u), torch.as_strided(base, shape, v)),
                      shape, -1, "here", "x")
+
+
+# ---- rotary tables ----
+
+def test_a_tables_one_fits_its_words():
+    """2^31 - 1 is the largest word; a quarter more rounds to it, 2^31 does not."""
+    top = 2.0 ** 31
+    for one in (top - 1, top - 0.75, 1 - top):
+        t, got = kv.rotary_table(3, 4, frac_bits=20, scale=one / 2.0 ** 20)
+        assert got == round(one) and (t[0, :, 0] == round(one)).all() and abs(t[0, 0, 0]) < top
+    for one in (top - 0.25, top, -top + 0.25, -top, float("nan"), float("inf"), -float("inf")):
+        with pytest.raises(ValueError, match="2\\^31"):
+            kv.rotary_table(3, 4, frac_bits=20, scale=one / 2.0 ** 20)
+
+
+@pytest.mark.parametrize("kw", [{"base": 0.0}, {"base": -2.0}, {"base": float("nan")},
+                                {"base": float("inf")}, {"scaling": ("linear", float("nan"))},
+                                {"scaling": ("linear", float("inf"))},
+                                {"scaling": ("parts", 2.0, float("nan"), 1, 4)},
+                                {"scaling": ("parts", 2.0, 64, 1, float("nan"))},
+                                {"scaling": ("parts", 2.0, 64)}, {"scaling": ()},
+                                {"scaling": ("linear",)}])
+def test_a_tables_angles_are_numbers(kw):
+    with pytest.raises(ValueError, match="rotary_table"):
+        kv.rotary_table(5, 8, **kw)
