@@ -483,6 +483,11 @@ class PagedCache:
     masks with its new tokens."""
 
     def __init__(self, pages, page_tokens, kv_heads, dim, v_dim=None, device="cuda"):
+        if not (pages >= 0 and kv_heads >= 1 and page_tokens >= 1 and
+                page_tokens & (page_tokens - 1) == 0 and 1 <= dim <= native.KV_MAX_DIM and
+                (v_dim is None or 1 <= v_dim <= native.KV_MAX_DIM)):
+            _fail("PagedCache", "pages >= 0, kv_heads >= 1, page_tokens a power of two and heads "
+                                "of 1 to %d values" % native.KV_MAX_DIM)
         shape = (pages, kv_heads, page_tokens)
         self.k, self.v = (
             Pool(*(torch.zeros(shape + (n,), dtype=torch.int64, device=device)

@@ -175,3 +175,13 @@ def test_a_tables_one_fits_its_words():
 def test_a_tables_angles_are_numbers(kw):
     with pytest.raises(ValueError, match="rotary_table"):
         kv.rotary_table(5, 8, **kw)
+
+
+@pytest.mark.parametrize("pages,page,heads,dim,v_dim", [
+    (4, 3, 1, 8, None), (4, 0, 1, 8, None), (4, -4, 1, 8, None), (-1, 4, 1, 8, None),
+    (4, 4, 0, 8, None), (4, 4, 1, 0, None), (4, 4, 1, 257, None), (4, 4, 1, 8, 0),
+    (4, 4, 1, 8, 257)])
+def test_a_cache_of_pages_that_no_call_takes_is_refused(pages, page, heads, dim, v_dim):
+    """When it is made, not at its first step."""
+    with pytest.raises(ValueError, match="PagedCache"):
+        kv.PagedCache(pages, page, heads, dim, v_dim, device="cpu")
