@@ -1469,6 +1469,17 @@ namespace {
 
 bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 unsigned clip(int64_t v, int64_t most) { return unsigned(v < 1 ? 1 : (v < most ? v : most)); }
+// A product of counts, or the largest number: bounds of a launch may be any.
+int64_t times(int64_t a, int64_t b) {
+  int64_t v;
+  return __builtin_mul_overflow(a, b, &v) ? INT64_MAX : v;
+}
+// Row tiles of a sequence with the bounds' most new tokens (no more than the
+// batch has).
+int64_t row_tiles_of(const sufhip_kv_batch& b, int group) {
+  const int64_t rows = times(b.max_new < b.tokens ? b.max_new : b.tokens, group);
+  return rows / 16 + (rows % 16 != 0);
+}
 
 // Compute units of the current device (256 without one: sizes asked for on a
 // host alone); asked of the runtime once a device.
@@ -1542,7 +1553,7 @@ int launch_scores_many(const ProductArgs& a, const dim3& grid, hipStream_t st) {
 template <bool kVec, bool kFull, bool kTrunc>
 int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st) {
   const int chunks = (a.pool.dim + 63) / 64;
-  const int64_t row_tiles = (int64_t(b.max_new) * a.group + 15) / 16;
+  const int64_t row_tiles = row_tiles_of(b, a.group);
   const int64_t zs = int64_t(a.b.seqs) * a.pool.heads;
   const int cus = cu_total();
   // One row tile a sequence streams the keys; with more, keys held as digits
@@ -1552,7 +1563,8 @@ int launch_scores(const ProductArgs& a, const sufhip_kv_batch& b, hipStream_t st
   if (row_tiles <= 1 || chunks > 2) {
     const int64_t tiles =
         b.max_keys > kKeyTile ? (int64_t(b.max_keys) + kKeyTile - 1) / kKeyTile : 1;
-    const dim3 grid(clip(zs * (row_tiles < 1 ? 1 : row_tiles) * (tiles + 1), 2 * int64_t(cus)));
+    const dim3 grid(
+        clip(times(times(zs, row_tiles < 1 ? 1 : row_tiles), tiles + 1), 2 * int64_t(cus)));
     return launch_scores_few<kVec, kFull, kTrunc>(a, grid, chunks, st);
   }
   constexpr int kGroups = kVec ? 2 : 1;  // of one chunk's kernel
@@ -1604,21 +1616,21 @@ struct ValuesPlan {
 ValuesPlan plan_values(const sufhip_kv_batch& b, const sufhip_kv_pool& p, int heads) {
   ValuesPlan v{};
   v.wide = p.page_tokens >= 16;
-  const int64_t rows = int64_t(b.max_new) * (heads / p.kv_heads);
-  v.row_tiles = rows < 1 ? 1 : (rows + 15) / 16;
+  v.row_tiles = row_tiles_of(b, heads / p.kv_heads);
+  if (v.row_tiles < 1) v.row_tiles = 1;
   v.zs = int64_t(b.seqs) * p.kv_heads;
   const int64_t tiles = b.max_keys > kKeyTile ? (int64_t(b.max_keys) + kKeyTile - 1) / kKeyTile : 1;
-  const int64_t items = v.zs * v.row_tiles * ((p.dim + 63) / 64);
-  v.few = tiles >= kFewMinTiles && (v.row_tiles == 1 || 2 * items <= cu_total());
+  const int64_t items = times(times(v.zs, v.row_tiles), (p.dim + 63) / 64);
+  v.few = tiles >= kFewMinTiles && (v.row_tiles == 1 || items <= cu_total() / 2);
   v.waves = v.few || !v.wide || p.dim <= 64 ? 4 : 8;
   v.blocks = (p.dim + 16 * v.waves - 1) / (16 * v.waves);
   if (v.few) {
-    v.groups = clip(v.zs * v.row_tiles * v.blocks * (tiles + 1), 2 * cu_total());
+    v.groups = clip(times(times(times(v.zs, v.row_tiles), v.blocks), tiles + 1), 2 * cu_total());
     v.part_bytes = size_t(v.groups) * 2 * kSlotWords * 8;
     v.info_bytes = size_t(b.tokens) * size_t(heads) * size_t(v.blocks) * 16;
   } else if (v.row_tiles >= kPlanesMinRows && tiles >= kFewMinTiles &&
-             int64_t(b.seqs) * tiles * kKeyTile <= 2 * int64_t(p.pages) * p.page_tokens &&
-             v.zs * tiles * ((p.dim + 15) / 16) <= kPlanesMost / kPlanesBytes) {
+             times(times(b.seqs, tiles), kKeyTile) <= 2 * int64_t(p.pages) * p.page_tokens &&
+             times(times(v.zs, tiles), (p.dim + 15) / 16) <= kPlanesMost / kPlanesBytes) {
     v.room = tiles;
     v.planes_bytes = size_t(v.zs) * size_t(tiles) * size_t((p.dim + 15) / 16) * kPlanesBytes;
   }
@@ -1703,7 +1715,7 @@ int sufhip_kv_values2(const sufhip_kv_product2_args* args, void* stream) {
       hipLaunchKernelGGL(kv_values2_few_kernel<false>, grid, dim3(256), 0, st, va);
     if (int rc = check_launch("kv_values2_few_kernel")) return rc;
     // Slots of an item: over four, more lanes take them.
-    if (v.groups > 4 * v.zs * v.row_tiles * v.blocks)
+    if ((v.groups - 1) / 4 >= times(times(v.zs, v.row_tiles), v.blocks))
       launch_join<16>(va, st);
     else
       launch_join<64>(va, st);

@@ -7,7 +7,7 @@ import torch
 
 from suf_amd import kv_attention as kv
 from suf_amd import native
-from test_kv_attention import append_args, batch, refused, rotary_args
+from test_kv_attention import append_args, batch, pool, product_args, refused, rotary_args
 
 
 @pytest.mark.parametrize("none", [{"seqs": 0}, {"tokens": 0}, {"seqs": 0, "tokens": 0}])
@@ -185,3 +185,25 @@ def test_a_cache_of_pages_that_no_call_takes_is_refused(pages, page, heads, dim,
     """When it is made, not at its first step."""
     with pytest.raises(ValueError, match="PagedCache"):
         kv.PagedCache(pages, page, heads, dim, v_dim, device="cpu")
+
+
+def work_bytes(heads, **kw):
+    a = product_args()
+    batch(a.batch, **kw)
+    pool(a.pool, pages=16, kv_heads=2, dim=128)
+    return native.load().sufhip_kv_values2_work_bytes(ctypes.byref(a.batch),
+                                                      ctypes.byref(a.pool), heads)
+
+
+@pytest.mark.parametrize("heads", [2, 1 << 10, 1 << 20, 1 << 28])
+@pytest.mark.parametrize("seqs", [1, 64, 1 << 16, 1 << 20])
+def test_any_bounds_lay_a_launch_out(heads, seqs):
+    """Products of bounds do not wrap: more new tokens than the batch has are
+    as many as it has, and more keys never take the layout of fewer."""
+    top = 2 ** 31 - 1
+    for keys in (32, 300, 1 << 20, top):
+        at = [work_bytes(heads, seqs=seqs, tokens=1, max_new=n, max_keys=keys)
+              for n in (1, 2, 1 << 16, top)]
+        assert len(set(at)) == 1, at
+        # Two slots of 16 KB for each of two workgroups a CU, 16 bytes a row.
+        assert at[0] <= (2 << 30) + 2 * 2 * 256 * 16384 + heads * 2 * 16, at
