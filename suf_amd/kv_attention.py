@@ -615,7 +615,8 @@ class CachedAttention:
         before = [self.cache.length(s) for s in seqs]
         batch = self.cache.extend(seqs, new)
         try:
-            step = AttentionStep(self, batch, seqs, new)
+            with torch.cuda.device(self.cache.device):
+                step = AttentionStep(self, batch, seqs, new)
         except BaseException:  # out of memory, an interrupt: no tokens without a step
             self.cache.shrink(seqs, before)
             raise
@@ -711,13 +712,18 @@ class AttentionStep:
         out: contiguous [tokens, heads, dim of v].  Returns out.  Raises for a
         step out of its order or of a closed sequence, and warns of a second
         run (a captured one's replays are not seen here)."""
-        att, cache, b, tr = self.att, self.att.cache, self.batch, self.tr
+        att, cache, b = self.att, self.att.cache, self.batch
         T, at = b.tokens, [0, 0]
         _rows(at, q, (T, att.heads, cache.k.dim), b.device, "run", "q")
         _rows(at, k, (T, cache.kv_heads, cache.k.dim), b.device, "run", "k")
         _rows(at, v, (T, cache.kv_heads, cache.v.dim), b.device, "run", "v")
         _ptr2(at, out, (T, att.heads, cache.v.dim), b.device, "run", "out")
         self._take_turn()
+        with torch.cuda.device(b.device):  # the gates' launches go to the current one
+            return self._run(q, k, v, out)
+
+    def _run(self, q, k, v, out):
+        att, cache, b, tr = self.att, self.att.cache, self.batch, self.tr
         prepare_batch(self.truncs())
         rotary2(q, att.q_rotary, self.positions, self.q, trunc=tr["q"])
         append2(b, cache.k, k, self.k_mask, cache.v, v, self.v_mask, rotary=att.k_rotary,

@@ -198,7 +198,7 @@ class SoftmaxBlock:
         self.nexp_table = nexp if nexp is not None else tables.nexp_table(frac_bits)
         self.nexp = spline.SplineGate(self.n, self.nexp_table[0], self.nexp_table[1],
                                       self.prg_state, frac_bits, seed=dealer.word() >> 1,
-                                      nonce=dealer.word())
+                                      nonce=dealer.word(), device=device)
         self.recip = Recip(self.rows, dealer, self.prg_state, frac_bits, recip, recip_iters,
                            device)
         row = np.repeat(np.arange(self.rows), np.diff(self.offsets))

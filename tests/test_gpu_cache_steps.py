@@ -8,7 +8,7 @@ import torch
 
 import oracle_lib as ol
 from suf_amd import kv_attention as kv
-from suf_amd import native
+from suf_amd import native, tasks
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +124,28 @@ def test_a_refused_call_does_not_use_a_step():
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         step.run(q, k, v, out)
+
+
+def test_a_step_is_dealt_and_run_on_the_caches_device(monkeypatch):
+    """Launches that go to the current device and its stream (the gates', the
+    softmax's) are issued with the cache's as the current one."""
+    real, inside, seen = torch.cuda.device, [], []
+
+    class Spy(real):
+        def __enter__(self):
+            inside.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *a):
+            inside.pop()
+            return super().__exit__(*a)
+
+    prepare, gen = kv.prepare_batch, tasks.pfss.trunc_gen
+    monkeypatch.setattr(torch.cuda, "device", Spy)
+    monkeypatch.setattr(kv, "prepare_batch", lambda t: (seen.append(list(inside)), prepare(t))[1])
+    monkeypatch.setattr(tasks.pfss, "trunc_gen",
+                        lambda *a, **k: (seen.append(list(inside)), gen(*a, **k))[1])
+    cache = kv.PagedCache(4, 4, 1, 8, device="cuda:0")
+    att = kv.CachedAttention(cache, 2, STATE, 8)
+    att.deal([cache.open()], [2]).run(*one(att, 2))
+    assert len(seen) > 4 and all(s and s[-1] == 0 for s in seen)

@@ -104,3 +104,27 @@ def test_softmax_chosen_by_positions(monkeypatch):
         make(4096, long_rows=False)
     with pytest.raises(ValueError, match="positions"):
         make((1 << 17) + 1)
+
+
+@pytest.mark.parametrize("make", [
+    lambda: softmax.SoftmaxBlock([0, 3, 5], bytes(128), device="cpu"),
+    lambda: softmax.LongRows([0, 3, 5], bytes(128), 12, [0, 1, 1], device="cpu")])
+def test_a_blocks_material_is_on_its_device(monkeypatch, make):
+    """Every tensor of a block, also those of its exponentials' gate."""
+    monkeypatch.setattr(softmax.torch.cuda, "Stream", lambda device=None: None)
+    monkeypatch.setattr(softmax.spline.pfss, "trunc_gen",
+                        lambda *a: [softmax.torch.empty(8, device=a[-1])] * 2)
+    seen = []
+
+    def walk(v):
+        if isinstance(v, softmax.torch.Tensor):
+            seen.append(v.device.type)
+        elif isinstance(v, (list, tuple)):
+            for w in v:
+                walk(w)
+        elif isinstance(v, dict):
+            walk(list(v.values()))
+        elif type(v).__module__.startswith("suf_amd") and hasattr(v, "__dict__"):
+            walk(list(vars(v).values()))
+    walk(make())
+    assert len(seen) > 50 and set(seen) == {"cpu"}
