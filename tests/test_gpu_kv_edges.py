@@ -170,3 +170,25 @@ def test_append_through_a_table_that_rotates_nothing():
     e = u64(cache.k.e[cache.seqs[0]["pages"][0]])[0]
     want = np.uint64(5) * (x[0] + x[1])[:, 0] - m[0][:, 0] - m[1][:, 0]
     assert np.array_equal(e[:2], want[:2]) and not e[2:].any()
+
+
+def test_append_writes_each_array_of_a_far_page():
+    """Pages whose words lie past 2^31 words, three arrays of their own."""
+    pages, heads, page, dim = 9000, 8, 128, 256  # 18.9 GB an array
+    if torch.cuda.mem_get_info()[0] < 70 << 30:
+        pytest.skip("70 GiB of device memory wanted")
+    rng = np.random.default_rng(1)
+    arrays = [torch.empty((pages, heads, page, dim), dtype=torch.int64, device="cuda")
+              for _ in range(3)]
+    for t in arrays:
+        t[-1].zero_()
+        t[0].zero_()
+    k, m = ([ref.words(rng, 2, heads, dim) for _ in range(2)] for _ in range(2))
+    batch = kv.Batch(i32([0, 1, 2]), i32([page, 1]), i32([[pages - 1], [0]]), tokens=2, max_new=1,
+                     max_keys=page)
+    kv.append2(batch, kv.Pool(*arrays), dev2(k), dev2(m))
+    for t, w in zip(arrays, (k[0] + k[1] - m[0] - m[1], m[0], m[1])):
+        assert np.array_equal(u64(t[-1][:, -1]), w[0]) and np.array_equal(u64(t[0][:, 0]), w[1])
+        assert not bool(t[-1][:, :-1].any()) and not bool(t[0][:, 1:].any())
+    del arrays, t, batch
+    torch.cuda.empty_cache()
