@@ -684,8 +684,10 @@ __global__ void __launch_bounds__(256, kVec ? 2 : 1)
 // barrier a tile).  Two groups of waves over one row tile (128 keys) where a
 // 64-wide chunk is all of a head: each thread then forms half as many digits.
 // Three prompts (1024, 517 after 200, 33), 12 heads of 64 on 4 cached ones:
-// 128 us, 342 MB; without its loads, stores and LDS writes the same work takes
-// seven tenths of that, two thirds of it matrix instructions.
+// 127 to 138 us on different cards; 342 MB needed, 493 moved, for each of the
+// 60 key tiles is loaded by up to 11 workgroups of its row tiles.  Without its
+// loads, stores and LDS writes the same work takes seven tenths of that, two
+// thirds of it matrix instructions.
 template <int kHeld, int kGroups, bool kVec, bool kFull, bool kTrunc, bool kBuffer>
 __global__ void __launch_bounds__(256 * kGroups, kGroups) kv_scores2_kernel(ProductArgs a) {
   constexpr int kRows = 256 * kGroups;  // rows looked up at once
@@ -1257,9 +1259,9 @@ __device__ __forceinline__ bool planes_run(const ProductArgs& a, const Row (&row
 
 // Many rows: a workgroup a row tile, cached head and column block.  Three
 // prompts (1024, 517 after 200, 33 tokens; 12 heads of 64 on 4 cached ones):
-// 123 us and 9 for the digits, 342 MB; the matrix cores are busy for 33% of
-// it.  The longest item is 16 chunks one after another; without the left
-// words' and the digits' traffic a chunk takes six tenths of its time.
+// 123 us and 9 for the digits; 342 MB needed, 419 moved; the matrix cores are
+// busy for 31% of it.  The longest item is 16 chunks one after another; without
+// the left words' and the digits' traffic a chunk takes six tenths of its time.
 template <int kWaves, bool kWide, bool kPlanes>
 __global__ void __launch_bounds__(64 * kWaves, kWide ? 2 : 1) kv_values2_kernel(ValuesArgs va) {
   const ProductArgs& a = va.p;

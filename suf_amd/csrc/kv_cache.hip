@@ -12,13 +12,14 @@
 // of each half; neighbours: 2 kP words in a row), for both parties, so nothing
 // is exchanged between lanes and an output may replace its input.  kP = 2
 // where every piece is 16-byte aligned: 2048 tokens of 32 heads of 128 rotate
-// in 50 us against 52 by single words, 2560 tokens of 8 heads append in 53
-// against 63.
+// in 52 us against 53 by single words (43 against 46 out of the last cache);
+// 2579 tokens append keys and values of 8 heads of 128 in 68 us either way, 57
+// against 59 out of the last cache.
 //
 // Measured: rotation of 2048 x 32 x 128 values 51 us (5.2 TB/s; a copy of
 // 2 GiB reaches 4.85), 1021 x 16 x 80 with 32 of them rotated 10.1; one token
 // of 12 heads 2.2 (the launch).  Append of 2579 tokens, 8 heads of 128, rotated
-// keys and values, 65 us (4.6 TB/s); of eight single tokens, 12 heads, 4.6: a
+// keys and values, 67 us (4.5 TB/s); of eight single tokens, 12 heads, 4.6: a
 // row's sequence, its length and its page are loads that wait for one another,
 // so the row's own words are asked for first.
 #include <hip/hip_runtime.h>

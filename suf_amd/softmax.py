@@ -20,6 +20,9 @@ Every truncation is a GapARS gate with its own key (the reference shares one
 trunc key among a task's truncations; reconstruction is the same exact
 shift); those by f are folded into the launch of the product they truncate
 (a table read, the key-only half prepared on a side stream beforehand).
+LongRows is the softmax for rows whose probabilities and reciprocals are too
+few steps of 2^-f, divided after the product with the values.
+
 Randomness: suf_amd.tasks.Dealer(seed).
 """
 import numpy as np
