@@ -540,7 +540,7 @@ class PagedCache:
         del self.free[ends[-1]:]
         return batch
 
-    def shrink(self, seqs, lens):
+    def _shrink(self, seqs, lens):
         """Takes back what the last extend() gave: seqs[i] has lens[i] tokens
         again, the pages past them are free."""
         for s, n in reversed(list(zip(seqs, lens))):
@@ -567,9 +567,10 @@ class CachedAttention:
 
     Softmax: steps of 2^-frac_bits in probabilities and reciprocals
     (SoftmaxBlock) while an equal share of max_positions keys is at least six
-    of them; a row of n keys so loses up to about 1.4 n 2^-frac_bits of its
-    weight (4 % at 100 keys, 18 % at 600, frac_bits 12).  Beyond, and wherever
-    long_rows asks for it, weights of 24 bits are divided after the product
+    of them; a row of n keys so loses up to about 2 n 2^-frac_bits of its
+    weight when its scores are close to each other (5 % at 100 keys, 29 % at
+    600, frac_bits 12), and long_rows asks for the other form there.  Beyond,
+    and wherever long_rows is given, weights of 24 bits are divided after the product
     with the values (LongRows): off by less than 0.1 % up to 8192 keys, 1.3 %
     at LONG_KEYS; the values have to stay below 2^(38 - frac_bits) over the
     keys in size.
@@ -621,7 +622,7 @@ class CachedAttention:
             with torch.cuda.device(self.cache.device):
                 step = AttentionStep(self, batch, seqs, new)
         except BaseException:  # out of memory, an interrupt: no tokens without a step
-            self.cache.shrink(seqs, before)
+            self.cache._shrink(seqs, before)
             raise
         for _, st, _ in step.turns:
             st["dealt"] += 1
