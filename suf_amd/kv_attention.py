@@ -27,6 +27,7 @@ it by a fresh triple for every new token; its attention is
 src/nn/attention_block.cpp:931-1900.
 """
 import ctypes
+import itertools
 import math
 import warnings
 
@@ -556,6 +557,9 @@ def _shares(dealer, shape, device):
     return tuple(dev(dealer.words(n), device).view(shape) for _ in range(2))
 
 
+_seeds = itertools.count(21)
+
+
 class CachedAttention:
     """Causal attention of new tokens over a PagedCache, grouped heads, with
     rotary positions; Q(frac_bits) shares in and out:
@@ -575,10 +579,14 @@ class CachedAttention:
     at LONG_KEYS; the values have to stay below 2^(38 - frac_bits) over the
     keys in size.
     deal(seqs, new) makes a step's dealer material and room in the cache,
-    step.run(q, k, v, out) computes it."""
+    step.run(q, k, v, out) computes it.
+
+    seed: of the dealer's words, another one for each object unless given (two
+    with one seed, a model's layers say, would open their keys under the same
+    masks)."""
 
     def __init__(self, cache, heads, prg_state, max_positions, frac_bits=12, table_bits=12,
-                 rot=None, base=10000.0, interleaved=False, scaling=None, seed=21,
+                 rot=None, base=10000.0, interleaved=False, scaling=None, seed=None,
                  long_rows=None):
         dim = cache.k.dim
         if heads % cache.kv_heads:
@@ -602,7 +610,7 @@ class CachedAttention:
         # Of rows that the block takes, a reciprocal that holds at every sum.
         self.recip_table = None if self.long_rows else tables.recip_wide_table(
             frac_bits, 2.0 ** max(10, int(max_positions).bit_length()))
-        self.dealer = Dealer(seed)
+        self.dealer = Dealer(next(_seeds) if seed is None else seed)
 
     def deal(self, seqs, new):
         """A step of new[i] tokens of sequence seqs[i].  Its material takes

@@ -130,3 +130,12 @@ def test_a_blocks_material_is_on_its_device(monkeypatch, make):
             walk(list(vars(v).values()))
     walk(make())
     assert len(seen) > 50 and set(seen) == {"cpu"}
+
+
+def test_each_attention_has_a_dealer_of_its_own(monkeypatch):
+    """Layers that open under the same masks tell their difference."""
+    monkeypatch.setattr(kv.Rotary, "build", classmethod(lambda *a, **k: None))
+    a, b, c, d = (kv.CachedAttention(Cache, 1, b"", 64, **kw).dealer
+                  for kw in ({}, {}, {"seed": 5}, {"seed": 5}))
+    wa, wb, wc, wd = (x.words(64) for x in (a, b, c, d))
+    assert not (wa == wb).any() and (wc == wd).all()
