@@ -1116,6 +1116,166 @@ int sufhip_matmul_public2(const uint64_t* d_X0, const uint64_t* d_X1, int M, int
                           uint64_t* d_zhat, uint64_t mask, const sufhip_trunc_epilogue* trunc,
                           void* d_work, size_t work_bytes, void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* The parts of a decoder around its attention, both parties on one GPU:    */
+/* the root-mean-square norm of the residual stream, products with public   */
+/* weights for any number of rows, products grouped by expert, and the      */
+/* weighted sum of the experts' outputs.  The reference has LayerNorm       */
+/* (include/runtime/phase_tasks.hpp:2186-2668) and dense public products    */
+/* (src/nn/matmul_publicW.cpp:17-36) only.                                  */
+/* ---------------------------------------------------------------------- */
+/* Rows of both parties: value c of row r of party p at
+ * p[p][r * row_stride + c] (u64 units, row_stride >= 0). */
+typedef struct sufhip_matrix2 {
+  const uint64_t* p[2];
+  int64_t row_stride;
+} sufhip_matrix2;
+
+/* Both parties' rows as balanced base-256 digits, 8 bits each with the scales
+ * 256^i: value c of row r of party p is the sum over i < 8 of
+ *   256^i * d_digits[((c / 32 * 2 rows + p rows + r) * 8 + i) * 32 + c % 32]
+ * mod 2^64.  Columns up to the next multiple of 32 are zeros.  16-byte
+ * aligned, sufhip_digits2_bytes() bytes. */
+typedef struct sufhip_digits2 {
+  int8_t* d_digits;
+  int rows, cols;
+} sufhip_digits2;
+/* 0 for rows or cols < 1 or past 2^24. */
+size_t sufhip_digits2_bytes(int rows, int cols);
+/* x (rows x cols) as digits. */
+int sufhip_digits2_split(const sufhip_matrix2* x, const sufhip_digits2* out, void* stream);
+
+/* Root-mean-square norm of rows x cols fixed-point values with f fractional
+ * bits, with the residual's addition before it (>> is the floor of a
+ * division, tr_* the table gates that compute it on shares):
+ *   s  = x + residual                     local; written to total, if given
+ *   ms = tr_ms[2](tr_ms[1](inv_len tr_ms[0](sum_c s s)))
+ *   y  = 1 / sqrt(ms + eps)               the chain SUFHIP_CHAIN_RSQRT, n = rows
+ *   o  = tr_norm(s y),  with weight: tr_weight(o weight[c])
+ * so that inv_len / 2^(bits of tr_ms[1] and tr_ms[2]) stands for 1 / cols.
+ * Dealer's material: a, the mask of s, serves both products, since the open
+ * s - a is the same; a2 [rows] are shares of each row's sum of a a, b [rows]
+ * of the mask of y, ab [rows][cols] of a b[row].  Every gate is a prepared
+ * GapARS table gate of at most 14 bits (its y and add are ignored); of the
+ * chain, x and out are ignored.  weight: public, [cols], or NULL.
+ * out (both or neither) and out_digits (d_digits NULL: none) receive o.
+ * total and out may each be x or residual itself (the same addresses and
+ * strides); no other output may meet an input. */
+typedef struct sufhip_rmsnorm2_args {
+  sufhip_matrix2 x;
+  sufhip_matrix2 residual; /* p NULL: none */
+  int rows, cols;
+  uint64_t inv_len, eps;
+  const uint64_t* a[2];
+  const uint64_t* a2[2];
+  const uint64_t* b[2];
+  const uint64_t* ab[2];
+  sufhip_trunc_epilogue tr_ms[3];
+  uint64_t ms_mask[3];
+  sufhip_chain2_args rsqrt;
+  sufhip_trunc_epilogue tr_norm;
+  uint64_t norm_mask;
+  const int64_t* d_weight;
+  sufhip_trunc_epilogue tr_weight;
+  uint64_t weight_mask;
+  uint64_t* total[2];
+  int64_t total_stride;
+  uint64_t* out[2];
+  int64_t out_stride;
+  sufhip_digits2 out_digits;
+} sufhip_rmsnorm2_args;
+int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream);
+
+/* Public weights of one or more matrices K x N ("experts") as `digits`
+ * balanced base-256 digits (sufhip_public_w_digits).  d_planes: an opaque
+ * layout, 16-byte aligned, of sufhip_linear_planes_bytes() bytes (0: bad
+ * extents), written once by sufhip_linear_prepare from d_W
+ * [experts][K][N].  d_bias: [experts][N] in the product's scale, or NULL. */
+typedef struct sufhip_linear_weights {
+  const int8_t* d_planes;
+  int experts, K, N, digits;
+  const int64_t* d_bias;
+} sufhip_linear_weights;
+size_t sufhip_linear_planes_bytes(int experts, int K, int N, int digits);
+int sufhip_linear_prepare(const int64_t* d_W, int experts, int K, int N, int digits,
+                          int8_t* d_planes, void* stream);
+
+#define SUFHIP_ACT_NONE 0
+#define SUFHIP_ACT_RELU 1
+#define SUFHIP_ACT_CUBIC 2
+/* Share x public weight for both parties, for any number of rows, with the
+ * bias, the truncation, an activation and a residual in its epilogue:
+ *   z = x[row] W[e] + bias[e]                   exact mod 2^64
+ *   y = act(trunc(z)),  out = y + residual
+ * Output row i reads x row d_rows[i] (d_rows NULL: row i; a number outside
+ * [0, x_rows) stands for a row of zeros), and the weights of the expert e with
+ * d_offsets[e] <= i < d_offsets[e + 1] ([experts + 1], not decreasing; NULL:
+ * all rows take the one expert).  Rows in no expert are left as they were.
+ * What stands in device memory is not checked; wrong offsets give wrong
+ * values, but no access outside the arrays.
+ * x: u64 shares [x_rows][K], or with x_digits.d_digits their digits.
+ * trunc: a prepared GapARS table gate fed with z_0 + z_1 + mask (no addend; its
+ * y are not used); NULL: z itself goes on, and act must be none.
+ * act: SUFHIP_ACT_RELU takes relu, the ReLU interval LUT of
+ * sufhip_relu_max_round2 (element index: row N + column); SUFHIP_ACT_CUBIC
+ * takes cubic, a SUFHIP_CHAIN_CUBIC chain with n = rows N, whose x and out are
+ * ignored and whose triples are indexed by row N + column.
+ * out (both or neither) with out_stride; out_digits (d_digits NULL: none):
+ * the outputs as digits; a row in no expert leaves its digits as they were.
+ * out may be residual itself (the same addresses and stride); it may meet no
+ * other input.
+ * K <= 65536, digits <= 4, digits K < 2^17; rows, x_rows <= 2^24; rows N <
+ * 2^31; experts <= 4096.  d_work: sufhip_linear2_work_bytes() bytes (asked
+ * for with the call's device current), 16-byte aligned, used by this call
+ * only until it ends; 0 bytes: none needed. */
+typedef struct sufhip_relu_key {
+  const uint8_t* key[2];
+  size_t key_bytes;
+  int intervals; /* <= 64 */
+  uint64_t mask;
+} sufhip_relu_key;
+typedef struct sufhip_linear2_args {
+  sufhip_linear_weights w;
+  sufhip_matrix2 x;
+  sufhip_digits2 x_digits;
+  int x_rows, rows;
+  const int32_t* d_rows;
+  const int32_t* d_offsets;
+  const sufhip_trunc_epilogue* trunc;
+  uint64_t mask;
+  int act;
+  sufhip_relu_key relu;
+  const sufhip_chain2_args* cubic;
+  sufhip_matrix2 residual; /* p NULL: none */
+  uint64_t* out[2];
+  int64_t out_stride;
+  sufhip_digits2 out_digits;
+  void* d_work;
+  size_t work_bytes;
+} sufhip_linear2_args;
+size_t sufhip_linear2_work_bytes(const sufhip_linear2_args* args);
+int sufhip_linear2(const sufhip_linear2_args* args, void* stream);
+
+/* The weighted sum of rows, e.g. of each token's experts:
+ *   out[t] = trunc(sum_{k < each} d_weights[t][k] z[d_slots[t][k]]) + residual[t]
+ * over cols values; a slot outside [0, z_rows) adds nothing.  The weights are
+ * public.  trunc: a prepared GapARS table gate (no addend; its y are not
+ * used), or NULL: the sum itself.  tokens <= 2^24, tokens cols < 2^31,
+ * each <= 1024.  out may be residual itself (the same addresses and stride);
+ * it may meet no other input. */
+typedef struct sufhip_expert_mix2_args {
+  sufhip_matrix2 z;
+  int z_rows, tokens, each, cols;
+  const int32_t* d_slots;
+  const int64_t* d_weights;
+  const sufhip_trunc_epilogue* trunc;
+  uint64_t mask;
+  sufhip_matrix2 residual; /* p NULL: none */
+  uint64_t* out[2];
+  int64_t out_stride;
+} sufhip_expert_mix2_args;
+int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* stream);
+
 /* launch_row_mean_kernel (:169-174): sum >> log2(L) for power-of-two L, else
  * the u64 sum divided by L as a plain integer (the reference's formula). */
 int sufhip_row_mean(const uint64_t* d_mat, int rows, int cols, const int* d_valid_lens,

@@ -1,0 +1,103 @@
+// The weighted sum of rows (sufhip_expert_mix2), both parties:
+//   out[t] = trunc(sum_k weights[t][k] z[slots[t][k]]) + residual[t]
+//
+// A lane takes two neighbouring columns of a token; the row numbers and
+// weights are the same for the whole wave's token mostly and come from the
+// caches.  Memory bounds it.
+#include <hip/hip_runtime.h>
+
+#include "feedforward_device.hpp"
+
+namespace sufhip {
+namespace {
+
+struct MixArgs {
+  Mat2 z, res;
+  int z_rows, tokens, each, cols;
+  const int32_t* slots;
+  const int64_t* weights;
+  TruncEpi epi;
+  uint64_t mask;
+  uint64_t* out[2];
+  int64_t out_stride;
+};
+
+__global__ void __launch_bounds__(256) expert_mix2_kernel(MixArgs a) {
+  const EpiHdrs eh = epi_hdrs(a.epi);
+  const size_t n = size_t(a.tokens) * a.cols;
+  for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += size_t(gridDim.x) * 256) {
+    const int t = int(uint32_t(i) / uint32_t(a.cols)), c = int(uint32_t(i) % uint32_t(a.cols));
+    uint64_t y[2] = {0, 0};
+    for (int k = 0; k < a.each; ++k) {
+      const int row = a.slots[size_t(t) * a.each + k];
+      if (row < 0 || row >= a.z_rows) continue;
+      const uint64_t w = uint64_t(a.weights[size_t(t) * a.each + k]);
+      y[0] += w * a.z.p[0][int64_t(row) * a.z.stride + c];
+      y[1] += w * a.z.p[1][int64_t(row) * a.z.stride + c];
+    }
+    if (a.epi.on) gate2(a.epi, eh, y[0] + y[1] + a.mask, y);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (a.res.p[0]) y[p] += a.res.p[p][int64_t(t) * a.res.stride + c];
+      a.out[p][int64_t(t) * a.out_stride + c] = y[p];
+    }
+  }
+}
+
+}  // namespace
+}  // namespace sufhip
+
+using namespace sufhip;
+
+extern "C" int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* stream) {
+  const char* what = "sufhip_expert_mix2";
+  SUFHIP_REQUIRE(args, "sufhip_expert_mix2: null args");
+  const sufhip_expert_mix2_args& g = *args;
+  if (g.tokens < 0 || g.cols < 0 || g.each < 0 || g.z_rows < 0 || g.tokens > kMaxRows ||
+      g.z_rows > kMaxRows || g.each > 1024 ||
+      uint64_t(g.tokens) * uint64_t(g.cols) >= (uint64_t(1) << 31))
+    return ff_fail(what, "tokens and z_rows in [0, 2^24], each in [0, 1024] and tokens cols < 2^31");
+  if (g.tokens == 0 || g.cols == 0) return SUFHIP_OK;
+  MixArgs a{};
+  a.z_rows = g.z_rows;
+  a.tokens = g.tokens;
+  a.each = g.each;
+  a.cols = g.cols;
+  a.slots = g.d_slots;
+  a.weights = g.d_weights;
+  if (g.each > 0 && (!g.d_slots || !g.d_weights)) return ff_fail(what, "null d_slots or d_weights");
+  if (g.each > 0 && g.z_rows > 0)
+    if (int rc = mat2_of(g.z, g.z_rows, g.cols, what, "z", &a.z)) return rc;
+  if (g.trunc)
+    if (int rc = gate_of(*g.trunc, size_t(g.tokens) * g.cols, what, &a.epi)) return rc;
+  a.mask = g.mask;
+  if ((g.residual.p[0] == nullptr) != (g.residual.p[1] == nullptr))
+    return ff_fail(what, "one share of the residual is missing");
+  if (g.residual.p[0])
+    if (int rc = mat2_of(g.residual, g.tokens, g.cols, what, "residual", &a.res)) return rc;
+  if (!g.out[0] || !g.out[1]) return ff_fail(what, "out is null");
+  if (g.out_stride < 0 || rows_overlap(g.out_stride, g.tokens, g.cols))
+    return ff_fail(what, "output rows overlap");
+  RowSet o[2];
+  for (int p = 0; p < 2; ++p) {
+    a.out[p] = g.out[p];
+    o[p] = {g.out[p], g.out_stride, g.tokens, g.cols};
+  }
+  a.out_stride = g.out_stride;
+  if (sets_meet(o[0], o[1])) return ff_fail(what, "the two shares of out meet");
+  for (int p = 0; p < 2; ++p)
+    for (int q = 0; q < 2; ++q) {
+      if (a.z.p[0] && sets_meet(o[p], row_set(a.z, q, g.z_rows, g.cols)))
+        return ff_fail(what, "out meets z");
+      if (a.res.p[0]) {
+        const RowSet r = row_set(a.res, q, g.tokens, g.cols);
+        if (sets_meet(o[p], r) && !(p == q && same_set(o[p], r)))
+          return ff_fail(what, "out meets the residual without being it");
+      }
+    }
+  const size_t n = size_t(g.tokens) * g.cols;
+  size_t grid = (n + 255) / 256;
+  if (grid > 16384) grid = 16384;
+  hipLaunchKernelGGL(expert_mix2_kernel, dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
+  return check_launch("expert_mix2_kernel");
+}

@@ -107,6 +107,14 @@ _SIGS = {
     "sufhip_kv_scores2": (c_int, [c_vp, c_vp]),
     "sufhip_kv_values2_work_bytes": (c_sz, [c_vp, c_vp, c_int]),
     "sufhip_kv_values2": (c_int, [c_vp, c_vp]),
+    "sufhip_digits2_bytes": (c_sz, [c_int, c_int]),
+    "sufhip_digits2_split": (c_int, [c_vp, c_vp, c_vp]),
+    "sufhip_rmsnorm2": (c_int, [c_vp, c_vp]),
+    "sufhip_linear_planes_bytes": (c_sz, [c_int, c_int, c_int, c_int]),
+    "sufhip_linear_prepare": (c_int, [c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp]),
+    "sufhip_linear2_work_bytes": (c_sz, [c_vp]),
+    "sufhip_linear2": (c_int, [c_vp, c_vp]),
+    "sufhip_expert_mix2": (c_int, [c_vp, c_vp]),
     "sufhip_public_w_digits": (c_int, [c_vp, c_sz]),
     "sufhip_public_w_planes_bytes": (c_sz, [c_int, c_int, c_int]),
     "sufhip_public_w_prepare": (c_int, [c_vp, c_int, c_int, c_int, c_vp, c_vp]),
@@ -335,6 +343,59 @@ class LayerNorm2Args(ctypes.Structure):
                 ("out", c_vp * 2), ("out_planes", XPlanes), ("in_slices", c_vp),
                 ("in_slice_count", c_int), ("tr_in", TruncEpilogue), ("in_mask", c_u64),
                 ("walk_jobs", c_vp), ("walk_count", c_int), ("walk_prg_state", c_vp)]
+
+
+class Matrix2(ctypes.Structure):
+    """sufhip_matrix2 (include/suf_hip.h)."""
+    _fields_ = [("p", c_vp * 2), ("row_stride", c_i64)]
+
+
+class Digits2(ctypes.Structure):
+    """sufhip_digits2 (include/suf_hip.h)."""
+    _fields_ = [("d_digits", c_vp), ("rows", c_int), ("cols", c_int)]
+
+
+class RmsNorm2Args(ctypes.Structure):
+    """sufhip_rmsnorm2_args (include/suf_hip.h)."""
+    _fields_ = [("x", Matrix2), ("residual", Matrix2), ("rows", c_int), ("cols", c_int),
+                ("inv_len", c_u64), ("eps", c_u64), ("a", c_vp * 2), ("a2", c_vp * 2),
+                ("b", c_vp * 2), ("ab", c_vp * 2), ("tr_ms", TruncEpilogue * 3),
+                ("ms_mask", c_u64 * 3), ("rsqrt", Chain2Args), ("tr_norm", TruncEpilogue),
+                ("norm_mask", c_u64), ("d_weight", c_vp), ("tr_weight", TruncEpilogue),
+                ("weight_mask", c_u64), ("total", c_vp * 2), ("total_stride", c_i64),
+                ("out", c_vp * 2), ("out_stride", c_i64), ("out_digits", Digits2)]
+
+
+ACT_NONE, ACT_RELU, ACT_CUBIC = range(3)
+
+
+class LinearWeights(ctypes.Structure):
+    """sufhip_linear_weights (include/suf_hip.h)."""
+    _fields_ = [("d_planes", c_vp), ("experts", c_int), ("K", c_int), ("N", c_int),
+                ("digits", c_int), ("d_bias", c_vp)]
+
+
+class ReluKey(ctypes.Structure):
+    """sufhip_relu_key (include/suf_hip.h)."""
+    _fields_ = [("key", c_vp * 2), ("key_bytes", c_sz), ("intervals", c_int), ("mask", c_u64)]
+
+
+class Linear2Args(ctypes.Structure):
+    """sufhip_linear2_args (include/suf_hip.h)."""
+    _fields_ = [("w", LinearWeights), ("x", Matrix2), ("x_digits", Digits2), ("x_rows", c_int),
+                ("rows", c_int), ("d_rows", c_vp), ("d_offsets", c_vp),
+                ("trunc", ctypes.POINTER(TruncEpilogue)), ("mask", c_u64), ("act", c_int),
+                ("relu", ReluKey), ("cubic", ctypes.POINTER(Chain2Args)), ("residual", Matrix2),
+                ("out", c_vp * 2), ("out_stride", c_i64), ("out_digits", Digits2),
+                ("d_work", c_vp), ("work_bytes", c_sz)]
+
+
+class ExpertMix2Args(ctypes.Structure):
+    """sufhip_expert_mix2_args (include/suf_hip.h)."""
+    _fields_ = [("z", Matrix2), ("z_rows", c_int), ("tokens", c_int), ("each", c_int),
+                ("cols", c_int), ("d_slots", c_vp), ("d_weights", c_vp),
+                ("trunc", ctypes.POINTER(TruncEpilogue)), ("mask", c_u64), ("residual", Matrix2),
+                ("out", c_vp * 2), ("out_stride", c_i64)]
 
 
 class ReluRoundKey(ctypes.Structure):

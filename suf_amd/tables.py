@@ -23,6 +23,8 @@ interval LUT of the gate carries.
                rsqrt_piecewise_affine_init.hpp:11-83) through
                build_rsqrt_affine_eval_suf (src/nn/transformer_layer.cpp:
                193-252): adj = a0 - (a1 * offset >> f), a1: 2 words.
+  rsqrt_wide_table
+               the same beyond its domain (it is a constant past 16): 2 words.
 
 Doubles are rounded with llround semantics (half away from zero); the last
 piece's end (~0 in the reference's interval lists) is the 2^64 wrap.
@@ -289,6 +291,24 @@ def rsqrt_table(frac_bits=12, eps=1.0 / 1024.0, vmax=16.0):
         adj = min(max(adj, INT64_MIN), INT64_MAX)
         pieces.append((start, off, [adj, a1]))
     pieces.sort(key=lambda p: p[0])
+    return _finish(pieces, 2)
+
+
+def rsqrt_wide_table(frac_bits=12, eps=1.0 / 1024.0, vmax=4096.0):
+    """rsqrt_table for mean squares past 16: its chords up to 16, where their
+    slopes, -0.29 2^(f - 1.5 k) on [2^k, 2^(k+1)), are whole words to a few per
+    cent, then constants, each within 4.5 % of 1/sqrt on a quarter of an octave,
+    which a Newton step takes to 0.3 %, up to vmax (a power of two)."""
+    alpha, coeffs = rsqrt_table(frac_bits, eps, min(16.0, vmax))
+    pieces = [(int(a), 0, [int(w) for w in c]) for a, c in zip(alpha, coeffs)][:-1]
+    L = min(16.0, vmax)
+    while L < vmax:
+        for i in range(4):
+            lo, hi = L * 2.0 ** (i / 4), L * 2.0 ** ((i + 1) / 4)
+            pieces.append((_enc(lo, frac_bits), 0,
+                           [_enc(0.5 * (lo ** -0.5 + hi ** -0.5), frac_bits), 0]))
+        L *= 2.0
+    pieces.append((_enc(vmax, frac_bits), 0, [_enc(vmax ** -0.5, frac_bits), 0]))
     return _finish(pieces, 2)
 
 
