@@ -130,20 +130,20 @@ __device__ __forceinline__ void put_output(const LinArgs& a, const EpiHdrs& eh, 
   }
 }
 
-// Few rows: a workgroup of four waves takes one row tile (kT / 2 tokens of
-// both parties), 64 columns and one k-slice; each wave a quarter of the
-// slice's steps, with its own streams of X and W straight into registers, and
-// the four sums are joined through LDS.
+// Few rows: a workgroup of four waves takes one row tile (kT / 2 tokens of both
+// parties), 128 columns, 32 a wave, and one k-slice.  W goes straight into
+// registers, each word read once; X's digits, which the four waves share, are
+// formed on the way into LDS (or come as digits), 64 k at a time, the next
+// chunk's loads in flight under this one's products.
 template <int kT, int J, bool kDigits>
-__global__ void __launch_bounds__(256, 1) linear_skinny_kernel(LinArgs a) {
+__global__ void __launch_bounds__(256, J <= 2 ? 2 : 1) linear_skinny_kernel(LinArgs a) {
   constexpr int kTok = kT / 2;
-  constexpr int kC = kT == 16 ? 4 : 1;      // column fragments
-  constexpr int kWide = kC * kT;            // columns: a weight tile's 64, or half of them
+  constexpr int kC = kT == 16 ? 2 : 1;      // column fragments of a wave
   constexpr int kR = kT == 16 ? 4 : 16;     // accumulator registers of one
-  constexpr int kStep = kT == 16 ? 2 : 1;   // 32-row k-blocks of a step
-  constexpr int kVals = kC * kR;            // values of a lane
+  constexpr int kSteps = kT == 16 ? 1 : 2;  // matrix steps of a chunk
+  constexpr int kPieces = kT / 8;           // of 16 bytes, a thread stores in a chunk
   typedef typename std::conditional<kT == 16, v4acc, v16acc>::type Acc;
-  __shared__ uint64_t red[4][kVals][64];
+  __shared__ __align__(16) int8_t lds[2][kSteps * 8 * 1024];  // [step][digit][lane] of 16 k
   const int l = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
   const int total = int(gridDim.x);
@@ -151,28 +151,100 @@ __global__ void __launch_bounds__(256, 1) linear_skinny_kernel(LinArgs a) {
   // Row tiles of the same weights run on one XCD, one after the other.
   if (total % 8 == 0) id = (id % 8) * (total / 8) + id / 8;
   const int ti = id % a.tiles, rest = id / a.tiles;
-  const int slice = rest % a.slices, c0 = rest / a.slices * kWide, g = c0 / kCols;
+  const int slice = rest % a.slices, c0 = rest / a.slices * 128 + 32 * w;
   const RowTile rt = row_tile(a, ti, kTok);
   if (rt.e < 0 || rt.begin >= rt.end) return;  // the whole workgroup
   const EpiHdrs eh = epi_hdrs(a.epi);
-  // This lane's row of the left operand.
-  const int r = l % kT, kl = l / kT;
+  // The row that this thread brings to LDS: a run of kT / 4 words of it, or
+  // (digits) its pieces of 16 bytes.
+  const int r = kDigits ? l % kT : int(threadIdx.x) / (256 / kT);
+  const int kq = int(threadIdx.x) % (256 / kT) * (kT / 4);  // first word in the chunk
   const int p = (r >> 1) & 1, t = 2 * (r >> 2) + (r & 1);
   int xr = rt.begin + t;
   bool live = xr < rt.end;
   if (live && a.map) xr = a.map[xr];
   live = live && xr >= 0 && xr < a.x_rows;
-  const uint64_t* xrow = (p ? a.x.p[1] : a.x.p[0]) + (live && !kDigits ? int64_t(xr) * a.x.stride : 0);
-  const int8_t* drow =
-      kDigits ? a.xd + (live ? (size_t(p) * a.x_rows + xr) * 256 + 16 * (kl & 1) : 0) : nullptr;
+  const uint64_t* xrow =
+      kDigits ? nullptr : (p ? a.x.p[1] : a.x.p[0]) + (live ? int64_t(xr) * a.x.stride : 0) + kq;
+  const int8_t* drow = kDigits ? a.xd + (live ? (size_t(p) * a.x_rows + xr) * 256 : 0) : nullptr;
   const size_t dstep = size_t(2) * a.x_rows * 256;
+  // This wave's columns; past the last weight tile it repeats the last one.
+  const int g = c0 / kCols < a.groups ? c0 / kCols : a.groups - 1;
   const int8_t* wl = a.w + size_t(rt.e) * a.expert_bytes + size_t(g) * a.kb * (J * kTileBytes) +
                      (c0 % kCols) * 32 +
                      (kT == 16 ? (l >> 5) * (J * kTileBytes) + (l & 15) * 32 + ((l >> 4) & 1) * 16
                                : (l & 31) * 32 + (l >> 5) * 16);
-  const int steps = a.kb / kStep;
-  const int s0 = int(int64_t(steps) * (slice * 4 + w) / (a.slices * 4));
-  const int s1 = int(int64_t(steps) * (slice * 4 + w + 1) / (a.slices * 4));
+  const int chunks = a.kb / 2;
+  const int q0 = int(int64_t(chunks) * slice / a.slices);
+  const int q1 = int(int64_t(chunks) * (slice + 1) / a.slices);
+  struct Wreg {
+    v4i v[kSteps][kC][J];
+  };
+  u64x2u xw[kDigits ? 1 : kT / 8];
+  v4i xd[kDigits ? kPieces : 1];
+  auto load_w = [&](Wreg& g, int q) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          g.v[s][c][j] = load16(wl + (size_t(q) * 2 + s) * (J * kTileBytes) + j * kTileBytes +
+                                c * (kT * 32));
+  };
+  auto load_x = [&](int q) {
+    if constexpr (kDigits) {
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        // Piece threadIdx + 256 u: step, digit and lane of the fragment.
+        const int piece = int(threadIdx.x) + 256 * u;
+        const int i = (piece >> 6) & 7;
+        const int sixteen = kT == 16 ? l / 16 : 2 * (piece >> 9) + l / 32;
+        const int kb = 2 * q + (sixteen >> 1);
+        xd[u] = v4i{0, 0, 0, 0};
+        if (live && 32 * kb < a.K)
+          xd[u] = load16(drow + size_t(kb) * dstep + 32 * i + 16 * (sixteen & 1));
+      }
+    } else {
+      const int k = 64 * q + kq;
+#pragma unroll
+      for (int u = 0; u < kT / 8; ++u) xw[u] = u64x2u{0, 0};
+      if (live && k + kT / 4 <= a.K) {
+#pragma unroll
+        for (int u = 0; u < kT / 8; ++u)
+          xw[u] = *reinterpret_cast<const u64x2u*>(xrow + 64 * q + 2 * u);
+      } else if (live) {
+#pragma unroll
+        for (int u = 0; u < kT / 8; ++u) {
+          if (k + 2 * u < a.K) xw[u][0] = xrow[64 * q + 2 * u];
+          if (k + 2 * u + 1 < a.K) xw[u][1] = xrow[64 * q + 2 * u + 1];
+        }
+      }
+    }
+  };
+  auto store_x = [&](int buf) {
+    if constexpr (kDigits) {
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u)
+        *reinterpret_cast<v4i*>(&lds[buf][(int(threadIdx.x) + 256 * u) * 16]) = xd[u];
+    } else {
+      const int lane = (kT == 16 ? kq >> 4 : (kq >> 4) & 1) * kT + r;
+      int8_t* at = &lds[buf][(kT == 16 ? 0 : kq >> 5) * 8192 + lane * 16 + (kq & 15)];
+      uint32_t d[kT / 16][8];
+#pragma unroll
+      for (int u = 0; u < kT / 16; ++u) {
+        const uint64_t v[4] = {xw[2 * u][0], xw[2 * u][1], xw[2 * u + 1][0], xw[2 * u + 1][1]};
+        digits_of4(v, d[u]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (kT == 16)
+          *reinterpret_cast<uint32_t*>(at + 1024 * i) = d[0][i];
+        else
+          *reinterpret_cast<uint2*>(at + 1024 * i) = make_uint2(d[0][i], d[1][i]);
+      }
+    }
+  };
   Acc acc[kC][8];
 #pragma unroll
   for (int c = 0; c < kC; ++c)
@@ -180,119 +252,89 @@ __global__ void __launch_bounds__(256, 1) linear_skinny_kernel(LinArgs a) {
     for (int s = 0; s < 8; ++s)
 #pragma unroll
       for (int q = 0; q < kR; ++q) acc[c][s][q] = 0;
-  struct Stage {
-    u64x2u x[8];       // 16 words of the row, or
-    v4i d[8];          // their digits
-    v4i w[kC][J];
-  };
-  auto load = [&](Stage& st, int step) {
+  auto products = [&](const Wreg& g, int buf) {
 #pragma unroll
-    for (int c = 0; c < kC; ++c)
+    for (int s = 0; s < kSteps; ++s) {
+      v4i d[8];
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-        st.w[c][j] = load16(wl + size_t(step) * (kStep * J * kTileBytes) + j * kTileBytes +
-                            c * (kT * 32));
-    const int k0 = 32 * kStep * step + 16 * kl;
-    if constexpr (kDigits) {
-      const int kbi = k0 >> 5;
-      const bool in = live && 32 * kbi < a.K;
+      for (int i = 0; i < 8; ++i)
+        d[i] = *reinterpret_cast<const v4i*>(&lds[buf][s * 8192 + i * 1024 + 16 * l]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) st.d[i] = v4i{0, 0, 0, 0};
-      if (in) {
+      for (int c = 0; c < kC; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) st.d[i] = load16(drow + size_t(kbi) * dstep + 32 * i);
-      }
-    } else {
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int q = 0; q < 8; ++q) st.x[q] = u64x2u{0, 0};
-      if (live && k0 + 16 <= a.K) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) st.x[q] = *reinterpret_cast<const u64x2u*>(xrow + k0 + 2 * q);
-      } else if (live) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (k0 + 2 * q < a.K) st.x[q][0] = xrow[k0 + 2 * q];
-          if (k0 + 2 * q + 1 < a.K) st.x[q][1] = xrow[k0 + 2 * q + 1];
-        }
-      }
+          for (int i = 0; i + j < 8; ++i) {
+            if constexpr (kT == 16)
+              acc[c][i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(d[i], g.v[s][c][j],
+                                                                    acc[c][i + j], 0, 0, 0);
+            else
+              acc[c][i + j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(d[i], g.v[s][c][j],
+                                                                    acc[c][i + j], 0, 0, 0);
+          }
     }
   };
-  auto products = [&](const Stage& st) {
-    v4i d[8];
-    if constexpr (kDigits) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] = st.d[i];
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint64_t v[4] = {st.x[2 * q][0], st.x[2 * q][1], st.x[2 * q + 1][0],
-                               st.x[2 * q + 1][1]};
-        uint32_t o[8];
-        digits_of4(v, o);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i][q] = int(o[i]);
-      }
+  auto step = [&](int q, const Wreg& cur, Wreg& next) {
+    if (q + 1 < q1) {
+      load_w(next, q + 1);
+      load_x(q + 1);
     }
-#pragma unroll
-    for (int c = 0; c < kC; ++c)
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int i = 0; i + j < 8; ++i) {
-          if constexpr (kT == 16)
-            acc[c][i + j] =
-                __builtin_amdgcn_mfma_i32_16x16x64_i8(d[i], st.w[c][j], acc[c][i + j], 0, 0, 0);
-          else
-            acc[c][i + j] =
-                __builtin_amdgcn_mfma_i32_32x32x32_i8(d[i], st.w[c][j], acc[c][i + j], 0, 0, 0);
-        }
+    products(cur, (q - q0) & 1);
+    if (q + 1 < q1) store_x((q + 1 - q0) & 1);
+    __syncthreads();
   };
-  if (s0 < s1) {
-    Stage sa, sb;
-    load(sa, s0);
-    int st = s0;
-    for (; st + 2 < s1; st += 2) {
-      load(sb, st + 1);
-      products(sa);
-      load(sa, st + 2);
-      products(sb);
-    }
-    if (st + 1 < s1) {
-      load(sb, st + 1);
-      products(sa);
-      products(sb);
-    } else {
-      products(sa);
+  if (q0 < q1) {
+    Wreg wa, wb;
+    load_w(wa, q0);
+    load_x(q0);
+    store_x(0);
+    __syncthreads();
+    for (int q = q0; q < q1; q += 2) {
+      step(q, wa, wb);
+      if (q + 1 < q1) step(q + 1, wb, wa);
     }
   }
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const int col = c0 + c * kT + l % kT;
+    if (col >= a.N) continue;
+#pragma unroll
+    for (int b = 0; b < kR / 4; ++b) {
+      uint64_t v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        v[q] = 0;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) v[q] += uint64_t(int64_t(acc[c][s][4 * b + q])) << (8 * s);
+      }
+      const int pairs = kT == 16 ? l / 16 : 2 * b + l / 32;  // of tokens, in the tile
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = rt.begin + 2 * pairs + h;
+        if (row < rt.end) put_output(a, eh, slice, rt.e, row, col, v[h], v[2 + h]);
+      }
+    }
+  }
+}
+
+// acc += a b with the accumulator in the accumulation registers for the whole
+// loop.  (The compiler keeps 256 of them in vector registers and copies them
+// to and from the others in every step.)  The wait before it covers a vector
+// instruction's write of an operand; between two products into one
+// accumulator lie at least six others.
+__device__ __forceinline__ void mfma_acc(v16acc& acc, v4i a, v4i b) {
+  asm volatile("s_nop 1\n\tv_mfma_i32_32x32x32_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+
+// Between mfma_acc and other uses of the accumulators: the last products' (or
+// the zeros') writes are done.  The ties keep every such use behind the wait.
+template <int kC, int kS>
+__device__ __forceinline__ void acc_settle(v16acc (&acc)[kC][kS]) {
+  asm volatile("s_nop 15\n\ts_nop 15" ::);
 #pragma unroll
   for (int c = 0; c < kC; ++c)
 #pragma unroll
-    for (int q = 0; q < kR; ++q) {
-      uint64_t v = 0;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) v += uint64_t(int64_t(acc[c][s][q])) << (8 * s);
-      red[w][c * kR + q][l] = v;
-    }
-  __syncthreads();
-  // Wave w joins a quarter of the values: fours of two tokens and both parties.
-#pragma unroll
-  for (int u = 0; u < kVals / 16; ++u) {
-    const int q0 = w * (kVals / 4) + 4 * u;
-    const int c = q0 / kR, qr = q0 % kR;
-    const int col = c0 + c * kT + (l % kT);
-    const int pairs = kT == 16 ? l / 16 : 2 * (qr / 4) + l / 32;  // of tokens, in the tile
-    uint64_t v[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      v[q] = red[0][q0 + q][l] + red[1][q0 + q][l] + red[2][q0 + q][l] + red[3][q0 + q][l];
-    if (col >= a.N) continue;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = rt.begin + 2 * pairs + h;
-      if (row < rt.end) put_output(a, eh, slice, rt.e, row, col, v[h], v[2 + h]);
-    }
-  }
+    for (int s = 0; s < kS; ++s) asm volatile("" : "+a"(acc[c][s]));
 }
 
 // Many rows: a workgroup takes 32 tokens of both parties (two tiles of 32
@@ -327,7 +369,8 @@ __global__ void __launch_bounds__(256, 1) linear_tile_kernel(LinArgs a) {
   bool live = xr < rt.end;
   if (live && a.map) xr = a.map[xr];
   live = live && xr >= 0 && xr < a.x_rows;
-  const int8_t* xl = a.xd + (live ? (size_t(p) * a.x_rows + xr) * 256 + half * 16 + n * 128 : 0);
+  // A row that is not there reads row 0 and is zeros in LDS.
+  const int8_t* xl = a.xd + (live ? (size_t(p) * a.x_rows + xr) * 256 : 0) + half * 16 + n * 128;
   const size_t xstep = size_t(2) * a.x_rows * 256;
   const int kb_x = (a.K + 31) / 32;
   const int8_t* wl[J];
@@ -341,24 +384,45 @@ __global__ void __launch_bounds__(256, 1) linear_tile_kernel(LinArgs a) {
   }
   const int b0 = int(int64_t(kb_x) * slice / a.slices);
   const int b1 = int(int64_t(kb_x) * (slice + 1) / a.slices);
-  v4i xv[4], wv[J];
-  auto load = [&](int kb) {
-    kb = kb < b1 ? kb : b1 - 1;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const v4i v = load16(xl + size_t(kb) * (live ? xstep : 0) + 32 * q);
-      xv[q] = live ? v : v4i{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int j = 0; j < J; ++j) wv[j] = load16(wl[j] + size_t(kb) * (J * kTileBytes));
+  // Registers for the k-blocks on their way to LDS (two ahead of the products)
+  // and for the fragments of this step and the next.
+  struct Staged {
+    v4i x[4], w[J];
   };
-  auto store = [&](int buf) {
+  struct Frags {
+    v4i x[8], w[2][J];
+  };
+  auto load_one = [&](Staged& g, int kb, int q) {
+    kb = kb < b1 ? kb : b1 - 1;
+    if (q < 4)
+      g.x[q] = load16(xl + size_t(kb) * xstep + 32 * q);
+    else
+      g.w[q - 4] = load16(wl[q - 4] + size_t(kb) * (J * kTileBytes));
+  };
+  auto store_one = [&](const Staged& g, int kb, int q) {
+    int8_t* at = lds[(kb - b0) & 1] + 16 * l;
+    if (q < 4)  // zeros for a row that is not there and past the last k-block
+      *reinterpret_cast<v4i*>(at + (m * 8 + n * 4 + q) * 1024) =
+          live && kb < b1 ? g.x[q] : v4i{0, 0, 0, 0};
+    else
+      *reinterpret_cast<v4i*>(at + (16 + w * J + q - 4) * 1024) = g.w[q - 4];
+  };
+  auto read_one = [&](Frags& f, int kb, int q) {
+    const int8_t* at = lds[(kb - b0) & 1] + 16 * l;
+    if (q < 8)
+      f.x[q] = *reinterpret_cast<const v4i*>(at + (m * 8 + q) * 1024);
+    else
+      f.w[(q - 8) / J][(q - 8) % J] = *reinterpret_cast<const v4i*>(
+          at + (16 + (n * J + (q - 8) % J) * 2 + (q - 8) / J) * 1024);
+  };
+  constexpr int kMoves = 4 + J, kReads = 8 + 2 * J;
+  auto load = [&](Staged& g, int kb) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<v4i*>(&lds[buf][(m * 8 + n * 4 + q) * 1024 + 16 * l]) = xv[q];
+    for (int q = 0; q < kMoves; ++q) load_one(g, kb, q);
+  };
+  auto store = [&](const Staged& g, int kb) {
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-      *reinterpret_cast<v4i*>(&lds[buf][(16 + w * J + j) * 1024 + 16 * l]) = wv[j];
+    for (int q = 0; q < kMoves; ++q) store_one(g, kb, q);
   };
   v16acc acc[2][8];
 #pragma unroll
@@ -367,38 +431,53 @@ __global__ void __launch_bounds__(256, 1) linear_tile_kernel(LinArgs a) {
     for (int s = 0; s < 8; ++s)
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[c][s][q] = 0;
-  if (b0 < b1) {
-    load(b0);
-    store(0);
-    load(b0 + 1);
+  // Step kb (its fragments in f): between its products the next step's
+  // fragments are read, the k-block after that is stored and another load of
+  // two steps ahead is issued.  Buffer kb & 1 held this step's k-block, whose
+  // readers passed the barrier at the end of the last step.
+  auto step = [&](int kb, const Frags& f, Frags& next, Staged& g) {
+    constexpr int kMfmas = 2 * (8 * J - J * (J - 1) / 2);
+    constexpr int kChores = kReads + 2 * kMoves;
+    int at = 0, done = 0;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i + j < 8; ++i) {
+          mfma_acc(acc[c][i + j], f.x[i], f.w[c][j]);
+          ++at;
+#pragma unroll
+          for (; done < at * kChores / kMfmas; ++done) {
+            if (done < kReads)
+              read_one(next, kb + 1, done);
+            else if (done < kReads + kMoves)
+              store_one(g, kb + 2, done - kReads);
+            else
+              load_one(g, kb + 4, done - kReads - kMoves);
+          }
+        }
     __syncthreads();
-    for (int kb = b0; kb < b1; ++kb) {
-      const int buf = (kb - b0) & 1;
-      // The other buffer's readers passed the barrier at the end of the last
-      // step.
-      store(buf ^ 1);
-      load(kb + 2);
-      v4i x[8], wf[2][J];
+  };
+  // Steps in pairs; past the last k-block X is zeros.
+  Staged ga, gb;
+  Frags fa, fb;
+  load(ga, b0);
+  load(gb, b0 + 1);
+  store(ga, b0);
+  load(ga, b0 + 2);
+  store(gb, b0 + 1);
+  load(gb, b0 + 3);
+  __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = *reinterpret_cast<const v4i*>(&lds[buf][(m * 8 + i) * 1024 + 16 * l]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-          wf[c][j] = *reinterpret_cast<const v4i*>(
-              &lds[buf][(16 + (n * J + j) * 2 + c) * 1024 + 16 * l]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-          for (int i = 0; i + j < 8; ++i)
-            acc[c][i + j] =
-                __builtin_amdgcn_mfma_i32_32x32x32_i8(x[i], wf[c][j], acc[c][i + j], 0, 0, 0);
-      __syncthreads();
-    }
+  for (int q = 0; q < kReads; ++q) read_one(fa, b0, q);
+  __syncthreads();  // buffer 0 is stored to in the first step
+  acc_settle(acc);
+  for (int kb = b0; kb < b1; kb += 2) {
+    step(kb, fa, fb, ga);
+    step(kb + 1, fb, fa, gb);
   }
+  acc_settle(acc);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int col = (2 * gp + n) * kCols + 32 * c + (l & 31);
@@ -652,9 +731,9 @@ Plan plan_linear(const sufhip_linear2_args& g) {
   p.tiles = g.d_offsets ? g.rows / per + (experts < g.rows ? experts : g.rows)
                         : (g.rows + per - 1) / per;
   const int cus = device_cus();
-  p.col_tiles = p.tile ? (groups + 1) / 2 : groups * (p.t == 32 ? 2 : 1);
+  p.col_tiles = (groups + 1) / 2;
   const int64_t wgs = int64_t(p.tiles) * p.col_tiles;
-  const int most = p.tile ? kb / 8 : (kb / 2 + 3) / 4;
+  const int most = p.tile ? kb / 8 : kb / 4;
   int64_t s = p.tile ? cus / wgs : (2 * cus + wgs - 1) / wgs;
   if (s > most) s = most;
   if (s > 16) s = 16;
