@@ -1219,7 +1219,8 @@ int sufhip_linear_prepare(const int64_t* d_W, int experts, int K, int N, int dig
  * act: SUFHIP_ACT_RELU takes relu, the ReLU interval LUT of
  * sufhip_relu_max_round2 (element index: row N + column); SUFHIP_ACT_CUBIC
  * takes cubic, a SUFHIP_CHAIN_CUBIC chain with n = rows N, whose x and out are
- * ignored and whose triples are indexed by row N + column.
+ * ignored and whose triples, indexed by row N + column, are plain arrays (no
+ * index, multiplier, shift or negation, all of stride 1 or all of stride 3).
  * out (both or neither) with out_stride; out_digits (d_digits NULL: none):
  * the outputs as digits; a row in no expert leaves its digits as they were.
  * out may be residual itself (the same addresses and stride); it may meet no

@@ -22,24 +22,60 @@ struct MixArgs {
   int64_t out_stride;
 };
 
+typedef uint64_t u64x2u __attribute__((ext_vector_type(2), aligned(8)));
+
+// Two neighbours from column c on, the second one if it is there.
+__device__ __forceinline__ u64x2u load2(const uint64_t* p, bool two) {
+  if (two) return *reinterpret_cast<const u64x2u*>(p);
+  return u64x2u{p[0], 0};
+}
+
 __global__ void __launch_bounds__(256) expert_mix2_kernel(MixArgs a) {
   const EpiHdrs eh = epi_hdrs(a.epi);
-  const size_t n = size_t(a.tokens) * a.cols;
+  const uint32_t half = uint32_t(a.cols + 1) / 2;
+  const size_t n = size_t(a.tokens) * half;
   for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += size_t(gridDim.x) * 256) {
-    const int t = int(uint32_t(i) / uint32_t(a.cols)), c = int(uint32_t(i) % uint32_t(a.cols));
-    uint64_t y[2] = {0, 0};
-    for (int k = 0; k < a.each; ++k) {
-      const int row = a.slots[size_t(t) * a.each + k];
-      if (row < 0 || row >= a.z_rows) continue;
-      const uint64_t w = uint64_t(a.weights[size_t(t) * a.each + k]);
-      y[0] += w * a.z.p[0][int64_t(row) * a.z.stride + c];
-      y[1] += w * a.z.p[1][int64_t(row) * a.z.stride + c];
+    const int t = int(uint32_t(i) / half), c = 2 * int(uint32_t(i) % half);
+    const bool two = c + 1 < a.cols;
+    const int32_t* slots = a.slots + size_t(t) * a.each;
+    const int64_t* weights = a.weights + size_t(t) * a.each;
+    uint64_t y[2][2] = {};
+    // Two rows at a time, their loads together; a row that is not there has
+    // weight 0 and reads row 0.
+    for (int k = 0; k < a.each; k += 2) {
+      const int k1 = k + 1 < a.each ? k + 1 : k;
+      int r0 = slots[k], r1 = slots[k1];
+      uint64_t w0 = uint64_t(weights[k]), w1 = k1 > k ? uint64_t(weights[k1]) : 0;
+      if (r0 < 0 || r0 >= a.z_rows) r0 = 0, w0 = 0;
+      if (r1 < 0 || r1 >= a.z_rows) r1 = 0, w1 = 0;
+      u64x2u v[2][2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        v[p][0] = load2(a.z.p[p] + int64_t(r0) * a.z.stride + c, two);
+        v[p][1] = load2(a.z.p[p] + int64_t(r1) * a.z.stride + c, two);
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) y[h][p] += w0 * v[p][0][h] + w1 * v[p][1][h];
     }
-    if (a.epi.on) gate2(a.epi, eh, y[0] + y[1] + a.mask, y);
+    u64x2u res[2] = {u64x2u{0, 0}, u64x2u{0, 0}};
+    if (a.res.p[0]) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) res[p] = load2(a.res.p[p] + int64_t(t) * a.res.stride + c, two);
+    }
+    if (a.epi.on) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) gate2(a.epi, eh, y[h][0] + y[h][1] + a.mask, y[h]);
+    }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      if (a.res.p[0]) y[p] += a.res.p[p][int64_t(t) * a.res.stride + c];
-      a.out[p][int64_t(t) * a.out_stride + c] = y[p];
+      uint64_t* o = a.out[p] + int64_t(t) * a.out_stride + c;
+      if (two) {
+        *reinterpret_cast<u64x2u*>(o) = u64x2u{y[0][p] + res[p][0], y[1][p] + res[p][1]};
+      } else {
+        o[0] = y[0][p] + res[p][0];
+      }
     }
   }
 }
@@ -61,7 +97,7 @@ extern "C" int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* str
   MixArgs a{};
   a.z_rows = g.z_rows;
   a.tokens = g.tokens;
-  a.each = g.each;
+  a.each = g.z_rows > 0 ? g.each : 0;  // without rows nothing is added
   a.cols = g.cols;
   a.slots = g.d_slots;
   a.weights = g.d_weights;
@@ -95,7 +131,7 @@ extern "C" int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* str
           return ff_fail(what, "out meets the residual without being it");
       }
     }
-  const size_t n = size_t(g.tokens) * g.cols;
+  const size_t n = size_t(g.tokens) * size_t((g.cols + 1) / 2);
   size_t grid = (n + 255) / 256;
   if (grid > 16384) grid = 16384;
   hipLaunchKernelGGL(expert_mix2_kernel, dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);

@@ -501,13 +501,27 @@ __global__ void __launch_bounds__(256, 1) linear_tile_kernel(LinArgs a) {
 }
 
 // The epilogue's own launch, where k-slices have to be summed, an activation
-// follows or the outputs go out as digits.
-constexpr int kEpiBlock = 512;
-using EpiAes = AesLds2<32>;
+// follows or the outputs go out as digits.  An activation's keystream binds a
+// large one (two AES blocks an element for a cubic): then workgroups of 1024
+// lanes with the four-table AES (128 KB of LDS), one a CU, else 512 lanes on
+// two tables.
+template <bool kWide>
+struct EpiCfg {
+  static constexpr int kBlock = 512;
+  using Aes = AesLds2<32>;
+  static constexpr int kTabWords = Aes::kSpanWords;
+};
+template <>
+struct EpiCfg<true> {
+  static constexpr int kBlock = 1024;
+  using Aes = AesLds4;
+  static constexpr int kTabWords = Aes::kWords;
+};
 
 // The ReLU's rows (c0, c1) at the masked open xh, both parties: c0 + c1 xh.
+template <class Aes>
 __device__ __forceinline__ void relu2(const ChainArgs& A, const ChainLds& L, const ChainKeyInfo& K,
-                                      const EpiAes& aes, size_t i, uint64_t (&y)[2]) {
+                                      const Aes& aes, size_t i, uint64_t (&y)[2]) {
   const uint64_t xh = y[0] + y[1] + A.lut_mask;
   uint32_t st[2][4];
   int iv[2];
@@ -563,12 +577,15 @@ struct EpiArgs {
 };
 static_assert(sizeof(EpiArgs) <= 4096, "kernel argument blocks must fit in 4 KB");
 
-template <int kAct>
-__global__ void __launch_bounds__(kEpiBlock) linear_epilogue_kernel(EpiArgs A) {
+template <int kAct, bool kWide>
+__global__ void __launch_bounds__(EpiCfg<kWide>::kBlock) linear_epilogue_kernel(EpiArgs A) {
+  using Cfg = EpiCfg<kWide>;
+  using EpiAes = typename Cfg::Aes;
+  constexpr int kEpiBlock = Cfg::kBlock;
   const LinArgs& a = A.a;
   constexpr bool kLut = kAct != SUFHIP_ACT_NONE;
   constexpr int W = kAct == SUFHIP_ACT_CUBIC ? 4 : 2;
-  __shared__ __align__(16) uint32_t tab[kLut ? EpiAes::kSpanWords : 4];
+  __shared__ __align__(16) uint32_t tab[kLut ? Cfg::kTabWords : 4];
   __shared__ ChainLds L;
   __shared__ TruncHdr th[3][2];
   if constexpr (kLut) {
@@ -599,7 +616,15 @@ __global__ void __launch_bounds__(kEpiBlock) linear_epilogue_kernel(EpiArgs A) {
     if (e < 0) continue;
     uint64_t y[2] = {0, 0}, open;
     if (a.slices > 1) {
-      for (int z = 0; z < a.slices; ++z) {
+      int z = 0;
+      for (; z + 4 <= a.slices; z += 4) {  // a group's loads before its sums
+        uint64_t v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = a.part[(size_t(z) * 2 + u) * mn + i];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) y[u & 1] += v[u];
+      }
+      for (; z < a.slices; ++z) {
         y[0] += a.part[size_t(z) * 2 * mn + i];
         y[1] += a.part[(size_t(z) * 2 + 1) * mn + i];
       }
@@ -613,7 +638,7 @@ __global__ void __launch_bounds__(kEpiBlock) linear_epilogue_kernel(EpiArgs A) {
     if constexpr (kAct == SUFHIP_ACT_CUBIC) {
       const Two x{{y[0], y[1]}};
       const Two o = chain_eval<SUFHIP_CHAIN_CUBIC, EpiAes>(
-          A.act, L, K, aes, i, x, chain_loader<SUFHIP_CHAIN_CUBIC>{&A.act, i}, th);
+          A.act, L, K, aes, i, x, plain_loader<SUFHIP_CHAIN_CUBIC>{&A.act, i}, th);
       y[0] = o.v[0];
       y[1] = o.v[1];
     }
@@ -892,6 +917,8 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
     if (!g.cubic || g.cubic->kind != SUFHIP_CHAIN_CUBIC || g.cubic->n != mn)
       return ff_fail(what, "cubic must be a SUFHIP_CHAIN_CUBIC chain with n = rows N");
     if (int rc = make_chain_args(*g.cubic, false, what, &act)) return rc;
+    if (!act.plain)
+      return ff_fail(what, "cubic's triples must be plain arrays, all of stride 1 or all of 3");
   } else if (g.act != SUFHIP_ACT_NONE) {
     return ff_fail(what, "unknown activation");
   }
@@ -986,16 +1013,21 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
   }
   if (!plan.epilogue) return SUFHIP_OK;
   const EpiArgs e{a, act};
-  size_t grid = (mn + kEpiBlock - 1) / kEpiBlock;
-  const size_t cap = size_t(device_cus()) * (g.act == SUFHIP_ACT_NONE ? 4 : 2);
+  const size_t cus = size_t(device_cus());
+  const bool wide = g.act == SUFHIP_ACT_CUBIC && mn >= 2 * cus * EpiCfg<true>::kBlock;
+  const size_t block = wide ? EpiCfg<true>::kBlock : EpiCfg<false>::kBlock;
+  size_t grid = (mn + block - 1) / block;
+  const size_t cap = cus * (wide ? 1 : (g.act == SUFHIP_ACT_NONE ? 4 : 2));
   if (grid > cap) grid = cap;
-  const dim3 gd{unsigned(grid)}, bd{kEpiBlock};
+  const dim3 gd{unsigned(grid)}, bd{unsigned(block)};
   if (g.act == SUFHIP_ACT_RELU)
-    hipLaunchKernelGGL(linear_epilogue_kernel<SUFHIP_ACT_RELU>, gd, bd, 0, s, e);
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_RELU, false>), gd, bd, 0, s, e);
+  else if (g.act == SUFHIP_ACT_CUBIC && wide)
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_CUBIC, true>), gd, bd, 0, s, e);
   else if (g.act == SUFHIP_ACT_CUBIC)
-    hipLaunchKernelGGL(linear_epilogue_kernel<SUFHIP_ACT_CUBIC>, gd, bd, 0, s, e);
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_CUBIC, false>), gd, bd, 0, s, e);
   else
-    hipLaunchKernelGGL(linear_epilogue_kernel<SUFHIP_ACT_NONE>, gd, bd, 0, s, e);
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_NONE, false>), gd, bd, 0, s, e);
   return check_launch("linear_epilogue_kernel");
 }
 

@@ -56,105 +56,142 @@ __device__ __forceinline__ const RmsArgs& rms_args() {
   return *(const RmsArgs*)p;
 }
 
-// A row's values in registers from its sum to its output: s less its mask, and
-// the mask's shares.
-template <int kPer>
-struct RmsRow {
-  uint64_t D[kPer], a0[kPer], a1[kPer];
-};
+// The lane's number afresh, for the same reason: addresses formed from it are
+// not held over the kernel.
+__device__ __forceinline__ int rms_lane() {
+  int t = int(threadIdx.x);
+  asm volatile("" : "+v"(t));
+  return t;
+}
 
-// Columns c0 + thread + k kBlock of row r.  again: for the output of a row that
-// was summed before (and whose total, if any, is written).
-template <int kPer, int kBlock>
-__device__ __forceinline__ void rms_load(RmsRow<kPer>& v, int r, int c0, bool again) {
-  const RmsArgs& A = rms_args();
-  const int cols = A.cols;
-  const size_t base = size_t(r) * size_t(cols);
-  uint64_t s[kPer][2];
+typedef uint64_t u64x2u __attribute__((ext_vector_type(2), aligned(8)));
+
+// Four neighbours from column c on; zeros past the row's end.
+__device__ __forceinline__ void load4(const uint64_t* row, int c, int cols, uint64_t (&v)[4]) {
+  if (c + 4 <= cols) {
+    const u64x2u a = *reinterpret_cast<const u64x2u*>(row + c);
+    const u64x2u b = *reinterpret_cast<const u64x2u*>(row + c + 2);
+    v[0] = a[0];
+    v[1] = a[1];
+    v[2] = b[0];
+    v[3] = b[1];
+  } else {
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int c = c0 + int(threadIdx.x) + k * kBlock;
-    s[k][0] = s[k][1] = v.a0[k] = v.a1[k] = 0;
-    if (c < cols) {
-      if (again && A.total[0]) {
-        s[k][0] = A.total[0][int64_t(r) * A.total_stride + c];
-        s[k][1] = A.total[1][int64_t(r) * A.total_stride + c];
-      } else {
-        s[k][0] = A.x.p[0][int64_t(r) * A.x.stride + c];
-        s[k][1] = A.x.p[1][int64_t(r) * A.x.stride + c];
-        if (A.r.p[0]) {
-          s[k][0] += A.r.p[0][int64_t(r) * A.r.stride + c];
-          s[k][1] += A.r.p[1][int64_t(r) * A.r.stride + c];
-        }
-      }
-      v.a0[k] = A.a[0][base + c];
-      v.a1[k] = A.a[1][base + c];
-    }
-    v.D[k] = (s[k][0] - v.a0[k]) + (s[k][1] - v.a1[k]);
-  }
-  if (!again && A.total[0]) {
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int c = c0 + int(threadIdx.x) + k * kBlock;
-      if (c < cols) {
-        A.total[0][int64_t(r) * A.total_stride + c] = s[k][0];
-        A.total[1][int64_t(r) * A.total_stride + c] = s[k][1];
-      }
-    }
+    for (int q = 0; q < 4; ++q) v[q] = c + q < cols ? row[c + q] : 0;
   }
 }
 
-// The outputs at those columns: b the shares of the row's mask, E the open of
-// its factor.
-template <int kPer, int kBlock>
-__device__ __forceinline__ void rms_put(const RmsRow<kPer>& v, int r, int c0, uint64_t b0,
+__device__ __forceinline__ void store4(uint64_t* row, int c, int cols, const uint64_t (&v)[4]) {
+  if (c + 4 <= cols) {
+    *reinterpret_cast<u64x2u*>(row + c) = u64x2u{v[0], v[1]};
+    *reinterpret_cast<u64x2u*>(row + c + 2) = u64x2u{v[2], v[3]};
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (c + q < cols) row[c + q] = v[q];
+  }
+}
+
+// One lane's four values of a row from its sum to its output: s less its mask,
+// and the mask's shares.
+struct RmsQuad {
+  uint64_t D[4], a0[4], a1[4];
+};
+
+// Columns c .. c + 3 of row r.  again: for the output of a row that was summed
+// before (and whose total, if any, is written).
+__device__ __forceinline__ void rms_load(RmsQuad& v, int r, int c, bool again) {
+  const RmsArgs& A = rms_args();
+  const int cols = A.cols;
+  const size_t base = size_t(r) * size_t(cols);
+  uint64_t s[2][4];
+  if (again && A.total[0]) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) load4(A.total[p] + int64_t(r) * A.total_stride, c, cols, s[p]);
+    load4(A.a[0] + base, c, cols, v.a0);
+    load4(A.a[1] + base, c, cols, v.a1);
+  } else {
+    uint64_t x[2][4];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) load4(A.x.p[p] + int64_t(r) * A.x.stride, c, cols, s[p]);
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[p][q] = 0;
+    if (A.r.p[0]) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) load4(A.r.p[p] + int64_t(r) * A.r.stride, c, cols, x[p]);
+    }
+    load4(A.a[0] + base, c, cols, v.a0);
+    load4(A.a[1] + base, c, cols, v.a1);
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s[p][q] += x[p][q];
+    if (!again && A.total[0]) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) store4(A.total[p] + int64_t(r) * A.total_stride, c, cols, s[p]);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v.D[q] = (s[0][q] - v.a0[q]) + (s[1][q] - v.a1[q]);
+}
+
+// The outputs at those columns: b0, b1 the shares of the row's mask, E the open
+// of its factor.
+__device__ __forceinline__ void rms_put(const RmsQuad& v, int r, int c, uint64_t b0,
                                         uint64_t b1, uint64_t E) {
   const RmsArgs& A = rms_args();
   const int cols = A.cols;
   const size_t base = size_t(r) * size_t(cols);
   const EpiHdrs hn = epi_hdrs(A.tr[kNorm]), hw = epi_hdrs(A.tr[kWeight]);
-  uint64_t open[kPer], y[kPer][2];
+  uint64_t z[2][4], y[2][4];
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int c = c0 + int(threadIdx.x) + k * kBlock;
-    uint64_t z0 = v.D[k] * b0 + v.a0[k] * E + v.D[k] * E, z1 = v.D[k] * b1 + v.a1[k] * E;
-    if (c < cols) {
-      z0 += A.ab[0][base + c];
-      z1 += A.ab[1][base + c];
-    }
-    open[k] = z0 + z1 + A.mask[kNorm];
+  for (int p = 0; p < 2; ++p) load4(A.ab[p] + base, c, cols, z[p]);
+  uint64_t w[4] = {0, 0, 0, 0};
+  if (A.w) load4(reinterpret_cast<const uint64_t*>(A.w), c, cols, w);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    z[0][q] += v.D[q] * b0 + v.a0[q] * E + v.D[q] * E;
+    z[1][q] += v.D[q] * b1 + v.a1[q] * E;
+    uint64_t o[2];
+    gate2(A.tr[kNorm], hn, z[0][q] + z[1][q] + A.mask[kNorm], o);
+    y[0][q] = o[0];
+    y[1][q] = o[1];
   }
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) gate2(A.tr[kNorm], hn, open[k], y[k]);
   if (A.w) {
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int c = c0 + int(threadIdx.x) + k * kBlock;
-      const uint64_t w = c < cols ? uint64_t(A.w[c]) : 0;
-      gate2(A.tr[kWeight], hw, y[k][0] * w + y[k][1] * w + A.mask[kWeight], y[k]);
+    for (int q = 0; q < 4; ++q) {
+      uint64_t o[2];
+      gate2(A.tr[kWeight], hw, y[0][q] * w[q] + y[1][q] * w[q] + A.mask[kWeight], o);
+      y[0][q] = o[0];
+      y[1][q] = o[1];
     }
   }
+  if (A.out[0]) {
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int c = c0 + int(threadIdx.x) + k * kBlock;
-    if (c >= cols) continue;
-    if (A.out[0]) {
-      A.out[0][int64_t(r) * A.out_stride + c] = y[k][0];
-      A.out[1][int64_t(r) * A.out_stride + c] = y[k][1];
-    }
-    if (A.digits) {
-      put_digits(A.digits, size_t(A.rows), size_t(r), c, 0, y[k][0]);
-      put_digits(A.digits, size_t(A.rows), size_t(r), c, 1, y[k][1]);
+    for (int p = 0; p < 2; ++p) store4(A.out[p] + int64_t(r) * A.out_stride, c, cols, y[p]);
+  }
+  if (A.digits) {  // zeros past the row's end, up to the next multiple of 32
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) y[p][q] = c + q < cols ? y[p][q] : 0;
+      uint32_t d[8];
+      digits_of4(y[p], d);
+      int8_t* at = A.digits + digit_off(size_t(p) * A.rows + r, c, size_t(A.rows));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(at + 32 * i) = d[i];
     }
   }
 }
 
-// A row of up to kPer * kBlock values stays in registers from the sum to the
+// A row of up to 4 kQuads kBlock values stays on the CU from the sum to the
 // output; with kLong a longer one is read again for the output.
-template <int kPer, int kBlock, bool kLong>
+template <int kQuads, int kBlock, bool kLong>
 __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs) {
   constexpr int kWaves = kBlock / 64;
-  constexpr int kSpan = kPer * kBlock;
+  constexpr int kSpan = 4 * kQuads * kBlock;
   constexpr int kProds = chain_products<SUFHIP_CHAIN_RSQRT>();
   __shared__ __align__(16) uint32_t tab[256 * kRmsCopies];
   __shared__ ChainLds L;
@@ -163,6 +200,9 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs
   __shared__ uint64_t red[2][kWaves];
   __shared__ uint64_t bc[4];
   __shared__ ChainPre pre;
+  // Wave 0's values of the row while it runs the row's chain, which needs their
+  // registers.
+  __shared__ uint64_t held[kLong ? 1 : 12 * kQuads][64];
   {
     const RmsArgs& A = rms_args();
     fill_ttable<kRmsCopies>(tab, kTDev.v);
@@ -178,23 +218,42 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs
     __syncthreads();
   }
   const int rows = rms_args().rows, cols = rms_args().cols;
+  // Lanes whose columns end before this write nothing, not even digits.
+  const int end = (cols + 31) / 32 * 32;
   for (int r = blockIdx.x; r < rows; r += int(gridDim.x)) {
-    if (threadIdx.x < 24)
-      pre.word(threadIdx.x) = chain_triple_word(rms_args().rs, threadIdx.x, size_t(r));
-    RmsRow<kPer> v;
+    if (const int t = rms_lane(); t < 24)
+      pre.word(t) = chain_triple_word(rms_args().rs, t, size_t(r));
+    RmsQuad v[kQuads];
     uint64_t q0 = 0, q1 = 0;
     for (int c0 = 0; c0 < (kLong ? cols : 1); c0 += kSpan) {
-      rms_load<kPer, kBlock>(v, r, c0, false);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        q0 += 2 * v.D[k] * v.a0[k] + v.D[k] * v.D[k];
-        q1 += 2 * v.D[k] * v.a1[k];
+      for (int k = 0; k < kQuads; ++k) {
+        const int c = c0 + 4 * (rms_lane() + k * kBlock);
+        rms_load(v[k], r, c, false);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          q0 += 2 * v[k].D[q] * v[k].a0[q] + v[k].D[q] * v[k].D[q];
+          q1 += 2 * v[k].D[q] * v[k].a1[q];
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     block_sum2_u64<kWaves>(q0, q1, red);
     if (threadIdx.x < 64) {
+      if constexpr (!kLong) {
+        const int t = rms_lane();
+#pragma unroll
+        for (int k = 0; k < kQuads; ++k)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            held[12 * k + q][t] = v[k].D[q];
+            held[12 * k + 4 + q][t] = v[k].a0[q];
+            held[12 * k + 8 + q][t] = v[k].a1[q];
+          }
+        asm volatile("" ::: "memory");  // and nothing of them stays in registers
+      }
       const RmsArgs& A = rms_args();
-      const RmsAes aes{tab, threadIdx.x % kRmsCopies};
+      const RmsAes aes{tab, uint32_t(rms_lane()) % kRmsCopies};
       const ChainKeyInfo K = chain_key_info(A.rs, L);
       auto gate = [&](int j, uint64_t x) {
         return Two{{trunc_table_eval_h(th[j][0], A.tr[j].table[0], A.tr[j].f, x),
@@ -205,40 +264,49 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs
       m = gate(kMs1, m.v[0] * A.inv_len + m.v[1] * A.inv_len + A.mask[kMs1]);
       m = gate(kMs2, m.v[0] + m.v[1] + A.mask[kMs2]);
       const Two ms{{m.v[0] + A.eps, m.v[1]}};
-      const Two y =
-          chain_eval_quad<SUFHIP_CHAIN_RSQRT, RmsAes>(A.rs, L, K, aes, size_t(r), ms, pre, rth);
+      const Two y = chain_eval_quad<SUFHIP_CHAIN_RSQRT, RmsAes>(rms_args().rs, L, K, aes,
+                                                                size_t(r), ms, pre, rth);
       if (threadIdx.x == 0) {
         bc[0] = b0;
         bc[1] = b1;
         bc[2] = (y.v[0] - b0) + (y.v[1] - b1);
       }
+      if constexpr (!kLong) {
+        asm volatile("" ::: "memory");
+        const int t = rms_lane();
+#pragma unroll
+        for (int k = 0; k < kQuads; ++k)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            v[k].D[q] = held[12 * k + q][t];
+            v[k].a0[q] = held[12 * k + 4 + q][t];
+            v[k].a1[q] = held[12 * k + 8 + q][t];
+          }
+      }
     }
     __syncthreads();
     const uint64_t b0 = bc[0], b1 = bc[1], E = bc[2];
     for (int c0 = 0; c0 < (kLong ? cols : 1); c0 += kSpan) {
-      if (kLong) rms_load<kPer, kBlock>(v, r, c0, true);
-      rms_put<kPer, kBlock>(v, r, c0, b0, b1, E);
-    }
-    const RmsArgs& A = rms_args();
-    if (A.digits) {  // up to the next multiple of 32
-      const int end = (cols + 31) / 32 * 32, c = cols + int(threadIdx.x);
-      if (c < end) {
-        put_digits(A.digits, size_t(rows), size_t(r), c, 0, 0);
-        put_digits(A.digits, size_t(rows), size_t(r), c, 1, 0);
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) {
+        const int c = c0 + 4 * (rms_lane() + k * kBlock);
+        if (kLong) rms_load(v[k], r, c, true);
+        if (c < end) rms_put(v[k], r, c, b0, b1, E);
+        __builtin_amdgcn_sched_barrier(0);  // one quad's registers at a time
       }
     }
     __syncthreads();  // bc and pre are rewritten for the next row
   }
 }
 
-template <int kPer, int kBlock, bool kLong>
+template <int kQuads, int kBlock, bool kLong>
 int launch_rms(const RmsArgs& A, hipStream_t s) {
   int dev = 0, cus = 256;
   if (hipGetDevice(&dev) == hipSuccess)
     (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
   const int cap = cus * (2048 / kBlock > 8 ? 8 : 2048 / kBlock);
   const int grid = A.rows < cap ? A.rows : cap;
-  hipLaunchKernelGGL((rmsnorm2_kernel<kPer, kBlock, kLong>), dim3(unsigned(grid)), dim3(kBlock), 0,
+  hipLaunchKernelGGL((rmsnorm2_kernel<kQuads, kBlock, kLong>), dim3(unsigned(grid)), dim3(kBlock), 0,
                      s, A);
   return check_launch("rmsnorm2_kernel");
 }
@@ -342,10 +410,10 @@ int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream) {
       if (range_meets(A.digits, bytes, outs[i])) return ff_fail(what, "out_digits meets an output");
   }
   hipStream_t s = as_stream(stream);
-  if (g.cols <= 1024) return launch_rms<4, 256, false>(A, s);
-  if (g.cols <= 2048) return launch_rms<4, 512, false>(A, s);
-  if (g.cols <= 4096) return launch_rms<8, 512, false>(A, s);
-  return launch_rms<4, 1024, true>(A, s);
+  if (g.cols <= 1024) return launch_rms<1, 256, false>(A, s);
+  if (g.cols <= 2048) return launch_rms<2, 256, false>(A, s);
+  if (g.cols <= 4096) return launch_rms<2, 512, false>(A, s);
+  return launch_rms<1, 1024, true>(A, s);
 }
 
 }  // extern "C"
