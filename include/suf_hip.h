@@ -1228,7 +1228,12 @@ int sufhip_linear_prepare(const int64_t* d_W, int experts, int K, int N, int dig
  * K <= 65536, digits <= 4, digits K < 2^17; rows, x_rows <= 2^24; rows N <
  * 2^31; experts <= 4096.  d_work: sufhip_linear2_work_bytes() bytes (asked
  * for with the call's device current), 16-byte aligned, used by this call
- * only until it ends; 0 bytes: none needed. */
+ * only until it ends; 0 bytes: none needed.
+ * walk_jobs (walk_count > 0): the key-only halves of truncation gates, as
+ * sufhip_trunc_prepare_batch(walk_prg_state, walk_jobs, walk_count) would
+ * write them, done by this call before it evaluates a gate, so that its own
+ * gates may be among them: beside the product where an epilogue's launch
+ * follows anyway or the outputs are few, else in their own launches first. */
 typedef struct sufhip_relu_key {
   const uint8_t* key[2];
   size_t key_bytes;
@@ -1253,6 +1258,9 @@ typedef struct sufhip_linear2_args {
   sufhip_digits2 out_digits;
   void* d_work;
   size_t work_bytes;
+  const sufhip_trunc_job* walk_jobs;
+  int walk_count;
+  const uint8_t* walk_prg_state;
 } sufhip_linear2_args;
 size_t sufhip_linear2_work_bytes(const sufhip_linear2_args* args);
 int sufhip_linear2(const sufhip_linear2_args* args, void* stream);

@@ -1,7 +1,7 @@
 // Share x public weight for both parties and any number of rows, dense or
 // grouped by expert, with the bias, the truncation, an activation and a
 // residual in its epilogue (sufhip_linear2), on the int8 matrix cores (gfx950
-// v_mfma_i32_16x16x64_i8 and 32x32x32_i8), exact mod 2^64.
+// v_mfma_i32_16x16x64_i8), exact mod 2^64.
 //
 // Both operands in balanced base-256 digits: x = sum_{i<8} x_i 256^i, W =
 // sum_{j<J} w_j 256^j, so that X W = sum_{s<8} 256^s S_s mod 2^64 with S_s =
@@ -18,12 +18,12 @@
 
 #include "chain_device.hpp"
 #include "feedforward_device.hpp"
+#include "walk_device.hpp"
 
 namespace sufhip {
 namespace {
 
 typedef int v4acc __attribute__((ext_vector_type(4)));
-typedef int v16acc __attribute__((ext_vector_type(16)));
 typedef uint64_t u64x2u __attribute__((ext_vector_type(2), aligned(8)));
 
 constexpr int kCols = 64;         // columns of a weight tile
@@ -47,6 +47,15 @@ struct LinArgs {
   uint64_t* out[2];
   int64_t out_stride;
   int8_t* digits;  // the outputs as digits (the epilogue's launch)
+};
+
+// The key-only walks that a launch does beside its own work, in its first
+// `groups` workgroups (a multiple of 8, so that the others' order over the XCDs
+// stays).
+constexpr int kLinWalks = 8;
+struct LinWalk {
+  WalkJobs<kLinWalks> jobs;
+  int groups;
 };
 
 // The expert of output row i and whether it has one.
@@ -130,392 +139,268 @@ __device__ __forceinline__ void put_output(const LinArgs& a, const EpiHdrs& eh, 
   }
 }
 
-// Few rows: a workgroup of four waves takes one row tile (kT / 2 tokens of both
-// parties), 128 columns, 32 a wave, and one k-slice.  W goes straight into
-// registers, each word read once; X's digits, which the four waves share, are
-// formed on the way into LDS (or come as digits), 64 k at a time, the next
-// chunk's loads in flight under this one's products.
-template <int kT, int J, bool kDigits>
-__global__ void __launch_bounds__(256, J <= 2 ? 2 : 1) linear_skinny_kernel(LinArgs a) {
-  constexpr int kTok = kT / 2;
-  constexpr int kC = kT == 16 ? 2 : 1;      // column fragments of a wave
-  constexpr int kR = kT == 16 ? 4 : 16;     // accumulator registers of one
-  constexpr int kSteps = kT == 16 ? 1 : 2;  // matrix steps of a chunk
-  constexpr int kPieces = kT / 8;           // of 16 bytes, a thread stores in a chunk
-  typedef typename std::conditional<kT == 16, v4acc, v16acc>::type Acc;
-  __shared__ __align__(16) int8_t lds[2][kSteps * 8 * 1024];  // [step][digit][lane] of 16 k
+// The order of the tiles.  Workgroups are dealt round-robin to the 8 XCDs, each
+// with an L2 of its own, so an XCD takes a contiguous eighth of the order; and
+// the order goes over 8 column tiles, then the row tiles, then the next 8
+// columns: the hundred workgroups that an XCD runs at once then share a dozen
+// row tiles of X and 8 column tiles of W, instead of one side alone being read
+// again by each (1000 x 2048 x 1024: 288 MB beyond the L2s, 66 us).
+struct TileId {
+  int row, col, slice;
+};
+__device__ __forceinline__ TileId tile_id(const LinArgs& a, int id, int total) {
+  const int each = total / 8, more = total % 8, x = id % 8;
+  id = x * each + (x < more ? x : more) + id / 8;
+  const int cols = (a.groups + 1) / 2;
+  const int plane = a.tiles * cols, slice = id / plane;
+  id -= slice * plane;
+  const int panel = id / (8 * a.tiles), left = cols - 8 * panel;
+  const int wide = left < 8 ? left : 8;
+  id -= 8 * a.tiles * panel;
+  return {id / wide, 8 * panel + id % wide, slice};
+}
+
+// A workgroup of four waves takes kRt row tiles (8 tokens of both parties
+// each), 128 columns, 32 a wave, and one k-slice.  W goes straight into registers; X's
+// digits, which the four waves share, are formed on the way into LDS (or come
+// as digits), 64 k at a time, the next chunk's loads in flight under this
+// one's products.
+constexpr int kTok = 8;
+constexpr int kFrags = 2;  // column fragments of a wave
+constexpr int kDepth = 2;  // chunks on their way
+template <int kRt, int J, bool kDigits, bool kWalk>
+__global__ void __launch_bounds__(256, 2) linear_product_kernel(LinArgs a, LinWalk wk) {
+  if constexpr (kWalk) {
+    if (int(blockIdx.x) < wk.groups) {
+      hosted_walk_role<kLinWalks, false>(wk.jobs, blockIdx.x * 256 + threadIdx.x);
+      return;
+    }
+  }
+  const int groups = kWalk ? wk.groups : 0;
+  // [digit][slot] of 16 k.  Row r's sixteen number kk is slot 16 kk + (r + 4 kk)
+  // % 16: a wave's dword writes (four rows, four sixteens) and its fragment
+  // reads then take every bank once.
+  __shared__ __align__(16) int8_t lds[2][kRt][8 * 1024];
   const int l = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-  const int total = int(gridDim.x);
-  int id = int(blockIdx.x);
-  // Row tiles of the same weights run on one XCD, one after the other.
-  if (total % 8 == 0) id = (id % 8) * (total / 8) + id / 8;
-  const int ti = id % a.tiles, rest = id / a.tiles;
-  const int slice = rest % a.slices, c0 = rest / a.slices * 128 + 32 * w;
-  const RowTile rt = row_tile(a, ti, kTok);
+  const int total = int(gridDim.x) - groups;
+  int id = int(blockIdx.x) - groups;
+  const TileId at = tile_id(a, id, total);
+  const int slice = at.slice, c0 = at.col * 128 + 32 * w;
+  const RowTile rt = row_tile(a, at.row, kRt * kTok);
   if (rt.e < 0 || rt.begin >= rt.end) return;  // the whole workgroup
   const EpiHdrs eh = epi_hdrs(a.epi);
-  // The row that this thread brings to LDS: a run of kT / 4 words of it, or
-  // (digits) its pieces of 16 bytes.
-  const int r = kDigits ? l % kT : int(threadIdx.x) / (256 / kT);
-  const int kq = int(threadIdx.x) % (256 / kT) * (kT / 4);  // first word in the chunk
+  // The row that this thread brings to LDS: four words of it from kq on, or
+  // (digits) two pieces of 16 bytes.
+  const int r = kDigits ? l % 16 : int(threadIdx.x) / 16;
+  const int kq = int(threadIdx.x) % 16 * 4;
+  const int slot = ((l & 48) + ((l + (l >> 4) * 4) & 15)) * 16;  // of this lane's fragment
   const int p = (r >> 1) & 1, t = 2 * (r >> 2) + (r & 1);
-  int xr = rt.begin + t;
-  bool live = xr < rt.end;
-  if (live && a.map) xr = a.map[xr];
-  live = live && xr >= 0 && xr < a.x_rows;
-  const uint64_t* xrow =
-      kDigits ? nullptr : (p ? a.x.p[1] : a.x.p[0]) + (live ? int64_t(xr) * a.x.stride : 0) + kq;
-  const int8_t* drow = kDigits ? a.xd + (live ? (size_t(p) * a.x_rows + xr) * 256 : 0) : nullptr;
+  bool live[kRt];
+  const uint64_t* xrow[kRt];
+  const int8_t* drow[kRt];
+#pragma unroll
+  for (int m = 0; m < kRt; ++m) {
+    int xr = rt.begin + kTok * m + t;
+    live[m] = xr < rt.end;
+    if (live[m] && a.map) xr = a.map[xr];
+    live[m] = live[m] && xr >= 0 && xr < a.x_rows;
+    if (kDigits)
+      drow[m] = a.xd + (live[m] ? (size_t(p) * a.x_rows + xr) * 256 : 0);
+    else
+      xrow[m] = (p ? a.x.p[1] : a.x.p[0]) + (live[m] ? int64_t(xr) * a.x.stride : 0) + kq;
+  }
   const size_t dstep = size_t(2) * a.x_rows * 256;
   // This wave's columns; past the last weight tile it repeats the last one.
   const int g = c0 / kCols < a.groups ? c0 / kCols : a.groups - 1;
   const int8_t* wl = a.w + size_t(rt.e) * a.expert_bytes + size_t(g) * a.kb * (J * kTileBytes) +
-                     (c0 % kCols) * 32 +
-                     (kT == 16 ? (l >> 5) * (J * kTileBytes) + (l & 15) * 32 + ((l >> 4) & 1) * 16
-                               : (l & 31) * 32 + (l >> 5) * 16);
+                     (c0 % kCols) * 32 + (l >> 5) * (J * kTileBytes) + (l & 15) * 32 +
+                     ((l >> 4) & 1) * 16;
   const int chunks = a.kb / 2;
   const int q0 = int(int64_t(chunks) * slice / a.slices);
   const int q1 = int(int64_t(chunks) * (slice + 1) / a.slices);
-  struct Wreg {
-    v4i v[kSteps][kC][J];
+  // Chunks on their way: W until its products, X until its place in LDS.
+  struct Chunk {
+    v4i w[kFrags][J];
+    u64x2u xw[kDigits ? 1 : kRt][2];
+    v4i xd[kDigits ? kRt : 1][2];
   };
-  u64x2u xw[kDigits ? 1 : kT / 8];
-  v4i xd[kDigits ? kPieces : 1];
-  auto load_w = [&](Wreg& g, int q) {
+  auto load_w = [&](Chunk& k, int q) {
+    if (q >= q1) return;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+    for (int c = 0; c < kFrags; ++c)
 #pragma unroll
-      for (int c = 0; c < kC; ++c)
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-          g.v[s][c][j] = load16(wl + (size_t(q) * 2 + s) * (J * kTileBytes) + j * kTileBytes +
-                                c * (kT * 32));
+      for (int j = 0; j < J; ++j)
+        k.w[c][j] = load16(wl + size_t(q) * (2 * J * kTileBytes) + j * kTileBytes + c * 512);
   };
-  auto load_x = [&](int q) {
-    if constexpr (kDigits) {
+  auto load_x = [&](Chunk& k, int q) {
+    if (q >= q1) return;
 #pragma unroll
-      for (int u = 0; u < kPieces; ++u) {
-        // Piece threadIdx + 256 u: step, digit and lane of the fragment.
-        const int piece = int(threadIdx.x) + 256 * u;
-        const int i = (piece >> 6) & 7;
-        const int sixteen = kT == 16 ? l / 16 : 2 * (piece >> 9) + l / 32;
-        const int kb = 2 * q + (sixteen >> 1);
-        xd[u] = v4i{0, 0, 0, 0};
-        if (live && 32 * kb < a.K)
-          xd[u] = load16(drow + size_t(kb) * dstep + 32 * i + 16 * (sixteen & 1));
-      }
-    } else {
-      const int k = 64 * q + kq;
-#pragma unroll
-      for (int u = 0; u < kT / 8; ++u) xw[u] = u64x2u{0, 0};
-      if (live && k + kT / 4 <= a.K) {
-#pragma unroll
-        for (int u = 0; u < kT / 8; ++u)
-          xw[u] = *reinterpret_cast<const u64x2u*>(xrow + 64 * q + 2 * u);
-      } else if (live) {
-#pragma unroll
-        for (int u = 0; u < kT / 8; ++u) {
-          if (k + 2 * u < a.K) xw[u][0] = xrow[64 * q + 2 * u];
-          if (k + 2 * u + 1 < a.K) xw[u][1] = xrow[64 * q + 2 * u + 1];
+    for (int m = 0; m < kRt; ++m) {
+      if constexpr (kDigits) {
+        // Digits w and w + 4 at this lane's place in the fragment.
+        const int kb = 2 * q + (l >> 5);
+        k.xd[m][0] = k.xd[m][1] = v4i{0, 0, 0, 0};
+        if (live[m] && 32 * kb < a.K) {
+          const int8_t* at = drow[m] + size_t(kb) * dstep + 16 * ((l >> 4) & 1) + 32 * w;
+          k.xd[m][0] = load16(at);
+          k.xd[m][1] = load16(at + 128);
+        }
+      } else {
+        const uint64_t* row = xrow[m] + 64 * q;
+        const int left = a.K - 64 * q - kq;
+        k.xw[m][0] = k.xw[m][1] = u64x2u{0, 0};
+        if (live[m] && left >= 4) {
+          k.xw[m][0] = *reinterpret_cast<const u64x2u*>(row);
+          k.xw[m][1] = *reinterpret_cast<const u64x2u*>(row + 2);
+        } else if (live[m]) {
+          if (left > 0) k.xw[m][0][0] = row[0];
+          if (left > 1) k.xw[m][0][1] = row[1];
+          if (left > 2) k.xw[m][1][0] = row[2];
         }
       }
     }
   };
-  auto store_x = [&](int buf) {
-    if constexpr (kDigits) {
+  auto store_x = [&](const Chunk& k, int buf) {
 #pragma unroll
-      for (int u = 0; u < kPieces; ++u)
-        *reinterpret_cast<v4i*>(&lds[buf][(int(threadIdx.x) + 256 * u) * 16]) = xd[u];
-    } else {
-      const int lane = (kT == 16 ? kq >> 4 : (kq >> 4) & 1) * kT + r;
-      int8_t* at = &lds[buf][(kT == 16 ? 0 : kq >> 5) * 8192 + lane * 16 + (kq & 15)];
-      uint32_t d[kT / 16][8];
+    for (int m = 0; m < kRt; ++m) {
+      if constexpr (kDigits) {
+        *reinterpret_cast<v4i*>(&lds[buf][m][w * 1024 + slot]) = k.xd[m][0];
+        *reinterpret_cast<v4i*>(&lds[buf][m][(w + 4) * 1024 + slot]) = k.xd[m][1];
+      } else {
+        int8_t* at =
+            &lds[buf][m][(kq & 48) * 16 + ((r + (kq >> 4) * 4) & 15) * 16 + (kq & 15)];
+        const uint64_t v[4] = {k.xw[m][0][0], k.xw[m][0][1], k.xw[m][1][0], k.xw[m][1][1]};
+        uint32_t d[8];
+        digits_of4(v, d);
 #pragma unroll
-      for (int u = 0; u < kT / 16; ++u) {
-        const uint64_t v[4] = {xw[2 * u][0], xw[2 * u][1], xw[2 * u + 1][0], xw[2 * u + 1][1]};
-        digits_of4(v, d[u]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (kT == 16)
-          *reinterpret_cast<uint32_t*>(at + 1024 * i) = d[0][i];
-        else
-          *reinterpret_cast<uint2*>(at + 1024 * i) = make_uint2(d[0][i], d[1][i]);
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(at + 1024 * i) = d[i];
       }
     }
   };
-  Acc acc[kC][8];
+  v4acc acc[kRt][kFrags][8];
 #pragma unroll
-  for (int c = 0; c < kC; ++c)
+  for (int m = 0; m < kRt; ++m)
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
+    for (int c = 0; c < kFrags; ++c)
 #pragma unroll
-      for (int q = 0; q < kR; ++q) acc[c][s][q] = 0;
-  auto products = [&](const Wreg& g, int buf) {
+      for (int s = 0; s < 8; ++s)
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
+        for (int q = 0; q < 4; ++q) acc[m][c][s][q] = 0;
+  auto products = [&](const Chunk& k, int buf) {
+#pragma unroll
+    for (int m = 0; m < kRt; ++m) {
       v4i d[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        d[i] = *reinterpret_cast<const v4i*>(&lds[buf][s * 8192 + i * 1024 + 16 * l]);
+        d[i] = *reinterpret_cast<const v4i*>(&lds[buf][m][i * 1024 + slot]);
 #pragma unroll
-      for (int c = 0; c < kC; ++c)
+      for (int c = 0; c < kFrags; ++c)
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
-          for (int i = 0; i + j < 8; ++i) {
-            if constexpr (kT == 16)
-              acc[c][i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(d[i], g.v[s][c][j],
-                                                                    acc[c][i + j], 0, 0, 0);
-            else
-              acc[c][i + j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(d[i], g.v[s][c][j],
-                                                                    acc[c][i + j], 0, 0, 0);
-          }
+          for (int i = 0; i + j < 8; ++i)
+            acc[m][c][i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(d[i], k.w[c][j],
+                                                                     acc[m][c][i + j], 0, 0, 0);
     }
   };
-  auto step = [&](int q, const Wreg& cur, Wreg& next) {
-    if (q + 1 < q1) {
-      load_w(next, q + 1);
-      load_x(q + 1);
-    }
-    products(cur, (q - q0) & 1);
-    if (q + 1 < q1) store_x((q + 1 - q0) & 1);
-    __syncthreads();
-  };
-  if (q0 < q1) {
-    Wreg wa, wb;
-    load_w(wa, q0);
-    load_x(q0);
-    store_x(0);
-    __syncthreads();
-    for (int q = q0; q < q1; q += 2) {
-      step(q, wa, wb);
-      if (q + 1 < q1) step(q + 1, wb, wa);
-    }
+  // Chunk q lies in ring[(q - q0) % kDepth]: its W is loaded kDepth steps ahead,
+  // when the slot's last products are issued; its X goes to LDS a step ahead.
+  Chunk ring[kDepth];
+#pragma unroll
+  for (int u = 0; u < kDepth; ++u) {
+    load_w(ring[u], q0 + u);
+    load_x(ring[u], q0 + u);
   }
-#pragma unroll
-  for (int c = 0; c < kC; ++c) {
-    const int col = c0 + c * kT + l % kT;
-    if (col >= a.N) continue;
-#pragma unroll
-    for (int b = 0; b < kR / 4; ++b) {
-      uint64_t v[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        v[q] = 0;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) v[q] += uint64_t(int64_t(acc[c][s][4 * b + q])) << (8 * s);
-      }
-      const int pairs = kT == 16 ? l / 16 : 2 * b + l / 32;  // of tokens, in the tile
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = rt.begin + 2 * pairs + h;
-        if (row < rt.end) put_output(a, eh, slice, rt.e, row, col, v[h], v[2 + h]);
-      }
-    }
-  }
-}
-
-// acc += a b with the accumulator in the accumulation registers for the whole
-// loop.  (The compiler keeps 256 of them in vector registers and copies them
-// to and from the others in every step.)  The wait before it covers a vector
-// instruction's write of an operand; between two products into one
-// accumulator lie at least six others.
-__device__ __forceinline__ void mfma_acc(v16acc& acc, v4i a, v4i b) {
-  asm volatile("s_nop 1\n\tv_mfma_i32_32x32x32_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
-}
-
-// Between mfma_acc and other uses of the accumulators: the last products' (or
-// the zeros') writes are done.  The ties keep every such use behind the wait.
-template <int kC, int kS>
-__device__ __forceinline__ void acc_settle(v16acc (&acc)[kC][kS]) {
-  asm volatile("s_nop 15\n\ts_nop 15" ::);
-#pragma unroll
-  for (int c = 0; c < kC; ++c)
-#pragma unroll
-    for (int s = 0; s < kS; ++s) asm volatile("" : "+a"(acc[c][s]));
-}
-
-// Many rows: a workgroup takes 32 tokens of both parties (two tiles of 32
-// rows) and 128 columns; wave (m, n) tile m and column tile n, 32 x 64 values
-// in 256 accumulator registers.  A k-block's operands, X's digits (gathered a
-// row at a time) and W's, pass through LDS in the fragments' order, the next
-// block's loads in flight under this one's products.
-constexpr int kBigTok = 32;
-
-template <int J>
-__global__ void __launch_bounds__(256, 1) linear_tile_kernel(LinArgs a) {
-  constexpr int kBlocks = 16 + 4 * J;  // of 1 KB: X (tile, digit), W (column tile, digit, half)
-  __shared__ __align__(16) int8_t lds[2][kBlocks * 1024];
-  const int l = threadIdx.x & 63;
-  const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-  const int total = int(gridDim.x);
-  int id = int(blockIdx.x);
-  // An XCD takes neighbouring column tiles of the same rows.
-  if (total % 8 == 0) id = (id % 8) * (total / 8) + id / 8;
-  const int gpairs = (a.groups + 1) / 2;
-  const int gp = id % gpairs, rest = id / gpairs;
-  const int slice = rest % a.slices, ti = rest / a.slices;
-  const RowTile rt = row_tile(a, ti, kBigTok);
-  if (rt.e < 0 || rt.begin >= rt.end) return;  // the whole workgroup
-  const EpiHdrs eh = epi_hdrs(a.epi);
-  const int m = w >> 1, n = w & 1;
-  // Loads of this thread: four X fragments of row tile m (digits 4 n .. 4 n +
-  // 3) and J of W's blocks, at its place in the fragment.
-  const int r = l & 31, half = l >> 5;
-  const int p = (r >> 1) & 1, t = 2 * (r >> 2) + (r & 1);
-  int xr = rt.begin + 16 * m + t;
-  bool live = xr < rt.end;
-  if (live && a.map) xr = a.map[xr];
-  live = live && xr >= 0 && xr < a.x_rows;
-  // A row that is not there reads row 0 and is zeros in LDS.
-  const int8_t* xl = a.xd + (live ? (size_t(p) * a.x_rows + xr) * 256 : 0) + half * 16 + n * 128;
-  const size_t xstep = size_t(2) * a.x_rows * 256;
-  const int kb_x = (a.K + 31) / 32;
-  const int8_t* wl[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int b = w * J + j;  // column tile, digit, half of its columns
-    int g = 2 * gp + b / (2 * J);
-    if (g >= a.groups) g = a.groups - 1;
-    wl[j] = a.w + size_t(rt.e) * a.expert_bytes + size_t(g) * a.kb * (J * kTileBytes) +
-            ((b >> 1) % J) * kTileBytes + (b & 1) * 1024 + (l & 31) * 32 + half * 16;
-  }
-  const int b0 = int(int64_t(kb_x) * slice / a.slices);
-  const int b1 = int(int64_t(kb_x) * (slice + 1) / a.slices);
-  // Registers for the k-blocks on their way to LDS (two ahead of the products)
-  // and for the fragments of this step and the next.
-  struct Staged {
-    v4i x[4], w[J];
-  };
-  struct Frags {
-    v4i x[8], w[2][J];
-  };
-  auto load_one = [&](Staged& g, int kb, int q) {
-    kb = kb < b1 ? kb : b1 - 1;
-    if (q < 4)
-      g.x[q] = load16(xl + size_t(kb) * xstep + 32 * q);
-    else
-      g.w[q - 4] = load16(wl[q - 4] + size_t(kb) * (J * kTileBytes));
-  };
-  auto store_one = [&](const Staged& g, int kb, int q) {
-    int8_t* at = lds[(kb - b0) & 1] + 16 * l;
-    if (q < 4)  // zeros for a row that is not there and past the last k-block
-      *reinterpret_cast<v4i*>(at + (m * 8 + n * 4 + q) * 1024) =
-          live && kb < b1 ? g.x[q] : v4i{0, 0, 0, 0};
-    else
-      *reinterpret_cast<v4i*>(at + (16 + w * J + q - 4) * 1024) = g.w[q - 4];
-  };
-  auto read_one = [&](Frags& f, int kb, int q) {
-    const int8_t* at = lds[(kb - b0) & 1] + 16 * l;
-    if (q < 8)
-      f.x[q] = *reinterpret_cast<const v4i*>(at + (m * 8 + q) * 1024);
-    else
-      f.w[(q - 8) / J][(q - 8) % J] = *reinterpret_cast<const v4i*>(
-          at + (16 + (n * J + (q - 8) % J) * 2 + (q - 8) / J) * 1024);
-  };
-  constexpr int kMoves = 4 + J, kReads = 8 + 2 * J;
-  auto load = [&](Staged& g, int kb) {
-#pragma unroll
-    for (int q = 0; q < kMoves; ++q) load_one(g, kb, q);
-  };
-  auto store = [&](const Staged& g, int kb) {
-#pragma unroll
-    for (int q = 0; q < kMoves; ++q) store_one(g, kb, q);
-  };
-  v16acc acc[2][8];
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-#pragma unroll
-    for (int s = 0; s < 8; ++s)
-#pragma unroll
-      for (int q = 0; q < 16; ++q) acc[c][s][q] = 0;
-  // Step kb (its fragments in f): between its products the next step's
-  // fragments are read, the k-block after that is stored and another load of
-  // two steps ahead is issued.  Buffer kb & 1 held this step's k-block, whose
-  // readers passed the barrier at the end of the last step.
-  auto step = [&](int kb, const Frags& f, Frags& next, Staged& g) {
-    constexpr int kMfmas = 2 * (8 * J - J * (J - 1) / 2);
-    constexpr int kChores = kReads + 2 * kMoves;
-    int at = 0, done = 0;
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int i = 0; i + j < 8; ++i) {
-          mfma_acc(acc[c][i + j], f.x[i], f.w[c][j]);
-          ++at;
-#pragma unroll
-          for (; done < at * kChores / kMfmas; ++done) {
-            if (done < kReads)
-              read_one(next, kb + 1, done);
-            else if (done < kReads + kMoves)
-              store_one(g, kb + 2, done - kReads);
-            else
-              load_one(g, kb + 4, done - kReads - kMoves);
-          }
-        }
-    __syncthreads();
-  };
-  // Steps in pairs; past the last k-block X is zeros.
-  Staged ga, gb;
-  Frags fa, fb;
-  load(ga, b0);
-  load(gb, b0 + 1);
-  store(ga, b0);
-  load(ga, b0 + 2);
-  store(gb, b0 + 1);
-  load(gb, b0 + 3);
+  store_x(ring[0], 0);
+  load_x(ring[0], q0 + kDepth);
   __syncthreads();
+  for (int q = q0; q < q1; q += kDepth) {
 #pragma unroll
-  for (int q = 0; q < kReads; ++q) read_one(fa, b0, q);
-  __syncthreads();  // buffer 0 is stored to in the first step
-  acc_settle(acc);
-  for (int kb = b0; kb < b1; kb += 2) {
-    step(kb, fa, fb, ga);
-    step(kb + 1, fb, fa, gb);
+    for (int u = 0; u < kDepth; ++u) {
+      if (q + u < q1) {
+        Chunk& next = ring[(u + 1) % kDepth];
+        const int buf = (q + u - q0) & 1;
+        products(ring[u], buf);
+        load_w(ring[u], q + u + kDepth);
+        store_x(next, buf ^ 1);
+        load_x(next, q + u + 1 + kDepth);
+        __syncthreads();
+      }
+    }
   }
-  acc_settle(acc);
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int col = (2 * gp + n) * kCols + 32 * c + (l & 31);
-    if (col >= a.N) continue;
+  for (int m = 0; m < kRt; ++m)
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
+    for (int c = 0; c < kFrags; ++c) {
+      const int col = c0 + 16 * c + l % 16;
+      if (col >= a.N) continue;
       uint64_t v[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         v[q] = 0;
 #pragma unroll
-        for (int s = 0; s < 8; ++s) v[q] += uint64_t(int64_t(acc[c][s][4 * b + q])) << (8 * s);
+        for (int s = 0; s < 8; ++s) v[q] += uint64_t(int64_t(acc[m][c][s][q])) << (8 * s);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int row = rt.begin + 16 * m + 2 * (2 * b + half) + h;
+        const int row = rt.begin + kTok * m + 2 * (l / 16) + h;
         if (row < rt.end) put_output(a, eh, slice, rt.e, row, col, v[h], v[2 + h]);
       }
     }
-  }
 }
 
 // The epilogue's own launch, where k-slices have to be summed, an activation
 // follows or the outputs go out as digits.  An activation's keystream binds a
-// large one (two AES blocks an element for a cubic): then workgroups of 1024
-// lanes with the four-table AES (128 KB of LDS), one a CU, else 512 lanes on
-// two tables.
-template <bool kWide>
-struct EpiCfg {
+// large one (two AES blocks an element for a cubic): workgroups of 1024 lanes
+// with the four-table AES (128 KB of LDS), one a CU.  A small one waits for its
+// tables first: 256 lanes and one table of 16 copies (16 KB).
+enum { kEpiSmall = 0, kEpiMid = 1, kEpiWide = 2 };
+template <int kSize>
+struct EpiCfg {  // kEpiMid
   static constexpr int kBlock = 512;
   using Aes = AesLds2<32>;
   static constexpr int kTabWords = Aes::kSpanWords;
+  template <class Cs, class Args>
+  __device__ __forceinline__ static Aes stage(uint32_t* tab, const Args& A, int W, ChainLds& L) {
+    typename Aes::template Filler<kBlock> tf;
+    Cs cs;
+    tf.load(kTDev.v);
+    cs.load(A, W);
+    cs.store(A, W, L);
+    tf.store(tab);
+    return Aes::make(tab);
+  }
 };
 template <>
-struct EpiCfg<true> {
+struct EpiCfg<kEpiWide> {
   static constexpr int kBlock = 1024;
   using Aes = AesLds4;
   static constexpr int kTabWords = Aes::kWords;
+  template <class Cs, class Args>
+  __device__ __forceinline__ static Aes stage(uint32_t* tab, const Args& A, int W, ChainLds& L) {
+    typename Aes::template Filler<kBlock> tf;
+    Cs cs;
+    tf.load(kTDev.v);
+    cs.load(A, W);
+    cs.store(A, W, L);
+    tf.store(tab);
+    return Aes::make(tab);
+  }
+};
+template <>
+struct EpiCfg<kEpiSmall> {
+  static constexpr int kBlock = 256;
+  using Aes = AesLds<16>;
+  static constexpr int kTabWords = 256 * 16;
+  template <class Cs, class Args>
+  __device__ __forceinline__ static Aes stage(uint32_t* tab, const Args& A, int W, ChainLds& L) {
+    Cs cs;
+    cs.load(A, W);
+    fill_ttable<16>(tab, kTDev.v);
+    cs.store(A, W, L);
+    return Aes{tab, uint32_t(threadIdx.x) % 16};
+  }
 };
 
 // The ReLU's rows (c0, c1) at the masked open xh, both parties: c0 + c1 xh.
@@ -577,9 +462,9 @@ struct EpiArgs {
 };
 static_assert(sizeof(EpiArgs) <= 4096, "kernel argument blocks must fit in 4 KB");
 
-template <int kAct, bool kWide>
-__global__ void __launch_bounds__(EpiCfg<kWide>::kBlock) linear_epilogue_kernel(EpiArgs A) {
-  using Cfg = EpiCfg<kWide>;
+template <int kAct, int kSize>
+__global__ void __launch_bounds__(EpiCfg<kSize>::kBlock) linear_epilogue_kernel(EpiArgs A) {
+  using Cfg = EpiCfg<kSize>;
   using EpiAes = typename Cfg::Aes;
   constexpr int kEpiBlock = Cfg::kBlock;
   const LinArgs& a = A.a;
@@ -588,23 +473,18 @@ __global__ void __launch_bounds__(EpiCfg<kWide>::kBlock) linear_epilogue_kernel(
   __shared__ __align__(16) uint32_t tab[kLut ? Cfg::kTabWords : 4];
   __shared__ ChainLds L;
   __shared__ TruncHdr th[3][2];
+  std::conditional_t<kLut, EpiAes, int> aes;
   if constexpr (kLut) {
-    typename EpiAes::template Filler<kEpiBlock> tf;
-    ChainStager<kEpiBlock, 2> cs;
-    tf.load(kTDev.v);
-    cs.load(A.act, W);
     if constexpr (kAct == SUFHIP_ACT_CUBIC) {
       TruncHdrStager<3> hs;
       hs.load(A.act, 0);
       hs.store(th);
     }
-    cs.store(A.act, W, L);
-    tf.store(tab);
+    aes = Cfg::template stage<ChainStager<kEpiBlock, 2>>(tab, A.act, W, L);
     __syncthreads();
     chain_compare(A.act, L);
     __syncthreads();
   }
-  const EpiAes aes = EpiAes::make(tab);
   ChainKeyInfo K{};
   if constexpr (kLut) K = chain_key_info(A.act, L);
   const EpiHdrs eh = epi_hdrs(a.epi);
@@ -729,13 +609,13 @@ int device_cus() {
 
 // How a call runs.
 struct Plan {
-  bool tile;       // linear_tile_kernel, else linear_skinny_kernel of t rows
-  int t;
+  int rt;          // row tiles of a workgroup
   int tiles;       // row tiles of the grid (an upper bound with experts)
   int col_tiles;
   int slices;
   bool epilogue;   // the epilogue's own launch
-  size_t digits_bytes, words;  // the workspace: x's digits, sums or opens
+  bool walk;       // the walks beside the product
+  size_t words;    // of the workspace: the slices' sums, or the opens
 };
 
 bool extents_ok(int experts, int K, int N, int digits) {
@@ -745,28 +625,35 @@ bool extents_ok(int experts, int K, int N, int digits) {
 
 Plan plan_linear(const sufhip_linear2_args& g) {
   Plan p{};
-  const int groups = (g.w.N + kCols - 1) / kCols;
-  const int kb = (g.w.K + 63) / 64 * 2;
-  const int experts = g.d_offsets ? g.w.experts : 1;
-  const int each = (g.rows + experts - 1) / experts;  // rows of an expert, on average
-  p.tile = each > 32;
-  p.t = each <= 8 ? 16 : 32;
-  const int per = p.tile ? kBigTok : p.t / 2;
   // Every expert may end inside a tile, and has one only if it has a row.
-  p.tiles = g.d_offsets ? g.rows / per + (experts < g.rows ? experts : g.rows)
-                        : (g.rows + per - 1) / per;
-  const int cus = device_cus();
-  p.col_tiles = (groups + 1) / 2;
+  const int experts = g.w.experts < g.rows ? g.w.experts : g.rows;
+  // Two row tiles a workgroup read W half as often: 1000 x 2048 x 1024 59 us
+  // against 67, 256 x 1024 x 4096 36 against 39; 128 x 4096 x 4096 68 against
+  // 63, for the half as many workgroups.  With three digits of W the sums do
+  // not fit the registers.
+  p.rt = g.w.digits <= 2 && g.rows / (g.d_offsets ? experts : 1) >= 192 ? 2 : 1;
+  const int per = p.rt * kTok;
+  p.tiles = g.d_offsets ? g.rows / per + experts : (g.rows + per - 1) / per;
+  p.col_tiles = (g.w.N + 127) / 128;
+  // k-slices up to two workgroups a CU, of three chunks at least: one row of
+  // 768 x 2304 8.4 us with 4, 10.5 with 1; 8 x 4096 x 4096 16.9 with 8, 20.7
+  // with 4, 18.4 with 16; 64 x 4096 x 4096 38.8 with 2, 50.2 with 1, 43 with 4.
   const int64_t wgs = int64_t(p.tiles) * p.col_tiles;
-  const int most = p.tile ? kb / 8 : kb / 4;
-  int64_t s = p.tile ? cus / wgs : (2 * cus + wgs - 1) / wgs;
+  int64_t s = 2 * int64_t(device_cus()) / wgs;
+  const int most = (g.w.K + 63) / 64 / 3;
   if (s > most) s = most;
-  if (s > 16) s = 16;
+  if (s > 8) s = 8;
   p.slices = s < 1 ? 1 : int(s);
   p.epilogue = p.slices > 1 || g.act != SUFHIP_ACT_NONE || g.out_digits.d_digits;
-  p.digits_bytes =
-      p.tile && !g.x_digits.d_digits ? sufhip_digits2_bytes(g.x_rows, g.w.K) : 0;
+  // Walks beside the product where its workgroups leave room, one round of the
+  // chip, and the epilogue's launch that evaluates the gates follows anyway or
+  // has little to do.  (One gate's walks alone take 13 us: logits of one token
+  // 42 -> 33 us.  Beside 504 workgroups of two row tiles, with a launch for a
+  // million outputs of its own, 85 us against 73.)
   const size_t mn = size_t(g.rows) * size_t(g.w.N);
+  p.walk = g.walk_count > 0 && g.walk_count <= kLinWalks && p.rt == 1 &&
+           wgs * p.slices <= 2 * device_cus() && (p.epilogue || mn <= (size_t(1) << 17));
+  p.epilogue = p.epilogue || p.walk;
   p.words = !p.epilogue ? 0 : (p.slices > 1 ? size_t(p.slices) * 2 * mn : mn);
   return p;
 }
@@ -783,28 +670,25 @@ int check_extents(const sufhip_linear2_args& g, const char* what) {
   return SUFHIP_OK;
 }
 
-template <int J>
-void launch_skinny(const LinArgs& a, int t, unsigned grid, hipStream_t s) {
-  if (t == 16) {
-    if (a.xd)
-      hipLaunchKernelGGL((linear_skinny_kernel<16, J, true>), dim3(grid), dim3(256), 0, s, a);
-    else
-      hipLaunchKernelGGL((linear_skinny_kernel<16, J, false>), dim3(grid), dim3(256), 0, s, a);
-  } else {
-    if (a.xd)
-      hipLaunchKernelGGL((linear_skinny_kernel<32, J, true>), dim3(grid), dim3(256), 0, s, a);
-    else
-      hipLaunchKernelGGL((linear_skinny_kernel<32, J, false>), dim3(grid), dim3(256), 0, s, a);
-  }
+template <int kRt, int J>
+void launch_tiles(const LinArgs& a, const LinWalk& w, unsigned wgs, hipStream_t s) {
+  const dim3 grid(wgs + unsigned(w.groups)), block(256);
+  if (a.xd && w.groups)
+    hipLaunchKernelGGL((linear_product_kernel<kRt, J, true, true>), grid, block, 0, s, a, w);
+  else if (a.xd)
+    hipLaunchKernelGGL((linear_product_kernel<kRt, J, true, false>), grid, block, 0, s, a, w);
+  else if (w.groups)
+    hipLaunchKernelGGL((linear_product_kernel<kRt, J, false, true>), grid, block, 0, s, a, w);
+  else
+    hipLaunchKernelGGL((linear_product_kernel<kRt, J, false, false>), grid, block, 0, s, a, w);
 }
 
-int launch_split(const Mat2& x, int rows, int cols, int8_t* digits, hipStream_t s) {
-  const size_t items = size_t(2) * rows * ((cols + 31) / 32 * 2);
-  size_t grid = (items + 255) / 256;
-  if (grid > 8192) grid = 8192;
-  hipLaunchKernelGGL(split_rows_kernel, dim3(unsigned(grid)), dim3(256), 0, s, x, rows, cols,
-                     digits);
-  return check_launch("split_rows_kernel");
+template <int J>
+void launch_product(const LinArgs& a, const LinWalk& w, int rt, unsigned wgs, hipStream_t s) {
+  if constexpr (J <= 2) {
+    if (rt == 2) return launch_tiles<2, J>(a, w, wgs, s);
+  }
+  launch_tiles<1, J>(a, w, wgs, s);
 }
 
 }  // namespace
@@ -832,7 +716,12 @@ int sufhip_digits2_split(const sufhip_matrix2* x, const sufhip_digits2* out, voi
     if (range_meets(out->d_digits, sufhip_digits2_bytes(out->rows, out->cols),
                     row_set(m, p, out->rows, out->cols)))
       return ff_fail(what, "out meets x");
-  return launch_split(m, out->rows, out->cols, out->d_digits, as_stream(stream));
+  const size_t items = size_t(2) * out->rows * ((out->cols + 31) / 32 * 2);
+  size_t grid = (items + 255) / 256;
+  if (grid > 8192) grid = 8192;
+  hipLaunchKernelGGL(split_rows_kernel, dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), m,
+                     out->rows, out->cols, out->d_digits);
+  return check_launch("split_rows_kernel");
 }
 
 size_t sufhip_linear_planes_bytes(int experts, int K, int N, int digits) {
@@ -862,8 +751,7 @@ int sufhip_linear_prepare(const int64_t* d_W, int experts, int K, int N, int dig
 size_t sufhip_linear2_work_bytes(const sufhip_linear2_args* args) {
   if (!args || check_extents(*args, "sufhip_linear2_work_bytes") != SUFHIP_OK) return 0;
   if (args->rows == 0 || args->x_rows == 0) return 0;
-  const Plan p = plan_linear(*args);
-  return p.digits_bytes + p.words * 8;
+  return plan_linear(*args).words * 8;
 }
 
 int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
@@ -934,8 +822,10 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
     if (int rc = digits2_of(g.out_digits, g.rows, g.w.N, what, "out_digits")) return rc;
   a.digits = g.out_digits.d_digits;
   a.out_stride = g.out_stride;
+  if (g.walk_count < 0 || (g.walk_count > 0 && (!g.walk_jobs || !g.walk_prg_state)))
+    return ff_fail(what, "walk_jobs and walk_prg_state are needed for walk_count jobs");
   const Plan plan = plan_linear(g);
-  const size_t need = plan.digits_bytes + plan.words * 8;
+  const size_t need = plan.words * 8;
   if (need && (!g.d_work || (reinterpret_cast<uintptr_t>(g.d_work) & 15) != 0 ||
                g.work_bytes < need))
     return ff_fail(what, "the workspace is null, not 16-byte aligned or too small");
@@ -980,54 +870,57 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
     if (bad) return ff_fail(what, "out_digits meets an input or the workspace");
   }
   hipStream_t s = as_stream(stream);
-  int8_t* work = static_cast<int8_t*>(g.d_work);
-  if (plan.digits_bytes) {
-    if (int rc = launch_split(a.x, g.x_rows, g.w.K, work, s)) return rc;
-    a.xd = work;
+  LinWalk w{};
+  if (plan.walk) {  // room for them: a workgroup a CU
+    size_t lanes = 0;
+    if (int rc = plan_hosted_walk(g.walk_prg_state, g.walk_jobs, g.walk_count,
+                                  size_t(device_cus()) * 256, stream, what, w.jobs, &lanes))
+      return rc;
+    w.groups = int((lanes + 256 * 8 - 1) / (256 * 8)) * 8;
+  } else if (g.walk_count > 0) {
+    if (int rc = sufhip_trunc_prepare_batch(g.walk_prg_state, g.walk_jobs, g.walk_count, stream))
+      return rc;
   }
-  uint64_t* words = reinterpret_cast<uint64_t*>(work + plan.digits_bytes);
+  uint64_t* words = static_cast<uint64_t*>(g.d_work);
   a.tiles = plan.tiles;
   a.slices = plan.slices;
   if (plan.slices > 1)
     a.part = words;
   else if (plan.epilogue)
     a.zhat = words;
-  if (plan.tile) {
-    const unsigned grid = unsigned(int64_t(plan.tiles) * plan.slices * plan.col_tiles);
-    switch (g.w.digits) {
-      case 1: hipLaunchKernelGGL(linear_tile_kernel<1>, dim3(grid), dim3(256), 0, s, a); break;
-      case 2: hipLaunchKernelGGL(linear_tile_kernel<2>, dim3(grid), dim3(256), 0, s, a); break;
-      case 3: hipLaunchKernelGGL(linear_tile_kernel<3>, dim3(grid), dim3(256), 0, s, a); break;
-      default: hipLaunchKernelGGL(linear_tile_kernel<4>, dim3(grid), dim3(256), 0, s, a); break;
-    }
-    if (int rc = check_launch("linear_tile_kernel")) return rc;
-  } else {
-    const unsigned grid = unsigned(int64_t(plan.tiles) * plan.slices * plan.col_tiles);
-    switch (g.w.digits) {
-      case 1: launch_skinny<1>(a, plan.t, grid, s); break;
-      case 2: launch_skinny<2>(a, plan.t, grid, s); break;
-      case 3: launch_skinny<3>(a, plan.t, grid, s); break;
-      default: launch_skinny<4>(a, plan.t, grid, s); break;
-    }
-    if (int rc = check_launch("linear_skinny_kernel")) return rc;
+  const unsigned wgs = unsigned(int64_t(plan.tiles) * plan.slices * plan.col_tiles);
+  switch (g.w.digits) {
+    case 1: launch_product<1>(a, w, plan.rt, wgs, s); break;
+    case 2: launch_product<2>(a, w, plan.rt, wgs, s); break;
+    case 3: launch_product<3>(a, w, plan.rt, wgs, s); break;
+    default: launch_product<4>(a, w, plan.rt, wgs, s); break;
   }
+  if (int rc = check_launch("linear_product_kernel")) return rc;
   if (!plan.epilogue) return SUFHIP_OK;
   const EpiArgs e{a, act};
   const size_t cus = size_t(device_cus());
-  const bool wide = g.act == SUFHIP_ACT_CUBIC && mn >= 2 * cus * EpiCfg<true>::kBlock;
-  const size_t block = wide ? EpiCfg<true>::kBlock : EpiCfg<false>::kBlock;
+  // Wide from two full passes of the chip on, as the chains' own launch; small
+  // below one of the mid form's.
+  const int size = g.act == SUFHIP_ACT_CUBIC && mn >= 2 * cus * 1024 ? kEpiWide
+                   : g.act != SUFHIP_ACT_NONE && mn < cus * 1024     ? kEpiSmall
+                                                                     : kEpiMid;
+  const size_t block = size == kEpiWide ? 1024 : (size == kEpiMid ? 512 : 256);
   size_t grid = (mn + block - 1) / block;
-  const size_t cap = cus * (wide ? 1 : (g.act == SUFHIP_ACT_NONE ? 4 : 2));
-  if (grid > cap) grid = cap;
+  const size_t cap = cus * (size == kEpiWide ? 1 : (g.act == SUFHIP_ACT_NONE ? 4 : 2));
+  if (grid > cap && size != kEpiSmall) grid = cap;
   const dim3 gd{unsigned(grid)}, bd{unsigned(block)};
-  if (g.act == SUFHIP_ACT_RELU)
-    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_RELU, false>), gd, bd, 0, s, e);
-  else if (g.act == SUFHIP_ACT_CUBIC && wide)
-    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_CUBIC, true>), gd, bd, 0, s, e);
-  else if (g.act == SUFHIP_ACT_CUBIC)
-    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_CUBIC, false>), gd, bd, 0, s, e);
+  if (g.act == SUFHIP_ACT_NONE)
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_NONE, kEpiMid>), gd, bd, 0, s, e);
+  else if (g.act == SUFHIP_ACT_RELU && size == kEpiSmall)
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_RELU, kEpiSmall>), gd, bd, 0, s, e);
+  else if (g.act == SUFHIP_ACT_RELU)
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_RELU, kEpiMid>), gd, bd, 0, s, e);
+  else if (size == kEpiSmall)
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_CUBIC, kEpiSmall>), gd, bd, 0, s, e);
+  else if (size == kEpiMid)
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_CUBIC, kEpiMid>), gd, bd, 0, s, e);
   else
-    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_NONE, false>), gd, bd, 0, s, e);
+    hipLaunchKernelGGL((linear_epilogue_kernel<SUFHIP_ACT_CUBIC, kEpiWide>), gd, bd, 0, s, e);
   return check_launch("linear_epilogue_kernel");
 }
 

@@ -118,16 +118,18 @@ class _Block:
         s = self.dealer.words(v.size).reshape(v.shape)
         return dev(s, self.device), dev(v - s, self.device)
 
+    def _jobs(self):
+        """(PRG state, jobs, count) of the gates' key-only halves."""
+        if self._walks is None:
+            self._walks = trunc_jobs(self.truncs())
+        return self._walks
+
     def _ready(self, prep):
         """The gates' key-only halves: issued here, or waited for."""
         if prep is not None:
             prep[0].wait(prep[1])
             return
-        if not self.truncs():
-            return
-        if self._walks is None:
-            self._walks = trunc_jobs(self.truncs())
-        state, jobs, count = self._walks
+        state, jobs, count = self._jobs()
         native.call("sufhip_trunc_prepare_batch", state, jobs, count,
                     torch._C._cuda_getCurrentRawStream(self.d))
 
@@ -382,7 +384,7 @@ class Linear(_Block):
         some = torch.empty(2, dtype=torch.int64, device=self.device).data_ptr()
         nb = 0
         for offsets in (None, some):
-            for digits in (None, some):
+            for digits in (None, some):  # with an epilogue of its own, as walks have it
                 a.d_offsets, a.out_digits.d_digits = offsets, digits
                 nb = max(nb, native.load().sufhip_linear2_work_bytes(ctypes.byref(a)))
         a.d_offsets = a.out_digits.d_digits = None
@@ -432,7 +434,11 @@ class Linear(_Block):
         elif out is None:
             _fail(what, "no output")
         with self._guard():
-            self._ready(prep)
+            if prep is not None:
+                self._ready(prep)
+            elif self.tr is not None:  # the call walks its gates' keys itself
+                state, jobs, a.walk_count = self._jobs()
+                a.walk_jobs, a.walk_prg_state = ctypes.addressof(jobs), ctypes.addressof(state)
             _call("sufhip_linear2", a, d)
         return out
 

@@ -387,7 +387,8 @@ class Linear2Args(ctypes.Structure):
                 ("trunc", ctypes.POINTER(TruncEpilogue)), ("mask", c_u64), ("act", c_int),
                 ("relu", ReluKey), ("cubic", ctypes.POINTER(Chain2Args)), ("residual", Matrix2),
                 ("out", c_vp * 2), ("out_stride", c_i64), ("out_digits", Digits2),
-                ("d_work", c_vp), ("work_bytes", c_sz)]
+                ("d_work", c_vp), ("work_bytes", c_sz), ("walk_jobs", c_vp),
+                ("walk_count", c_int), ("walk_prg_state", c_vp)]
 
 
 class ExpertMix2Args(ctypes.Structure):
