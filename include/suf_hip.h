@@ -1160,7 +1160,12 @@ int sufhip_digits2_split(const sufhip_matrix2* x, const sufhip_digits2* out, voi
  * chain, x and out are ignored.  weight: public, [cols], or NULL.
  * out (both or neither) and out_digits (d_digits NULL: none) receive o.
  * total and out may each be x or residual itself (the same addresses and
- * strides); no other output may meet an input. */
+ * strides); no other output may meet an input.
+ * d_work: sufhip_rmsnorm2_work_bytes() bytes, 16-byte aligned, used by this
+ * call only until it ends; 0 bytes: none needed.  walk_jobs (walk_count > 0):
+ * the key-only halves of truncation gates, as sufhip_trunc_prepare_batch(
+ * walk_prg_state, walk_jobs, walk_count) would write them, done by this call
+ * before it evaluates a gate, so that its own gates may be among them. */
 typedef struct sufhip_rmsnorm2_args {
   sufhip_matrix2 x;
   sufhip_matrix2 residual; /* p NULL: none */
@@ -1183,7 +1188,13 @@ typedef struct sufhip_rmsnorm2_args {
   uint64_t* out[2];
   int64_t out_stride;
   sufhip_digits2 out_digits;
+  void* d_work;
+  size_t work_bytes;
+  const sufhip_trunc_job* walk_jobs;
+  int walk_count;
+  const uint8_t* walk_prg_state;
 } sufhip_rmsnorm2_args;
+size_t sufhip_rmsnorm2_work_bytes(int rows, int cols);
 int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream);
 
 /* Public weights of one or more matrices K x N ("experts") as `digits`

@@ -30,11 +30,20 @@ __device__ __forceinline__ u64x2u load2(const uint64_t* p, bool two) {
   return u64x2u{p[0], 0};
 }
 
-__global__ void __launch_bounds__(256) expert_mix2_kernel(MixArgs a) {
+// kLds: the gate's tables in LDS, for many outputs.
+template <bool kLds>
+__global__ void __launch_bounds__(kLds ? 1024 : 256, kLds ? 8 : 4) expert_mix2_kernel(MixArgs a) {
+  __shared__ __align__(16) uint64_t tables[kLds ? sizeof(LdsGate) / 8 : 1];
+  LdsGate& lds = reinterpret_cast<LdsGate&>(tables);
+  if constexpr (kLds) {
+    stage_gate(a.epi, lds);
+    __syncthreads();
+  }
   const EpiHdrs eh = epi_hdrs(a.epi);
   const uint32_t half = uint32_t(a.cols + 1) / 2;
   const size_t n = size_t(a.tokens) * half;
-  for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += size_t(gridDim.x) * 256) {
+  for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+       i += size_t(gridDim.x) * blockDim.x) {
     const int t = int(uint32_t(i) / half), c = 2 * int(uint32_t(i) % half);
     const bool two = c + 1 < a.cols;
     const int32_t* slots = a.slots + size_t(t) * a.each;
@@ -66,7 +75,13 @@ __global__ void __launch_bounds__(256) expert_mix2_kernel(MixArgs a) {
     }
     if (a.epi.on) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) gate2(a.epi, eh, y[h][0] + y[h][1] + a.mask, y[h]);
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t open = y[h][0] + y[h][1] + a.mask;
+        if constexpr (kLds)
+          gate2(a.epi, eh, lds, open, y[h]);
+        else
+          gate2(a.epi, eh, open, y[h]);
+      }
     }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
@@ -132,8 +147,16 @@ extern "C" int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* str
       }
     }
   const size_t n = size_t(g.tokens) * size_t((g.cols + 1) / 2);
-  size_t grid = (n + 255) / 256;
-  if (grid > 16384) grid = 16384;
-  hipLaunchKernelGGL(expert_mix2_kernel, dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
+  hipStream_t s = as_stream(stream);
+  if (a.epi.on && a.epi.f <= kLdsGateBits && n >= (size_t(1) << 19)) {
+    int dev = 0, cus = 256;
+    if (hipGetDevice(&dev) == hipSuccess)
+      (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+    hipLaunchKernelGGL(expert_mix2_kernel<true>, dim3(unsigned(2 * cus)), dim3(1024), 0, s, a);
+  } else {
+    size_t grid = (n + 255) / 256;
+    if (grid > 16384) grid = 16384;
+    hipLaunchKernelGGL(expert_mix2_kernel<false>, dim3(unsigned(grid)), dim3(256), 0, s, a);
+  }
   return check_launch("expert_mix2_kernel");
 }

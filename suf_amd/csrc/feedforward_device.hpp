@@ -77,6 +77,30 @@ __device__ __forceinline__ void gate2(const TruncEpi& e, const EpiHdrs& eh, uint
   y[1] = trunc_table_out(eh.h[1], e.f, open, w1);
 }
 
+// Gates of up to kLdsGateBits bits with their tables in LDS, for streaming
+// kernels: read from memory, each of a wave's 64 places in a 32 KB table is a
+// line of the L1 cache to fetch, which four tables do not fit (the large
+// norm's outputs: 94 -> 62 us).
+constexpr int kLdsGateBits = 12;
+typedef uint64_t LdsGate[2][1 << kLdsGateBits];
+
+// Both parties' tables of gate e; the caller syncs.
+__device__ __forceinline__ void stage_gate(const TruncEpi& e, LdsGate& t) {
+  const int n = 1 << (e.f - 1);  // pairs
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+    for (int i = threadIdx.x; i < n; i += blockDim.x)
+      reinterpret_cast<uint4*>(t[p])[i] = e.table[p][i];
+}
+
+__device__ __forceinline__ void gate2(const TruncEpi& e, const EpiHdrs& eh, const LdsGate& t,
+                                      uint64_t open, uint64_t (&y)[2]) {
+  const uint64_t at = open & ((uint64_t(1) << e.f) - 1);
+  const uint64_t w0 = t[0][at], w1 = t[1][at];
+  y[0] = trunc_table_out(eh.h[0], e.f, open, w0);
+  y[1] = trunc_table_out(eh.h[1], e.f, open, w1);
+}
+
 // ---- host ----
 
 inline int ff_fail(const char* what, const std::string& msg) {

@@ -16,6 +16,7 @@
 #include "chain_device.hpp"
 #include "feedforward_device.hpp"
 #include "reduce_device.hpp"
+#include "walk_device.hpp"
 
 namespace sufhip {
 namespace {
@@ -42,8 +43,18 @@ struct RmsArgs {
   uint64_t* out[2];
   int64_t out_stride;
   int8_t* digits;
+  uint64_t* sums;   // the launches of a large norm: [2][rows] sums of s s
+  uint64_t* opens;  // [rows] opens of the rows' factors
 };
-static_assert(sizeof(RmsArgs) <= 4096, "kernel argument blocks must fit in 4 KB");
+
+// Key-only walks beside a large norm's sums: its own nine gates of both parties.
+constexpr int kRmsWalks = 18;
+struct RmsWalk {
+  WalkJobs<kRmsWalks> jobs;
+  int groups;  // workgroups of them, the launch's first
+};
+static_assert(sizeof(RmsArgs) + sizeof(RmsWalk) <= 4096,
+              "kernel argument blocks must fit in 4 KB");
 
 // The kernel's argument read afresh from the kernarg segment, an opaque copy of
 // its address per phase of a row: a phase's pointers are scalar loads where
@@ -138,9 +149,11 @@ __device__ __forceinline__ void rms_load(RmsQuad& v, int r, int c, bool again) {
 }
 
 // The outputs at those columns: b0, b1 the shares of the row's mask, E the open
-// of its factor.
+// of its factor; lds: the elements' gates' tables (the norm's, the weight's), or
+// none, to read them in memory.
+template <bool kLds = false>
 __device__ __forceinline__ void rms_put(const RmsQuad& v, int r, int c, uint64_t b0,
-                                        uint64_t b1, uint64_t E) {
+                                        uint64_t b1, uint64_t E, const LdsGate* lds = nullptr) {
   const RmsArgs& A = rms_args();
   const int cols = A.cols;
   const size_t base = size_t(r) * size_t(cols);
@@ -155,7 +168,11 @@ __device__ __forceinline__ void rms_put(const RmsQuad& v, int r, int c, uint64_t
     z[0][q] += v.D[q] * b0 + v.a0[q] * E + v.D[q] * E;
     z[1][q] += v.D[q] * b1 + v.a1[q] * E;
     uint64_t o[2];
-    gate2(A.tr[kNorm], hn, z[0][q] + z[1][q] + A.mask[kNorm], o);
+    const uint64_t open = z[0][q] + z[1][q] + A.mask[kNorm];
+    if constexpr (kLds)
+      gate2(A.tr[kNorm], hn, lds[0], open, o);
+    else
+      gate2(A.tr[kNorm], hn, open, o);
     y[0][q] = o[0];
     y[1][q] = o[1];
   }
@@ -163,7 +180,11 @@ __device__ __forceinline__ void rms_put(const RmsQuad& v, int r, int c, uint64_t
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       uint64_t o[2];
-      gate2(A.tr[kWeight], hw, y[0][q] * w[q] + y[1][q] * w[q] + A.mask[kWeight], o);
+      const uint64_t open = y[0][q] * w[q] + y[1][q] * w[q] + A.mask[kWeight];
+      if constexpr (kLds)
+        gate2(A.tr[kWeight], hw, lds[1], open, o);
+      else
+        gate2(A.tr[kWeight], hw, open, o);
       y[0][q] = o[0];
       y[1][q] = o[1];
     }
@@ -186,6 +207,44 @@ __device__ __forceinline__ void rms_put(const RmsQuad& v, int r, int c, uint64_t
   }
 }
 
+// The row's factor from its sums: the gates of the mean square and the chain,
+// on one wave, every lane with the same values.  The caller staged the chain's
+// LUT, triples and headers.  Returns the shares.
+__device__ __forceinline__ Two rms_factor(const uint32_t* tab, const ChainLds& L,
+                                          const TruncHdr (*th)[2], const TruncHdr (*rth)[2],
+                                          const ChainPre& pre, int r, uint64_t s0, uint64_t s1) {
+  const RmsArgs& A = rms_args();
+  const RmsAes aes{tab, uint32_t(rms_lane()) % kRmsCopies};
+  const ChainKeyInfo K = chain_key_info(A.rs, L);
+  auto gate = [&](int j, uint64_t x) {
+    return Two{{trunc_table_eval_h(th[j][0], A.tr[j].table[0], A.tr[j].f, x),
+                trunc_table_eval_h(th[j][1], A.tr[j].table[1], A.tr[j].f, x)}};
+  };
+  Two m = gate(kMs0, (s0 + A.a2[0][r]) + (s1 + A.a2[1][r]) + A.mask[kMs0]);
+  m = gate(kMs1, m.v[0] * A.inv_len + m.v[1] * A.inv_len + A.mask[kMs1]);
+  m = gate(kMs2, m.v[0] + m.v[1] + A.mask[kMs2]);
+  const Two ms{{m.v[0] + A.eps, m.v[1]}};
+  return chain_eval_quad<SUFHIP_CHAIN_RSQRT, RmsAes>(rms_args().rs, L, K, aes, size_t(r), ms, pre,
+                                                     rth);
+}
+
+// What rms_factor needs in LDS; ends with a barrier.
+__device__ __forceinline__ void rms_stage(uint32_t* tab, ChainLds& L, TruncHdr (*th)[2],
+                                          TruncHdr (*rth)[2]) {
+  const RmsArgs& A = rms_args();
+  fill_ttable<kRmsCopies>(tab, kTDev.v);
+  chain_stage(A.rs, 2, L);
+  if (int(threadIdx.x) < 2 * kNorm)
+    th[threadIdx.x >> 1][threadIdx.x & 1] =
+        read_trunc_hdr(A.tr[threadIdx.x >> 1].key[threadIdx.x & 1]);
+  TruncHdrStager<chain_products<SUFHIP_CHAIN_RSQRT>()> hs;
+  hs.load(A.rs, 64);
+  hs.store(rth);
+  __syncthreads();
+  chain_compare(A.rs, L);
+  __syncthreads();
+}
+
 // A row of up to 4 kQuads kBlock values stays on the CU from the sum to the
 // output; with kLong a longer one is read again for the output.
 template <int kQuads, int kBlock, bool kLong>
@@ -203,20 +262,7 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs
   // Wave 0's values of the row while it runs the row's chain, which needs their
   // registers.
   __shared__ uint64_t held[kLong ? 1 : 12 * kQuads][64];
-  {
-    const RmsArgs& A = rms_args();
-    fill_ttable<kRmsCopies>(tab, kTDev.v);
-    chain_stage(A.rs, 2, L);
-    if (int(threadIdx.x) < 2 * kNorm)
-      th[threadIdx.x >> 1][threadIdx.x & 1] =
-          read_trunc_hdr(A.tr[threadIdx.x >> 1].key[threadIdx.x & 1]);
-    TruncHdrStager<kProds> hs;
-    hs.load(A.rs, 64);
-    hs.store(rth);
-    __syncthreads();
-    chain_compare(A.rs, L);
-    __syncthreads();
-  }
+  rms_stage(tab, L, th, rth);
   const int rows = rms_args().rows, cols = rms_args().cols;
   // Lanes whose columns end before this write nothing, not even digits.
   const int end = (cols + 31) / 32 * 32;
@@ -252,20 +298,8 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs
           }
         asm volatile("" ::: "memory");  // and nothing of them stays in registers
       }
-      const RmsArgs& A = rms_args();
-      const RmsAes aes{tab, uint32_t(rms_lane()) % kRmsCopies};
-      const ChainKeyInfo K = chain_key_info(A.rs, L);
-      auto gate = [&](int j, uint64_t x) {
-        return Two{{trunc_table_eval_h(th[j][0], A.tr[j].table[0], A.tr[j].f, x),
-                    trunc_table_eval_h(th[j][1], A.tr[j].table[1], A.tr[j].f, x)}};
-      };
-      const uint64_t b0 = A.b[0][r], b1 = A.b[1][r];
-      Two m = gate(kMs0, (q0 + A.a2[0][r]) + (q1 + A.a2[1][r]) + A.mask[kMs0]);
-      m = gate(kMs1, m.v[0] * A.inv_len + m.v[1] * A.inv_len + A.mask[kMs1]);
-      m = gate(kMs2, m.v[0] + m.v[1] + A.mask[kMs2]);
-      const Two ms{{m.v[0] + A.eps, m.v[1]}};
-      const Two y = chain_eval_quad<SUFHIP_CHAIN_RSQRT, RmsAes>(rms_args().rs, L, K, aes,
-                                                                size_t(r), ms, pre, rth);
+      const Two y = rms_factor(tab, L, th, rth, pre, r, q0, q1);
+      const uint64_t b0 = rms_args().b[0][r], b1 = rms_args().b[1][r];
       if (threadIdx.x == 0) {
         bc[0] = b0;
         bc[1] = b1;
@@ -299,12 +333,146 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs
   }
 }
 
-template <int kQuads, int kBlock, bool kLong>
-int launch_rms(const RmsArgs& A, hipStream_t s) {
+// A large norm in three launches, each at the memory's pace: the rows' sums (and
+// total), with the gates' walks beside them; the rows' factors, a wave a row;
+// the outputs.  Row by row in one launch, the workgroups all wait for their
+// chains at the same time, and behind each other's loads: 1999 x 2048 with
+// total and weight 134 us after 22 of walks.
+//
+// kWaveRow: a wave a row (rows of up to 1024 values), else a workgroup a row.
+template <bool kWaveRow, bool kWalk>
+__global__ void __launch_bounds__(256) rms_sum_kernel(RmsArgs, RmsWalk wk) {
+  if constexpr (kWalk) {
+    if (int(blockIdx.x) < wk.groups) {
+      hosted_walk_role<kRmsWalks, false>(wk.jobs, blockIdx.x * 256 + threadIdx.x);
+      return;
+    }
+  }
+  __shared__ uint64_t red[2][4];
+  const int first = int(blockIdx.x) - (kWalk ? wk.groups : 0);
+  const int step = int(gridDim.x) - (kWalk ? wk.groups : 0);
+  const int rows = rms_args().rows, cols = rms_args().cols;
+  const int wave = int(threadIdx.x) >> 6, lane = kWaveRow ? int(threadIdx.x) & 63 : int(threadIdx.x);
+  constexpr int kPerGroup = kWaveRow ? 4 : 1, kSpan = kWaveRow ? 256 : 1024;
+  for (int r = first * kPerGroup + (kWaveRow ? wave : 0); r < rows; r += step * kPerGroup) {
+    uint64_t q0 = 0, q1 = 0;
+    for (int c = 4 * lane; c < cols; c += kSpan) {
+      RmsQuad v;
+      rms_load(v, r, c, false);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        q0 += 2 * v.D[q] * v.a0[q] + v.D[q] * v.D[q];
+        q1 += 2 * v.D[q] * v.a1[q];
+      }
+    }
+    if constexpr (kWaveRow) {
+      q0 = wave_sum_u64(q0);
+      q1 = wave_sum_u64(q1);
+    } else {
+      block_sum2_u64<4>(q0, q1, red);
+    }
+    if (lane == 0) {
+      rms_args().sums[r] = q0;
+      rms_args().sums[size_t(rows) + r] = q1;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) rms_factor_kernel(RmsArgs) {
+  __shared__ __align__(16) uint32_t tab[256 * kRmsCopies];
+  __shared__ ChainLds L;
+  __shared__ TruncHdr th[kNorm][2];
+  __shared__ TruncHdr rth[chain_products<SUFHIP_CHAIN_RSQRT>()][2];
+  __shared__ ChainPre pre[4];
+  rms_stage(tab, L, th, rth);
+  const int rows = rms_args().rows;
+  const int wave = int(threadIdx.x) >> 6, lane = int(threadIdx.x) & 63;
+  // Every wave of a workgroup makes the same number of rounds (the barriers).
+  for (int r0 = int(blockIdx.x) * 4; r0 < rows; r0 += int(gridDim.x) * 4) {
+    const int r = r0 + wave < rows ? r0 + wave : rows - 1;
+    if (lane < 24) pre[wave].word(lane) = chain_triple_word(rms_args().rs, lane, size_t(r));
+    __syncthreads();
+    const RmsArgs& A = rms_args();
+    const Two y =
+        rms_factor(tab, L, th, rth, pre[wave], r, A.sums[r], A.sums[size_t(rows) + r]);
+    if (lane == 0 && r0 + wave < rows)
+      rms_args().opens[r] =
+          (y.v[0] - rms_args().b[0][r]) + (y.v[1] - rms_args().b[1][r]);
+    __syncthreads();  // pre is rewritten for the next row
+  }
+}
+
+// kGates: of the elements' gates, the norm's and the weight's, how many have
+// their tables in LDS (all or none).
+template <int kGates>
+__global__ void __launch_bounds__(kGates ? 1024 : 256) rms_out_kernel(RmsArgs) {
+  __shared__ __align__(16) LdsGate lds[kGates ? kGates : 1];
+  if constexpr (kGates > 0) {
+    stage_gate(rms_args().tr[kNorm], lds[0]);
+    if constexpr (kGates > 1) stage_gate(rms_args().tr[kWeight], lds[1]);
+    __syncthreads();
+  }
+  const int rows = rms_args().rows, cols = rms_args().cols;
+  const uint32_t quads = uint32_t((cols + 31) / 32) * 8;  // with the digits' padding
+  const size_t n = size_t(rows) * quads;
+  for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+       i += size_t(gridDim.x) * blockDim.x) {
+    const int r = int(i / quads), c = 4 * int(i % quads);
+    RmsQuad v;
+    rms_load(v, r, c, true);
+    const RmsArgs& A = rms_args();
+    rms_put<(kGates > 0)>(v, r, c, A.b[0][r], A.b[1][r], A.opens[r], lds);
+  }
+}
+
+int device_cus() {
   int dev = 0, cus = 256;
   if (hipGetDevice(&dev) == hipSuccess)
     (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
-  const int cap = cus * (2048 / kBlock > 8 ? 8 : 2048 / kBlock);
+  return cus;
+}
+
+// Whether a norm takes the three launches.
+bool rms_large(int rows, int cols) { return size_t(rows) * size_t(cols) >= (size_t(3) << 19); }
+
+int launch_large(const RmsArgs& A, const RmsWalk& w, hipStream_t s) {
+  const int cus = device_cus();
+  const bool wave = A.cols <= 1024;
+  int groups = wave ? (A.rows + 3) / 4 : A.rows;
+  if (groups > 8 * cus) groups = 8 * cus;
+  const dim3 g(unsigned(groups + w.groups)), b(256);
+  if (wave && w.groups)
+    hipLaunchKernelGGL((rms_sum_kernel<true, true>), g, b, 0, s, A, w);
+  else if (wave)
+    hipLaunchKernelGGL((rms_sum_kernel<true, false>), g, b, 0, s, A, w);
+  else if (w.groups)
+    hipLaunchKernelGGL((rms_sum_kernel<false, true>), g, b, 0, s, A, w);
+  else
+    hipLaunchKernelGGL((rms_sum_kernel<false, false>), g, b, 0, s, A, w);
+  if (int rc = check_launch("rms_sum_kernel")) return rc;
+  groups = (A.rows + 3) / 4;
+  if (groups > 4 * cus) groups = 4 * cus;
+  hipLaunchKernelGGL(rms_factor_kernel, dim3(unsigned(groups)), b, 0, s, A);
+  if (int rc = check_launch("rms_factor_kernel")) return rc;
+  if (!A.out[0] && !A.digits) return SUFHIP_OK;
+  const size_t n = size_t(A.rows) * size_t((A.cols + 31) / 32) * 8;
+  if (A.tr[kNorm].f <= kLdsGateBits && (!A.w || A.tr[kWeight].f <= kLdsGateBits)) {
+    const dim3 lg{unsigned(cus)}, lb{1024};
+    if (A.w)
+      hipLaunchKernelGGL(rms_out_kernel<2>, lg, lb, 0, s, A);
+    else
+      hipLaunchKernelGGL(rms_out_kernel<1>, lg, lb, 0, s, A);
+  } else {
+    size_t out = (n + 255) / 256;
+    if (out > size_t(32) * cus) out = size_t(32) * cus;
+    hipLaunchKernelGGL(rms_out_kernel<0>, dim3(unsigned(out)), b, 0, s, A);
+  }
+  return check_launch("rms_out_kernel");
+}
+
+template <int kQuads, int kBlock, bool kLong>
+int launch_rms(const RmsArgs& A, hipStream_t s) {
+  const int cap = device_cus() * (2048 / kBlock > 8 ? 8 : 2048 / kBlock);
   const int grid = A.rows < cap ? A.rows : cap;
   hipLaunchKernelGGL((rmsnorm2_kernel<kQuads, kBlock, kLong>), dim3(unsigned(grid)), dim3(kBlock), 0,
                      s, A);
@@ -317,6 +485,11 @@ int launch_rms(const RmsArgs& A, hipStream_t s) {
 using namespace sufhip;
 
 extern "C" {
+
+size_t sufhip_rmsnorm2_work_bytes(int rows, int cols) {
+  if (rows < 1 || cols < 1 || rows > kMaxRows || cols > (1 << 20)) return 0;
+  return rms_large(rows, cols) ? (size_t(rows) * 24 + 15) / 16 * 16 : 0;
+}
 
 int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream) {
   const char* what = "sufhip_rmsnorm2";
@@ -409,7 +582,32 @@ int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream) {
     for (int i = 0; i < count; ++i)
       if (range_meets(A.digits, bytes, outs[i])) return ff_fail(what, "out_digits meets an output");
   }
+  if (g.walk_count < 0 || (g.walk_count > 0 && (!g.walk_jobs || !g.walk_prg_state)))
+    return ff_fail(what, "walk_jobs and walk_prg_state are needed for walk_count jobs");
+  const size_t need = sufhip_rmsnorm2_work_bytes(g.rows, g.cols);
+  if (need) {
+    if (!g.d_work || (reinterpret_cast<uintptr_t>(g.d_work) & 15) != 0 || g.work_bytes < need)
+      return ff_fail(what, "the workspace is null, not 16-byte aligned or too small");
+    for (int i = 0; i < count; ++i)
+      if (range_meets(g.d_work, need, outs[i])) return ff_fail(what, "the workspace meets an output");
+  }
   hipStream_t s = as_stream(stream);
+  if (need) {
+    A.sums = static_cast<uint64_t*>(g.d_work);
+    A.opens = A.sums + 2 * size_t(g.rows);
+    RmsWalk w{};
+    if (g.walk_count > 0) {
+      size_t lanes = 0;  // room for a workgroup a CU
+      if (int rc = plan_hosted_walk(g.walk_prg_state, g.walk_jobs, g.walk_count,
+                                    size_t(device_cus()) * 256, stream, what, w.jobs, &lanes))
+        return rc;
+      w.groups = int((lanes + 255) / 256);
+    }
+    return launch_large(A, w, s);
+  }
+  if (g.walk_count > 0)
+    if (int rc = sufhip_trunc_prepare_batch(g.walk_prg_state, g.walk_jobs, g.walk_count, stream))
+      return rc;
   if (g.cols <= 1024) return launch_rms<1, 256, false>(A, s);
   if (g.cols <= 2048) return launch_rms<2, 256, false>(A, s);
   if (g.cols <= 4096) return launch_rms<2, 512, false>(A, s);

@@ -124,6 +124,14 @@ class _Block:
             self._walks = trunc_jobs(self.truncs())
         return self._walks
 
+    def _walks_of(self, a, prep):
+        """The gates' key-only halves: done by the call a, or waited for."""
+        if prep is not None:
+            prep[0].wait(prep[1])
+            return
+        state, jobs, a.walk_count = self._jobs()
+        a.walk_jobs, a.walk_prg_state = ctypes.addressof(jobs), ctypes.addressof(state)
+
     def _ready(self, prep):
         """The gates' key-only halves: issued here, or waited for."""
         if prep is not None:
@@ -234,6 +242,9 @@ class RMSNorm(_Block):
                               self.tr_rsqrt, self.b)
         a.rsqrt.out[:] = none
         a.tr_norm, a.norm_mask = _epi(self.tr_norm), self.tr_norm.mask & M64
+        nb = native.load().sufhip_rmsnorm2_work_bytes(rows, cols)
+        self.work = torch.empty((nb + 7) // 8, dtype=torch.int64, device=self.device)
+        a.d_work, a.work_bytes = (self.work.data_ptr() if nb else None), nb
         if weight is not None:
             a.d_weight = self.weight.data_ptr()
             a.tr_weight, a.weight_mask = _epi(self.tr_weight), self.tr_weight.mask & M64
@@ -261,7 +272,7 @@ class RMSNorm(_Block):
         if out is None and digits is None and total is None:
             _fail(what, "no output")
         with self._guard():
-            self._ready(prep)
+            self._walks_of(a, prep)
             _call("sufhip_rmsnorm2", a, d)
         return out
 
@@ -434,11 +445,8 @@ class Linear(_Block):
         elif out is None:
             _fail(what, "no output")
         with self._guard():
-            if prep is not None:
-                self._ready(prep)
-            elif self.tr is not None:  # the call walks its gates' keys itself
-                state, jobs, a.walk_count = self._jobs()
-                a.walk_jobs, a.walk_prg_state = ctypes.addressof(jobs), ctypes.addressof(state)
+            if prep is not None or self.tr is not None:
+                self._walks_of(a, prep)
             _call("sufhip_linear2", a, d)
         return out
 

@@ -109,6 +109,7 @@ _SIGS = {
     "sufhip_kv_values2": (c_int, [c_vp, c_vp]),
     "sufhip_digits2_bytes": (c_sz, [c_int, c_int]),
     "sufhip_digits2_split": (c_int, [c_vp, c_vp, c_vp]),
+    "sufhip_rmsnorm2_work_bytes": (c_sz, [c_int, c_int]),
     "sufhip_rmsnorm2": (c_int, [c_vp, c_vp]),
     "sufhip_linear_planes_bytes": (c_sz, [c_int, c_int, c_int, c_int]),
     "sufhip_linear_prepare": (c_int, [c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp]),
@@ -363,7 +364,9 @@ class RmsNorm2Args(ctypes.Structure):
                 ("ms_mask", c_u64 * 3), ("rsqrt", Chain2Args), ("tr_norm", TruncEpilogue),
                 ("norm_mask", c_u64), ("d_weight", c_vp), ("tr_weight", TruncEpilogue),
                 ("weight_mask", c_u64), ("total", c_vp * 2), ("total_stride", c_i64),
-                ("out", c_vp * 2), ("out_stride", c_i64), ("out_digits", Digits2)]
+                ("out", c_vp * 2), ("out_stride", c_i64), ("out_digits", Digits2),
+                ("d_work", c_vp), ("work_bytes", c_sz), ("walk_jobs", c_vp),
+                ("walk_count", c_int), ("walk_prg_state", c_vp)]
 
 
 ACT_NONE, ACT_RELU, ACT_CUBIC = range(3)

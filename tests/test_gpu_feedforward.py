@@ -55,7 +55,9 @@ def _empty(*shape):
 # ---- the norm ----
 
 NORM_SHAPES = [(1, 1), (1, 768), (3, 33), (5, 64), (2, 255), (7, 1000), (4, 1024), (3, 1025),
-               (300, 96), (2, 2048), (2, 2049), (3, 4096), (2, 4097), (1, 9001)]
+               (300, 96), (2, 2048), (2, 2049), (3, 4096), (2, 4097), (1, 9001),
+              # in three launches (3 * 2^19 values and more): waves and workgroups a row
+              (2100, 1000), (70000, 30), (1000, 2100), (30, 70001)]
 
 
 @pytest.mark.parametrize("rows,cols", NORM_SHAPES)
@@ -396,7 +398,7 @@ def test_wrong_offsets_stay_inside(off, rows):
 
 
 @pytest.mark.parametrize("tokens,each,cols", [(1, 1, 1), (1, 2, 1024), (7, 3, 33), (40, 8, 130),
-                                              (3, 0, 20), (300, 2, 65)])
+                                              (3, 0, 20), (300, 2, 65), (1050, 3, 1001)])
 def test_mix(tokens, each, cols):
     say("mix %d %d %d" % (tokens, each, cols))
     rng = np.random.default_rng(tokens + cols)
