@@ -433,7 +433,7 @@ int device_cus() {
 }
 
 // Whether a norm takes the three launches.
-bool rms_large(int rows, int cols) { return size_t(rows) * size_t(cols) >= (size_t(3) << 19); }
+bool rms_large(int rows, int cols) { return size_t(rows) * size_t(cols) >= (size_t(1) << 21); }
 
 int launch_large(const RmsArgs& A, const RmsWalk& w, hipStream_t s) {
   const int cus = device_cus();

@@ -56,7 +56,7 @@ def _empty(*shape):
 
 NORM_SHAPES = [(1, 1), (1, 768), (3, 33), (5, 64), (2, 255), (7, 1000), (4, 1024), (3, 1025),
                (300, 96), (2, 2048), (2, 2049), (3, 4096), (2, 4097), (1, 9001),
-              # in three launches (3 * 2^19 values and more): waves and workgroups a row
+              # in three launches (2^21 values and more): waves and workgroups a row
               (2100, 1000), (70000, 30), (1000, 2100), (30, 70001)]
 
 
