@@ -297,16 +297,27 @@ def rsqrt_table(frac_bits=12, eps=1.0 / 1024.0, vmax=16.0):
 def rsqrt_wide_table(frac_bits=12, eps=1.0 / 1024.0, vmax=4096.0):
     """rsqrt_table for mean squares past 16: its chords up to 16, where their
     slopes, -0.29 2^(f - 1.5 k) on [2^k, 2^(k+1)), are whole words to a few per
-    cent, then constants, each within 4.5 % of 1/sqrt on a quarter of an octave,
-    which a Newton step takes to 0.3 %, up to vmax (a power of two)."""
+    cent, then a constant on each quarter of an octave up to vmax (a power of
+    two).  A Newton step takes a quarter octave's 4.5 % to 0.3 %, but for the
+    floor of y y to 2^-f, which loses up to a share v 2^-f of it: so each
+    constant is the one whose result, floors and all, is nearest to 1/sqrt over
+    its piece.  With 12 fractional bits y is then off by 0.5 % at most up to 256,
+    0.9 % up to 1024 and 2.5 % up to 4096, where one of its steps is 1.6 %."""
     alpha, coeffs = rsqrt_table(frac_bits, eps, min(16.0, vmax))
     pieces = [(int(a), 0, [int(w) for w in c]) for a, c in zip(alpha, coeffs)][:-1]
+
+    one = math.ldexp(1.0, frac_bits)
     L = min(16.0, vmax)
     while L < vmax:
         for i in range(4):
             lo, hi = L * 2.0 ** (i / 4), L * 2.0 ** ((i + 1) / 4)
-            pieces.append((_enc(lo, frac_bits), 0,
-                           [_enc(0.5 * (lo ** -0.5 + hi ** -0.5), frac_bits), 0]))
+            v = (one * np.linspace(lo, hi, 33)).astype(np.int64)
+            want = one * (v / one) ** -0.5
+            y = np.arange(max(1, int(0.6 * want[-1])), int(1.4 * want[0]) + 2)[:, None]
+            h = (v * ((y * y) >> frac_bits)) >> (frac_bits + 1)
+            got = (y * ((3 << (frac_bits - 1)) - h)) >> frac_bits
+            best = int(y[np.abs(got / want - 1).max(1).argmin(), 0])
+            pieces.append((_enc(lo, frac_bits), 0, [best, 0]))
         L *= 2.0
     pieces.append((_enc(vmax, frac_bits), 0, [_enc(vmax ** -0.5, frac_bits), 0]))
     return _finish(pieces, 2)
