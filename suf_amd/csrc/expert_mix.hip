@@ -118,17 +118,17 @@ extern "C" int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* str
   a.weights = g.d_weights;
   if (g.each > 0 && (!g.d_slots || !g.d_weights)) return ff_fail(what, "null d_slots or d_weights");
   if (g.each > 0 && g.z_rows > 0)
-    if (int rc = mat2_of(g.z, g.z_rows, g.cols, what, "z", &a.z)) return rc;
+    if (int rc = mat2_of(g.z, g.z_rows, what, "z", &a.z)) return rc;
   if (g.trunc)
     if (int rc = gate_of(*g.trunc, size_t(g.tokens) * g.cols, what, &a.epi)) return rc;
   a.mask = g.mask;
   if ((g.residual.p[0] == nullptr) != (g.residual.p[1] == nullptr))
     return ff_fail(what, "one share of the residual is missing");
   if (g.residual.p[0])
-    if (int rc = mat2_of(g.residual, g.tokens, g.cols, what, "residual", &a.res)) return rc;
+    if (int rc = mat2_of(g.residual, g.tokens, what, "residual", &a.res)) return rc;
   if (!g.out[0] || !g.out[1]) return ff_fail(what, "out is null");
-  if (g.out_stride < 0 || rows_overlap(g.out_stride, g.tokens, g.cols))
-    return ff_fail(what, "output rows overlap");
+  if (bad_out_stride(g.out_stride, g.tokens, g.cols))
+    return ff_fail(what, "output rows overlap, or lie more than 2^35 apart");
   RowSet o[2];
   for (int p = 0; p < 2; ++p) {
     a.out[p] = g.out[p];
@@ -136,7 +136,11 @@ extern "C" int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* str
   }
   a.out_stride = g.out_stride;
   if (sets_meet(o[0], o[1])) return ff_fail(what, "the two shares of out meet");
-  for (int p = 0; p < 2; ++p)
+  const size_t listed = size_t(g.tokens) * g.each;
+  for (int p = 0; p < 2; ++p) {
+    if (range_meets(Range{g.d_slots, listed * 4}, o[p]) ||
+        range_meets(Range{g.d_weights, listed * 8}, o[p]))
+      return ff_fail(what, "out meets the slots or the weights");
     for (int q = 0; q < 2; ++q) {
       if (a.z.p[0] && sets_meet(o[p], row_set(a.z, q, g.z_rows, g.cols)))
         return ff_fail(what, "out meets z");
@@ -146,6 +150,7 @@ extern "C" int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* str
           return ff_fail(what, "out meets the residual without being it");
       }
     }
+  }
   const size_t n = size_t(g.tokens) * size_t((g.cols + 1) / 2);
   hipStream_t s = as_stream(stream);
   if (a.epi.on && a.epi.f <= kLdsGateBits && n >= (size_t(1) << 19)) {

@@ -161,10 +161,10 @@ __device__ __forceinline__ TileId tile_id(const LinArgs& a, int id, int total) {
 }
 
 // A workgroup of four waves takes kRt row tiles (8 tokens of both parties
-// each), 128 columns, 32 a wave, and one k-slice.  W goes straight into registers; X's
-// digits, which the four waves share, are formed on the way into LDS (or come
-// as digits), 64 k at a time, the next chunk's loads in flight under this
-// one's products.
+// each), 128 columns, 32 a wave, and one k-slice.  W goes straight into
+// registers; X's digits, which the four waves share, are formed on the way into
+// LDS (or come as digits), 64 k at a time, the next chunk's loads in flight
+// under this one's products.
 constexpr int kTok = 8;
 constexpr int kFrags = 2;  // column fragments of a wave
 constexpr int kDepth = 2;  // chunks on their way
@@ -183,9 +183,7 @@ __global__ void __launch_bounds__(256, 2) linear_product_kernel(LinArgs a, LinWa
   __shared__ __align__(16) int8_t lds[2][kRt][8 * 1024];
   const int l = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-  const int total = int(gridDim.x) - groups;
-  int id = int(blockIdx.x) - groups;
-  const TileId at = tile_id(a, id, total);
+  const TileId at = tile_id(a, int(blockIdx.x) - groups, int(gridDim.x) - groups);
   const int slice = at.slice, c0 = at.col * 128 + 32 * w;
   const RowTile rt = row_tile(a, at.row, kRt * kTok);
   if (rt.e < 0 || rt.begin >= rt.end) return;  // the whole workgroup
@@ -711,7 +709,7 @@ int sufhip_digits2_split(const sufhip_matrix2* x, const sufhip_digits2* out, voi
     return ff_fail(what, "rows and cols in [1, 2^24], and a buffer");
   if (int rc = digits2_of(*out, out->rows, out->cols, what, "out")) return rc;
   Mat2 m;
-  if (int rc = mat2_of(*x, out->rows, out->cols, what, "x", &m)) return rc;
+  if (int rc = mat2_of(*x, out->rows, what, "x", &m)) return rc;
   for (int p = 0; p < 2; ++p)
     if (range_meets(out->d_digits, sufhip_digits2_bytes(out->rows, out->cols),
                     row_set(m, p, out->rows, out->cols)))
@@ -782,7 +780,7 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
   if (g.x_digits.d_digits) {
     if (int rc = digits2_of(g.x_digits, g.x_rows, g.w.K, what, "x_digits")) return rc;
     a.xd = g.x_digits.d_digits;
-  } else if (int rc = mat2_of(g.x, g.x_rows, g.w.K, what, "x", &a.x)) {
+  } else if (int rc = mat2_of(g.x, g.x_rows, what, "x", &a.x)) {
     return rc;
   }
   const size_t mn = size_t(g.rows) * size_t(g.w.N);
@@ -814,7 +812,7 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
   if ((g.residual.p[0] == nullptr) != (g.residual.p[1] == nullptr))
     return ff_fail(what, "one share of the residual is missing");
   if (g.residual.p[0])
-    if (int rc = mat2_of(g.residual, g.rows, g.w.N, what, "residual", &a.res)) return rc;
+    if (int rc = mat2_of(g.residual, g.rows, what, "residual", &a.res)) return rc;
   if ((g.out[0] == nullptr) != (g.out[1] == nullptr))
     return ff_fail(what, "give both share outputs or neither");
   if (!g.out[0] && !g.out_digits.d_digits) return ff_fail(what, "no output");
@@ -825,15 +823,40 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
   if (g.walk_count < 0 || (g.walk_count > 0 && (!g.walk_jobs || !g.walk_prg_state)))
     return ff_fail(what, "walk_jobs and walk_prg_state are needed for walk_count jobs");
   const Plan plan = plan_linear(g);
+  const uint64_t tiles = uint64_t(plan.tiles) * plan.slices * plan.col_tiles;
+  if (tiles >= (uint64_t(1) << 24) - 4096)  // a launch holds 2^32 lanes
+    return ff_fail(what, "more than 2^24 tiles of 8 rows and 128 columns");
   const size_t need = plan.words * 8;
   if (need && (!g.d_work || (reinterpret_cast<uintptr_t>(g.d_work) & 15) != 0 ||
                g.work_bytes < need))
     return ff_fail(what, "the workspace is null, not 16-byte aligned or too small");
-  const size_t dig_bytes = g.out_digits.d_digits ? sufhip_digits2_bytes(g.rows, g.w.N) : 0;
-  const size_t xd_bytes = a.xd ? sufhip_digits2_bytes(g.x_rows, g.w.K) : 0;
+  // Nothing that the call writes meets what it reads, but for out as the
+  // residual itself.
+  const Range xd{a.xd, a.xd ? sufhip_digits2_bytes(g.x_rows, g.w.K) : 0};
+  const Range outd{a.digits, a.digits ? sufhip_digits2_bytes(g.rows, g.w.N) : 0};
+  const Range work{g.d_work, need};
+  const Range reads[5] = {
+      {g.w.d_planes, sufhip_linear_planes_bytes(g.w.experts, g.w.K, g.w.N, g.w.digits)},
+      {g.w.d_bias, size_t(g.w.experts) * g.w.N * 8},
+      {g.d_rows, size_t(g.rows) * 4},
+      {g.d_offsets, (size_t(g.w.experts) + 1) * 4},
+      xd};
+  RowSet x[2], res[2];
+  for (int q = 0; q < 2; ++q) {
+    x[q] = row_set(a.x, q, a.xd ? 0 : g.x_rows, g.w.K);
+    res[q] = row_set(a.res, q, a.res.p[0] ? g.rows : 0, g.w.N);
+  }
+  for (const Range& r : reads)
+    if (ranges_meet(outd, r) || ranges_meet(work, r))
+      return ff_fail(what, "out_digits or the workspace meets an input");
+  if (ranges_meet(outd, work)) return ff_fail(what, "out_digits meets the workspace");
+  for (int q = 0; q < 2; ++q)
+    for (const RowSet* in : {&x[q], &res[q]})
+      if (range_meets(outd, *in) || range_meets(work, *in))
+        return ff_fail(what, "out_digits or the workspace meets an input");
   if (g.out[0]) {
-    if (g.out_stride < 0 || rows_overlap(g.out_stride, g.rows, g.w.N))
-      return ff_fail(what, "output rows overlap");
+    if (bad_out_stride(g.out_stride, g.rows, g.w.N))
+      return ff_fail(what, "output rows overlap, or lie more than 2^35 apart");
     RowSet o[2];
     for (int p = 0; p < 2; ++p) {
       a.out[p] = g.out[p];
@@ -842,32 +865,15 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
     if (sets_meet(o[0], o[1])) return ff_fail(what, "the two shares of out meet");
     for (int p = 0; p < 2; ++p) {
       for (int q = 0; q < 2; ++q) {
-        if (!a.xd && sets_meet(o[p], row_set(a.x, q, g.x_rows, g.w.K)))
-          return ff_fail(what, "out meets x");
-        if (a.res.p[0]) {
-          const RowSet r = row_set(a.res, q, g.rows, g.w.N);
-          if (sets_meet(o[p], r) && !(p == q && same_set(o[p], r)))
-            return ff_fail(what, "out meets the residual without being it");
-        }
+        if (sets_meet(o[p], x[q])) return ff_fail(what, "out meets x");
+        if (sets_meet(o[p], res[q]) && !(p == q && same_set(o[p], res[q])))
+          return ff_fail(what, "out meets the residual without being it");
       }
-      if ((a.xd && range_meets(a.xd, xd_bytes, o[p])) ||
-          (need && range_meets(g.d_work, need, o[p])) ||
-          (dig_bytes && range_meets(g.out_digits.d_digits, dig_bytes, o[p])))
-        return ff_fail(what, "out meets a buffer of digits or the workspace");
+      for (const Range& r : reads)
+        if (range_meets(r, o[p])) return ff_fail(what, "out meets an input");
+      if (range_meets(outd, o[p]) || range_meets(work, o[p]))
+        return ff_fail(what, "out meets out_digits or the workspace");
     }
-  }
-  auto bytes_meet = [](const void* x, size_t nx, const void* y, size_t ny) {
-    const char *cx = static_cast<const char*>(x), *cy = static_cast<const char*>(y);
-    return nx && ny && cx < cy + ny && cy < cx + nx;
-  };
-  if (dig_bytes) {
-    const void* d = g.out_digits.d_digits;
-    bool bad = bytes_meet(d, dig_bytes, a.xd, xd_bytes) ||
-               bytes_meet(d, dig_bytes, g.d_work, need);
-    for (int q = 0; q < 2; ++q)
-      bad = bad || (!a.xd && range_meets(d, dig_bytes, row_set(a.x, q, g.x_rows, g.w.K))) ||
-            (a.res.p[0] && range_meets(d, dig_bytes, row_set(a.res, q, g.rows, g.w.N)));
-    if (bad) return ff_fail(what, "out_digits meets an input or the workspace");
   }
   hipStream_t s = as_stream(stream);
   LinWalk w{};
@@ -888,7 +894,7 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
     a.part = words;
   else if (plan.epilogue)
     a.zhat = words;
-  const unsigned wgs = unsigned(int64_t(plan.tiles) * plan.slices * plan.col_tiles);
+  const unsigned wgs = unsigned(tiles);
   switch (g.w.digits) {
     case 1: launch_product<1>(a, w, plan.rt, wgs, s); break;
     case 2: launch_product<2>(a, w, plan.rt, wgs, s); break;

@@ -504,11 +504,11 @@ int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream) {
   A.cols = g.cols;
   A.inv_len = g.inv_len;
   A.eps = g.eps;
-  if (int rc = mat2_of(g.x, g.rows, g.cols, what, "x", &A.x)) return rc;
+  if (int rc = mat2_of(g.x, g.rows, what, "x", &A.x)) return rc;
   if ((g.residual.p[0] == nullptr) != (g.residual.p[1] == nullptr))
     return ff_fail(what, "one share of the residual is missing");
   if (g.residual.p[0])
-    if (int rc = mat2_of(g.residual, g.rows, g.cols, what, "residual", &A.r)) return rc;
+    if (int rc = mat2_of(g.residual, g.rows, what, "residual", &A.r)) return rc;
   for (int p = 0; p < 2; ++p) {
     if (!g.a[p] || !g.a2[p] || !g.b[p] || !g.ab[p])
       return ff_fail(what, "a, a2, b and ab are needed for both parties");
@@ -550,46 +550,42 @@ int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream) {
     if (g.out[0]) outs[count++] = {g.out[p], g.out_stride, g.rows, g.cols};
   }
   for (int i = 0; i < count; ++i) {
-    if (outs[i].stride < 0 || rows_overlap(outs[i].stride, g.rows, g.cols))
-      return ff_fail(what, "output rows overlap");
+    if (bad_out_stride(outs[i].stride, g.rows, g.cols))
+      return ff_fail(what, "output rows overlap, or lie more than 2^35 apart");
     const int p = g.total[0] && g.out[0] ? i / 2 : i;
     for (int q = 0; q < 2; ++q) {
       const RowSet in[2] = {row_set(A.x, q, g.rows, g.cols), row_set(A.r, q, g.rows, g.cols)};
       for (int k = 0; k < (A.r.p[0] ? 2 : 1); ++k)
         if (sets_meet(outs[i], in[k]) && !(p == q && same_set(outs[i], in[k])))
           return ff_fail(what, "an output meets x or the residual without being it");
-      const RowSet mat[4] = {{g.a[q], 0, 1, 0}, {g.ab[q], 0, 1, 0}, {g.a2[q], 0, 1, g.rows},
-                             {g.b[q], 0, 1, g.rows}};
-      for (int k = 0; k < 4; ++k) {
-        RowSet m = mat[k];
-        if (k < 2) m = {m.p, g.cols, g.rows, g.cols};
-        if (sets_meet(outs[i], m)) return ff_fail(what, "an output meets the dealer's material");
-      }
     }
     for (int j = 0; j < i; ++j)
       if (sets_meet(outs[i], outs[j])) return ff_fail(what, "two outputs meet");
   }
-  if (A.digits) {
-    const size_t bytes = sufhip_digits2_bytes(g.rows, g.cols);
-    for (int q = 0; q < 2; ++q) {
-      const RowSet in[4] = {row_set(A.x, q, g.rows, g.cols),
-                            row_set(A.r, q, A.r.p[0] ? g.rows : 0, g.cols),
-                            {g.a[q], g.cols, g.rows, g.cols},
-                            {g.ab[q], g.cols, g.rows, g.cols}};
-      for (const RowSet& s : in)
-        if (range_meets(A.digits, bytes, s)) return ff_fail(what, "out_digits meets an input");
-    }
-    for (int i = 0; i < count; ++i)
-      if (range_meets(A.digits, bytes, outs[i])) return ff_fail(what, "out_digits meets an output");
-  }
   if (g.walk_count < 0 || (g.walk_count > 0 && (!g.walk_jobs || !g.walk_prg_state)))
     return ff_fail(what, "walk_jobs and walk_prg_state are needed for walk_count jobs");
   const size_t need = sufhip_rmsnorm2_work_bytes(g.rows, g.cols);
-  if (need) {
-    if (!g.d_work || (reinterpret_cast<uintptr_t>(g.d_work) & 15) != 0 || g.work_bytes < need)
-      return ff_fail(what, "the workspace is null, not 16-byte aligned or too small");
-    for (int i = 0; i < count; ++i)
-      if (range_meets(g.d_work, need, outs[i])) return ff_fail(what, "the workspace meets an output");
+  if (need && (!g.d_work || (reinterpret_cast<uintptr_t>(g.d_work) & 15) != 0 ||
+               g.work_bytes < need))
+    return ff_fail(what, "the workspace is null, not 16-byte aligned or too small");
+  const Range outd{A.digits, A.digits ? sufhip_digits2_bytes(g.rows, g.cols) : 0};
+  const Range work{g.d_work, need};
+  if (ranges_meet(outd, work)) return ff_fail(what, "out_digits meets the workspace");
+  for (int i = 0; i < count; ++i)
+    if (range_meets(outd, outs[i]) || range_meets(work, outs[i]))
+      return ff_fail(what, "an output meets out_digits or the workspace");
+  for (int q = 0; q < 2; ++q) {
+    for (const RowSet& in : {row_set(A.x, q, g.rows, g.cols),
+                             row_set(A.r, q, A.r.p[0] ? g.rows : 0, g.cols)})
+      if (range_meets(outd, in) || range_meets(work, in))
+        return ff_fail(what, "out_digits or the workspace meets an input");
+    for (const Range& m : {Range{g.a[q], n * 8}, Range{g.ab[q], n * 8},
+                           Range{g.a2[q], size_t(g.rows) * 8}, Range{g.b[q], size_t(g.rows) * 8},
+                           Range{g.d_weight, size_t(g.cols) * 8}}) {
+      bool bad = ranges_meet(outd, m) || ranges_meet(work, m);
+      for (int i = 0; i < count; ++i) bad = bad || range_meets(m, outs[i]);
+      if (bad) return ff_fail(what, "an output or the workspace meets the dealer's material");
+    }
   }
   hipStream_t s = as_stream(stream);
   if (need) {

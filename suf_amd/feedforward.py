@@ -38,9 +38,9 @@ import numpy as np
 import torch
 
 from . import native, tables
-from .kv_attention import _call, _device, _fail, _ptr
+from .kv_attention import _call, _fail, _ptr
 from .tasks import (M64, RELU_ALPHA, TABLE_BITS, CoeffLut, Dealer, Triples, Trunc, chain2_args,
-                    dev, pair, relu_coeffs_for, trunc_jobs)
+                    dev, relu_coeffs_for, trunc_jobs)
 
 MAX_ROWS = 1 << 24
 LEN_BITS = 26  # of a norm's public 1 / cols, truncated by two gates of 13 bits
@@ -82,8 +82,7 @@ def _out(a, t2, shape, d, what, name):
 
 
 def _gate_bits(frac_bits, most, what):
-    if not 1 <= frac_bits <= most:
-        _fail(what, "frac_bits must be in [1, %d]" % most)
+    _extent(frac_bits, 1, most, what, "frac_bits")
 
 
 def _extent(v, least, most, what, name):
@@ -92,14 +91,21 @@ def _extent(v, least, most, what, name):
     return int(v)
 
 
+def _gpu(device, what):
+    """The GPU that a name or number stands for, with its index."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        _fail(what, "device must be a GPU, not %s" % device)
+    return torch.device("cuda", torch.cuda.current_device() if device.index is None
+                        else device.index)
+
+
 class _Block:
     """What the operators share: a dealer, the key-only halves of the gates,
     the device."""
 
     def __init__(self, prg_state, seed, device):
-        device = torch.device(device)
-        self.device = torch.device("cuda", torch.cuda.current_device()
-                                   if device.index is None else device.index)
+        self.device = _gpu(device, type(self).__name__)
         self.d = self.device.index
         self.prg_state = bytes(prg_state)
         self.dealer = Dealer(next(_seeds) if seed is None else seed)
@@ -148,6 +154,7 @@ class Digits:
     def __init__(self, rows, cols, device="cuda"):
         rows = _extent(rows, 1, MAX_ROWS, "Digits", "rows")
         cols = _extent(cols, 1, MAX_ROWS, "Digits", "cols")
+        device = _gpu(device, "Digits")
         nb = native.load().sufhip_digits2_bytes(rows, cols)
         # Zeros: rows that no call writes stand for 0.
         self.buffer = torch.zeros(nb, dtype=torch.int8, device=device)
@@ -302,7 +309,7 @@ class PublicWeights:
             bias = torch.as_tensor(bias)
             if bias.dtype is not torch.int64 or tuple(bias.shape) != lead + (self.N,):
                 _fail(what, "bias must be int64 %s" % (list(lead + (self.N,)),))
-        device = W.device if W.is_cuda else torch.device(device)
+        device = _gpu(W.device if W.is_cuda else device, what)
         with torch.cuda.device(device):
             W = W.to(device).contiguous()
             self.d = W.get_device()
@@ -498,3 +505,108 @@ class ExpertMix(_Block):
             self._ready(prep)
             _call("sufhip_expert_mix2", a, d)
         return out
+
+
+# ---- blocks ----
+
+def route(experts_of, experts):
+    """The tables of a public choice: experts_of int [tokens, each], on any
+    device.  Returns int32 tensors there: offsets [experts + 1] and rows
+    [tokens * each] for Linear (the pairs in the order of their experts, a
+    token's before the next one's), slots [tokens, each] for ExpertMix.  A
+    number outside [0, experts) is in no expert and adds nothing to its
+    token's sum.  Sorts, so not for a captured stream."""
+    if experts_of.dim() != 2 or experts_of.dtype not in (torch.int32, torch.int64):
+        _fail("route", "experts_of must be int32 or int64 [tokens, each]")
+    tokens, each = experts_of.shape
+    e = experts_of.reshape(-1).to(torch.int64)
+    e = torch.where((e >= 0) & (e < experts), e, experts)
+    order = torch.argsort(e, stable=True)
+    offsets = torch.searchsorted(e[order], torch.arange(experts + 1, device=e.device))
+    place = torch.empty_like(order)
+    place[order] = torch.arange(tokens * each, device=e.device)
+    slots = torch.where(e < experts, place, -1).view(tokens, each)
+    rows = torch.div(order, max(each, 1), rounding_mode="floor")
+    return offsets.to(torch.int32), rows.to(torch.int32), slots.to(torch.int32)
+
+
+class FeedForward:
+    """out = s + down(act(up(norm(s)))) with s = x + residual, over rows tokens:
+    what follows a decoder's attention, from its output and the residual
+    stream.  The norm hands its output on as digits, up its activations.
+    up, down: PublicWeights of [cols, hidden] and [hidden, cols]; act as in
+    Linear; weight, eps, table as in RMSNorm.  seed: of the three parts'
+    material (seed, seed + 1, seed + 2)."""
+
+    def __init__(self, rows, up, down, prg_state, frac_bits=12, act="relu", weight=None,
+                 eps=1.0 / 1024.0, table=None, seed=None):
+        _pair("FeedForward", up, down, 1)
+        dev_ = torch.device("cuda", up.d)
+        seeds = [None if seed is None else seed + i for i in range(3)]
+        self.rows, self.cols = rows, up.K
+        self.norm = RMSNorm(rows, up.K, prg_state, frac_bits, weight, eps, table, seeds[0], dev_)
+        self.up = Linear(up, rows, prg_state, frac_bits, act, seed=seeds[1])
+        self.down = Linear(down, rows, prg_state, frac_bits, seed=seeds[2])
+        self.total = [torch.empty(rows, up.K, dtype=torch.int64, device=dev_) for _ in range(2)]
+        self.normed, self.hidden = Digits(rows, up.K, dev_), Digits(rows, up.N, dev_)
+
+    def truncs(self):
+        return self.norm.truncs() + self.up.truncs() + self.down.truncs()
+
+    def eval2(self, x, out, residual=None, prep=None):
+        """x, out, residual: pairs of int64 [rows, cols] with any row stride;
+        out may be x or residual.  Returns out."""
+        self.norm.eval2(x, None, residual, self.total, self.normed, prep)
+        self.up.eval2(self.normed, None, digits=self.hidden, prep=prep)
+        return self.down.eval2(self.hidden, out, self.total, prep=prep)
+
+
+class ExpertFeedForward:
+    """out[t] = s[t] + sum_k weights[t, k] down_e(act(up_e(norm(s)[t]))), e the
+    k-th expert of token t, with s = x + residual: FeedForward with `each`
+    experts a token.  up, down: PublicWeights of [experts, cols, hidden] and
+    [experts, hidden, cols]; the rest as in FeedForward (seed .. seed + 3)."""
+
+    def __init__(self, tokens, each, up, down, prg_state, frac_bits=12, act="relu", weight=None,
+                 eps=1.0 / 1024.0, table=None, seed=None):
+        what = "ExpertFeedForward"
+        tokens = _extent(tokens, 1, MAX_ROWS, what, "tokens")
+        each = _extent(each, 1, 1024, what, "each")
+        _pair(what, up, down, None)
+        dev_ = torch.device("cuda", up.d)
+        seeds = [None if seed is None else seed + i for i in range(4)]
+        n = tokens * each
+        self.tokens, self.each, self.cols = tokens, each, up.K
+        self.norm = RMSNorm(tokens, up.K, prg_state, frac_bits, weight, eps, table, seeds[0],
+                            dev_)
+        self.up = Linear(up, n, prg_state, frac_bits, act, x_rows=tokens, seed=seeds[1])
+        self.down = Linear(down, n, prg_state, frac_bits, seed=seeds[2])
+        self.mix = ExpertMix(tokens, up.K, prg_state, frac_bits, seeds[3], dev_)
+        self.total = [torch.empty(tokens, up.K, dtype=torch.int64, device=dev_)
+                      for _ in range(2)]
+        # Zeros: pairs in no expert are not written, nor read by the sum.
+        self.z = [torch.zeros(n, up.K, dtype=torch.int64, device=dev_) for _ in range(2)]
+        self.normed, self.hidden = Digits(tokens, up.K, dev_), Digits(n, up.N, dev_)
+
+    def truncs(self):
+        return self.norm.truncs() + self.up.truncs() + self.down.truncs() + self.mix.truncs()
+
+    def eval2(self, x, out, offsets, rows, slots, weights, residual=None, prep=None):
+        """x, out, residual as in FeedForward; offsets, rows, slots: route() of
+        the tokens' experts, on the GPU; weights: int64 [tokens, each] in
+        Q(frac_bits) on the GPU.  Returns out."""
+        self.norm.eval2(x, None, residual, self.total, self.normed, prep)
+        self.up.eval2(self.normed, None, offsets=offsets, rows=rows, digits=self.hidden,
+                      prep=prep)
+        self.down.eval2(self.hidden, self.z, offsets=offsets, prep=prep)
+        return self.mix.eval2(self.z, slots, weights, out, self.total, prep)
+
+
+def _pair(what, up, down, experts):
+    """up and down fit each other."""
+    if not isinstance(up, PublicWeights) or not isinstance(down, PublicWeights):
+        _fail(what, "up and down must be PublicWeights")
+    if (up.K, up.N, up.experts, up.d) != (down.N, down.K, down.experts, down.d):
+        _fail(what, "up [%d, %d] and down [%d, %d] do not fit" % (up.K, up.N, down.K, down.N))
+    if experts is not None and up.experts != experts:
+        _fail(what, "of %d matrices ExpertFeedForward makes one" % up.experts)
