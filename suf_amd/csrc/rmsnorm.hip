@@ -605,8 +605,12 @@ int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream) {
     if (int rc = sufhip_trunc_prepare_batch(g.walk_prg_state, g.walk_jobs, g.walk_count, stream))
       return rc;
   if (g.cols <= 1024) return launch_rms<1, 256, false>(A, s);
-  if (g.cols <= 2048) return launch_rms<2, 256, false>(A, s);
-  if (g.cols <= 4096) return launch_rms<2, 512, false>(A, s);
+  // A row's latency counts where a CU has two at most (1 x 2048: 16.8 us, 19.4
+  // with half the lanes), their number where it has more (1000 x 2048: 53 us, 61
+  // with twice the lanes).
+  if (g.cols <= 2048 && g.rows > 2 * device_cus()) return launch_rms<2, 256, false>(A, s);
+  if (g.cols <= 2048) return launch_rms<1, 512, false>(A, s);
+  if (g.cols <= 4096) return launch_rms<1, 1024, false>(A, s);
   return launch_rms<1, 1024, true>(A, s);
 }
 

@@ -208,7 +208,7 @@ def test_two_objects_on_two_streams():
 
 # ---- each operator at its edges ----
 
-@pytest.mark.parametrize("rows,cols,weight", [(5, 40, True), (2100, 1000, False),
+@pytest.mark.parametrize("rows,cols,weight", [(5, 40, True), (600, 1501, True), (2100, 1000, False),
                                               (1000, 2100, True)])
 def test_norm_prepared_elsewhere_and_outputs_alone(rows, cols, weight):
     say("norm %d x %d, prepared" % (rows, cols))
@@ -218,6 +218,8 @@ def test_norm_prepared_elsewhere_and_outputs_alone(rows, cols, weight):
     norm = ff.RMSNorm(rows, cols, STATE, weight=w, seed=9)
     xs, rs, out = _share(rng, x), _share(rng, r), _empty(rows, cols)
     norm.eval2(xs, out, residual=rs)
+    assert np.array_equal(_open(out), ref.rmsnorm(x, r, norm.inv_len, norm.eps_q, norm.table, F,
+                                                  w)[1])
     want = [o.clone() for o in out]
     prep = (tasks.Prepared(torch.cuda.Stream(), [norm.truncs()]), 0)
     norm.eval2(xs, out, residual=rs, prep=prep)
