@@ -107,7 +107,7 @@ extern "C" int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* str
   if (g.tokens < 0 || g.cols < 0 || g.each < 0 || g.z_rows < 0 || g.tokens > kMaxRows ||
       g.z_rows > kMaxRows || g.each > 1024 ||
       uint64_t(g.tokens) * uint64_t(g.cols) >= (uint64_t(1) << 31))
-    return ff_fail(what, "tokens and z_rows in [0, 2^24], each in [0, 1024] and tokens cols < 2^31");
+    return ff_fail(what, "tokens and z_rows in [0, 2^24], each in [0, 1024], tokens cols < 2^31");
   if (g.tokens == 0 || g.cols == 0) return SUFHIP_OK;
   MixArgs a{};
   a.z_rows = g.z_rows;

@@ -165,6 +165,13 @@ __device__ __forceinline__ TileId tile_id(const LinArgs& a, int id, int total) {
 // registers; X's digits, which the four waves share, are formed on the way into
 // LDS (or come as digits), 64 k at a time, the next chunk's loads in flight
 // under this one's products.
+//
+// Few rows: the stream of W bounds it (logits of one row, 2048 x 32000, 131 MB
+// in 27 us).  Many rows: 1000 x 2048 x 1024 takes 62 us, 2.0 POP/s of int8;
+// with the matrix instructions alone it would be 38, and X's loads and digits
+// cost 11 of the rest, the fragments' reads from LDS as much, W's loads 3.  A
+// deeper ring, larger tiles (32 tokens x 128 columns, 256 accumulators a wave:
+// 72 us) and fragments read a step ahead gain nothing.
 constexpr int kTok = 8;
 constexpr int kFrags = 2;  // column fragments of a wave
 constexpr int kDepth = 2;  // chunks on their way

@@ -1,5 +1,5 @@
 // Root-mean-square norm with the residual's addition (sufhip_rmsnorm2), both
-// parties, a workgroup a row.
+// parties: a workgroup a row, or three launches for a large one.
 //
 //   s = x + residual,  S = sum s s,  v = S / cols + eps,  o = s / sqrt(v)
 //
@@ -246,7 +246,10 @@ __device__ __forceinline__ void rms_stage(uint32_t* tab, ChainLds& L, TruncHdr (
 }
 
 // A row of up to 4 kQuads kBlock values stays on the CU from the sum to the
-// output; with kLong a longer one is read again for the output.
+// output; with kLong a longer one is read again for the output.  One row is
+// bound by latency, seven gates and a LUT one after the other: 15 us for 768
+// values.  Many stream their 12 words a value: 1000 x 2048 with total and
+// weight 53 us, 3.7 TB/s, the workgroups' chains between their loads.
 template <int kQuads, int kBlock, bool kLong>
 __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs) {
   constexpr int kWaves = kBlock / 64;
@@ -337,7 +340,9 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs
 // total), with the gates' walks beside them; the rows' factors, a wave a row;
 // the outputs.  Row by row in one launch, the workgroups all wait for their
 // chains at the same time, and behind each other's loads: 1999 x 2048 with
-// total and weight 134 us after 22 of walks.
+// total and weight 134 us after 22 of walks.  In three: 57 us of sums and walks
+// (262 MB, 4.6 TB/s), 17 of factors, 54 of outputs (262 MB, 4.8 TB/s: as a
+// copy).  Factors in the outputs' launch: 72 us for the two.
 //
 // kWaveRow: a wave a row (rows of up to 1024 values), else a workgroup a row.
 template <bool kWaveRow, bool kWalk>
@@ -352,7 +357,8 @@ __global__ void __launch_bounds__(256) rms_sum_kernel(RmsArgs, RmsWalk wk) {
   const int first = int(blockIdx.x) - (kWalk ? wk.groups : 0);
   const int step = int(gridDim.x) - (kWalk ? wk.groups : 0);
   const int rows = rms_args().rows, cols = rms_args().cols;
-  const int wave = int(threadIdx.x) >> 6, lane = kWaveRow ? int(threadIdx.x) & 63 : int(threadIdx.x);
+  const int wave = int(threadIdx.x) >> 6;
+  const int lane = kWaveRow ? int(threadIdx.x) & 63 : int(threadIdx.x);
   constexpr int kPerGroup = kWaveRow ? 4 : 1, kSpan = kWaveRow ? 256 : 1024;
   for (int r = first * kPerGroup + (kWaveRow ? wave : 0); r < rows; r += step * kPerGroup) {
     uint64_t q0 = 0, q1 = 0;
@@ -474,8 +480,8 @@ template <int kQuads, int kBlock, bool kLong>
 int launch_rms(const RmsArgs& A, hipStream_t s) {
   const int cap = device_cus() * (2048 / kBlock > 8 ? 8 : 2048 / kBlock);
   const int grid = A.rows < cap ? A.rows : cap;
-  hipLaunchKernelGGL((rmsnorm2_kernel<kQuads, kBlock, kLong>), dim3(unsigned(grid)), dim3(kBlock), 0,
-                     s, A);
+  hipLaunchKernelGGL((rmsnorm2_kernel<kQuads, kBlock, kLong>), dim3(unsigned(grid)),
+                     dim3(kBlock), 0, s, A);
   return check_launch("rmsnorm2_kernel");
 }
 
