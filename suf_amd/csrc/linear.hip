@@ -38,7 +38,7 @@ struct LinArgs {
   const int64_t* bias;
   const int32_t* map;
   const int32_t* offsets;
-  int tiles, slices;
+  int tiles, cols, slices;
   uint64_t* part;  // several k-slices: [slices][2][rows][N] sums
   uint64_t* zhat;  // the masked opens [rows][N], for the epilogue's launch
   uint64_t mask;
@@ -72,15 +72,17 @@ __device__ __forceinline__ int expert_of(const LinArgs& a, int row) {
   return a.offsets[lo] <= row && row < a.offsets[lo + 1] ? lo : -1;
 }
 
-// Row tile number ti, of `per` rows: its expert and rows.  Every lane of the
+constexpr int kTok = 8;  // rows of a row tile
+
+// Row tile number ti: its expert and rows.  Every lane of the
 // wave takes part; experts are counted 64 at a time.
 struct RowTile {
   int e, begin, end;
 };
-__device__ __forceinline__ RowTile row_tile(const LinArgs& a, int ti, int per) {
+__device__ __forceinline__ RowTile row_tile(const LinArgs& a, int ti) {
   if (!a.offsets) {
-    const int begin = ti * per;
-    const int end = begin + per < a.rows ? begin + per : a.rows;
+    const int begin = ti * kTok;
+    const int end = begin + kTok < a.rows ? begin + kTok : a.rows;
     return {begin < a.rows ? 0 : -1, begin, end};
   }
   const int lane = threadIdx.x & 63;
@@ -94,7 +96,7 @@ __device__ __forceinline__ RowTile row_tile(const LinArgs& a, int ti, int per) {
       lo = lo < 0 ? 0 : (lo > a.rows ? a.rows : lo);
       hi = hi < lo ? lo : (hi > a.rows ? a.rows : hi);
     }
-    const int n = (hi - lo + per - 1) / per;
+    const int n = (hi - lo + kTok - 1) / kTok;
     int incl = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -106,8 +108,8 @@ __device__ __forceinline__ RowTile row_tile(const LinArgs& a, int ti, int per) {
       const int f = __builtin_ctzll(over);
       const int first = base + __shfl(incl - n, f, 64);
       const int flo = __shfl(lo, f, 64), fhi = __shfl(hi, f, 64);
-      const int begin = flo + (ti - first) * per;
-      return {e0 + f, begin, begin + per < fhi ? begin + per : fhi};
+      const int begin = flo + (ti - first) * kTok;
+      return {e0 + f, begin, begin + kTok < fhi ? begin + kTok : fhi};
     }
     base += __shfl(incl, 63, 64);
   }
@@ -141,41 +143,41 @@ __device__ __forceinline__ void put_output(const LinArgs& a, const EpiHdrs& eh, 
 
 // The order of the tiles.  Workgroups are dealt round-robin to the 8 XCDs, each
 // with an L2 of its own, so an XCD takes a contiguous eighth of the order; and
-// the order goes over 8 column tiles, then the row tiles, then the next 8
-// columns: the hundred workgroups that an XCD runs at once then share a dozen
-// row tiles of X and 8 column tiles of W, instead of one side alone being read
-// again by each (1000 x 2048 x 1024: 288 MB beyond the L2s, 66 us).
+// the order goes over 1024 columns (kPanel tiles), then the row tiles, then the
+// next columns: the sixty workgroups that an XCD runs at once then share some row
+// tiles of X and 1024 columns of W, instead of one side alone being read again
+// by each (1000 x 2048 x 1024: 288 MB beyond the L2s, 66 us with tiles of 128
+// columns row by row; 512 or 2048 columns at a time: within 2 %).
 struct TileId {
   int row, col, slice;
 };
+template <int kPanel>
 __device__ __forceinline__ TileId tile_id(const LinArgs& a, int id, int total) {
   const int each = total / 8, more = total % 8, x = id % 8;
   id = x * each + (x < more ? x : more) + id / 8;
-  const int cols = (a.groups + 1) / 2;
+  const int cols = a.cols;
   const int plane = a.tiles * cols, slice = id / plane;
   id -= slice * plane;
-  const int panel = id / (8 * a.tiles), left = cols - 8 * panel;
-  const int wide = left < 8 ? left : 8;
-  id -= 8 * a.tiles * panel;
-  return {id / wide, 8 * panel + id % wide, slice};
+  const int panel = id / (kPanel * a.tiles), left = cols - kPanel * panel;
+  const int wide = left < kPanel ? left : kPanel;
+  id -= kPanel * a.tiles * panel;
+  return {id / wide, kPanel * panel + id % wide, slice};
 }
 
-// A workgroup of four waves takes kRt row tiles (8 tokens of both parties
-// each), 128 columns, 32 a wave, and one k-slice.  W goes straight into
+// A workgroup of four waves takes a row tile (8 tokens of both parties), 64
+// kFrags columns, 16 kFrags a wave, and one k-slice.  W goes straight into
 // registers; X's digits, which the four waves share, are formed on the way into
 // LDS (or come as digits), 64 k at a time, the next chunk's loads in flight
 // under this one's products.
 //
 // Few rows: the stream of W bounds it (logits of one row, 2048 x 32000, 131 MB
-// in 27 us).  Many rows: 1000 x 2048 x 1024 takes 62 us, 2.0 POP/s of int8;
-// with the matrix instructions alone it would be 38, and X's loads and digits
-// cost 11 of the rest, the fragments' reads from LDS as much, W's loads 3.  A
+// in 27 us).  Many rows: 1000 x 2048 x 1024 takes 56 us from digits, 2.25 POP/s
+// of int8, and 60 from shares; with the matrix instructions alone it would be
+// 37, and X's way costs 7, W's loads 5, the fragments' reads from LDS 10.  A
 // deeper ring, larger tiles (32 tokens x 128 columns, 256 accumulators a wave:
-// 72 us) and fragments read a step ahead gain nothing.
-constexpr int kTok = 8;
-constexpr int kFrags = 2;  // column fragments of a wave
+// 72 us) and fragments read a step ahead (57 us) gain nothing.
 constexpr int kDepth = 2;  // chunks on their way
-template <int kRt, int J, bool kDigits, bool kWalk>
+template <int kFrags, int J, bool kDigits, bool kWalk>
 __global__ void __launch_bounds__(256, 2) linear_product_kernel(LinArgs a, LinWalk wk) {
   if constexpr (kWalk) {
     if (int(blockIdx.x) < wk.groups) {
@@ -187,12 +189,13 @@ __global__ void __launch_bounds__(256, 2) linear_product_kernel(LinArgs a, LinWa
   // [digit][slot] of 16 k.  Row r's sixteen number kk is slot 16 kk + (r + 4 kk)
   // % 16: a wave's dword writes (four rows, four sixteens) and its fragment
   // reads then take every bank once.
-  __shared__ __align__(16) int8_t lds[2][kRt][8 * 1024];
+  __shared__ __align__(16) int8_t lds[2][8 * 1024];
   const int l = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-  const TileId at = tile_id(a, int(blockIdx.x) - groups, int(gridDim.x) - groups);
-  const int slice = at.slice, c0 = at.col * 128 + 32 * w;
-  const RowTile rt = row_tile(a, at.row, kRt * kTok);
+  constexpr int kPanel = kFrags > 2 ? 4 : 8;
+  const TileId at = tile_id<kPanel>(a, int(blockIdx.x) - groups, int(gridDim.x) - groups);
+  const int slice = at.slice, c0 = (at.col * 4 + w) * 16 * kFrags;
+  const RowTile rt = row_tile(a, at.row);
   if (rt.e < 0 || rt.begin >= rt.end) return;  // the whole workgroup
   const EpiHdrs eh = epi_hdrs(a.epi);
   // The row that this thread brings to LDS: four words of it from kq on, or
@@ -201,20 +204,13 @@ __global__ void __launch_bounds__(256, 2) linear_product_kernel(LinArgs a, LinWa
   const int kq = int(threadIdx.x) % 16 * 4;
   const int slot = ((l & 48) + ((l + (l >> 4) * 4) & 15)) * 16;  // of this lane's fragment
   const int p = (r >> 1) & 1, t = 2 * (r >> 2) + (r & 1);
-  bool live[kRt];
-  const uint64_t* xrow[kRt];
-  const int8_t* drow[kRt];
-#pragma unroll
-  for (int m = 0; m < kRt; ++m) {
-    int xr = rt.begin + kTok * m + t;
-    live[m] = xr < rt.end;
-    if (live[m] && a.map) xr = a.map[xr];
-    live[m] = live[m] && xr >= 0 && xr < a.x_rows;
-    if (kDigits)
-      drow[m] = a.xd + (live[m] ? (size_t(p) * a.x_rows + xr) * 256 : 0);
-    else
-      xrow[m] = (p ? a.x.p[1] : a.x.p[0]) + (live[m] ? int64_t(xr) * a.x.stride : 0) + kq;
-  }
+  int xr = rt.begin + t;
+  bool live = xr < rt.end;
+  if (live && a.map) xr = a.map[xr];
+  live = live && xr >= 0 && xr < a.x_rows;
+  const uint64_t* xrow =
+      kDigits ? nullptr : (p ? a.x.p[1] : a.x.p[0]) + (live ? int64_t(xr) * a.x.stride : 0) + kq;
+  const int8_t* drow = kDigits ? a.xd + (live ? (size_t(p) * a.x_rows + xr) * 256 : 0) : nullptr;
   const size_t dstep = size_t(2) * a.x_rows * 256;
   // This wave's columns; past the last weight tile it repeats the last one.
   const int g = c0 / kCols < a.groups ? c0 / kCols : a.groups - 1;
@@ -224,97 +220,95 @@ __global__ void __launch_bounds__(256, 2) linear_product_kernel(LinArgs a, LinWa
   const int chunks = a.kb / 2;
   const int q0 = int(int64_t(chunks) * slice / a.slices);
   const int q1 = int(int64_t(chunks) * (slice + 1) / a.slices);
-  // Chunks on their way: W until its products, X until its place in LDS.
-  struct Chunk {
-    v4i w[kFrags][J];
-    u64x2u xw[kDigits ? 1 : kRt][2];
-    v4i xd[kDigits ? kRt : 1][2];
-  };
-  auto load_w = [&](Chunk& k, int q) {
+  // W on its way, until its products: kDepth chunks, or (four fragments, whose
+  // registers are many) one, a fragment's loads leaving behind its products.
+  constexpr int kWays = kFrags > 2 ? 1 : kDepth;
+  v4i wr[kWays][kFrags][J];
+  auto load_w = [&](int u, int c, int q) {
     if (q >= q1) return;
 #pragma unroll
-    for (int c = 0; c < kFrags; ++c)
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-        k.w[c][j] = load16(wl + size_t(q) * (2 * J * kTileBytes) + j * kTileBytes + c * 512);
+    for (int j = 0; j < J; ++j)
+      wr[u][c][j] = load16(wl + size_t(q) * (2 * J * kTileBytes) + j * kTileBytes + c * 512);
+  };
+  // X on its way, until its place in LDS.
+  struct Chunk {
+    u64x2u w[kDigits ? 1 : 2];
+    v4i d[kDigits ? 2 : 1];
   };
   auto load_x = [&](Chunk& k, int q) {
     if (q >= q1) return;
-#pragma unroll
-    for (int m = 0; m < kRt; ++m) {
-      if constexpr (kDigits) {
-        // Digits w and w + 4 at this lane's place in the fragment.
-        const int kb = 2 * q + (l >> 5);
-        k.xd[m][0] = k.xd[m][1] = v4i{0, 0, 0, 0};
-        if (live[m] && 32 * kb < a.K) {
-          const int8_t* at = drow[m] + size_t(kb) * dstep + 16 * ((l >> 4) & 1) + 32 * w;
-          k.xd[m][0] = load16(at);
-          k.xd[m][1] = load16(at + 128);
-        }
-      } else {
-        const uint64_t* row = xrow[m] + 64 * q;
-        const int left = a.K - 64 * q - kq;
-        k.xw[m][0] = k.xw[m][1] = u64x2u{0, 0};
-        if (live[m] && left >= 4) {
-          k.xw[m][0] = *reinterpret_cast<const u64x2u*>(row);
-          k.xw[m][1] = *reinterpret_cast<const u64x2u*>(row + 2);
-        } else if (live[m]) {
-          if (left > 0) k.xw[m][0][0] = row[0];
-          if (left > 1) k.xw[m][0][1] = row[1];
-          if (left > 2) k.xw[m][1][0] = row[2];
-        }
+    if constexpr (kDigits) {
+      // Digits w and w + 4 at this lane's place in the fragment.
+      const int kb = 2 * q + (l >> 5);
+      k.d[0] = k.d[1] = v4i{0, 0, 0, 0};
+      if (live && 32 * kb < a.K) {
+        const int8_t* at = drow + size_t(kb) * dstep + 16 * ((l >> 4) & 1) + 32 * w;
+        k.d[0] = load16(at);
+        k.d[1] = load16(at + 128);
+      }
+    } else {
+      const uint64_t* row = xrow + 64 * q;
+      const int left = a.K - 64 * q - kq;
+      k.w[0] = k.w[1] = u64x2u{0, 0};
+      if (live && left >= 4) {
+        k.w[0] = *reinterpret_cast<const u64x2u*>(row);
+        k.w[1] = *reinterpret_cast<const u64x2u*>(row + 2);
+      } else if (live) {
+        if (left > 0) k.w[0][0] = row[0];
+        if (left > 1) k.w[0][1] = row[1];
+        if (left > 2) k.w[1][0] = row[2];
       }
     }
   };
   auto store_x = [&](const Chunk& k, int buf) {
+    if constexpr (kDigits) {
+      *reinterpret_cast<v4i*>(&lds[buf][w * 1024 + slot]) = k.d[0];
+      *reinterpret_cast<v4i*>(&lds[buf][(w + 4) * 1024 + slot]) = k.d[1];
+    } else {
+      int8_t* at = &lds[buf][(kq & 48) * 16 + ((r + (kq >> 4) * 4) & 15) * 16 + (kq & 15)];
+      const uint64_t v[4] = {k.w[0][0], k.w[0][1], k.w[1][0], k.w[1][1]};
+      uint32_t d[8];
+      digits_of4(v, d);
 #pragma unroll
-    for (int m = 0; m < kRt; ++m) {
-      if constexpr (kDigits) {
-        *reinterpret_cast<v4i*>(&lds[buf][m][w * 1024 + slot]) = k.xd[m][0];
-        *reinterpret_cast<v4i*>(&lds[buf][m][(w + 4) * 1024 + slot]) = k.xd[m][1];
-      } else {
-        int8_t* at =
-            &lds[buf][m][(kq & 48) * 16 + ((r + (kq >> 4) * 4) & 15) * 16 + (kq & 15)];
-        const uint64_t v[4] = {k.xw[m][0][0], k.xw[m][0][1], k.xw[m][1][0], k.xw[m][1][1]};
-        uint32_t d[8];
-        digits_of4(v, d);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(at + 1024 * i) = d[i];
-      }
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(at + 1024 * i) = d[i];
     }
   };
-  v4acc acc[kRt][kFrags][8];
+  v4acc acc[kFrags][8];
 #pragma unroll
-  for (int m = 0; m < kRt; ++m)
+  for (int c = 0; c < kFrags; ++c)
 #pragma unroll
-    for (int c = 0; c < kFrags; ++c)
+    for (int s = 0; s < 8; ++s)
 #pragma unroll
-      for (int s = 0; s < 8; ++s)
+      for (int q = 0; q < 4; ++q) acc[c][s][q] = 0;
+  // Chunk q, its W in wr[u], its X in LDS; W of chunk q + kWays follows.
+  auto products = [&](int u, int buf, int q) {
+    v4i d[8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[m][c][s][q] = 0;
-  auto products = [&](const Chunk& k, int buf) {
+    for (int i = 0; i < 8; ++i) d[i] = *reinterpret_cast<const v4i*>(&lds[buf][i * 1024 + slot]);
 #pragma unroll
-    for (int m = 0; m < kRt; ++m) {
-      v4i d[8];
+    for (int c = 0; c < kFrags; ++c) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        d[i] = *reinterpret_cast<const v4i*>(&lds[buf][m][i * 1024 + slot]);
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int c = 0; c < kFrags; ++c)
+        for (int i = 0; i + j < 8; ++i)
+          acc[c][i + j] =
+              __builtin_amdgcn_mfma_i32_16x16x64_i8(d[i], wr[u][c][j], acc[c][i + j], 0, 0, 0);
+      if (kWays == 1) load_w(u, c, q + 1);
+    }
+    if (kWays > 1) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-          for (int i = 0; i + j < 8; ++i)
-            acc[m][c][i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(d[i], k.w[c][j],
-                                                                     acc[m][c][i + j], 0, 0, 0);
+      for (int c = 0; c < kFrags; ++c) load_w(u, c, q + kWays);
     }
   };
-  // Chunk q lies in ring[(q - q0) % kDepth]: its W is loaded kDepth steps ahead,
-  // when the slot's last products are issued; its X goes to LDS a step ahead.
+  // Chunk q's X lies in ring[(q - q0) % kDepth], then in LDS, a step ahead of
+  // its products.
   Chunk ring[kDepth];
 #pragma unroll
   for (int u = 0; u < kDepth; ++u) {
-    load_w(ring[u], q0 + u);
+    if (u < kWays) {
+#pragma unroll
+      for (int c = 0; c < kFrags; ++c) load_w(u, c, q0 + u);
+    }
     load_x(ring[u], q0 + u);
   }
   store_x(ring[0], 0);
@@ -326,8 +320,7 @@ __global__ void __launch_bounds__(256, 2) linear_product_kernel(LinArgs a, LinWa
       if (q + u < q1) {
         Chunk& next = ring[(u + 1) % kDepth];
         const int buf = (q + u - q0) & 1;
-        products(ring[u], buf);
-        load_w(ring[u], q + u + kDepth);
+        products(u % kWays, buf, q + u);
         store_x(next, buf ^ 1);
         load_x(next, q + u + 1 + kDepth);
         __syncthreads();
@@ -335,24 +328,22 @@ __global__ void __launch_bounds__(256, 2) linear_product_kernel(LinArgs a, LinWa
     }
   }
 #pragma unroll
-  for (int m = 0; m < kRt; ++m)
+  for (int c = 0; c < kFrags; ++c) {
+    const int col = c0 + 16 * c + l % 16;
+    if (col >= a.N) continue;
+    uint64_t v[4];
 #pragma unroll
-    for (int c = 0; c < kFrags; ++c) {
-      const int col = c0 + 16 * c + l % 16;
-      if (col >= a.N) continue;
-      uint64_t v[4];
+    for (int q = 0; q < 4; ++q) {
+      v[q] = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        v[q] = 0;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) v[q] += uint64_t(int64_t(acc[m][c][s][q])) << (8 * s);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = rt.begin + kTok * m + 2 * (l / 16) + h;
-        if (row < rt.end) put_output(a, eh, slice, rt.e, row, col, v[h], v[2 + h]);
-      }
+      for (int s = 0; s < 8; ++s) v[q] += uint64_t(int64_t(acc[c][s][q])) << (8 * s);
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = rt.begin + 2 * (l / 16) + h;
+      if (row < rt.end) put_output(a, eh, slice, rt.e, row, col, v[h], v[2 + h]);
+    }
+  }
 }
 
 // The epilogue's own launch, where k-slices have to be summed, an activation
@@ -614,7 +605,7 @@ int device_cus() {
 
 // How a call runs.
 struct Plan {
-  int rt;          // row tiles of a workgroup
+  bool wide;       // 256 columns a workgroup, else 128
   int tiles;       // row tiles of the grid (an upper bound with experts)
   int col_tiles;
   int slices;
@@ -632,14 +623,16 @@ Plan plan_linear(const sufhip_linear2_args& g) {
   Plan p{};
   // Every expert may end inside a tile, and has one only if it has a row.
   const int experts = g.w.experts < g.rows ? g.w.experts : g.rows;
-  // Two row tiles a workgroup read W half as often: 1000 x 2048 x 1024 59 us
-  // against 67, 256 x 1024 x 4096 36 against 39; 128 x 4096 x 4096 68 against
-  // 63, for the half as many workgroups.  With three digits of W the sums do
-  // not fit the registers.
-  p.rt = g.w.digits <= 2 && g.rows / (g.d_offsets ? experts : 1) >= 192 ? 2 : 1;
-  const int per = p.rt * kTok;
-  p.tiles = g.d_offsets ? g.rows / per + experts : (g.rows + per - 1) / per;
-  p.col_tiles = (g.w.N + 127) / 128;
+  // 256 columns a workgroup read X's digits from LDS half as often, where there
+  // are workgroups enough: 1000 x 2048 x 1024 (500 of them) 56 us against 67, 400
+  // x 2048 x 2048 (400) 52 against 65, 256 x 768 x 2304 (288) 24 against 21; by
+  // expert, whose tiles are ragged, 2000 rows x 1024 x 2048 of 16 (2000) 135
+  // against 145, 1000 rows (1000) 76 either way, 500 rows 50 against 44.  With
+  // three digits of W the sums do not fit the registers.
+  const int64_t full = int64_t(g.rows / kTok) * ((g.w.N + 255) / 256);
+  p.wide = g.w.digits <= 2 && 2 * full >= (g.d_offsets ? 9 : 3) * int64_t(device_cus());
+  p.tiles = g.d_offsets ? g.rows / kTok + experts : (g.rows + kTok - 1) / kTok;
+  p.col_tiles = p.wide ? (g.w.N + 255) / 256 : (g.w.N + 127) / 128;
   // k-slices up to two workgroups a CU, of three chunks at least: one row of
   // 768 x 2304 8.4 us with 4, 10.5 with 1; 8 x 4096 x 4096 16.9 with 8, 20.7
   // with 4, 18.4 with 16; 64 x 4096 x 4096 38.8 with 2, 50.2 with 1, 43 with 4.
@@ -653,10 +646,10 @@ Plan plan_linear(const sufhip_linear2_args& g) {
   // Walks beside the product where its workgroups leave room, one round of the
   // chip, and the epilogue's launch that evaluates the gates follows anyway or
   // has little to do.  (One gate's walks alone take 13 us: logits of one token
-  // 42 -> 33 us.  Beside 504 workgroups of two row tiles, with a launch for a
+  // 42 -> 33 us.  Beside as many workgroups of 256 columns, with a launch for a
   // million outputs of its own, 85 us against 73.)
   const size_t mn = size_t(g.rows) * size_t(g.w.N);
-  p.walk = g.walk_count > 0 && g.walk_count <= kLinWalks && p.rt == 1 &&
+  p.walk = g.walk_count > 0 && g.walk_count <= kLinWalks && !p.wide &&
            wgs * p.slices <= 2 * device_cus() && (p.epilogue || mn <= (size_t(1) << 17));
   p.epilogue = p.epilogue || p.walk;
   p.words = !p.epilogue ? 0 : (p.slices > 1 ? size_t(p.slices) * 2 * mn : mn);
@@ -675,25 +668,25 @@ int check_extents(const sufhip_linear2_args& g, const char* what) {
   return SUFHIP_OK;
 }
 
-template <int kRt, int J>
+template <int kFrags, int J>
 void launch_tiles(const LinArgs& a, const LinWalk& w, unsigned wgs, hipStream_t s) {
   const dim3 grid(wgs + unsigned(w.groups)), block(256);
   if (a.xd && w.groups)
-    hipLaunchKernelGGL((linear_product_kernel<kRt, J, true, true>), grid, block, 0, s, a, w);
+    hipLaunchKernelGGL((linear_product_kernel<kFrags, J, true, true>), grid, block, 0, s, a, w);
   else if (a.xd)
-    hipLaunchKernelGGL((linear_product_kernel<kRt, J, true, false>), grid, block, 0, s, a, w);
+    hipLaunchKernelGGL((linear_product_kernel<kFrags, J, true, false>), grid, block, 0, s, a, w);
   else if (w.groups)
-    hipLaunchKernelGGL((linear_product_kernel<kRt, J, false, true>), grid, block, 0, s, a, w);
+    hipLaunchKernelGGL((linear_product_kernel<kFrags, J, false, true>), grid, block, 0, s, a, w);
   else
-    hipLaunchKernelGGL((linear_product_kernel<kRt, J, false, false>), grid, block, 0, s, a, w);
+    hipLaunchKernelGGL((linear_product_kernel<kFrags, J, false, false>), grid, block, 0, s, a, w);
 }
 
 template <int J>
-void launch_product(const LinArgs& a, const LinWalk& w, int rt, unsigned wgs, hipStream_t s) {
+void launch_product(const LinArgs& a, const LinWalk& w, bool wide, unsigned wgs, hipStream_t s) {
   if constexpr (J <= 2) {
-    if (rt == 2) return launch_tiles<2, J>(a, w, wgs, s);
+    if (wide) return launch_tiles<4, J>(a, w, wgs, s);
   }
-  launch_tiles<1, J>(a, w, wgs, s);
+  launch_tiles<2, J>(a, w, wgs, s);
 }
 
 }  // namespace
@@ -896,6 +889,7 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
   }
   uint64_t* words = static_cast<uint64_t*>(g.d_work);
   a.tiles = plan.tiles;
+  a.cols = plan.col_tiles;
   a.slices = plan.slices;
   if (plan.slices > 1)
     a.part = words;
@@ -903,10 +897,10 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
     a.zhat = words;
   const unsigned wgs = unsigned(tiles);
   switch (g.w.digits) {
-    case 1: launch_product<1>(a, w, plan.rt, wgs, s); break;
-    case 2: launch_product<2>(a, w, plan.rt, wgs, s); break;
-    case 3: launch_product<3>(a, w, plan.rt, wgs, s); break;
-    default: launch_product<4>(a, w, plan.rt, wgs, s); break;
+    case 1: launch_product<1>(a, w, plan.wide, wgs, s); break;
+    case 2: launch_product<2>(a, w, plan.wide, wgs, s); break;
+    case 3: launch_product<3>(a, w, plan.wide, wgs, s); break;
+    default: launch_product<4>(a, w, plan.wide, wgs, s); break;
   }
   if (int rc = check_launch("linear_product_kernel")) return rc;
   if (!plan.epilogue) return SUFHIP_OK;
