@@ -825,7 +825,7 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
   const Plan plan = plan_linear(g);
   const uint64_t tiles = uint64_t(plan.tiles) * plan.slices * plan.col_tiles;
   if (tiles >= (uint64_t(1) << 24) - 4096)  // a launch holds 2^32 lanes
-    return ff_fail(what, "more than 2^24 tiles of 8 rows and 128 columns");
+    return ff_fail(what, "more than 2^24 tiles of 8 rows and 128 or 256 columns");
   const size_t need = plan.words * 8;
   if (need && (!g.d_work || (reinterpret_cast<uintptr_t>(g.d_work) & 15) != 0 ||
                g.work_bytes < need))

@@ -137,9 +137,11 @@ def test_linear2_refuses_gates_and_workspaces():
     for meets in (at(0), at(1), at(3), at(9)):
         refused("sufhip_linear2", linear_args(**d, d_work=meets), "workspace")
     does_nothing("sufhip_linear2", linear_args(rows=0))
-    # 2^17 column tiles for each row tile of 127 experts: past a launch's lanes.
+    # 2^17 column tiles of 128 (three digits) for each row tile of 127 experts:
+    # past a launch's lanes.
     refused("sufhip_linear2", linear_args(rows=127, x_rows=127, w__N=1 << 24, w__experts=127,
-                                          d_offsets=at(22), out_stride=1 << 24), "tiles")
+                                          w__digits=3, d_offsets=at(22), out_stride=1 << 24),
+            "tiles")
 
 
 def test_sizes():
