@@ -1125,7 +1125,7 @@ int sufhip_matmul_public2(const uint64_t* d_X0, const uint64_t* d_X1, int M, int
 /* (src/nn/matmul_publicW.cpp:17-36) only.                                  */
 /* ---------------------------------------------------------------------- */
 /* Rows of both parties: value c of row r of party p at
- * p[p][r * row_stride + c] (u64 units, row_stride >= 0). */
+ * p[p][r * row_stride + c] (u64 units; row_stride in [0, 2^35], of one row any). */
 typedef struct sufhip_matrix2 {
   const uint64_t* p[2];
   int64_t row_stride;
@@ -1237,7 +1237,8 @@ int sufhip_linear_prepare(const int64_t* d_W, int experts, int K, int N, int dig
  * out may be residual itself (the same addresses and stride); it may meet no
  * other input.
  * K <= 65536, digits <= 4, digits K < 2^17; rows, x_rows <= 2^24; rows N <
- * 2^31; experts <= 4096.  d_work: sufhip_linear2_work_bytes() bytes (asked
+ * 2^31; experts <= 4096; fewer than 2^24 tiles of 8 rows (an expert's last one
+ * may be ragged) and 128 columns.  d_work: sufhip_linear2_work_bytes() bytes (asked
  * for with the call's device current), 16-byte aligned, used by this call
  * only until it ends; 0 bytes: none needed.
  * walk_jobs (walk_count > 0): the key-only halves of truncation gates, as

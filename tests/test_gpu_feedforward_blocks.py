@@ -232,6 +232,22 @@ def test_norm_prepared_elsewhere_and_outputs_alone(rows, cols, weight):
     assert all(torch.equal(t, a + b) for t, a, b in zip(total, xs, rs))
 
 
+@pytest.mark.parametrize("rows,cols", [(2100, 1000), (300, 7001)])
+def test_large_norm_in_place(rows, cols):
+    say("large norm in place, %d x %d" % (rows, cols))
+    rng = np.random.default_rng(rows)
+    x, r = _values(rng, rows, cols), _values(rng, rows, cols)
+    norm = ff.RMSNorm(rows, cols, STATE, seed=20)
+    xs, rs = _share(rng, x), _share(rng, r)
+    norm.eval2(xs, xs, residual=rs, total=rs)
+    s, want = ref.rmsnorm(x, r, norm.inv_len, norm.eps_q, norm.table, F)
+    assert np.array_equal(_open(rs), s) and np.array_equal(_open(xs), want)
+    xs = _share(rng, x)
+    norm.eval2(xs, xs)
+    assert np.array_equal(_open(xs), ref.rmsnorm(x, None, norm.inv_len, norm.eps_q, norm.table,
+                                                 F)[1])
+
+
 @pytest.mark.parametrize("f", [9, 13])
 @pytest.mark.parametrize("weight", [False, True])
 def test_large_norm_other_fraction(f, weight):
@@ -375,3 +391,52 @@ def test_eval2_refuses():
             call()
     torch.cuda.synchronize()
     assert all(bool((t == -7).all()) for t in x + y)
+
+
+# ---- many rows: 256 columns a workgroup ----
+
+MANY = [
+    # rows, K, N, bits, act, residual, digits in; one to five chunks of 64 k
+    (400, 40, 2100, 12, None, True, True),
+    (1603, 96, 500, 6, "relu", False, False),
+    (393, 200, 2050, 13, "gelu", True, False),
+    (410, 130, 1999, 7, None, False, True),
+    (3100, 300, 256, 12, "relu", True, True),
+    (395, 64, 2049, 22, None, True, False),  # three digits: 128 columns
+]
+
+
+@pytest.mark.parametrize("rows,K,N,bits,act,residual,split", MANY)
+def test_linear_many_rows(rows, K, N, bits, act, residual, split):
+    say("linear %dx%dx%d bits=%d act=%s digits=%s" % (rows, K, N, bits, act, split))
+    rng = np.random.default_rng(rows + K)
+    x, W = _values(rng, rows, K), _weights(rng, bits, K, N)
+    W.flat[0], W.flat[-1] = -2 ** bits, 2 ** bits - 1
+    bias = _bias(rng, N)
+    res = _values(rng, rows, N) if residual else None
+    lin = ff.Linear(ff.PublicWeights(W, bias), rows, STATE, act=_act(act), seed=21)
+    xs = _share(rng, x, pad=6)
+    out, digits = _empty(rows, N), ff.Digits(rows, N)
+    lin.eval2(ff.Digits(rows, K).split(xs) if split else xs, out, digits=digits,
+              residual=None if res is None else _share(rng, res))
+    assert np.array_equal(_open(out), ref.linear(x, W, bias, F, _act(act), res)[0])
+    assert all(torch.equal(a, b) for a, b in zip(digits.values(), out))
+
+
+@pytest.mark.parametrize("bits", [7, 12])
+@pytest.mark.parametrize("split", [False, True])
+def test_experts_many_rows(bits, split):
+    """Ragged experts, one without rows; rows in no expert between guard rows."""
+    say("experts, many rows, bits=%d digits=%s" % (bits, split))
+    rng = np.random.default_rng(bits)
+    n_rows, T, K, N, E = 2500, 700, 70, 1000, 6
+    off = np.array([3, 900, 900, 1001, 1003, 2200, 2491])
+    src = rng.integers(-1, T + 1, n_rows)
+    x, W, bias = _values(rng, T, K), _weights(rng, bits, E, K, N), _bias(rng, E, N)
+    lin = ff.Linear(ff.PublicWeights(W, bias), n_rows, STATE, x_rows=T, seed=22)
+    xs = _share(rng, x)
+    out = _empty(n_rows, N)
+    lin.eval2(ff.Digits(T, K).split(xs) if split else xs, out, offsets=_i32(off), rows=_i32(src))
+    want, written = ref.linear(x, W, bias, F, offsets=off, rows=src)
+    assert np.array_equal(_open(out)[written], want[written])
+    assert all(bool((o[~torch.from_numpy(written)] == -7).all()) for o in out)
