@@ -158,6 +158,8 @@ class Digits:
         nb = native.load().sufhip_digits2_bytes(rows, cols)
         # Zeros: rows that no call writes stand for 0.
         self.buffer = torch.zeros(nb, dtype=torch.int8, device=device)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()  # any stream may write them next
         self.shape, self.d = (rows, cols), self.buffer.get_device()
         self.arg = native.Digits2()
         self.arg.d_digits, self.arg.rows, self.arg.cols = self.buffer.data_ptr(), rows, cols
@@ -584,8 +586,8 @@ class ExpertFeedForward:
         self.mix = ExpertMix(tokens, up.K, prg_state, frac_bits, seeds[3], dev_)
         self.total = [torch.empty(tokens, up.K, dtype=torch.int64, device=dev_)
                       for _ in range(2)]
-        # Zeros: pairs in no expert are not written, nor read by the sum.
-        self.z = [torch.zeros(n, up.K, dtype=torch.int64, device=dev_) for _ in range(2)]
+        # Pairs in no expert are not written, nor read by the sum.
+        self.z = [torch.empty(n, up.K, dtype=torch.int64, device=dev_) for _ in range(2)]
         self.normed, self.hidden = Digits(tokens, up.K, dev_), Digits(n, up.N, dev_)
 
     def truncs(self):

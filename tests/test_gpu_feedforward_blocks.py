@@ -206,6 +206,27 @@ def test_two_objects_on_two_streams():
         assert np.array_equal(_open(o), want(v, None))
 
 
+def test_objects_of_a_busy_stream():
+    """Made on a stream with work before them, used on another at once."""
+    say("objects of a busy stream")
+    rng = np.random.default_rng(23)
+    x = _values(rng, 50, 70)
+    xs = _share(rng, x)
+    weights = _weights(rng, 10, 70, 40)
+    torch.cuda.synchronize()
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(20000000)
+        digits = ff.Digits(50, 70)
+        torch.cuda._sleep(20000000)
+        lin = ff.Linear(ff.PublicWeights(weights), 50, STATE, seed=23)
+        outs = ff.Digits(50, 40)
+    with torch.cuda.stream(other):
+        lin.eval2(digits.split(xs), None, digits=outs)
+    torch.cuda.synchronize()
+    assert np.array_equal(_open(outs.values()), ref.linear(x, weights, None, F)[0])
+
+
 # ---- each operator at its edges ----
 
 @pytest.mark.parametrize("rows,cols,weight", [(5, 40, True), (600, 1501, True), (2100, 1000, False),
