@@ -39,8 +39,9 @@ struct LinArgs {
   const int32_t* map;
   const int32_t* offsets;
   int tiles, cols, slices;
-  uint64_t* part;  // several k-slices: [slices][2][rows][N] sums
-  uint64_t* zhat;  // the masked opens [rows][N], for the epilogue's launch
+  // For the epilogue's launch, one of them:
+  uint64_t* part;  // both shares [slices][2][rows][N], of several k-slices or without a gate
+  uint64_t* zhat;  // the masked opens [rows][N]
   uint64_t mask;
   TruncEpi epi;
   Mat2 res;
@@ -116,12 +117,12 @@ __device__ __forceinline__ RowTile row_tile(const LinArgs& a, int ti) {
   return {-1, 0, 0};
 }
 
-// Both shares of output (row, col) where a launch finishes them: bias, then
-// the k-slices' sums, the masked open, or the truncation and the residual.
+// Both shares of output (row, col) as the product leaves them: for the
+// epilogue's launch, or with bias, truncation and residual.
 __device__ __forceinline__ void put_output(const LinArgs& a, const EpiHdrs& eh, int slice, int e,
                                            int row, int col, uint64_t y0, uint64_t y1) {
   const size_t i = size_t(row) * a.N + col;
-  if (a.slices > 1) {
+  if (a.part) {
     const size_t mn = size_t(a.rows) * a.N;
     a.part[size_t(slice) * 2 * mn + i] = y0;
     a.part[(size_t(slice) * 2 + 1) * mn + i] = y1;
@@ -491,7 +492,7 @@ __global__ void __launch_bounds__(EpiCfg<kSize>::kBlock) linear_epilogue_kernel(
     const int e = expert_of(a, row);
     if (e < 0) continue;
     uint64_t y[2] = {0, 0}, open;
-    if (a.slices > 1) {
+    if (a.part) {
       int z = 0;
       for (; z + 4 <= a.slices; z += 4) {  // a group's loads before its sums
         uint64_t v[8];
@@ -611,7 +612,8 @@ struct Plan {
   int slices;
   bool epilogue;   // the epilogue's own launch
   bool walk;       // the walks beside the product
-  size_t words;    // of the workspace: the slices' sums, or the opens
+  bool shares;     // the epilogue is handed shares, of each slice, else opens
+  size_t words;    // of the workspace, which holds them
 };
 
 bool extents_ok(int experts, int K, int N, int digits) {
@@ -652,7 +654,9 @@ Plan plan_linear(const sufhip_linear2_args& g) {
   p.walk = g.walk_count > 0 && g.walk_count <= kLinWalks && !p.wide &&
            wgs * p.slices <= 2 * device_cus() && (p.epilogue || mn <= (size_t(1) << 17));
   p.epilogue = p.epilogue || p.walk;
-  p.words = !p.epilogue ? 0 : (p.slices > 1 ? size_t(p.slices) * 2 * mn : mn);
+  // Without a gate nothing is opened: a party's output is its own share.
+  p.shares = p.slices > 1 || !g.trunc;
+  p.words = !p.epilogue ? 0 : (p.shares ? size_t(p.slices) * 2 * mn : mn);
   return p;
 }
 
@@ -891,10 +895,7 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
   a.tiles = plan.tiles;
   a.cols = plan.col_tiles;
   a.slices = plan.slices;
-  if (plan.slices > 1)
-    a.part = words;
-  else if (plan.epilogue)
-    a.zhat = words;
+  if (plan.epilogue) (plan.shares ? a.part : a.zhat) = words;
   const unsigned wgs = unsigned(tiles);
   switch (g.w.digits) {
     case 1: launch_product<1>(a, w, plan.wide, wgs, s); break;
