@@ -20,7 +20,8 @@ A program that has to hide the choice runs every token through every expert
 (a Linear each) and adds them up by shared weights.
 
 Each object holds one use's dealer material, drawn by its own Dealer unless it
-is given a seed (two with one seed would open under the same masks).  eval2
+is given a seed (two with one seed would open under the same masks; a block's
+parts draw from the block's one Dealer).  eval2
 issues the key-only halves of its gates first, or waits for `prep` =
 (tasks.Prepared, batch) where they were issued before.  Calls of one object go
 one after the other (they share its workspace), in one stream or in streams
@@ -46,6 +47,14 @@ MAX_ROWS = 1 << 24
 LEN_BITS = 26  # of a norm's public 1 / cols, truncated by two gates of 13 bits
 
 _seeds = itertools.count(0x5eed0001)
+
+
+def _dealer(seed):
+    """The Dealer of a seed; a block's parts are given its own, from which they
+    draw one after the other."""
+    if isinstance(seed, Dealer):
+        return seed
+    return Dealer(next(_seeds) if seed is None else seed)
 
 
 # ---- arguments ----
@@ -108,7 +117,7 @@ class _Block:
         self.device = _gpu(device, type(self).__name__)
         self.d = self.device.index
         self.prg_state = bytes(prg_state)
-        self.dealer = Dealer(next(_seeds) if seed is None else seed)
+        self.dealer = _dealer(seed)
         self._walks = None
 
     def _guard(self):
@@ -537,18 +546,18 @@ class FeedForward:
     what follows a decoder's attention, from its output and the residual
     stream.  The norm hands its output on as digits, up its activations.
     up, down: PublicWeights of [cols, hidden] and [hidden, cols]; act as in
-    Linear; weight, eps, table as in RMSNorm.  seed: of the three parts'
-    material (seed, seed + 1, seed + 2)."""
+    Linear; weight, eps, table as in RMSNorm.  seed: of the block's dealer, from
+    which its parts draw."""
 
     def __init__(self, rows, up, down, prg_state, frac_bits=12, act="relu", weight=None,
                  eps=1.0 / 1024.0, table=None, seed=None):
         _pair("FeedForward", up, down, 1)
         dev_ = torch.device("cuda", up.d)
-        seeds = [None if seed is None else seed + i for i in range(3)]
+        deal = _dealer(seed)
         self.rows, self.cols = rows, up.K
-        self.norm = RMSNorm(rows, up.K, prg_state, frac_bits, weight, eps, table, seeds[0], dev_)
-        self.up = Linear(up, rows, prg_state, frac_bits, act, seed=seeds[1])
-        self.down = Linear(down, rows, prg_state, frac_bits, seed=seeds[2])
+        self.norm = RMSNorm(rows, up.K, prg_state, frac_bits, weight, eps, table, deal, dev_)
+        self.up = Linear(up, rows, prg_state, frac_bits, act, seed=deal)
+        self.down = Linear(down, rows, prg_state, frac_bits, seed=deal)
         self.total = [torch.empty(rows, up.K, dtype=torch.int64, device=dev_) for _ in range(2)]
         self.normed, self.hidden = Digits(rows, up.K, dev_), Digits(rows, up.N, dev_)
 
@@ -567,7 +576,7 @@ class ExpertFeedForward:
     """out[t] = s[t] + sum_k weights[t, k] down_e(act(up_e(norm(s)[t]))), e the
     k-th expert of token t, with s = x + residual: FeedForward with `each`
     experts a token.  up, down: PublicWeights of [experts, cols, hidden] and
-    [experts, hidden, cols]; the rest as in FeedForward (seed .. seed + 3)."""
+    [experts, hidden, cols]; the rest as in FeedForward."""
 
     def __init__(self, tokens, each, up, down, prg_state, frac_bits=12, act="relu", weight=None,
                  eps=1.0 / 1024.0, table=None, seed=None):
@@ -576,14 +585,13 @@ class ExpertFeedForward:
         each = _extent(each, 1, 1024, what, "each")
         _pair(what, up, down, None)
         dev_ = torch.device("cuda", up.d)
-        seeds = [None if seed is None else seed + i for i in range(4)]
+        deal = _dealer(seed)
         n = tokens * each
         self.tokens, self.each, self.cols = tokens, each, up.K
-        self.norm = RMSNorm(tokens, up.K, prg_state, frac_bits, weight, eps, table, seeds[0],
-                            dev_)
-        self.up = Linear(up, n, prg_state, frac_bits, act, x_rows=tokens, seed=seeds[1])
-        self.down = Linear(down, n, prg_state, frac_bits, seed=seeds[2])
-        self.mix = ExpertMix(tokens, up.K, prg_state, frac_bits, seeds[3], dev_)
+        self.norm = RMSNorm(tokens, up.K, prg_state, frac_bits, weight, eps, table, deal, dev_)
+        self.up = Linear(up, n, prg_state, frac_bits, act, x_rows=tokens, seed=deal)
+        self.down = Linear(down, n, prg_state, frac_bits, seed=deal)
+        self.mix = ExpertMix(tokens, up.K, prg_state, frac_bits, deal, dev_)
         self.total = [torch.empty(tokens, up.K, dtype=torch.int64, device=dev_)
                       for _ in range(2)]
         # Pairs in no expert are not written, nor read by the sum.

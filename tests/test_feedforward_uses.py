@@ -1,10 +1,14 @@
 """The feed-forward operators on the CPU: workspaces, and what stands between
 one use of an object and the next."""
+import contextlib
 import ctypes
 
+import numpy as np
 import pytest
+import torch
 
-from suf_amd import native
+from suf_amd import feedforward as ff
+from suf_amd import native, tables, tasks
 from test_feedforward_arguments import at, linear_args
 
 
@@ -24,3 +28,71 @@ def test_a_product_without_a_gate_hands_over_both_shares(rows, K, N):
         assert words(False, **kw) >= 2 * rows * N
         assert words(True, **kw) >= rows * N
     assert words(False) in (0, words(False, walk_count=2))
+
+
+# ---- whose words are whose ----
+
+class HostWeights(ff.PublicWeights):
+    """The extents of public weights."""
+
+    def __init__(self, K, N, experts=1):
+        self.K, self.N, self.experts, self.digits, self.d = K, N, experts, 2, -1
+        a = self.arg = native.LinearWeights()
+        a.experts, a.K, a.N, a.digits = experts, K, N, 2
+
+
+@pytest.fixture
+def on_host(monkeypatch):
+    """Material is dealt on the host; here it stays there."""
+    cpu = torch.device("cpu")
+    monkeypatch.setattr(ff, "_gpu", lambda device, what: cpu)
+    monkeypatch.setattr(ff._Block, "_guard", lambda self: contextlib.nullcontext())
+    monkeypatch.setattr(ff, "Digits", lambda *a: None)
+    monkeypatch.setattr(torch, "device", lambda *a: cpu)
+    monkeypatch.setattr(tasks.pfss, "trunc_gen",
+                        lambda *a: [torch.zeros(8, dtype=torch.uint8)] * 2)
+
+
+def words_of(o, names):
+    """All words that an object's dealer drew or derived, by part, without the
+    small numbers of layouts and headers."""
+    out = set()
+
+    def walk(v):
+        if isinstance(v, torch.Tensor):
+            if v.dtype is torch.int64:
+                out.update(v.reshape(-1).tolist())
+        elif isinstance(v, np.ndarray):
+            if v.dtype in (np.uint64, np.int64):
+                out.update(v.reshape(-1).view(np.int64).tolist())
+        elif isinstance(v, (list, tuple)):
+            for w in v:
+                walk(w)
+        elif isinstance(v, (ff.Trunc, ff.Triples, ff.CoeffLut)):
+            walk([w for k, w in vars(v).items() if k not in ("work", "blobs", "keys")])
+    walk([vars(o)[k] for k in names if k in vars(o)])
+    return {w for w in out if abs(w) > 1 << 40}
+
+
+MATERIAL = ("a", "a2", "b", "ab", "tr_ms", "tr_rsqrt", "tr_norm", "tr_weight", "tri", "tr",
+            "tr_act")
+
+
+def parts(block):
+    return [words_of(p, MATERIAL) for p in
+            (block.norm, block.up, block.down) + ((block.mix,) if hasattr(block, "mix") else ())]
+
+
+@pytest.mark.parametrize("experts", [1, 3])
+def test_blocks_of_neighbouring_seeds_share_no_material(on_host, experts):
+    """A model's layers, seeded 0, 1, 2 and so on: no word of one part's masks,
+    triples and gates is another's, in a block or between two."""
+    up, down = HostWeights(8, 6, experts), HostWeights(6, 8, experts)
+    kw = dict(act=tables.gelu_table(12), weight=torch.full((8,), 5000))
+    make = (lambda s: ff.FeedForward(3, up, down, bytes(range(128)), seed=s, **kw)) if experts == 1 else \
+        (lambda s: ff.ExpertFeedForward(3, 2, up, down, bytes(range(128)), seed=s, **kw))
+    sets = [p for s in range(6) for p in parts(make(s))]
+    assert all(len(p) > 8 for p in sets)
+    assert len(set().union(*sets)) == sum(len(p) for p in sets)
+    again = parts(make(2))  # one seed, one material
+    assert again == sets[2 * len(again):3 * len(again)]
