@@ -27,7 +27,6 @@ it by a fresh triple for every new token; its attention is
 src/nn/attention_block.cpp:931-1900.
 """
 import ctypes
-import itertools
 import math
 import warnings
 
@@ -36,7 +35,7 @@ import torch
 
 from . import native, tables
 from .softmax import LONG_KEYS, LongRows, SoftmaxBlock
-from .tasks import TABLE_BITS, Dealer, Trunc, dev, dev_i32, prepare_batch
+from .tasks import TABLE_BITS, Dealer, Trunc, dev, dev_i32, own_seed, prepare_batch
 
 M64 = (1 << 64) - 1
 I32 = (1 << 31) - 1       # the library counts tokens, heads and pages in 32 bits
@@ -557,9 +556,6 @@ def _shares(dealer, shape, device):
     return tuple(dev(dealer.words(n), device).view(shape) for _ in range(2))
 
 
-_seeds = itertools.count(21)
-
-
 class CachedAttention:
     """Causal attention of new tokens over a PagedCache, grouped heads, with
     rotary positions; Q(frac_bits) shares in and out:
@@ -610,7 +606,7 @@ class CachedAttention:
         # Of rows that the block takes, a reciprocal that holds at every sum.
         self.recip_table = None if self.long_rows else tables.recip_wide_table(
             frac_bits, 2.0 ** max(10, int(max_positions).bit_length()))
-        self.dealer = Dealer(next(_seeds) if seed is None else seed)
+        self.dealer = Dealer(own_seed() if seed is None else seed)
 
     def deal(self, seqs, new):
         """A step of new[i] tokens of sequence seqs[i].  Its material takes

@@ -17,6 +17,8 @@ current stream.
                1248-1384), rotated by the gate's r_in
   term/operand the generalised operands of sufhip_lin2 / sufhip_mul2x
 """
+import os
+
 import numpy as np
 import torch
 
@@ -62,6 +64,13 @@ class Dealer:
 
     def word(self):
         return int(self.words(1)[0])
+
+
+def own_seed():
+    """A Dealer's seed where the caller gives none: another one each time, in
+    every process (what two objects open under the same masks tells their
+    difference)."""
+    return int.from_bytes(os.urandom(8), "little")
 
 
 def term(pair, index=None, stride=1, off=0, shift=0, neg=False, length=None, mul=1):

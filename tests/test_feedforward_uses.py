@@ -2,6 +2,9 @@
 one use of an object and the next."""
 import contextlib
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -96,3 +99,18 @@ def test_blocks_of_neighbouring_seeds_share_no_material(on_host, experts):
     assert len(set().union(*sets)) == sum(len(p) for p in sets)
     again = parts(make(2))  # one seed, one material
     assert again == sets[2 * len(again):3 * len(again)]
+
+
+def test_unseeded_objects_differ_between_processes():
+    """Two runs of a program do not open their values under the same masks."""
+    code = ("from suf_amd import feedforward as ff, kv_attention as kv\n"
+            "kv.Rotary.build = classmethod(lambda *a, **k: None)\n"
+            "class Cache:\n"
+            "    class k: dim = 8\n"
+            "    kv_heads, device = 1, 'cpu'\n"
+            "att = kv.CachedAttention(Cache, 1, b'', 64).dealer.seed\n"
+            "print(next(ff._seeds), next(ff._seeds), att)\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    runs = [subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                           check=True).stdout.split() for _ in range(2)]
+    assert len(runs[0]) == 3 and len(set(runs[0] + runs[1])) == 6
