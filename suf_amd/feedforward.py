@@ -25,14 +25,16 @@ parts draw from the block's one Dealer).  eval2
 issues the key-only halves of its gates first, or waits for `prep` =
 (tasks.Prepared, batch) where they were issued before.  Calls of one object go
 one after the other (they share its workspace), in one stream or in streams
-that wait for each other.  Of a captured call's replays each opens under the
-same masks.
+that wait for each other.  A second call of an object with gates opens other
+values under the same masks: eval2 warns of it, but not of a captured call's
+replays, of which each is one.
 
 The reference has LayerNorm (include/runtime/phase_tasks.hpp:2186-2668) and
 dense public products (src/nn/matmul_publicW.cpp:17-36); it has no experts.
 """
 import contextlib
 import ctypes
+import warnings
 
 import numpy as np
 import torch
@@ -118,12 +120,23 @@ class _Block:
         self.prg_state = bytes(prg_state)
         self.dealer = _dealer(seed)
         self._walks = None
+        self.spent = False  # whether its masks have hidden a value
+        # Who warns of a second use, and how far above _use its caller stands: of
+        # a block's parts the first one, for the block.
+        self.warns = (type(self).__name__, 3)
 
     def _guard(self):
         """Makes the object's device the current one, where it is not."""
         if torch._C._cuda_getDevice() == self.d:
             return contextlib.nullcontext()
         return torch.cuda.device(self.d)
+
+    def _use(self):
+        """Warns of a second use."""
+        if self.spent and self.warns:
+            warnings.warn("%s.eval2: an object is for one use; a second one opens other values "
+                          "under the same masks, whose difference is then public" % self.warns[0],
+                          RuntimeWarning, stacklevel=self.warns[1])
 
     def _gate(self, bits, n):
         return Trunc(self.dealer, bits, n, self.prg_state, device=self.device)
@@ -288,9 +301,11 @@ class RMSNorm(_Block):
             _digits(a.out_digits, digits, shape, d, what, "digits")
         if out is None and digits is None and total is None:
             _fail(what, "no output")
+        self._use()
         with self._guard():
             self._walks_of(a, prep)
             _call("sufhip_rmsnorm2", a, d)
+        self.spent = True
         return out
 
 
@@ -461,10 +476,12 @@ class Linear(_Block):
             _digits(a.out_digits, digits, shape, d, what, "digits")
         elif out is None:
             _fail(what, "no output")
+        self._use()
         with self._guard():
             if prep is not None or self.tr is not None:
                 self._walks_of(a, prep)
             _call("sufhip_linear2", a, d)
+        self.spent = self.tr is not None
         return out
 
 
@@ -511,9 +528,11 @@ class ExpertMix(_Block):
         if residual is not None:
             _matrix(a.residual, residual, shape, d, what, "residual")
         _out(a, out, shape, d, what, "out")
+        self._use()
         with self._guard():
             self._ready(prep)
             _call("sufhip_expert_mix2", a, d)
+        self.spent = True
         return out
 
 
@@ -559,6 +578,7 @@ class FeedForward:
         self.down = Linear(down, rows, prg_state, frac_bits, seed=deal)
         self.total = [torch.empty(rows, up.K, dtype=torch.int64, device=dev_) for _ in range(2)]
         self.normed, self.hidden = Digits(rows, up.K, dev_), Digits(rows, up.N, dev_)
+        self.norm.warns, self.up.warns, self.down.warns = ("FeedForward", 4), None, None
 
     def truncs(self):
         return self.norm.truncs() + self.up.truncs() + self.down.truncs()
@@ -596,6 +616,8 @@ class ExpertFeedForward:
         # Pairs in no expert are not written, nor read by the sum.
         self.z = [torch.empty(n, up.K, dtype=torch.int64, device=dev_) for _ in range(2)]
         self.normed, self.hidden = Digits(tokens, up.K, dev_), Digits(n, up.N, dev_)
+        self.norm.warns = ("ExpertFeedForward", 4)
+        self.up.warns = self.down.warns = self.mix.warns = None
 
     def truncs(self):
         return self.norm.truncs() + self.up.truncs() + self.down.truncs() + self.mix.truncs()

@@ -1,0 +1,93 @@
+"""What stands between one use of a feed-forward operator and the next."""
+import warnings
+
+import numpy as np
+import pytest
+import torch
+
+import oracle_lib as ol
+from gpu_util import say
+from suf_amd import feedforward as ff
+from suf_amd import native
+
+pytestmark = pytest.mark.gpu
+
+STATE = ol.mt64_bytes(6, ol.PRG_STATE_BYTES).tobytes()
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _init():
+    native.call("sufhip_init", 0)
+
+
+def _pair(*shape):
+    return tuple(torch.zeros(shape, dtype=torch.int64, device="cuda") for _ in range(2))
+
+
+def _public(*shape):
+    return ff.PublicWeights(np.arange(np.prod(shape)).reshape(shape) % 200 - 100)
+
+
+def _tables(tokens, each, experts):
+    chosen = torch.arange(tokens * each, device="cuda").reshape(tokens, each) % experts
+    return (*ff.route(chosen, experts), torch.ones(tokens, each, dtype=torch.int64, device="cuda"))
+
+
+def _norm():
+    o = ff.RMSNorm(3, 40, STATE, seed=1)
+    return (lambda: o.eval2(_pair(3, 40), _pair(3, 40))), (lambda: o.eval2(_pair(3, 41), None))
+
+
+def _linear():
+    o = ff.Linear(_public(40, 24), 3, STATE, act="relu", seed=1)
+    return (lambda: o.eval2(_pair(3, 40), _pair(3, 24))), (lambda: o.eval2(_pair(3, 40), None))
+
+
+def _mix():
+    o, slots = ff.ExpertMix(3, 24, STATE, seed=1), torch.zeros(3, 2, dtype=torch.int32).cuda()
+    w = torch.ones(3, 2, dtype=torch.int64, device="cuda")
+    return (lambda: o.eval2(_pair(4, 24), slots, w, _pair(3, 24))), \
+        (lambda: o.eval2(_pair(4, 24), slots, w, _pair(3, 25)))
+
+
+def _block():
+    o = ff.FeedForward(3, _public(40, 24), _public(24, 40), STATE, seed=1)
+    return (lambda: o.eval2(_pair(3, 40), _pair(3, 40))), \
+        (lambda: o.eval2(_pair(3, 41), _pair(3, 40)))
+
+
+def _experts():
+    o = ff.ExpertFeedForward(3, 2, _public(4, 40, 24), _public(4, 24, 40), STATE, seed=1)
+    tabs = _tables(3, 2, 4)
+    return (lambda: o.eval2(_pair(3, 40), _pair(3, 40), *tabs)), \
+        (lambda: o.eval2(_pair(3, 41), _pair(3, 40), *tabs))
+
+
+@pytest.mark.parametrize("make", [_norm, _linear, _mix, _block, _experts])
+def test_a_second_use_is_warned_of(make):
+    """Once for a call, where the call stands; a refused call is no use."""
+    say("second use, %s" % make.__name__)
+    call, *refused = make()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        for bad in refused:
+            with pytest.raises(ValueError):
+                bad()
+        call()
+        for bad in refused:
+            with pytest.raises(ValueError):
+                bad()
+    with pytest.warns(RuntimeWarning, match="one use") as seen:
+        call()
+    assert len(seen) == 1 and seen[0].filename == __file__
+    torch.cuda.synchronize()
+
+
+def test_a_product_that_opens_nothing_may_be_used_again():
+    say("untruncated product, twice")
+    o = ff.Linear(_public(40, 24), 3, STATE, trunc=False)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        for _ in range(2):
+            o.eval2(_pair(3, 40), _pair(3, 24), digits=ff.Digits(3, 24))
+    torch.cuda.synchronize()
