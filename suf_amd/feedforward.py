@@ -586,6 +586,9 @@ class FeedForward:
     def eval2(self, x, out, residual=None, prep=None):
         """x, out, residual: pairs of int64 [rows, cols] with any row stride;
         out may be x or residual.  Returns out."""
+        # Before the norm uses up its masks.
+        _matrix(native.Matrix2(), out, (self.rows, self.cols), self.norm.d, "FeedForward.eval2",
+                "out", written=True)
         self.norm.eval2(x, None, residual, self.total, self.normed, prep)
         self.up.eval2(self.normed, None, digits=self.hidden, prep=prep)
         return self.down.eval2(self.hidden, out, self.total, prep=prep)
@@ -626,6 +629,16 @@ class ExpertFeedForward:
         """x, out, residual as in FeedForward; offsets, rows, slots: route() of
         the tokens' experts, on the GPU; weights: int64 [tokens, each] in
         Q(frac_bits) on the GPU.  Returns out."""
+        what, d, experts = "ExpertFeedForward.eval2", self.norm.d, self.up.weights.experts
+        # Before the norm uses up its masks.
+        _matrix(native.Matrix2(), out, (self.tokens, self.cols), d, what, "out", written=True)
+        if experts > 1 or offsets is not None:
+            _ptr(offsets, (experts + 1,), d, what, "offsets", torch.int32)
+        if self.each > 1 or rows is not None:
+            _ptr(rows, (self.up.rows,), d, what, "rows", torch.int32)
+        each = slots.shape[1] if getattr(slots, "ndim", 0) == 2 else self.each
+        _ptr(slots, (self.tokens, each), d, what, "slots", torch.int32)
+        _ptr(weights, (self.tokens, each), d, what, "weights")
         self.norm.eval2(x, None, residual, self.total, self.normed, prep)
         self.up.eval2(self.normed, None, offsets=offsets, rows=rows, digits=self.hidden,
                       prep=prep)

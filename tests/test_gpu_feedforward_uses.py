@@ -53,14 +53,20 @@ def _mix():
 def _block():
     o = ff.FeedForward(3, _public(40, 24), _public(24, 40), STATE, seed=1)
     return (lambda: o.eval2(_pair(3, 40), _pair(3, 40))), \
-        (lambda: o.eval2(_pair(3, 41), _pair(3, 40)))
+        (lambda: o.eval2(_pair(3, 41), _pair(3, 40))), (lambda: o.eval2(_pair(3, 40), None)), \
+        (lambda: o.eval2(_pair(3, 40), _pair(3, 40), _pair(3, 39)))
 
 
 def _experts():
     o = ff.ExpertFeedForward(3, 2, _public(4, 40, 24), _public(4, 24, 40), STATE, seed=1)
     tabs = _tables(3, 2, 4)
     return (lambda: o.eval2(_pair(3, 40), _pair(3, 40), *tabs)), \
-        (lambda: o.eval2(_pair(3, 41), _pair(3, 40), *tabs))
+        (lambda: o.eval2(_pair(3, 41), _pair(3, 40), *tabs)), \
+        (lambda: o.eval2(_pair(3, 40), _pair(3, 41), *tabs)), \
+        (lambda: o.eval2(_pair(3, 40), _pair(3, 40), tabs[0][1:], *tabs[1:])), \
+        (lambda: o.eval2(_pair(3, 40), _pair(3, 40), tabs[0], tabs[1][1:], *tabs[2:])), \
+        (lambda: o.eval2(_pair(3, 40), _pair(3, 40), *tabs[:2], tabs[2][:, :1], tabs[3])), \
+        (lambda: o.eval2(_pair(3, 40), _pair(3, 40), *tabs[:3], tabs[3].int()))
 
 
 @pytest.mark.parametrize("make", [_norm, _linear, _mix, _block, _experts])
@@ -91,3 +97,20 @@ def test_a_product_that_opens_nothing_may_be_used_again():
         for _ in range(2):
             o.eval2(_pair(3, 40), _pair(3, 24), digits=ff.Digits(3, 24))
     torch.cuda.synchronize()
+
+
+def test_one_expert_needs_no_tables():
+    """With one expert, one for each token, the tokens' own order will do; the
+    sum may take fewer rows than there are."""
+    say("one expert, no tables")
+    up, down = _public(40, 24), _public(24, 40)
+    x = tuple(torch.full((3, 40), v, dtype=torch.int64, device="cuda") for v in (5000, -77))
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    w = torch.full((3, 1), 4096, dtype=torch.int64, device="cuda")
+    got = [ff.ExpertFeedForward(3, 1, up, down, STATE).eval2(x, _pair(3, 40), *t, slots, w)
+           for t in ((None, None), ff.route(torch.zeros(3, 1, dtype=torch.int64).cuda(), 1)[:2])]
+    assert torch.equal(*(a[0] + a[1] for a in got))
+    two = ff.route(torch.zeros(3, 2, dtype=torch.int64).cuda(), 1)
+    out = ff.ExpertFeedForward(3, 2, up, down, STATE).eval2(x, _pair(3, 40), *two[:2],
+                                                            2 * slots, w)
+    assert torch.equal(out[0] + out[1], got[0][0] + got[0][1])
