@@ -217,8 +217,9 @@ class RMSNorm(_Block):
 
     In whole numbers, with >> a floor: ms = (((sum s s) >> f) inv) >> 26 with inv
     = round(2^26 / cols); y from `table` (pieces' starts and words (c0, c1) in
-    the unsigned order of ms + eps: tables.rsqrt_wide_table, up to mean squares
-    of 4096) and a Newton step; out = (s y) >> f, then (out weight) >> f.
+    the unsigned order of ms + eps: tables.rsqrt_wide_table, for mean squares up
+    to 4096, rougher up to 65536, where y stops falling) and a Newton step; out =
+    (s y) >> f, then (out weight) >> f.
     y is a Q(f) number: at a mean square of 4096 it is 2^(f - 6) steps.
     weight: public int64 [cols] in Q(f), or None.  frac_bits at most 13."""
 

@@ -302,24 +302,40 @@ def rsqrt_wide_table(frac_bits=12, eps=1.0 / 1024.0, vmax=4096.0):
     floor of y y to 2^-f, which loses up to a share v 2^-f of it: so each
     constant is the one whose result, floors and all, is nearest to 1/sqrt over
     its piece.  With 12 fractional bits y is then off by 0.5 % at most up to 256,
-    0.9 % up to 1024 and 2.5 % up to 4096, where one of its steps is 1.6 %."""
+    0.9 % up to 1024 and 2.5 % up to 4096, where one of its steps is 1.6 %.
+
+    Past vmax a constant that the step overshoots would leave y negative.  There
+    the constants go on (quarters of an octave to 2 vmax, halves to 16 vmax, as
+    many as a LUT of 64 intervals takes: all of them for an eps of 2^-14 and
+    more; y is off by 6 % and 13 % at 12 bits), and the last one's y y rounds to
+    0, so that the step makes 1.5 times of it whatever the mean square is: y
+    stays at 1 / (4 sqrt(vmax))."""
     alpha, coeffs = rsqrt_table(frac_bits, eps, min(16.0, vmax))
     pieces = [(int(a), 0, [int(w) for w in c]) for a, c in zip(alpha, coeffs)][:-1]
 
     one = math.ldexp(1.0, frac_bits)
+
+    def constant(lo, hi):
+        v = (one * np.linspace(lo, hi, 33)).astype(np.int64)
+        want = one * (v / one) ** -0.5
+        y = np.arange(max(1, int(0.6 * want[-1])), int(1.4 * want[0]) + 2)[:, None]
+        h = (v * ((y * y) >> frac_bits)) >> (frac_bits + 1)
+        got = (y * ((3 << (frac_bits - 1)) - h)) >> frac_bits
+        best = int(y[np.abs(got / want - 1).max(1).argmin(), 0])
+        pieces.append((_enc(lo, frac_bits), 0, [best, 0]))
+
     L = min(16.0, vmax)
     while L < vmax:
         for i in range(4):
-            lo, hi = L * 2.0 ** (i / 4), L * 2.0 ** ((i + 1) / 4)
-            v = (one * np.linspace(lo, hi, 33)).astype(np.int64)
-            want = one * (v / one) ** -0.5
-            y = np.arange(max(1, int(0.6 * want[-1])), int(1.4 * want[0]) + 2)[:, None]
-            h = (v * ((y * y) >> frac_bits)) >> (frac_bits + 1)
-            got = (y * ((3 << (frac_bits - 1)) - h)) >> frac_bits
-            best = int(y[np.abs(got / want - 1).max(1).argmin(), 0])
-            pieces.append((_enc(lo, frac_bits), 0, [best, 0]))
+            constant(L * 2.0 ** (i / 4), L * 2.0 ** ((i + 1) / 4))
         L *= 2.0
-    pieces.append((_enc(vmax, frac_bits), 0, [_enc(vmax ** -0.5, frac_bits), 0]))
+    # 62 pieces and the last one are 64 intervals once the mask has wrapped one.
+    ends = [L * 2.0 ** e for e in (0, 0.25, 0.5, 0.75, 1, 1.5, 2, 2.5, 3, 3.5, 4)]
+    ends = ends[:max(1, 63 - len(pieces))]
+    for lo, hi in zip(ends, ends[1:]):
+        constant(lo, hi)
+    last = min(int(one * ends[-1] ** -0.5 / 1.5 + 0.5), math.isqrt((1 << frac_bits) - 1))
+    pieces.append((_enc(ends[-1], frac_bits), 0, [last, 0]))
     return _finish(pieces, 2)
 
 

@@ -10,9 +10,12 @@ import numpy as np
 import pytest
 import torch
 
+import feedforward_reference as ref
 from suf_amd import feedforward as ff
 from suf_amd import native, tables, tasks
 from test_feedforward_arguments import at, linear_args
+
+M64 = (1 << 64) - 1
 
 
 @pytest.mark.parametrize("rows,K,N", [(4, 64, 32), (1, 1, 1), (500, 64, 96), (4, 1000, 70)])
@@ -114,3 +117,25 @@ def test_unseeded_objects_differ_between_processes():
     runs = [subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
                            check=True).stdout.split() for _ in range(2)]
     assert len(runs[0]) == 3 and len(set(runs[0] + runs[1])) == 6
+
+
+# ---- the norm's range ----
+
+@pytest.mark.parametrize("f", [8, 10, 12, 13])
+@pytest.mark.parametrize("eps", [1.0 / 1024.0, 1e-5, 1e-6])
+def test_norm_of_large_mean_squares(f, eps):
+    """Past the table's range y neither turns negative nor grows, up to sums that
+    wrap; at 12 bits it is as near as the table says."""
+    alpha, words = tables.rsqrt_wide_table(f, eps)
+    assert np.all(alpha[1:] > alpha[:-1]) and len(alpha) <= 63
+    v = np.concatenate([np.exp2(np.linspace(12, 16, 4001)), np.exp2(np.arange(16, 63 - f))])
+    v = np.concatenate([np.rint(v * 2.0 ** f).astype(np.uint64),
+                        np.array([1 << 63, M64], np.uint64)])
+    y = ref.rsqrt(v, (alpha, words), f).view(np.int64) / 2.0 ** f
+    top = 1.13 / 64 + 1.5 * 2.0 ** -f  # a constant's half octave, a step of 1.5 y
+    assert np.all((y >= 0) & (y <= top))
+    assert len(set(y[v >= 65536 << f])) == 1
+    if f == 12 and eps > 1e-4:
+        off = np.abs(y * np.sqrt(v / 2.0 ** f) - 1)
+        assert off[v < 8192 << f].max() <= 0.061 and off[v < 65536 << f].max() <= 0.13
+        assert y[-1] == 1 / 256
