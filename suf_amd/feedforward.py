@@ -220,7 +220,11 @@ class RMSNorm(_Block):
     the unsigned order of ms + eps: tables.rsqrt_wide_table, for mean squares up
     to 4096, rougher up to 65536, where y stops falling) and a Newton step; out =
     (s y) >> f, then (out weight) >> f.
-    y is a Q(f) number: at a mean square of 4096 it is 2^(f - 6) steps.
+    y is a Q(f) number: at a mean square of 4096 it is 2^(f - 6) steps.  So are
+    ms and eps: an eps of less than half a step is 0, and a row whose ms + eps is
+    n steps has its y off by a share of up to 0.75 / n (default eps, 12 bits: n
+    is 4 at least; a model's 1e-5 is none).  eps must be positive, and at least
+    2^-25 for the default table; a table has at most 63 pieces.
     weight: public int64 [cols] in Q(f), or None.  frac_bits at most 13."""
 
     def __init__(self, rows, cols, prg_state, frac_bits=12, weight=None, eps=1.0 / 1024.0,
@@ -229,14 +233,17 @@ class RMSNorm(_Block):
         self.rows = rows = _extent(rows, 1, MAX_ROWS, what, "rows")
         self.cols = cols = _extent(cols, 1, 1 << 20, what, "cols")
         _gate_bits(frac_bits, TABLE_BITS - 1, what)
+        if table is None:
+            table = tables.rsqrt_wide_table(frac_bits, eps)
+        if len(table[0]) > 63:  # 64 intervals, one of them wrapped by the mask
+            _fail(what, "a table of %d pieces (eps %r), at most 63 are taken" %
+                  (len(table[0]), eps))
         super().__init__(prg_state, seed, device)
         with self._guard():
             self._deal(rows, cols, frac_bits, weight, eps, table, what)
 
     def _deal(self, rows, cols, f, weight, eps, table, what):
         deal, n = self.dealer, rows * cols
-        if table is None:
-            table = tables.rsqrt_wide_table(f, eps)
         self.table, self.f = table, f
         self.inv_len = tables.llround(2.0 ** LEN_BITS / cols)
         self.eps_q = tables.eps_qf(eps, f)

@@ -255,6 +255,8 @@ def rsqrt_table(frac_bits=12, eps=1.0 / 1024.0, vmax=16.0):
     """1/sqrt(x) affine init: constant 1/sqrt(eps) below eps, chords on
     [eps 2^k, eps 2^(k+1)) up to vmax, constant 1/sqrt(vmax) above, as the
     x-form words (a0 - (a1 * offset >> f), a1)."""
+    if not 0 < eps < math.inf:
+        raise ValueError("rsqrt_table: eps must be a positive number, not %r" % (eps,))
     scale = math.ldexp(1.0, frac_bits)
     eps_q = _enc(eps, frac_bits)
     if eps_q == 0:

@@ -139,3 +139,31 @@ def test_norm_of_large_mean_squares(f, eps):
         off = np.abs(y * np.sqrt(v / 2.0 ** f) - 1)
         assert off[v < 8192 << f].max() <= 0.061 and off[v < 65536 << f].max() <= 0.13
         assert y[-1] == 1 / 256
+
+
+@pytest.mark.parametrize("eps", [0, 0.0, -1e-5, float("nan"), float("inf"), 1e-8, 2.0 ** -26])
+def test_norm_refuses_an_epsilon_that_no_table_takes(eps):
+    with pytest.raises(ValueError, match="eps"):
+        ff.RMSNorm(1, 8, bytes(range(128)), eps=eps)
+
+
+def test_norm_refuses_long_tables():
+    with pytest.raises(ValueError, match="63"):
+        ff.RMSNorm(1, 8, bytes(range(128)), table=(np.arange(64), np.zeros((64, 2))))
+    assert len(tables.rsqrt_wide_table(12, 2.0 ** -25)[0]) == 63
+
+
+@pytest.mark.parametrize("f", [10, 12])
+@pytest.mark.parametrize("eps", [1.0 / 1024.0, 1e-5, 1e-6])
+def test_norm_of_small_mean_squares(f, eps):
+    """What the mean square's and the epsilon's own steps leave of 1/sqrt(ms +
+    eps), n steps of them: the floor of ms up to a step, eps half of one, so 1.5
+    steps of n, half of it in the root; and the table's 1.5 e^2, e <= 6.25 % (a
+    chord of an octave, or of one of the first steps, which are shorter)."""
+    table = tables.rsqrt_wide_table(f, eps)
+    ms = np.exp2(np.linspace(-f - 3, 0, 20001))
+    n = np.floor(ms * 2.0 ** f) + tables.eps_qf(eps, f)
+    at = n >= 1
+    y = ref.rsqrt(n[at].astype(np.uint64), table, f).view(np.int64) / 2.0 ** f
+    off = np.abs(y * np.sqrt(ms[at] + eps) - 1)
+    assert np.all(off <= 0.75 / n[at] + 1.5 * 0.0625 ** 2 + 4 * 2.0 ** -f)
