@@ -328,8 +328,11 @@ class PublicWeights:
     """Public weights on the GPU as int8 digits: W int64 [K, N], or [experts,
     K, N], a numpy array or a tensor; bias int64 [N] or [experts, N] in the
     scale of the products (twice the fractional bits of a Q(f) W and x), or
-    None.  Weights of up to 8 b - 1 bits and a sign take b bytes each; at most
-    4, and b K < 2^17."""
+    None.  Every weight takes as many digits, a byte each, as the largest one:
+    1 hold [-128, 127], 2 [-32896, 32639], 3 [-8421504, 8355711], 4
+    [-2155905152, 2139062143], so that 15 bits and a sign take 3 where some are
+    past 32639 (21 int8 products where 2 take 15).  At most 4, and digits
+    K < 2^17."""
 
     def __init__(self, W, bias=None, device="cuda"):
         what = "PublicWeights"
@@ -351,8 +354,9 @@ class PublicWeights:
             lib = native.load()
             nb = lib.sufhip_linear_planes_bytes(self.experts, self.K, self.N, self.digits)
             if nb == 0:
-                _fail(what, "1 to 4096 experts, K up to 65536, N up to 2^24, weights of up to 4 "
-                            "digits with digits K < 2^17")
+                _fail(what, "1 to 4096 experts, K up to 65536, N up to 2^24, weights in "
+                            "[-2155905152, 2139062143] (4 digits), digits K < 2^17; these %d x "
+                            "%d x %d take %d digits" % (self.experts, self.K, self.N, self.digits))
             self.planes = torch.empty((nb + 7) // 8, dtype=torch.int64, device=W.device)
             native.call("sufhip_linear_prepare", W.data_ptr(), self.experts, self.K, self.N,
                         self.digits, self.planes.data_ptr(),

@@ -114,3 +114,16 @@ def test_one_expert_needs_no_tables():
     out = ff.ExpertFeedForward(3, 2, up, down, STATE).eval2(x, _pair(3, 40), *two[:2],
                                                             2 * slots, w)
     assert torch.equal(out[0] + out[1], got[0][0] + got[0][1])
+
+
+@pytest.mark.parametrize("most,digits", [(127, 1), (128, 2), (32639, 2), (32640, 3), (32767, 3),
+                                         (2139062143, 4), (2139062144, 5), (2 ** 31 - 1, 5)])
+def test_digits_of_the_largest_weight(most, digits):
+    """As many as the documentation says; a refusal names them and the range."""
+    say("digits of %d" % most)
+    W = np.array([[3, -5], [most, 0]])
+    if digits <= 4:
+        assert ff.PublicWeights(W).digits == digits
+    else:
+        with pytest.raises(ValueError, match=r"-2155905152, 2139062143\].* 5 digits"):
+            ff.PublicWeights(W)
