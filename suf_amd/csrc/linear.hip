@@ -761,7 +761,12 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
   SUFHIP_REQUIRE(args, "sufhip_linear2: null args");
   const sufhip_linear2_args& g = *args;
   if (int rc = check_extents(g, what)) return rc;
-  if (g.rows == 0) return SUFHIP_OK;
+  if (g.walk_count < 0 || (g.walk_count > 0 && (!g.walk_jobs || !g.walk_prg_state)))
+    return ff_fail(what, "walk_jobs and walk_prg_state are needed for walk_count jobs");
+  if (g.rows == 0)  // the walks may be other operators' gates'
+    return g.walk_count > 0
+             ? sufhip_trunc_prepare_batch(g.walk_prg_state, g.walk_jobs, g.walk_count, stream)
+             : SUFHIP_OK;
   if (g.x_rows == 0) return ff_fail(what, "x has no rows");
   if (!g.w.d_planes || (reinterpret_cast<uintptr_t>(g.w.d_planes) & 15) != 0)
     return ff_fail(what, "the weights' planes are null or not 16-byte aligned");
@@ -824,8 +829,6 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
     if (int rc = digits2_of(g.out_digits, g.rows, g.w.N, what, "out_digits")) return rc;
   a.digits = g.out_digits.d_digits;
   a.out_stride = g.out_stride;
-  if (g.walk_count < 0 || (g.walk_count > 0 && (!g.walk_jobs || !g.walk_prg_state)))
-    return ff_fail(what, "walk_jobs and walk_prg_state are needed for walk_count jobs");
   const Plan plan = plan_linear(g);
   const uint64_t tiles = uint64_t(plan.tiles) * plan.slices * plan.col_tiles;
   if (tiles >= (uint64_t(1) << 24) - 4096)  // a launch holds 2^32 lanes

@@ -503,7 +503,12 @@ int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream) {
   const sufhip_rmsnorm2_args& g = *args;
   if (g.rows < 0 || g.cols < 0 || g.rows > kMaxRows || g.cols > (1 << 20))
     return ff_fail(what, "rows in [0, 2^24] and cols in [0, 2^20]");
-  if (g.rows == 0 || g.cols == 0) return SUFHIP_OK;
+  if (g.walk_count < 0 || (g.walk_count > 0 && (!g.walk_jobs || !g.walk_prg_state)))
+    return ff_fail(what, "walk_jobs and walk_prg_state are needed for walk_count jobs");
+  if (g.rows == 0 || g.cols == 0)  // the walks may be other operators' gates'
+    return g.walk_count > 0
+             ? sufhip_trunc_prepare_batch(g.walk_prg_state, g.walk_jobs, g.walk_count, stream)
+             : SUFHIP_OK;
   const size_t n = size_t(g.rows) * size_t(g.cols);
   RmsArgs A{};
   A.rows = g.rows;
@@ -568,8 +573,6 @@ int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream) {
     for (int j = 0; j < i; ++j)
       if (sets_meet(outs[i], outs[j])) return ff_fail(what, "two outputs meet");
   }
-  if (g.walk_count < 0 || (g.walk_count > 0 && (!g.walk_jobs || !g.walk_prg_state)))
-    return ff_fail(what, "walk_jobs and walk_prg_state are needed for walk_count jobs");
   const size_t need = sufhip_rmsnorm2_work_bytes(g.rows, g.cols);
   if (need && (!g.d_work || (reinterpret_cast<uintptr_t>(g.d_work) & 15) != 0 ||
                g.work_bytes < need))

@@ -12,8 +12,8 @@ import torch
 
 import feedforward_reference as ref
 from suf_amd import feedforward as ff
-from suf_amd import native, tables, tasks
-from test_feedforward_arguments import at, linear_args
+from suf_amd import native, pfss, tables, tasks
+from test_feedforward_arguments import at, linear_args, norm_args, refused
 
 M64 = (1 << 64) - 1
 
@@ -34,6 +34,20 @@ def test_a_product_without_a_gate_hands_over_both_shares(rows, K, N):
         assert words(False, **kw) >= 2 * rows * N
         assert words(True, **kw) >= rows * N
     assert words(False) in (0, words(False, walk_count=2))
+
+
+@pytest.mark.parametrize("name,args", [("sufhip_linear2", lambda **kw: linear_args(rows=0, **kw)),
+                                       ("sufhip_rmsnorm2", lambda **kw: norm_args(rows=0, **kw)),
+                                       ("sufhip_rmsnorm2", lambda **kw: norm_args(cols=0, **kw))])
+def test_walks_of_a_call_without_rows(name, args):
+    """They are issued all the same: a job that no launch takes is refused."""
+    refused(name, args(walk_count=1), "walk_jobs")
+    refused(name, args(walk_count=-1), "walk_jobs")
+    state, jobs = ctypes.create_string_buffer(pfss.PRG_STATE_BYTES), (native.TruncJob * 1)()
+    jobs[0].kind = 77
+    a = args(walk_count=1, walk_jobs=ctypes.addressof(jobs),
+             walk_prg_state=ctypes.addressof(state))
+    assert getattr(native.load(), name)(ctypes.byref(a), None) == -1
 
 
 # ---- whose words are whose ----

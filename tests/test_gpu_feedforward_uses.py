@@ -1,4 +1,5 @@
 """What stands between one use of a feed-forward operator and the next."""
+import ctypes
 import warnings
 
 import numpy as np
@@ -8,7 +9,7 @@ import torch
 import oracle_lib as ol
 from gpu_util import say
 from suf_amd import feedforward as ff
-from suf_amd import native
+from suf_amd import native, tasks
 
 pytestmark = pytest.mark.gpu
 
@@ -127,3 +128,24 @@ def test_digits_of_the_largest_weight(most, digits):
     else:
         with pytest.raises(ValueError, match=r"-2155905152, 2139062143\].* 5 digits"):
             ff.PublicWeights(W)
+
+
+@pytest.mark.parametrize("name", ["sufhip_linear2", "sufhip_rmsnorm2"])
+def test_walks_of_a_call_without_rows(name):
+    """The key-only halves that come with a call are done though it has no rows."""
+    say("walks without rows, %s" % name)
+    gate = tasks.Trunc(tasks.Dealer(33), 12, 100, STATE)
+    gate.prepare()
+    torch.cuda.synchronize()
+    tables = [t[:1 << 12].clone() for t in gate.work]
+    for t in gate.work:
+        t.fill_(-7)
+    if name == "sufhip_linear2":
+        a = native.Linear2Args.from_buffer_copy(ff.Linear(_public(40, 24), 3, STATE)._args)
+    else:
+        a = native.RmsNorm2Args.from_buffer_copy(ff.RMSNorm(3, 40, STATE)._args)
+    a.rows = 0
+    state, jobs, a.walk_count = tasks.trunc_jobs([gate])
+    a.walk_jobs, a.walk_prg_state = ctypes.addressof(jobs), ctypes.addressof(state)
+    native.call(name, ctypes.byref(a), torch.cuda.current_stream().cuda_stream)
+    assert all(torch.equal(t[:1 << 12], w) for t, w in zip(gate.work, tables))
