@@ -137,10 +137,13 @@ extern "C" int sufhip_expert_mix2(const sufhip_expert_mix2_args* args, void* str
   a.out_stride = g.out_stride;
   if (sets_meet(o[0], o[1])) return ff_fail(what, "the two shares of out meet");
   const size_t listed = size_t(g.tokens) * g.each;
+  Material keys;
+  keys.gate(a.epi);
   for (int p = 0; p < 2; ++p) {
     if (range_meets(Range{g.d_slots, listed * 4}, o[p]) ||
         range_meets(Range{g.d_weights, listed * 8}, o[p]))
       return ff_fail(what, "out meets the slots or the weights");
+    if (keys.meets(o[p])) return ff_fail(what, "out meets the gate");
     for (int q = 0; q < 2; ++q) {
       if (a.z.p[0] && sets_meet(o[p], row_set(a.z, q, g.z_rows, g.cols)))
         return ff_fail(what, "out meets z");

@@ -8,6 +8,7 @@
 #include <cstdint>
 #include <string>
 
+#include "chain_device.hpp"
 #include "digit_planes.hpp"
 #include "suf_hip.h"
 #include "sufhip_internal.hpp"
@@ -196,5 +197,53 @@ inline int gate_of(const sufhip_trunc_epilogue& g, size_t n, const char* what, T
   t.y[0] = t.y[1] = nullptr;
   return make_epi(&t, n, what, out, false);
 }
+
+// What a call's gates, LUTs and triples are read from, and nothing that it
+// writes may meet.
+struct Material {
+  Range r[64];
+  RowSet t[24];
+  int n = 0, m = 0;
+
+  void add(const void* p, size_t bytes) { r[n++] = {p, bytes}; }
+  void gate(const uint8_t* const (&key)[2], const uint4* const (&table)[2], int f) {
+    for (int p = 0; p < 2; ++p) {
+      add(key[p], sufhip_trunc_key_bytes(SUFHIP_TRUNC_GAPARS, f));
+      add(table[p], size_t(8) << f);
+    }
+  }
+  void gate(const TruncEpi& e) {
+    if (e.on) gate(e.key, e.table, e.f);
+  }
+  // Triples of n < 2^31 elements; one with an index may read all its rows.
+  void chain(const ChainArgs& c, int prods, size_t lut_key_bytes) {
+    for (int p = 0; p < 2; ++p) add(c.lut[p], lut_key_bytes);
+    for (int k = 0; k < prods; ++k) {
+      gate(c.tkey[k], c.ttab[k], c.tf[k]);
+      for (const sufhip_term2* w : {&c.a[k], &c.b[k], &c.c[k]})
+        for (int p = 0; p < 2; ++p) {
+          if (w->index)
+            add(w->p[p], w->len * w->stride * 8);
+          else
+            t[m++] = {w->p[p] + w->off, int64_t(w->stride), int(c.n), 1};
+        }
+    }
+  }
+
+  bool meets(const RowSet& w) const {
+    for (int i = 0; i < n; ++i)
+      if (range_meets(r[i], w)) return true;
+    for (int i = 0; i < m; ++i)
+      if (sets_meet(t[i], w)) return true;
+    return false;
+  }
+  bool meets(const Range& w) const {
+    for (int i = 0; i < n; ++i)
+      if (ranges_meet(r[i], w)) return true;
+    for (int i = 0; i < m; ++i)
+      if (range_meets(w, t[i])) return true;
+    return false;
+  }
+};
 
 }  // namespace sufhip

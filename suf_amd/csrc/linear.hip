@@ -857,6 +857,14 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
     if (ranges_meet(outd, r) || ranges_meet(work, r))
       return ff_fail(what, "out_digits or the workspace meets an input");
   if (ranges_meet(outd, work)) return ff_fail(what, "out_digits meets the workspace");
+  Material keys;
+  keys.gate(a.epi);
+  if (g.act == SUFHIP_ACT_RELU)
+    for (int p = 0; p < 2; ++p) keys.add(g.relu.key[p], g.relu.key_bytes);
+  if (g.act == SUFHIP_ACT_CUBIC)
+    keys.chain(act, chain_products<SUFHIP_CHAIN_CUBIC>(), g.cubic->lut_key_bytes);
+  if (keys.meets(outd) || keys.meets(work))
+    return ff_fail(what, "out_digits or the workspace meets a gate, a LUT or a triple");
   for (int q = 0; q < 2; ++q)
     for (const RowSet* in : {&x[q], &res[q]})
       if (range_meets(outd, *in) || range_meets(work, *in))
@@ -878,6 +886,7 @@ int sufhip_linear2(const sufhip_linear2_args* args, void* stream) {
       }
       for (const Range& r : reads)
         if (range_meets(r, o[p])) return ff_fail(what, "out meets an input");
+      if (keys.meets(o[p])) return ff_fail(what, "out meets a gate, a LUT or a triple");
       if (range_meets(outd, o[p]) || range_meets(work, o[p]))
         return ff_fail(what, "out meets out_digits or the workspace");
     }

@@ -596,6 +596,12 @@ int sufhip_rmsnorm2(const sufhip_rmsnorm2_args* args, void* stream) {
       if (bad) return ff_fail(what, "an output or the workspace meets the dealer's material");
     }
   }
+  Material keys;
+  for (int k = 0; k < kGates; ++k) keys.gate(A.tr[k]);
+  keys.chain(A.rs, chain_products<SUFHIP_CHAIN_RSQRT>(), g.rsqrt.lut_key_bytes);
+  bool bad = keys.meets(outd) || keys.meets(work);
+  for (int i = 0; i < count; ++i) bad = bad || keys.meets(outs[i]);
+  if (bad) return ff_fail(what, "an output or the workspace meets a gate, a LUT or a triple");
   hipStream_t s = as_stream(stream);
   if (need) {
     A.sums = static_cast<uint64_t*>(g.d_work);

@@ -13,7 +13,7 @@ import torch
 import feedforward_reference as ref
 from suf_amd import feedforward as ff
 from suf_amd import native, pfss, tables, tasks
-from test_feedforward_arguments import at, linear_args, norm_args, refused
+from test_feedforward_arguments import at, gate, linear_args, mix_args, norm_args, put, refused
 
 M64 = (1 << 64) - 1
 
@@ -48,6 +48,63 @@ def test_walks_of_a_call_without_rows(name, args):
     a = args(walk_count=1, walk_jobs=ctypes.addressof(jobs),
              walk_prg_state=ctypes.addressof(state))
     assert getattr(native.load(), name)(ctypes.byref(a), None) == -1
+
+
+# ---- outputs over what the gates are read from ----
+
+def cubic_args(stride=1, **kw):
+    """A product of 4 x 32 outputs with a cubic's chain: gates at 40 to 43, the
+    LUT at 50, triples at 52 and 53."""
+    a = linear_args(act=native.ACT_CUBIC)
+    c = native.Chain2Args()
+    c.kind, c.frac_bits, c.n = native.CHAIN_CUBIC, 12, 4 * 32
+    c.lut[0], c.lut[1], c.intervals = at(50), at(51), 4
+    c.lut_key_bytes = native.load().sufhip_interval_lut_key_bytes(4, 4)
+    for t in list(c.a[:3]) + list(c.b[:3]) + list(c.c[:3]):
+        t.p[0], t.p[1], t.len, t.stride, t.mul = at(52), at(53), 4 * 32, stride, 1
+    for e in c.trunc[:3]:
+        gate(e)
+    a.cubic = ctypes.pointer(c)
+    return put(a, **kw)
+
+
+def relu_args(**kw):
+    size = native.load().sufhip_interval_lut_key_bytes(3, 2)
+    return linear_args(act=native.ACT_RELU, relu__key0=at(20), relu__key1=at(21),
+                       relu__intervals=3, relu__key_bytes=size, **kw)
+
+
+def large_norm(**kw):
+    return norm_args(rows=1 << 12, cols=1 << 9, x__row_stride=1 << 9, out_stride=1 << 9,
+                     rsqrt__n=1 << 12, **{"d_work": at(30), "work_bytes": 1 << 20, **kw})
+
+
+def digits(p, rows, cols):
+    return dict(out_digits__d_digits=p, out_digits__rows=rows, out_digits__cols=cols)
+
+
+OVER = [("sufhip_linear2", f, kw) for f, places in
+        ((linear_args, (40, 41, 42, 43)), (relu_args, (20, 21, 40)),
+         (cubic_args, (40, 42, 50, 51, 52, 53)))
+        for k in places for kw in (dict(out0=at(k)), dict(out1=at(k)), dict(d_work=at(k)),
+                                   digits(at(k), 4, 32))
+        if "d_work" not in kw or f is not linear_args]
+OVER += [("sufhip_linear2", cubic_args, dict(out0=at(52) + 8 * 127)),
+         ("sufhip_linear2", lambda **kw: cubic_args(stride=3, **kw),
+          dict(out0=at(53) + 8 * 3 * 127)),
+         ("sufhip_linear2", linear_args, dict(out0=at(42) + (8 << 12) - 8)),
+         ("sufhip_linear2", linear_args, dict(d_work=at(43), **digits(at(9), 4, 32)))]
+OVER += [("sufhip_rmsnorm2", f, kw) for k in (40, 41, 42, 43, 50, 51, 52, 53)
+         for f, kw in ((norm_args, dict(out0=at(k))), (norm_args, digits(at(k), 3, 40)),
+                       (norm_args, dict(total0=at(k), total1=at(31), total_stride=40)),
+                       (large_norm, dict(d_work=at(k))))]
+OVER += [("sufhip_expert_mix2", mix_args, dict([(o, at(k))])) for k in (40, 41, 42, 43)
+         for o in ("out0", "out1")]
+
+
+@pytest.mark.parametrize("name,args,kw", OVER)
+def test_outputs_over_keys_tables_and_triples(name, args, kw):
+    refused(name, args(**kw), "gate")
 
 
 # ---- whose words are whose ----
