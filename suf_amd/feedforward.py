@@ -101,6 +101,13 @@ def _extent(v, least, most, what, name):
     return int(v)
 
 
+def _settle(device):
+    """Waits for the current stream: any stream may use what it has written, and
+    the memory that it had before."""
+    if not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(device).synchronize()
+
+
 def _gpu(device, what):
     """The GPU that a name or number stands for, with its index."""
     device = torch.device(device)
@@ -179,8 +186,7 @@ class Digits:
         nb = native.load().sufhip_digits2_bytes(rows, cols)
         # Zeros: rows that no call writes stand for 0.
         self.buffer = torch.zeros(nb, dtype=torch.int8, device=device)
-        if not torch.cuda.is_current_stream_capturing():
-            torch.cuda.current_stream(device).synchronize()  # any stream may write them next
+        _settle(device)
         self.shape, self.d = (rows, cols), self.buffer.get_device()
         self.arg = native.Digits2()
         self.arg.d_digits, self.arg.rows, self.arg.cols = self.buffer.data_ptr(), rows, cols
@@ -241,6 +247,7 @@ class RMSNorm(_Block):
         super().__init__(prg_state, seed, device)
         with self._guard():
             self._deal(rows, cols, frac_bits, weight, eps, table, what)
+            _settle(self.device)
 
     def _deal(self, rows, cols, f, weight, eps, table, what):
         deal, n = self.dealer, rows * cols
@@ -361,7 +368,7 @@ class PublicWeights:
             native.call("sufhip_linear_prepare", W.data_ptr(), self.experts, self.K, self.N,
                         self.digits, self.planes.data_ptr(),
                         torch._C._cuda_getCurrentRawStream(self.d))
-            torch.cuda.current_stream().synchronize()  # any stream may read the planes
+            _settle(W.device)
         a = self.arg = native.LinearWeights()
         a.d_planes, a.experts, a.K, a.N, a.digits = (self.planes.data_ptr(), self.experts, self.K,
                                                      self.N, self.digits)
@@ -404,6 +411,7 @@ class Linear(_Block):
         super().__init__(prg_state, seed, torch.device("cuda", weights.d))
         with self._guard():
             self._deal(frac_bits, act, trunc)
+            _settle(self.device)
 
     def _deal(self, f, act, trunc):
         n = self.rows * self.weights.N
@@ -513,6 +521,7 @@ class ExpertMix(_Block):
         a.tokens, a.cols = self.tokens, self.cols
         with self._guard():
             self.tr = self._gate(frac_bits, self.tokens * self.cols)
+            _settle(self.device)
         self._epi = _epi(self.tr)
         a.trunc, a.mask = ctypes.pointer(self._epi), self.tr.mask & M64
 

@@ -125,6 +125,7 @@ def on_host(monkeypatch):
     monkeypatch.setattr(ff, "_gpu", lambda device, what: cpu)
     monkeypatch.setattr(ff._Block, "_guard", lambda self: contextlib.nullcontext())
     monkeypatch.setattr(ff, "Digits", lambda *a: None)
+    monkeypatch.setattr(ff, "_settle", lambda device: None, raising=False)
     monkeypatch.setattr(torch, "device", lambda *a: cpu)
     monkeypatch.setattr(tasks.pfss, "trunc_gen",
                         lambda *a: [torch.zeros(8, dtype=torch.uint8)] * 2)

@@ -9,7 +9,7 @@ import torch
 import oracle_lib as ol
 from gpu_util import say
 from suf_amd import feedforward as ff
-from suf_amd import native, tasks
+from suf_amd import native, tables, tasks
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +149,53 @@ def test_walks_of_a_call_without_rows(name):
     a.walk_jobs, a.walk_prg_state = ctypes.addressof(jobs), ctypes.addressof(state)
     native.call(name, ctypes.byref(a), torch.cuda.current_stream().cuda_stream)
     assert all(torch.equal(t[:1 << 12], w) for t, w in zip(gate.work, tables))
+
+
+MADE = [
+    lambda: ff.RMSNorm(3, 40, STATE), lambda: ff.RMSNorm(3, 40, STATE, weight=[4096] * 40),
+    lambda: ff.Linear(_public(40, 24), 3, STATE), lambda: ff.ExpertMix(3, 24, STATE),
+    lambda: ff.Linear(_public(40, 24), 3, STATE, act="relu"),
+    lambda: ff.Linear(_public(40, 24), 3, STATE, act=tables.gelu_table(12)),
+    lambda: ff.Linear(_public(40, 24), 3, STATE, trunc=False),
+    lambda: ff.PublicWeights(torch.ones(40, 24, dtype=torch.int64, device="cuda")),
+    lambda: ff.FeedForward(3, _public(40, 24), _public(24, 40), STATE),
+    lambda: ff.ExpertFeedForward(3, 2, _public(4, 40, 24), _public(4, 24, 40), STATE),
+]
+
+
+@pytest.mark.parametrize("which", range(len(MADE)))
+def test_objects_are_whole_when_they_are_made(which, monkeypatch):
+    """Whatever their stream was doing, and however long the gates' keys take:
+    another stream may use them at once."""
+    say("made on a busy stream, %d" % which)
+    gen = tasks.pfss.trunc_gen
+    monkeypatch.setattr(tasks.pfss, "trunc_gen",
+                        lambda *a: (torch.cuda._sleep(2000000), gen(*a))[1])
+    busy = torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(2000000)
+        made = MADE[which]()
+        assert busy.query()
+    assert made is not None
+
+
+@pytest.mark.parametrize("act", [None, "relu"])
+def test_another_stream_uses_them_at_once(act, monkeypatch):
+    say("used on another stream, act=%s" % act)
+    gen = tasks.pfss.trunc_gen
+    monkeypatch.setattr(tasks.pfss, "trunc_gen",
+                        lambda *a: (torch.cuda._sleep(2000000), gen(*a))[1])
+    x = tuple(torch.full((3, 40), v, dtype=torch.int64, device="cuda") for v in (50000, -77))
+    outs = [_pair(3, 24) for _ in range(2)]
+    public = _public(40, 24)
+    torch.cuda.synchronize()
+    for out in outs:
+        busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+        with torch.cuda.stream(busy):
+            o = ff.Linear(public, 3, STATE, act=act)
+            with torch.cuda.stream(other):
+                o.eval2(x, out)
+        torch.cuda.synchronize()
+    z = (50000 - 77) * (np.arange(40 * 24).reshape(40, 24) % 200 - 100).sum(0) >> 12
+    want = torch.from_numpy(np.maximum(z, 0) if act else z).cuda().expand(3, 24)
+    assert all(torch.equal(a + b, want) for a, b in outs)
