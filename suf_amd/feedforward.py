@@ -25,7 +25,8 @@ parts draw from the block's one Dealer).  eval2
 issues the key-only halves of its gates first, or waits for `prep` =
 (tasks.Prepared, batch) where they were issued before.  Calls of one object go
 one after the other (they share its workspace), in one stream or in streams
-that wait for each other.  A second call of an object with gates opens other
+that wait for each other; on another stream than it was made on, it has to
+live until they have run.  A second call of an object with gates opens other
 values under the same masks: eval2 warns of it, but not of a captured call's
 replays, of which each is one.
 
@@ -259,7 +260,7 @@ class RMSNorm(_Block):
             w = torch.as_tensor(weight)
             if w.dtype is not torch.int64 or tuple(w.shape) != (cols,):
                 _fail(what, "weight must be int64 [%d]" % cols)
-            self.weight = w.to(self.device).contiguous()
+            self.weight = w.to(self.device, copy=True).contiguous()
         # a is the mask of s in both products: s - a is opened once.
         a = deal.words(n).reshape(rows, cols)
         b = deal.words(rows)
@@ -356,7 +357,7 @@ class PublicWeights:
         with torch.cuda.device(device):
             W = W.to(device).contiguous()
             self.d = W.get_device()
-            self.bias = None if bias is None else bias.to(W.device).contiguous()
+            self.bias = None if bias is None else bias.to(W.device, copy=True).contiguous()
             self.digits = self._digits_of(int(W.min()), int(W.max()))
             lib = native.load()
             nb = lib.sufhip_linear_planes_bytes(self.experts, self.K, self.N, self.digits)

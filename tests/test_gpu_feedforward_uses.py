@@ -199,3 +199,25 @@ def test_another_stream_uses_them_at_once(act, monkeypatch):
     z = (50000 - 77) * (np.arange(40 * 24).reshape(40, 24) % 200 - 100).sum(0) >> 12
     want = torch.from_numpy(np.maximum(z, 0) if act else z).cuda().expand(3, 24)
     assert all(torch.equal(a + b, want) for a, b in outs)
+
+
+def test_public_values_are_the_objects_own():
+    """A buffer that weights were given in may be filled anew."""
+    say("public values, given in tensors of the GPU")
+    W = torch.arange(40 * 24, device="cuda").reshape(40, 24) % 200 - 100
+    bias = torch.arange(24, device="cuda") << 14
+    weight = torch.arange(40, device="cuda") * 300
+    x = tuple(torch.full((3, 40), v, dtype=torch.int64, device="cuda") for v in (50000, -77))
+
+    def run(spoil):
+        lin = ff.Linear(ff.PublicWeights(W.clone(), given[0]), 3, STATE)
+        norm = ff.RMSNorm(3, 40, STATE, weight=given[1])
+        if spoil:
+            for t in given:
+                t.fill_(-1)
+        return [a + b for a, b in (lin.eval2(x, _pair(3, 24)), norm.eval2(x, _pair(3, 40)))]
+    given = bias.clone(), weight.clone()
+    want = run(False)
+    assert all(torch.equal(a, b) for a, b in zip(run(True), want))
+    given = bias.cpu(), weight.cpu()
+    assert all(torch.equal(a, b) for a, b in zip(run(True), want))
