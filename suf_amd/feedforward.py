@@ -27,8 +27,8 @@ issues the key-only halves of its gates first, or waits for `prep` =
 one after the other (they share its workspace), in one stream or in streams
 that wait for each other; on another stream than it was made on, it has to
 live until they have run.  A second call of an object with gates opens other
-values under the same masks: eval2 warns of it, but not of a captured call's
-replays, of which each is one.
+values under the same masks: eval2 warns of it once, and not of a captured
+call's replays, of which each is one.
 
 The reference has LayerNorm (include/runtime/phase_tasks.hpp:2186-2668) and
 dense public products (src/nn/matmul_publicW.cpp:17-36); it has no experts.
@@ -140,11 +140,12 @@ class _Block:
         return torch.cuda.device(self.d)
 
     def _use(self):
-        """Warns of a second use."""
+        """Warns of a second use, once (a warning takes some microseconds)."""
         if self.spent and self.warns:
             warnings.warn("%s.eval2: an object is for one use; a second one opens other values "
                           "under the same masks, whose difference is then public" % self.warns[0],
                           RuntimeWarning, stacklevel=self.warns[1])
+            self.warns = None
 
     def _gate(self, bits, n):
         return Trunc(self.dealer, bits, n, self.prg_state, device=self.device)

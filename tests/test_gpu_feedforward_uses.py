@@ -72,7 +72,7 @@ def _experts():
 
 @pytest.mark.parametrize("make", [_norm, _linear, _mix, _block, _experts])
 def test_a_second_use_is_warned_of(make):
-    """Once for a call, where the call stands; a refused call is no use."""
+    """Once, where the call stands; a refused call is no use."""
     say("second use, %s" % make.__name__)
     call, *refused = make()
     with warnings.catch_warnings():
@@ -87,6 +87,9 @@ def test_a_second_use_is_warned_of(make):
     with pytest.warns(RuntimeWarning, match="one use") as seen:
         call()
     assert len(seen) == 1 and seen[0].filename == __file__
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        call()  # said once
     torch.cuda.synchronize()
 
 
