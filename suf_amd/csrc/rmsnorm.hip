@@ -247,9 +247,10 @@ __device__ __forceinline__ void rms_stage(uint32_t* tab, ChainLds& L, TruncHdr (
 
 // A row of up to 4 kQuads kBlock values stays on the CU from the sum to the
 // output; with kLong a longer one is read again for the output.  One row is
-// bound by latency, seven gates and a LUT one after the other: 15 us for 768
-// values.  Many stream their 12 words a value: 1000 x 2048 with total and
-// weight 53 us, 3.7 TB/s, the workgroups' chains between their loads.
+// bound by latency, seven gates and a LUT one after the other: 14 us for 768
+// values in a captured graph, 18 after other work.  Many stream their 12 words a
+// value: 1000 x 2048 with its total 55 us, 3.6 TB/s (with a weight too 67), the
+// workgroups' chains between their loads.
 template <int kQuads, int kBlock, bool kLong>
 __global__ void __launch_bounds__(kBlock, 1024 / kBlock) rmsnorm2_kernel(RmsArgs) {
   constexpr int kWaves = kBlock / 64;
@@ -438,7 +439,12 @@ int device_cus() {
   return cus;
 }
 
-// Whether a norm takes the three launches.
+// Whether a norm takes the three launches.  One launch / three, in us, the nine
+// gates' walks included, with residual and total: 512 x 1024 47 / 57, 512 x 2048
+// 54 / 65, 1000 x 2048 76 / 82, 1999 x 2048 with a weight 156 / 130.  The shape
+// counts too, which the rule leaves out: 488 x 4096 87 / 82, and with rows of
+// more than 4096 values, read twice either way, 64 x 16384 87 / 61; with many
+// short ones, a chain each, 20000 x 96 327 / 117.
 bool rms_large(int rows, int cols) { return size_t(rows) * size_t(cols) >= (size_t(1) << 21); }
 
 int launch_large(const RmsArgs& A, const RmsWalk& w, hipStream_t s) {
