@@ -227,7 +227,8 @@ class RMSNorm(_Block):
     = round(2^26 / cols); y from `table` (pieces' starts and words (c0, c1) in
     the unsigned order of ms + eps: tables.rsqrt_wide_table, for mean squares up
     to 4096, rougher up to 65536, where y stops falling) and a Newton step; out =
-    (s y) >> f, then (out weight) >> f.
+    (s y) >> f, then (out weight) >> f.  The gates take 62 bits: a row's sum of
+    squares has to stay below 2^(62 - 2 f), its mean square below 2^(36 - f).
     y is a Q(f) number: at a mean square of 4096 it is 2^(f - 6) steps.  So are
     ms and eps: an eps of less than half a step is 0, and a row whose ms + eps is
     n steps has its y off by a share of up to 0.75 / n (default eps, 12 bits: n

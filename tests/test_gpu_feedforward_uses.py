@@ -1,4 +1,5 @@
-"""What stands between one use of a feed-forward operator and the next."""
+"""What stands between one use of a feed-forward operator and the next, and what
+its public values and its rows may be."""
 import ctypes
 import warnings
 
@@ -6,8 +7,9 @@ import numpy as np
 import pytest
 import torch
 
+import feedforward_reference as ref
 import oracle_lib as ol
-from gpu_util import say
+from gpu_util import dev, say, u64
 from suf_amd import feedforward as ff
 from suf_amd import native, tables, tasks
 
@@ -224,3 +226,29 @@ def test_public_values_are_the_objects_own():
     assert all(torch.equal(a, b) for a, b in zip(run(True), want))
     given = bias.cpu(), weight.cpu()
     assert all(torch.equal(a, b) for a, b in zip(run(True), want))
+
+
+@pytest.mark.parametrize("rows,cols", [(9, 96), (2100, 1000)])
+@pytest.mark.parametrize("eps", [1.0 / 1024.0, 2.0 ** -25])
+def test_norm_of_rows_of_any_size(rows, cols, eps):
+    """Rows whose mean squares go from 0 to 2^22, through tables of up to 64
+    intervals: the definition, and outputs of their inputs' signs that saturate
+    where the table ends."""
+    say("norm %d x %d of rows of any size, eps %g" % (rows, cols, eps))
+    rng = np.random.default_rng(rows)
+    size = np.exp2(np.linspace(-14, 11, rows))[:, None]
+    x = np.rint(rng.standard_normal((rows, cols)) * size * 4096).astype(np.int64)
+    x[0] = 0
+    s = rng.integers(0, 1 << 64, x.shape, dtype=np.uint64)
+    norm = ff.RMSNorm(rows, cols, STATE, eps=eps)
+    assert len(norm.table[0]) == (58 if eps > 1e-4 else 63)
+    out = norm.eval2((dev(s), dev(x.view(np.uint64) - s)), _pair(rows, cols))
+    got = u64(out[0] + out[1])
+    assert np.array_equal(got, ref.rmsnorm(x.view(np.uint64), None, norm.inv_len, norm.eps_q,
+                                           norm.table, 12)[1])
+    # A floor takes a small value of either sign to -1 step at least.
+    got = got.view(np.int64)
+    assert np.all(np.where(x < 0, got <= 0, got >= 0))
+    last = size[:, 0] ** 2 > 2 * 65536  # past the table's end by more than a row's own spread
+    steps = int(norm.table[1][-1][0]) * 3 // 2
+    assert last.any() and np.array_equal(got[last], (x[last] * steps) >> 12)
